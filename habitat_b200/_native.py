@@ -160,6 +160,28 @@ EXPORTS = {
         ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p]),
     "hb_partials_sum_allreduce": (ctypes.c_int32, [
         ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p]),
+    "hb_quantize_rows": (ctypes.c_int32, [
+        ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64,
+        ctypes.c_void_p, ctypes.c_void_p]),
+    "hb_int8_matmul": (ctypes.c_int32, [
+        ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p,
+        ctypes.c_int32, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64,
+        ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]),
+    "hb_int8_matmul_quantized": (ctypes.c_int32, [
+        ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p,
+        ctypes.c_int32, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
+        ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]),
+    "hb_int8_workspace_bytes": (ctypes.c_int64, [
+        ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
+        ctypes.c_int32]),
+    "hb_orthogonalize": (ctypes.c_int32, [
+        ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
+        ctypes.c_int32, ctypes.POINTER(ctypes.c_double), ctypes.c_double, ctypes.c_int32, ctypes.c_void_p, ctypes.c_int64,
+        ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]),
+    "hb_orthogonalize_workspace_bytes": (ctypes.c_int64, [
+        ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32]),
+    "hb_dense_status": (ctypes.c_int32, [ctypes.POINTER(ctypes.c_int32)]),
+    "hb_dense_inject_status": (ctypes.c_int32, [ctypes.c_int32]),
     "hb_peer_allreduce": (ctypes.c_int32, [
         ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p]),
 }

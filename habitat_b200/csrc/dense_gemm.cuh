@@ -1,0 +1,440 @@
+// The matrix product behind the dense-layer operators (dense_int8.cu, orthogonalize.cu): D = A B^T on two-SM pairs.
+//
+// A pair of CTAs (cta_group::2) computes tiles of 256 x BN: each CTA brings its 128 rows of A and its BN / 2 rows of B
+// into a ring of 128-byte-wide slots by TMA (128-byte swizzle, no multicast), the even CTA's elected lane issues the MMAs for
+// both, and the accumulators (32-bit) lie in TMEM twice, so that eight epilogue warps per CTA drain one tile while the
+// next one is multiplied.  Per slot the pair moves 2 (128 + BN / 2) x 128 bytes for 4 MMAs; with BN = 256 that is 64
+// bytes per clock and SM, half of what two separate SMs with 128 x 256 tiles would need of L2.  A slot is 128 bytes of K
+// whatever the type, 128 8-bit integers or 64 half-precision values, so both share the ring and the issue loop.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "mlp_common.cuh"
+
+namespace dense {
+
+constexpr int kPairRows = 256;             // rows of a pair's tile
+constexpr int kCtaRows = 128;
+constexpr int kSlotK = 128;                // bytes of K per slot
+constexpr int kThreads = 384;              // warps: 0 TMA, 1 MMA, 2 TMEM, 3 none, 4-11 epilogue
+constexpr int kEpiWarp0 = 4;
+constexpr int kEpiWarps = 8;
+constexpr int kStageOutBytes = 32 * 128;   // an epilogue warp's staging: 32 rows x 128 bytes
+
+enum OutType : int32_t { kF32 = 0, kBF16 = 1, kF16 = 2 };
+
+template <int BN>
+struct Shape {
+  static constexpr int kBRows = BN / 2;                               // rows of B (columns of D) per CTA
+  static constexpr int kSlotBytes = (kCtaRows + kBRows) * kSlotK;     // per CTA
+  static constexpr int kSlots = BN == 256 ? 5 : BN == 128 ? 7 : 8;
+  static constexpr int kTmemCols = 2 * BN;
+};
+
+// Shared memory behind the ring: staging, channel scales and biases, row maxima of other CTAs, barriers.
+struct Tail {
+  uint8_t staging[kEpiWarps * kStageOutBytes];
+  float scale[2][256];
+  float bias[2][256];
+  float row_max[2][4][2][kCtaRows];
+  uint64_t full[8], empty[8], acc_full[2], acc_empty[2], exchange[2], drain;
+  uint32_t tmem;
+  int abort;
+};
+
+template <int BN>
+constexpr int smem_bytes() { return Shape<BN>::kSlots * Shape<BN>::kSlotBytes + static_cast<int>(sizeof(Tail)) + 1024; }
+
+// What a launch multiplies: `batches` products of M x N with kblocks slots of K each.  With `segments` 3 the operands are
+// pairs of planes, high and low parts (the low ones lie `batches` matrices behind), and the sum is hi hi + hi lo + lo hi.
+struct Product {
+  CUtensorMap a, b;        // [matrices][rows][K], boxes of 128 (a) and BN / 2 (b) rows x 128 bytes; b K-major or MN-major
+  int32_t M, N, kblocks, segments, batches;
+  int32_t tiles_m, tiles_n, num_tiles;   // num_tiles: over all batches
+  int32_t lower;           // 1: D is symmetric, only tiles that reach its lower triangle are computed
+  int32_t group;           // slots of K that one accumulator takes before it is drained; several groups: see Epi::kGrouped
+  int32_t* status;
+};
+
+struct Tile {
+  int batch, m0, n0;
+};
+
+// Tile `t` of a launch.  Full products go through groups of eight row blocks, column by column, so that the tiles in
+// flight share rows and columns in L2.
+template <int BN>
+__device__ __forceinline__ Tile tile_of(const Product& p, int t) {
+  const int per_batch = p.num_tiles / p.batches;
+  Tile r;
+  r.batch = t / per_batch;
+  t -= r.batch * per_batch;
+  int mt, nt;
+  if (p.lower) {
+    constexpr int kPer = kPairRows / BN;
+    mt = 0;
+    nt = t;
+    for (;;) {
+      const int row = min((mt + 1) * kPer, p.tiles_n);
+      if (nt < row) break;
+      nt -= row;
+      ++mt;
+    }
+  } else {
+    constexpr int kGroup = 8;
+    const int per_group = kGroup * p.tiles_n;
+    const int g = t / per_group;
+    const int rows = min(kGroup, p.tiles_m - g * kGroup);
+    const int in = t - g * per_group;
+    mt = g * kGroup + in % rows;
+    nt = in / rows;
+  }
+  r.m0 = mt * kPairRows;
+  r.n0 = nt * BN;
+  return r;
+}
+
+__device__ __forceinline__ void tma_3d_2sm(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, int32_t z,
+                                           uint32_t cluster_mbar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(cluster_mbar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+// Commits to the barriers of both CTAs of the pair; `pair` is its index in the cluster.
+__device__ __forceinline__ void commit_pair(uint32_t bar, uint32_t pair) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+      "h"(static_cast<uint16_t>(3u << (2 * pair)))
+      : "memory");
+}
+template <bool I8>
+__device__ __forceinline__ void mma_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  if (I8)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// 32 lanes x 32 columns without the wait (tc_wait_ld follows).
+__device__ __forceinline__ void tc_ld32_async(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// max(x, 0) that keeps NaN
+__device__ __forceinline__ float relu_nan(float x) { return max_nan(x, 0.0f); }
+
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  const __half2 p = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+
+// Where results go: rows of `ld` elements, matrices `batch_stride` elements apart; `vec`: every row starts on 16 bytes.
+struct Out {
+  void* base;
+  int64_t ld, batch_stride;
+  int32_t type;
+  int32_t vec;
+};
+
+// Stores a warp's 32 x 32 results: lane `lane` has row m0 + lane, columns n0 .. n0 + 31 in v.  Through the warp's staging
+// the rows leave in whole 64- or 128-byte pieces: 16-byte stores of 32 different rows fill half a sector each.
+__device__ __forceinline__ void store_rows(const Out& out, int batch, int M, int N, int m0, int n0, const float (&v)[32],
+                                           uint8_t* staging, int lane) {
+  __syncwarp();   // the last chunk's reads of the staging are done
+  if (out.type == kF32) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      *reinterpret_cast<float4*>(staging + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+          make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    __syncwarp();
+    float* base = static_cast<float*>(out.base) + batch * out.batch_stride;
+    if (out.vec && n0 + 32 <= N) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = 4 * i + (lane >> 3), c = lane & 7;
+        const float4 x = *reinterpret_cast<const float4*>(staging + r * 128 + ((c ^ (r & 7)) << 4));
+        if (m0 + r < M) *reinterpret_cast<float4*>(base + static_cast<int64_t>(m0 + r) * out.ld + n0 + 4 * c) = x;
+      }
+    } else if (n0 + lane < N) {
+#pragma unroll 4
+      for (int r = 0; r < 32 && m0 + r < M; ++r)
+        base[static_cast<int64_t>(m0 + r) * out.ld + n0 + lane] =
+            *reinterpret_cast<const float*>(staging + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + 4 * (lane & 3));
+    }
+  } else {
+    uint32_t w[16];
+    if (out.type == kBF16) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) w[i] = pack_f16(v[2 * i], v[2 * i + 1]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      *reinterpret_cast<uint4*>(staging + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) =
+          make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+    __syncwarp();
+    uint16_t* base = static_cast<uint16_t*>(out.base) + batch * out.batch_stride;
+    if (out.vec && n0 + 32 <= N) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 8 * i + (lane >> 2), c = lane & 3;
+        const uint4 x = *reinterpret_cast<const uint4*>(staging + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+        if (m0 + r < M) *reinterpret_cast<uint4*>(base + static_cast<int64_t>(m0 + r) * out.ld + n0 + 8 * c) = x;
+      }
+    } else if (n0 + lane < N) {
+#pragma unroll 4
+      for (int r = 0; r < 32 && m0 + r < M; ++r)
+        base[static_cast<int64_t>(m0 + r) * out.ld + n0 + lane] =
+            *reinterpret_cast<const uint16_t*>(staging + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + 2 * (lane & 7));
+    }
+  }
+}
+
+// What a tile's epilogue may use.
+struct EpiContext {
+  Tail* tail;
+  uint32_t tmem;          // this warp's lanes and first column of its half of the tile
+  int warp, lane, half;   // epilogue warp 0 .. 7, its half of the columns
+  int row;                // row of the CTA's 128 that the lane has
+  int m0, n0;             // first row of the CTA and first column of the warp's half, in the matrix
+  int batch;
+  uint32_t n_tile;        // how many tiles the CTA has drained before
+  bool first, last;       // group of the tile
+  uint32_t rank;          // in the cluster
+  bool* ok;
+};
+
+// Adds a group's accumulators to a lane's sums.
+template <int BN, class Release>
+__device__ __forceinline__ void add_group(const EpiContext& c, float (&sums)[BN / 2], Release release) {
+#pragma unroll
+  for (int chunk = 0; chunk < BN / 64; ++chunk) {
+    uint32_t acc[32];
+    tc_ld32_async(c.tmem + chunk * 32, acc);
+    tc_wait_ld();
+    if (chunk == BN / 64 - 1) release();
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const float x = __uint_as_float(acc[i]);
+      sums[32 * chunk + i] = c.first ? x : sums[32 * chunk + i] + x;
+    }
+  }
+}
+
+// The kernel.  Epilogue: a policy with `Params`, static kInt8, kMnMajorB, kGrouped, kClusterCtas (0: a pair; else the CTAs of a
+// cluster that share rows, one pair per BN columns) and
+//   static void begin(const Params&, const Product&, EpiContext&)                  before the accumulators are waited for (tables)
+//   static void drain(const Params&, const Product&, EpiContext&, sums, release)   calls release() once the accumulators are read
+// kGrouped: the tensor core adds 16 products of K at a time to its float32 sums and cuts what does not fit, which over
+// long K is off by as many units as there are additions, all to the same side.  So a tile's K goes to the accumulators in
+// groups, and drain() adds the groups in registers (sums), rounded to nearest; it acts on the last one.
+template <int BN, class Epi>
+__global__ void __launch_bounds__(kThreads, 1)
+gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ typename Epi::Params ep) {
+  using S = Shape<BN>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  Tail* tail = reinterpret_cast<Tail*>(ring + S::kSlots * S::kSlotBytes);
+  const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31);
+  const uint32_t rank = cluster_ctarank();
+  const uint32_t side = rank & 1u, pair = rank >> 1;
+  const uint32_t leader = rank & ~1u;
+  constexpr int kCluster = Epi::kClusterCtas ? Epi::kClusterCtas : 2;
+  volatile int* abort_flag = &tail->abort;
+  const uint32_t full = smem_u32(tail->full), empty = smem_u32(tail->empty), acc_full = smem_u32(tail->acc_full),
+                 acc_empty = smem_u32(tail->acc_empty);
+
+  if (threadIdx.x == 32) {
+    for (int s = 0; s < S::kSlots; ++s) {
+      mbar_init(full + 8 * s, 1);       // the leader's: its producer's expect_tx; both CTAs' copies count there
+      mbar_init(empty + 8 * s, 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(acc_full + 8 * s, 1);
+      mbar_init(acc_empty + 8 * s, 2 * kEpiWarps);
+      mbar_init(smem_u32(&tail->exchange[s]), kEpiWarps * (kCluster / 2));
+    }
+    mbar_init(smem_u32(&tail->drain), 1);
+    tail->abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tail->tmem)),
+                 "r"(static_cast<uint32_t>(S::kTmemCols))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  hb_grid_dependency_wait();   // the set-up above overlaps the end of the launch before it on the stream
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem = tail->tmem;
+
+  // a tile of the list per pair, or, where a cluster shares rows, per cluster (its pairs take neighbouring columns)
+  const int workers = static_cast<int>(gridDim.x) / kCluster * (Epi::kClusterCtas ? 1 : kCluster / 2);
+  const int worker = static_cast<int>(blockIdx.x) / (Epi::kClusterCtas ? kCluster : 2);
+  auto locate = [&](int t) {
+    if (Epi::kClusterCtas) return Tile{0, t * kPairRows, static_cast<int>(pair) * BN};
+    return tile_of<BN>(p, t);
+  };
+  const int total_kb = p.kblocks * p.segments;
+  const int group = Epi::kGrouped ? p.group : total_kb;
+
+  if (warp == 0) {
+    // ------------------------------ copies ------------------------------
+    if (lane == 0) {
+      const uint32_t ring_addr = smem_u32(ring);
+      uint32_t s = 0, ph = 1;
+      bool ok = true;
+      for (int t = worker; t < p.num_tiles && ok; t += workers) {
+        const Tile tile = locate(t);
+        for (int seg = 0; seg < p.segments && ok; ++seg) {
+          const int za = tile.batch + (seg == 2 ? p.batches : 0), zb = tile.batch + (seg == 1 ? p.batches : 0);
+          for (int kb = 0; kb < p.kblocks; ++kb) {
+            ok = mbar_wait(empty + 8 * s, ph, abort_flag, p.status, 0x511);
+            if (!ok) break;
+            const uint32_t bar = map_to_cta(full + 8 * s, leader);
+            if (side == 0) mbar_expect_tx(full + 8 * s, 2 * S::kSlotBytes);
+            const uint32_t dst = ring_addr + s * S::kSlotBytes;
+            constexpr int kElems = Epi::kInt8 ? kSlotK : kSlotK / 2;
+            tma_3d_2sm(dst, &p.a, kb * kElems, tile.m0 + static_cast<int>(side) * kCtaRows, za, bar);
+            const int n = tile.n0 + static_cast<int>(side) * S::kBRows;
+            if (Epi::kMnMajorB) {
+              // [64 rows of K][64 columns] per slab
+#pragma unroll
+              for (int j = 0; j < S::kBRows / 64; ++j)
+                tma_3d_2sm(dst + kCtaRows * kSlotK + j * 8192, &p.b, n + 64 * j, kb * kElems, zb, bar);
+            } else {
+              tma_3d_2sm(dst + kCtaRows * kSlotK, &p.b, kb * kElems, n, zb, bar);
+            }
+            if (++s == S::kSlots) { s = 0; ph ^= 1u; }
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------ MMAs (leader) ------------------------------
+    if (side == 0 && elect_one()) {
+      // D: 32-bit integers (2) or float (1); A and B: signed 8-bit (1) or f16 (0); B MN-major: bit 16; N, M
+      constexpr uint32_t idesc = (Epi::kInt8 ? (2u << 4) | (1u << 7) | (1u << 10) : (1u << 4)) |
+                                 (Epi::kMnMajorB ? 1u << 16 : 0u) | (static_cast<uint32_t>(BN >> 3) << 17) |
+                                 (static_cast<uint32_t>(kPairRows >> 4) << 24);
+      // 8 rows of a swizzle atom are 1,024 bytes; MN-major: slabs of 64 columns are 8 KB apart
+      constexpr uint64_t kDesc = (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) |
+                                 (static_cast<uint64_t>(2) << 61);
+      constexpr uint64_t a_hi = kDesc | (static_cast<uint64_t>(1) << 16);
+      constexpr uint64_t b_hi = kDesc | (static_cast<uint64_t>(Epi::kMnMajorB ? 8192 >> 4 : 1) << 16);
+      constexpr uint32_t b_step = Epi::kMnMajorB ? 2048 >> 4 : 32 >> 4;
+      const uint32_t a0 = (smem_u32(ring) & 0x3FFFF) >> 4;
+      uint32_t s = 0, ph = 0, n = 0;
+      bool ok = true;
+      for (int t = worker; t < p.num_tiles && ok; t += workers) {
+        for (int kb0 = 0; kb0 < total_kb && ok; kb0 += group, ++n) {
+          const uint32_t st = n & 1u;
+          ok = mbar_wait_cluster(acc_empty + 8 * st, ((n >> 1) & 1u) ^ 1u, abort_flag, p.status, 0x521);
+          tc_fence_after();
+          const uint32_t d = tmem + st * BN;
+          const int kb1 = min(kb0 + group, total_kb);
+          for (int kb = kb0; kb < kb1 && ok; ++kb) {
+            ok = mbar_wait_cluster(full + 8 * s, ph, abort_flag, p.status, 0x522);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t a_lo = a0 + s * (S::kSlotBytes >> 4);
+            const uint32_t b_lo = a_lo + (kCtaRows * kSlotK >> 4);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              mma_pair<Epi::kInt8>(d, a_hi | (a_lo + 2 * k), b_hi | (b_lo + b_step * k), idesc, (kb != kb0 || k) ? 1u : 0u);
+            commit_pair(empty + 8 * s, pair);
+            if (++s == S::kSlots) { s = 0; ph ^= 1u; }
+          }
+          if (ok) commit_pair(acc_full + 8 * st, pair);
+        }
+      }
+    }
+  } else if (warp >= kEpiWarp0) {
+    // ------------------------------ epilogue ------------------------------
+    const int w = warp - kEpiWarp0;
+    const int quad = warp & 3;
+    bool ok = true;
+    EpiContext c;
+    c.tail = tail; c.warp = w; c.lane = lane; c.half = w >> 2; c.row = quad * 32 + lane; c.rank = rank; c.ok = &ok;
+    uint32_t n = 0;
+    const uint32_t acc_empty_leader = map_to_cta(acc_empty, leader);
+    float sums[Epi::kGrouped ? BN / 2 : 1];
+    c.n_tile = 0;
+    for (int t = worker; t < p.num_tiles && ok; t += workers, ++c.n_tile) {
+      const Tile tile = locate(t);
+      c.m0 = tile.m0 + static_cast<int>(side) * kCtaRows;
+      c.n0 = tile.n0 + c.half * (BN / 2);
+      c.batch = tile.batch;
+      Epi::template begin<BN>(ep, p, c);
+      for (int kb0 = 0; kb0 < total_kb && ok; kb0 += group, ++n) {
+        const uint32_t st = n & 1u;
+        c.tmem = tmem + (static_cast<uint32_t>(quad * 32) << 16) + st * BN + static_cast<uint32_t>(c.half * (BN / 2));
+        c.first = kb0 == 0;
+        c.last = kb0 + group >= total_kb;
+        if (!mbar_wait(acc_full + 8 * st, (n >> 1) & 1u, abort_flag, p.status, 0x531)) { ok = false; break; }
+        tc_fence_after();
+        Epi::template drain<BN>(ep, p, c, sums, [&] {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if (side == 0) mbar_arrive(acc_empty + 8 * st);
+            else mbar_arrive_remote(acc_empty_leader + 8 * st);
+          }
+        });
+      }
+    }
+  }
+
+  // ------------------------------ teardown ------------------------------
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    // given up: wait, within limits, for MMAs and copies in flight
+    if (side == 0 && warp == 1 && elect_one()) {
+      commit_pair(smem_u32(&tail->drain), pair);
+      const long long t0 = clock64();
+      while (!mbar_try_wait_cluster(smem_u32(&tail->drain), 0) && clock64() - t0 <= kWaitCycles) {}
+    }
+    if (threadIdx.x == 0)
+      for (const long long t0 = clock64(); clock64() - t0 < 1000000;) {}
+    __syncthreads();
+  }
+  cluster_sync_all();   // no CTA leaves while another may still touch its memory
+  if (warp == 2) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(static_cast<uint32_t>(S::kTmemCols))
+                 : "memory");
+  }
+}
+
+}  // namespace dense

@@ -1,0 +1,660 @@
+// Dense layers in 8-bit integers: rows quantised with one scale each, products with one scale per row and per output
+// channel, and the same with the result handed on as quantised rows.
+//
+// Definition (float32 arithmetic, every operation rounded to nearest): amax = max |x| of the row, q = rint(x * (127 / amax)),
+// scale = amax / 127; y = (float(sum q w) * channel scale) * row scale + bias, then ReLU.  The integer sums are exact, so
+// results do not depend on the order of the additions: all kernels here, and any other program that follows the
+// definition, give the same bits.  A row whose amax is below 2^-119 counts as zeros (127 / amax would overflow); a row with
+// an infinity or a NaN gets zeros and the scale NaN, so that its results are NaN and not finite numbers that look like some.
+#include <atomic>
+
+#include "dense_gemm.cuh"
+#include "dense_host.h"
+
+namespace dense {
+namespace {
+
+constexpr int64_t kMostK = 131071;      // 128 * 128 * K stays below 2^31
+constexpr int64_t kMostRows = 0x7FFFFF00;
+
+// ---------------------------------------------------------------------------
+// Quantisation
+// ---------------------------------------------------------------------------
+struct RowScale {
+  float inverse, scale;
+  bool bad;
+};
+__device__ __forceinline__ RowScale row_scale(float amax) {
+  RowScale r;
+  r.bad = !(amax < __int_as_float(0x7F800000));
+  const bool zero = amax < 0x1p-119f;
+  r.inverse = r.bad || zero ? 0.0f : __fdiv_rn(127.0f, amax);
+  r.scale = r.bad ? __int_as_float(0x7FFFFFFF) : zero ? 0.0f : __fdiv_rn(amax, 127.0f);
+  return r;
+}
+// The integer nearest to x * inverse (ties to even) in the low byte: adding 1.5 * 2^23 leaves it in the last bits.
+__device__ __forceinline__ uint32_t quantized(float x, float inverse) {
+  return __float_as_uint(__fadd_rn(__fmul_rn(x, inverse), 12582912.0f));
+}
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
+template <typename T>
+__device__ __forceinline__ float to_float(T x);
+template <>
+__device__ __forceinline__ float to_float(float x) { return x; }
+template <>
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <>
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+
+constexpr int kQuantThreads = 256;
+constexpr int kQuantVecs = 8;           // 16-byte pieces of a row per thread
+
+// The largest value over the TPR threads that share a row, for all of them.
+template <int TPR>
+__device__ __forceinline__ float row_max(float v, float* scratch) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1) v = max_nan(v, __shfl_xor_sync(0xFFFFFFFFu, v, d));
+  if (TPR == 32) return v;
+  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = scratch[0];
+#pragma unroll
+  for (int i = 1; i < TPR / 32; ++i) v = max_nan(v, scratch[i]);
+  return v;
+}
+
+// Bound by memory: a row is read once, into registers (TPR threads x eight pieces of 16 bytes: 4 KB with a warp per row, 32 KB
+// with a block), and written from there.
+template <typename T, int TPR>
+__global__ void __launch_bounds__(kQuantThreads)
+quantize_vec_kernel(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t pitch, int8_t* __restrict__ q, int64_t q_pitch,
+                    float* __restrict__ scales) {
+  constexpr int kPer = 16 / static_cast<int>(sizeof(T));
+  __shared__ float scratch[kQuantThreads / 32];
+  hb_grid_dependency_wait();
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kQuantThreads / TPR) + threadIdx.x / TPR;
+  if (row >= rows) return;   // whole warps, and with TPR = 256 whole blocks
+  const int t = static_cast<int>(threadIdx.x) % TPR;
+  const T* xr = x + row * pitch;
+  union Piece {
+    uint4 u;
+    T e[kPer];
+  };
+  Piece v[kQuantVecs];
+  float amax = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kQuantVecs; ++i) {
+    const int64_t at = (static_cast<int64_t>(i) * TPR + t) * kPer;
+    v[i].u = make_uint4(0, 0, 0, 0);
+    if (at + kPer <= cols) {
+      v[i].u = *reinterpret_cast<const uint4*>(xr + at);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j)
+        if (at + j < cols) v[i].e[j] = xr[at + j];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kQuantVecs; ++i)
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) amax = max_nan(amax, fabsf(to_float(v[i].e[j])));
+  const RowScale s = row_scale(row_max<TPR>(amax, scratch));
+  if (t == 0) scales[row] = s.scale;
+  int8_t* qr = q + row * q_pitch;
+#pragma unroll
+  for (int i = 0; i < kQuantVecs; ++i) {
+    const int64_t at = (static_cast<int64_t>(i) * TPR + t) * kPer;
+    if (at >= cols) break;
+    uint32_t w[kPer / 4];
+#pragma unroll
+    for (int j = 0; j < kPer / 4; ++j) {
+      w[j] = low_bytes(quantized(to_float(v[i].e[4 * j]), s.inverse), quantized(to_float(v[i].e[4 * j + 1]), s.inverse),
+                       quantized(to_float(v[i].e[4 * j + 2]), s.inverse), quantized(to_float(v[i].e[4 * j + 3]), s.inverse));
+      if (s.bad) w[j] = 0;
+    }
+    if (at + kPer <= cols) {
+#pragma unroll
+      for (int j = 0; j < kPer / 4; ++j) reinterpret_cast<uint32_t*>(qr + at)[j] = w[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j)
+        if (at + j < cols) qr[at + j] = static_cast<int8_t>(w[j / 4] >> (8 * (j % 4)));
+    }
+  }
+}
+
+// Rows that start anywhere, or are longer than a block's registers: element by element, read twice (the second time from
+// cache).
+template <typename T, int TPR>
+__global__ void __launch_bounds__(kQuantThreads)
+quantize_any_kernel(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t pitch, int8_t* __restrict__ q, int64_t q_pitch,
+                    float* __restrict__ scales) {
+  __shared__ float scratch[kQuantThreads / 32];
+  hb_grid_dependency_wait();
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kQuantThreads / TPR) + threadIdx.x / TPR;
+  if (row >= rows) return;
+  const int t = static_cast<int>(threadIdx.x) % TPR;
+  const T* xr = x + row * pitch;
+  float amax = 0.0f;
+#pragma unroll 4
+  for (int64_t i = t; i < cols; i += TPR) amax = max_nan(amax, fabsf(to_float(xr[i])));
+  const RowScale s = row_scale(row_max<TPR>(amax, scratch));
+  if (t == 0) scales[row] = s.scale;
+#pragma unroll 4
+  for (int64_t i = t; i < cols; i += TPR)
+    q[row * q_pitch + i] = s.bad ? 0 : static_cast<int8_t>(quantized(to_float(xr[i]), s.inverse));
+}
+
+template <typename T>
+cudaError_t launch_quantize(const void* x, int64_t rows, int64_t cols, int64_t pitch, int8_t* q, int64_t q_pitch, float* scales,
+                            cudaStream_t s) {
+  constexpr int64_t kPer = 16 / sizeof(T);
+  const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && pitch % kPer == 0 && reinterpret_cast<uintptr_t>(q) % 4 == 0 &&
+                   q_pitch % 4 == 0;
+  const T* xt = static_cast<const T*>(x);
+  constexpr int64_t kWarpRow = 32 * kQuantVecs * kPer, kBlockRow = kQuantThreads * kQuantVecs * kPer;
+  // a warp per row while its registers hold one, and for single elements up to 512 of them
+  const bool warp_row = cols <= (vec ? kWarpRow : 512);
+  const int64_t per = warp_row ? kQuantThreads / 32 : 1;
+  const dim3 grid(static_cast<unsigned>((rows + per - 1) / per));
+  auto kernel = vec && cols <= kBlockRow ? (warp_row ? quantize_vec_kernel<T, 32> : quantize_vec_kernel<T, kQuantThreads>)
+                                         : (warp_row ? quantize_any_kernel<T, 32> : quantize_any_kernel<T, kQuantThreads>);
+  return hb::launch_overlapped(kernel, grid, dim3(kQuantThreads), 0, s, xt, rows, cols, pitch, q, q_pitch, scales);
+}
+
+// Rows of bytes that start anywhere -> rows that start on 16 bytes (TMA reads nothing else).
+__global__ void __launch_bounds__(256) align_rows_kernel(const int8_t* __restrict__ x, int64_t cols, int64_t pitch, int8_t* __restrict__ out,
+                                                         int64_t out_pitch) {
+  hb_grid_dependency_wait();
+  const int8_t* xr = x + static_cast<int64_t>(blockIdx.x) * pitch;
+  uint32_t* o = reinterpret_cast<uint32_t*>(out + static_cast<int64_t>(blockIdx.x) * out_pitch);
+  const uintptr_t start = reinterpret_cast<uintptr_t>(xr);
+  const uint32_t shift = static_cast<uint32_t>(start & 3u) * 8u;
+  const uint32_t* xw = reinterpret_cast<const uint32_t*>(start & ~static_cast<uintptr_t>(3));
+  for (int64_t i = threadIdx.x; 4 * i < cols; i += blockDim.x) {
+    // whole words inside the row are loaded as such; its last bytes one by one
+    uint32_t w = 0;
+    if (4 * i + 8 <= cols) {
+      w = shift ? __funnelshift_r(xw[i], xw[i + 1], shift) : xw[i];
+      if (i == 0 && shift) {
+        w = 0;
+        for (int j = 0; j < 4; ++j) w |= static_cast<uint32_t>(static_cast<uint8_t>(xr[j])) << (8 * j);
+      }
+    } else {
+      for (int j = 0; j < 4 && 4 * i + j < cols; ++j) w |= static_cast<uint32_t>(static_cast<uint8_t>(xr[4 * i + j])) << (8 * j);
+    }
+    o[i] = w;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Epilogues
+// ---------------------------------------------------------------------------
+struct LayerScales {
+  const float* row;
+  const float* channel;
+  const float* bias;     // or null
+  int32_t relu;
+};
+
+// Channel scales and biases of a warp group's half of the tile into shared memory (zeros outside the matrix).
+template <int BN>
+__device__ __forceinline__ void load_channels(const LayerScales& s, const Product& p, const EpiContext& c) {
+  const int i = (c.warp & 3) * 32 + c.lane;   // 0 .. 127 among the half's warps
+  const uint32_t buf = c.n_tile & 1u;
+  if (i < BN / 2) {
+    const int n = c.n0 + i;
+    c.tail->scale[buf][c.half * (BN / 2) + i] = n < p.N ? s.channel[n] : 0.0f;
+    c.tail->bias[buf][c.half * (BN / 2) + i] = n < p.N && s.bias ? s.bias[n] : 0.0f;
+  }
+  asm volatile("bar.sync %0, 128;" ::"r"(1 + c.half) : "memory");
+}
+
+// 32 accumulators of a row -> results.
+template <int BN>
+__device__ __forceinline__ void finish(const LayerScales& s, const EpiContext& c, float row_scale, int chunk, const uint32_t* acc,
+                                       float* v) {
+  const uint32_t buf = c.n_tile & 1u;
+  const float4* sc = reinterpret_cast<const float4*>(&c.tail->scale[buf][c.half * (BN / 2) + chunk * 32]);
+  const float4* bi = reinterpret_cast<const float4*>(&c.tail->bias[buf][c.half * (BN / 2) + chunk * 32]);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float4 w = sc[j], b = bi[j];
+    const float ws[4] = {w.x, w.y, w.z, w.w}, bs[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float y = __fadd_rn(__fmul_rn(__fmul_rn(__int2float_rn(static_cast<int>(acc[4 * j + i])), ws[i]), row_scale), bs[i]);
+      v[4 * j + i] = s.relu ? relu_nan(y) : y;
+    }
+  }
+}
+
+struct FloatOut {
+  static constexpr bool kInt8 = true, kMnMajorB = false, kGrouped = false;
+  static constexpr int kClusterCtas = 0;
+  struct Params {
+    LayerScales s;
+    Out out;
+  };
+  template <int BN>
+  static __device__ __forceinline__ void begin(const Params& ep, const Product& p, const EpiContext& c) {
+    load_channels<BN>(ep.s, p, c);
+  }
+  template <int BN, class Release>
+  static __device__ __forceinline__ void drain(const Params& ep, const Product& p, const EpiContext& c, float (&)[1], Release release) {
+    const int row = c.m0 + c.row;
+    const float rs = row < p.M ? __ldg(ep.s.row + row) : 0.0f;
+#pragma unroll 1
+    for (int chunk = 0; chunk < BN / 64; ++chunk) {
+      uint32_t acc[32];
+      float v[32];
+      tc_ld32_async(c.tmem + chunk * 32, acc);
+      tc_wait_ld();
+      if (chunk == BN / 64 - 1) release();
+      finish<BN>(ep.s, c, rs, chunk, acc, v);
+      store_rows(ep.out, 0, p.M, p.N, c.m0 + (c.row & ~31), c.n0 + chunk * 32, v, c.tail->staging + c.warp * kStageOutBytes, c.lane);
+    }
+  }
+};
+
+// The result as quantised rows.  The CTAs of a cluster hold whole rows between them (one pair per 256 columns): every lane
+// keeps its 128 results in registers, sends their largest magnitude to all CTAs of its row half through distributed shared
+// memory, and quantises when the others' are there.  The accumulators are free before the exchange, so the next tile's
+// MMAs run during it.
+template <int kCtas>
+struct QuantOut {
+  static constexpr bool kInt8 = true, kMnMajorB = false, kGrouped = false;
+  static constexpr int kClusterCtas = kCtas;
+  struct Params {
+    LayerScales s;
+    int8_t* q;
+    int64_t pitch;       // a multiple of 16, as is the address
+    float* scales;
+  };
+  template <int BN>
+  static __device__ __forceinline__ void begin(const Params& ep, const Product& p, const EpiContext& c) {
+    load_channels<BN>(ep.s, p, c);
+  }
+  template <int BN, class Release>
+  static __device__ __forceinline__ void drain(const Params& ep, const Product& p, const EpiContext& c, float (&)[1], Release release) {
+    static_assert(BN == 256, "128 columns per lane");
+    const int row = c.m0 + c.row;
+    const float rs = row < p.M ? __ldg(ep.s.row + row) : 0.0f;
+    float v[128];
+    float amax = 0.0f;
+#pragma unroll
+    for (int chunk = 0; chunk < 4; ++chunk) {
+      uint32_t acc[32];
+      tc_ld32_async(c.tmem + chunk * 32, acc);
+      tc_wait_ld();
+      finish<BN>(ep.s, c, rs, chunk, acc, v + 32 * chunk);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) amax = max_nan(amax, fabsf(v[32 * chunk + i]));
+    }
+    release();
+    const uint32_t buf = c.n_tile & 1u, side = c.rank & 1u;
+    const uint32_t bar = smem_u32(&c.tail->exchange[buf]);
+    const uint32_t mine = smem_u32(&c.tail->row_max[buf][c.rank >> 1][c.half][c.row]);
+#pragma unroll
+    for (int i = 0; i < kCtas / 2; ++i) st_cluster_f32(map_to_cta(mine, 2 * i + side), amax);
+    __syncwarp();
+    if (c.lane < kCtas / 2) mbar_arrive_remote(map_to_cta(bar, 2 * c.lane + side));
+    if (!mbar_wait_cluster(bar, (c.n_tile >> 1) & 1u, &c.tail->abort, p.status, 0x541)) {
+      *c.ok = false;
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < kCtas / 2; ++i)
+      amax = max_nan(amax, max_nan(c.tail->row_max[buf][i][0][c.row], c.tail->row_max[buf][i][1][c.row]));
+    const RowScale s = row_scale(amax);
+    if (c.rank < 2 && c.half == 0 && row < p.M) ep.scales[row] = s.scale;
+    uint8_t* staging = c.tail->staging + c.warp * kStageOutBytes;
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float* x = v + 16 * j + 4 * i;
+        w[i] = low_bytes(quantized(x[0], s.inverse), quantized(x[1], s.inverse), quantized(x[2], s.inverse), quantized(x[3], s.inverse));
+        if (s.bad) w[i] = 0;
+      }
+      *reinterpret_cast<uint4*>(staging + c.lane * 128 + ((j ^ (c.lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    __syncwarp();
+    const int m0 = c.m0 + (c.row & ~31);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = 4 * i + (c.lane >> 3), ch = c.lane & 7;
+      const uint8_t* at = staging + r * 128 + ((ch ^ (r & 7)) << 4);
+      const int n = c.n0 + 16 * ch;
+      if (m0 + r >= p.M) continue;
+      int8_t* to = ep.q + static_cast<int64_t>(m0 + r) * ep.pitch + n;
+      if (n + 16 <= p.N) {
+        *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(at);
+      } else {
+        for (int e = 0; n + e < p.N && e < 16; ++e) to[e] = static_cast<int8_t>(at[e]);
+      }
+    }
+  }
+};
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
+bool tma_rows(const void* p, int64_t pitch) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && pitch % 16 == 0; }
+
+struct Operands {
+  const int8_t* q;
+  int64_t q_pitch;
+  const int8_t* w;
+  int64_t w_pitch;
+};
+
+hb_status check_product(const char* name, const int8_t* q, int64_t q_pitch, const float* q_scales, const int8_t* w, int64_t w_pitch,
+                        const float* w_scales, int64_t M, int64_t N, int64_t K) {
+  if (M < 0 || N < 0 || K < 1 || q_pitch < K || w_pitch < K) {
+    hb::set_error("%s: M and N must not be negative, K at least 1, pitches at least K", name);
+    return HB_ERR_INVALID_ARGUMENT;
+  }
+  if (M > kMostRows || N > kMostRows || K > kMostK) {
+    hb::set_error("%s: K is at most 131071 (the sums are 32-bit integers), M and N below 2^31", name);
+    return HB_ERR_TOO_LARGE;
+  }
+  if (M && N && (!q || !q_scales || !w || !w_scales)) {
+    hb::set_error("%s: NULL argument", name);
+    return HB_ERR_INVALID_ARGUMENT;
+  }
+  return HB_OK;
+}
+
+int64_t align_bytes(int64_t rows, int64_t K, bool aligned) { return aligned ? 0 : round_up(rows * round_up(K, 16), 256); }
+
+// Operands that TMA can read: as they are, or copied to the workspace.
+hb_status align_operands(const char* name, Operands* o, int64_t M, int64_t N, int64_t K, uint8_t* workspace, int64_t workspace_bytes,
+                         int64_t more, cudaStream_t s) {
+  const bool q_ok = tma_rows(o->q, o->q_pitch), w_ok = tma_rows(o->w, o->w_pitch);
+  const int64_t need = align_bytes(M, K, q_ok) + align_bytes(N, K, w_ok) + more;
+  if (need > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256)) {
+    hb::set_error("%s: the workspace has to have %lld bytes, on a 256-byte boundary", name, static_cast<long long>(need));
+    return HB_ERR_INVALID_ARGUMENT;
+  }
+  const int64_t pitch = round_up(K, 16);
+  auto copy = [&](const int8_t** x, int64_t* x_pitch, int64_t rows) -> hb_status {
+    HB_CUDA_TRY(hb::launch_overlapped(align_rows_kernel, dim3(static_cast<unsigned>(rows)), dim3(K > 512 ? 256 : 64), 0, s, *x, K, *x_pitch,
+                                      reinterpret_cast<int8_t*>(workspace), pitch));
+    *x = reinterpret_cast<const int8_t*>(workspace);
+    *x_pitch = pitch;
+    workspace += align_bytes(rows, K, false);
+    return HB_OK;
+  };
+  if (!q_ok)
+    if (const hb_status st = copy(&o->q, &o->q_pitch, M)) return st;
+  if (!w_ok)
+    if (const hb_status st = copy(&o->w, &o->w_pitch, N)) return st;
+  return HB_OK;
+}
+
+hb_status describe(Product* p, const Operands& o, int64_t M, int64_t N, int64_t K, int bn, int32_t* status) {
+  HB_CUDA_TRY(encode_planes(&p->a, o.q, 1, K, M, 1, o.q_pitch, 0, kCtaRows));
+  HB_CUDA_TRY(encode_planes(&p->b, o.w, 1, K, N, 1, o.w_pitch, 0, bn / 2));
+  p->M = static_cast<int32_t>(M);
+  p->N = static_cast<int32_t>(N);
+  p->kblocks = static_cast<int32_t>((K + kSlotK - 1) / kSlotK);
+  p->segments = 1;
+  p->batches = 1;
+  p->tiles_m = static_cast<int32_t>((M + kPairRows - 1) / kPairRows);
+  p->tiles_n = static_cast<int32_t>((N + bn - 1) / bn);
+  p->lower = 0;
+  p->status = status;
+  return HB_OK;
+}
+
+template <int BN>
+hb_status launch_float(const Operands& o, int64_t M, int64_t N, int64_t K, const FloatOut::Params& ep, int32_t* status, cudaStream_t s) {
+  static std::atomic<int> held[64];
+  int pairs = 0;
+  auto kernel = gemm_kernel<BN, FloatOut>;
+  if (const hb_status st = max_clusters(kernel, 2, kThreads, smem_bytes<BN>(), held, &pairs)) return st;
+  Product p{};
+  if (const hb_status st = describe(&p, o, M, N, K, BN, status)) return st;
+  const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
+  if (tiles > 0x7FFFFFFF) {
+    hb::set_error("hb_int8_matmul: M x N too large for one launch");
+    return HB_ERR_TOO_LARGE;
+  }
+  p.num_tiles = static_cast<int32_t>(tiles);
+  const int clusters = p.num_tiles < pairs ? p.num_tiles : pairs;
+  HB_CUDA_TRY(launch_clusters(kernel, clusters, 2, kThreads, smem_bytes<BN>(), s, p, ep));
+  return HB_OK;
+}
+
+template <int kCtas>
+hb_status launch_quant(const Operands& o, int64_t M, int64_t N, int64_t K, const typename QuantOut<kCtas>::Params& ep, int32_t* status,
+                       cudaStream_t s) {
+  static std::atomic<int> held[64];
+  int clusters = 0;
+  auto kernel = gemm_kernel<256, QuantOut<kCtas>>;
+  if (const hb_status st = max_clusters(kernel, kCtas, kThreads, smem_bytes<256>(), held, &clusters)) return st;
+  Product p{};
+  if (const hb_status st = describe(&p, o, M, N, K, 256, status)) return st;
+  p.num_tiles = p.tiles_m;
+  if (p.num_tiles < clusters) clusters = p.num_tiles;
+  HB_CUDA_TRY(launch_clusters(kernel, clusters, kCtas, kThreads, smem_bytes<256>(), s, p, ep));
+  return HB_OK;
+}
+
+// The tile width whose rounds of tiles take least: a round costs its columns and about 24 columns' time beside.
+int tile_columns(int64_t M, int64_t N, int pairs) {
+  int best = 256;
+  int64_t least = INT64_MAX;
+  for (const int bn : {256, 128, 64}) {
+    const int64_t tiles = ((M + kPairRows - 1) / kPairRows) * ((N + bn - 1) / bn);
+    const int64_t cost = (tiles + pairs - 1) / pairs * (bn + 24);
+    if (cost < least) {
+      least = cost;
+      best = bn;
+    }
+  }
+  return best;
+}
+
+}  // namespace
+
+hb_status sm_count(int* sms) {
+  int dev = 0;
+  HB_CUDA_TRY(cudaGetDevice(&dev));
+  HB_CUDA_TRY(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev));
+  return HB_OK;
+}
+
+cudaError_t encode_planes(CUtensorMap* map, const void* base, int elem_bytes, int64_t cols, int64_t rows, int64_t planes, int64_t pitch,
+                          int64_t plane_stride, int box_rows) {
+  using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static std::atomic<void*> encode{nullptr};
+  void* fn = encode.load();
+  if (!fn) {
+    cudaDriverEntryPointQueryResult found;
+    const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found);
+    if (e != cudaSuccess) return e;
+    if (!fn || found != cudaDriverEntryPointSuccess) return cudaErrorNotSupported;
+    encode.store(fn);
+  }
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(planes)};
+  // one plane: its stride is never used, but has to be a multiple of 16 bytes
+  const cuuint64_t row_bytes = static_cast<cuuint64_t>(pitch) * elem_bytes;
+  const cuuint64_t strides[2] = {row_bytes, planes > 1 ? static_cast<cuuint64_t>(plane_stride) * elem_bytes : row_bytes};
+  const cuuint32_t box[3] = {static_cast<cuuint32_t>(128 / elem_bytes), static_cast<cuuint32_t>(box_rows), 1};
+  const cuuint32_t elem[3] = {1, 1, 1};
+  return reinterpret_cast<EncodeFn>(fn)(map, elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                                        const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? cudaSuccess
+             : cudaErrorInvalidValue;
+}
+
+namespace {
+std::mutex g_status_mu;
+int32_t* g_status[64];
+}  // namespace
+
+hb_status status_word(int32_t** word) {
+  int dev = 0;
+  HB_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) {
+    hb::set_error("device ordinal %d out of range", dev);
+    return HB_ERR_UNSUPPORTED;
+  }
+  std::lock_guard<std::mutex> lock(g_status_mu);
+  if (!g_status[dev]) {
+    void* p = nullptr;
+    HB_CUDA_TRY(cudaHostAlloc(&p, 64, cudaHostAllocDefault));
+    g_status[dev] = static_cast<int32_t*>(p);
+    *static_cast<volatile int32_t*>(g_status[dev]) = 0;
+  }
+  *word = g_status[dev];
+  return HB_OK;
+}
+
+hb_status begin_call(const char* name, int32_t** word) {
+  if (const hb_status st = status_word(word)) return st;
+  volatile int32_t* w = *word;
+  if (const int32_t code = *w) {
+    *w = 0;
+    hb::set_error("%s: an earlier dense-layer launch gave up on a bounded wait (code 0x%x)", name, code);
+    return HB_ERR_DEVICE_TIMEOUT;
+  }
+  return HB_OK;
+}
+
+}  // namespace dense
+
+extern "C" hb_status hb_dense_status(int32_t* device_status) {
+  if (!device_status) {
+    hb::set_error("hb_dense_status: NULL argument");
+    return HB_ERR_INVALID_ARGUMENT;
+  }
+  int32_t* word = nullptr;
+  if (const hb_status st = dense::status_word(&word)) return st;
+  HB_CUDA_TRY(cudaDeviceSynchronize());
+  volatile int32_t* w = word;
+  *device_status = *w;
+  *w = 0;
+  if (*device_status) {
+    hb::set_error("a dense-layer launch gave up on a bounded wait (code 0x%x)", *device_status);
+    return HB_ERR_DEVICE_TIMEOUT;
+  }
+  return HB_OK;
+}
+
+extern "C" hb_status hb_dense_inject_status(int32_t device_status) {
+  int32_t* word = nullptr;
+  if (const hb_status st = dense::status_word(&word)) return st;
+  *static_cast<volatile int32_t*>(word) = device_status;
+  return HB_OK;
+}
+
+extern "C" hb_status hb_quantize_rows(const void* x, int32_t x_type, int64_t rows, int64_t cols, int64_t x_pitch, int8_t* q,
+                                      int64_t q_pitch, float* scales, void* stream) {
+  if (rows < 0 || cols < 1 || x_pitch < cols || q_pitch < cols || x_type < HB_F32 || x_type > HB_F16) {
+    hb::set_error("hb_quantize_rows: rows must not be negative, cols at least 1, pitches at least cols");
+    return HB_ERR_INVALID_ARGUMENT;
+  }
+  if (rows == 0) return HB_OK;
+  if (!x || !q || !scales) {
+    hb::set_error("hb_quantize_rows: NULL argument");
+    return HB_ERR_INVALID_ARGUMENT;
+  }
+  if (rows > dense::kMostRows) {
+    hb::set_error("hb_quantize_rows: rows are below 2^31");
+    return HB_ERR_TOO_LARGE;
+  }
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  auto launch = x_type == HB_F32 ? dense::launch_quantize<float>
+                                 : x_type == HB_BF16 ? dense::launch_quantize<__nv_bfloat16> : dense::launch_quantize<__half>;
+  HB_CUDA_TRY(launch(x, rows, cols, x_pitch, q, q_pitch, scales, s));
+  return HB_OK;
+}
+
+extern "C" int64_t hb_int8_workspace_bytes(const int8_t* q, int64_t q_pitch, const int8_t* w, int64_t w_pitch, int64_t M, int64_t N,
+                                           int64_t K, int32_t quantized) {
+  if (M < 0 || N < 0 || K < 1) return -1;
+  int64_t bytes = dense::align_bytes(M, K, dense::tma_rows(q, q_pitch)) + dense::align_bytes(N, K, dense::tma_rows(w, w_pitch));
+  if (quantized && N > 1024) bytes += dense::round_up(M * dense::round_up(N, 4) * 4, 256);
+  return bytes;
+}
+
+extern "C" hb_status hb_int8_matmul(const int8_t* q, int64_t q_pitch, const float* q_scales, const int8_t* w, int64_t w_pitch,
+                                    const float* w_scales, const float* bias, int32_t relu, int64_t M, int64_t N, int64_t K, void* out,
+                                    int32_t out_type, int64_t out_pitch, void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace dense;
+  const char* name = "hb_int8_matmul";
+  if (const hb_status st = check_product(name, q, q_pitch, q_scales, w, w_pitch, w_scales, M, N, K)) return st;
+  if (out_type < HB_F32 || out_type > HB_F16 || out_pitch < N || (M && N && !out)) {
+    hb::set_error("%s: out has to be given, with a pitch of at least N and a type of 0 to 2", name);
+    return HB_ERR_INVALID_ARGUMENT;
+  }
+  int32_t* status = nullptr;
+  if (const hb_status st = begin_call(name, &status)) return st;
+  if (M == 0 || N == 0) return HB_OK;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  Operands o{q, q_pitch, w, w_pitch};
+  if (const hb_status st = align_operands(name, &o, M, N, K, static_cast<uint8_t*>(workspace), workspace_bytes, 0, s)) return st;
+  const int per = out_type == HB_F32 ? 4 : 8;
+  FloatOut::Params ep{{q_scales, w_scales, bias, relu}, {out, out_pitch, 0, out_type, 0}};
+  ep.out.vec = reinterpret_cast<uintptr_t>(out) % 16 == 0 && out_pitch % per == 0;
+  int sms = 0;
+  if (const hb_status st = sm_count(&sms)) return st;
+  switch (tile_columns(M, N, sms / 2)) {
+    case 256: return launch_float<256>(o, M, N, K, ep, status, s);
+    case 128: return launch_float<128>(o, M, N, K, ep, status, s);
+    default: return launch_float<64>(o, M, N, K, ep, status, s);
+  }
+}
+
+extern "C" hb_status hb_int8_matmul_quantized(const int8_t* q, int64_t q_pitch, const float* q_scales, const int8_t* w, int64_t w_pitch,
+                                              const float* w_scales, const float* bias, int32_t relu, int64_t M, int64_t N, int64_t K,
+                                              int8_t* out, int64_t out_pitch, float* out_scales, void* workspace, int64_t workspace_bytes,
+                                              void* stream) {
+  using namespace dense;
+  const char* name = "hb_int8_matmul_quantized";
+  if (const hb_status st = check_product(name, q, q_pitch, q_scales, w, w_pitch, w_scales, M, N, K)) return st;
+  if (M && (N < 1 || !out || !out_scales || !tma_rows(out, out_pitch) || out_pitch < N)) {
+    hb::set_error("%s: out and out_scales have to be given, N at least 1, out's rows on 16-byte boundaries", name);
+    return HB_ERR_INVALID_ARGUMENT;
+  }
+  int32_t* status = nullptr;
+  if (const hb_status st = begin_call(name, &status)) return st;
+  if (M == 0) return HB_OK;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  Operands o{q, q_pitch, w, w_pitch};
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  if (N > 1024) {
+    // wider rows than a cluster of eight holds: through memory, in float32
+    const int64_t pitch = round_up(N, 4), bytes = round_up(M * pitch * 4, 256);
+    const int64_t before = align_bytes(M, K, tma_rows(q, q_pitch)) + align_bytes(N, K, tma_rows(w, w_pitch));
+    if (!ws || workspace_bytes < before + bytes || reinterpret_cast<uintptr_t>(ws) % 256) {
+      hb::set_error("%s: the workspace has to have %lld bytes, on a 256-byte boundary", name, static_cast<long long>(before + bytes));
+      return HB_ERR_INVALID_ARGUMENT;
+    }
+    float* y = reinterpret_cast<float*>(ws + before);
+    if (const hb_status st = hb_int8_matmul(q, q_pitch, q_scales, w, w_pitch, w_scales, bias, relu, M, N, K, y, HB_F32, pitch, ws, before, stream))
+      return st;
+    return hb_quantize_rows(y, HB_F32, M, N, pitch, out, out_pitch, out_scales, stream);
+  }
+  if (const hb_status st = align_operands(name, &o, M, N, K, ws, workspace_bytes, 0, s)) return st;
+  const LayerScales scales{q_scales, w_scales, bias, relu};
+  switch ((N + 255) / 256) {
+    case 1: return launch_quant<2>(o, M, N, K, {scales, out, out_pitch, out_scales}, status, s);
+    case 2: return launch_quant<4>(o, M, N, K, {scales, out, out_pitch, out_scales}, status, s);
+    case 3: return launch_quant<6>(o, M, N, K, {scales, out, out_pitch, out_scales}, status, s);
+    default: return launch_quant<8>(o, M, N, K, {scales, out, out_pitch, out_scales}, status, s);
+  }
+}

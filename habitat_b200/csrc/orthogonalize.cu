@@ -1,0 +1,486 @@
+// Updates of weight matrices made nearly orthogonal by Newton-Schulz steps:
+//   X = G / (|G|_F + eps);   `steps` times:  A = X X^T,  B = a I + b A + c A^2,  X <- B X
+// (on G^T where G has more rows than columns), which drives all singular values towards one while the singular vectors
+// stay.  Three products per step on the tensor cores (dense_gemm.cuh); A and B are symmetric, so only tiles that reach their lower
+// triangle are computed and the rest is mirrored: s^2 l + s^3 + 2 s^2 l operations per step for sides s <= l.
+//
+// Numbers.  Operands are half precision (11 bits, against bfloat16's 8, at the same rate) scaled by powers of two: X, A and B by
+// 2^8, which keeps entries of matrices with a norm near one far from the subnormal numbers, and G, for the first step,
+// so that its Frobenius norm is in [2^13, 2^14).  The exact factor 1 / (|G| + eps) enters the first step's results in
+// float32, so a 16-bit G is multiplied unrounded.  Sums are float32, the norm float64.  With `split` every operand is a
+// pair of half-precision matrices, high and low parts (22 bits), and a product three (hi hi + hi lo + lo hi): float32
+// updates, whose results are held to float32's accuracy.
+#include <atomic>
+#include <cmath>
+#include <type_traits>
+
+#include "dense_gemm.cuh"
+#include "dense_host.h"
+
+namespace dense {
+namespace {
+
+constexpr float kScale = 256.0f;          // of stored X, A and B
+constexpr int kNormThreads = 256;
+constexpr int kMostPartials = 64;
+constexpr int kGroup = 4;                 // slots of K (256 values, 16 additions) per accumulation, with `split`
+
+template <typename T>
+__device__ __forceinline__ float element(const void* base, int64_t at) { return static_cast<float>(static_cast<const T*>(base)[at]); }
+__device__ __forceinline__ float load_element(const void* base, int type, int64_t at) {
+  return type == kF32 ? element<float>(base, at) : type == kBF16 ? element<__nv_bfloat16>(base, at) : element<__half>(base, at);
+}
+
+struct Source {
+  const void* base;
+  int64_t ld, batch_stride;
+  int32_t type, rows, cols;
+};
+
+// Sums of squares of G's elements, one per block.
+__global__ void __launch_bounds__(kNormThreads) norm_kernel(Source g, double* partials) {
+  __shared__ double scratch[kNormThreads / 32];
+  hb_grid_dependency_wait();
+  const int64_t base = blockIdx.y * g.batch_stride;
+  const int64_t n = static_cast<int64_t>(g.rows) * g.cols;
+  double sum = 0.0;
+  if (g.ld == g.cols) {
+#pragma unroll 4
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kNormThreads + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * kNormThreads) {
+      const double x = load_element(g.base, g.type, base + i);
+      sum += x * x;
+    }
+  } else {
+    for (int64_t r = blockIdx.x; r < g.rows; r += gridDim.x)
+      for (int64_t i = threadIdx.x; i < g.cols; i += kNormThreads) {
+        const double x = load_element(g.base, g.type, base + r * g.ld + i);
+        sum += x * x;
+      }
+  }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < kNormThreads / 32; ++i) sum += scratch[i];
+    partials[blockIdx.y * gridDim.x + blockIdx.x] = sum;
+  }
+}
+
+// G as half-precision operands: X0 [s][l] = G p (or G^T p), p the power of two that brings its norm to [2^13, 2^14); the
+// block at the origin leaves 1 / ((norm + eps) p), NaN where the norm is not finite.
+struct Planes {
+  __half* hi;
+  int64_t ld, batch_stride, low;   // low: elements from a high part to its low part, 0 without
+};
+__global__ void __launch_bounds__(256) operand_kernel(Source g, const double* partials, int n_partials, double eps, int flip, Planes x,
+                                                      float* factor) {
+  __shared__ float tile[32][33];
+  __shared__ float power;
+  hb_grid_dependency_wait();
+  const int batch = blockIdx.z;
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  if (ty == 0) {
+    double sum = 0.0;
+    for (int i = tx; i < n_partials; i += 32) sum += partials[batch * n_partials + i];
+#pragma unroll
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+    if (tx == 0) {
+      const double norm = sqrt(sum);
+      const bool fine = norm < static_cast<double>(INFINITY);
+      const int e = fine && norm > 0.0 ? max(-149, min(127, 13 - ilogb(norm))) : 0;
+      power = static_cast<float>(ldexp(1.0, e));
+      if (blockIdx.x == 0 && blockIdx.y == 0)
+        factor[batch] = fine ? static_cast<float>(1.0 / ((norm + eps) * ldexp(1.0, e))) : __int_as_float(0x7FFFFFFF);
+    }
+  }
+  __syncthreads();
+  const float p = power;
+  const int64_t base = batch * g.batch_stride;
+  const int s = flip ? g.cols : g.rows, l = flip ? g.rows : g.cols;
+  const int r0 = blockIdx.y * 32, c0 = blockIdx.x * 32;   // in X
+#pragma unroll
+  for (int i = 0; i < 32; i += 8) {
+    // read along G's rows
+    const int gr = (flip ? c0 : r0) + ty + i, gc = (flip ? r0 : c0) + tx;
+    tile[ty + i][tx] = gr < g.rows && gc < g.cols ? load_element(g.base, g.type, base + static_cast<int64_t>(gr) * g.ld + gc) * p : 0.0f;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 32; i += 8) {
+    const int r = r0 + ty + i, c = c0 + tx;
+    if (r >= s || c >= l) continue;
+    const float v = flip ? tile[tx][ty + i] : tile[ty + i][tx];
+    __half* at = x.hi + batch * x.batch_stride + static_cast<int64_t>(r) * x.ld + c;
+    const __half hi = __float2half_rn(v);
+    *at = hi;
+    if (x.low) at[x.low] = __float2half_rn(v - __half2float(hi));
+  }
+}
+
+// float32 values -> what their half-precision parts leave.
+__device__ __forceinline__ void take_half(float (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] -= __half2float(__float2half_rn(v[i]));
+}
+
+// Calls work(chunk, values) for the lane's 32-column chunks: as they leave the accumulators, or, where K comes in groups, from
+// the sums behind the last group.
+template <int BN, bool kGrouped, class Release, class Work>
+__device__ __forceinline__ void for_chunks(const EpiContext& c, float* sums, Release release, Work work) {
+  if constexpr (kGrouped) {
+    add_group<BN>(c, *reinterpret_cast<float(*)[BN / 2]>(sums), release);
+    if (!c.last) return;
+#pragma unroll
+    for (int chunk = 0; chunk < BN / 64; ++chunk) {
+      float v[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = sums[32 * chunk + i];
+      work(chunk, v);
+    }
+  } else {
+#pragma unroll 1
+    for (int chunk = 0; chunk < BN / 64; ++chunk) {
+      uint32_t acc[32];
+      float v[32];
+      tc_ld32_async(c.tmem + chunk * 32, acc);
+      tc_wait_ld();
+      if (chunk == BN / 64 - 1) release();
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(acc[i]);
+      work(chunk, v);
+    }
+  }
+}
+
+// v += factor * 32 half-precision values
+__device__ __forceinline__ void add_halves(float (&v)[32], const __half* at, float factor) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint4 x = *reinterpret_cast<const uint4*>(at + 8 * j);
+    const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&xs[i]));
+      v[8 * j + 2 * i] = fmaf(factor, f.x, v[8 * j + 2 * i]);
+      v[8 * j + 2 * i + 1] = fmaf(factor, f.y, v[8 * j + 2 * i + 1]);
+    }
+  }
+}
+
+// Symmetric results: A = X X^T, or B = a I + b A + c A^2, as half-precision operands (kSplit: high and low parts).
+template <bool kSplit>
+struct SymmetricOut {
+  static constexpr bool kInt8 = false, kMnMajorB = false, kGrouped = kSplit;
+  static constexpr int kClusterCtas = 0;
+  struct Params {
+    Planes out;
+    Planes a;               // of B: A; else hi is null
+    const float* factor;    // of the first A: X = X0 * factor; else null
+    float scale;            // of the accumulators
+    float on_a, on_diagonal;
+  };
+  template <int BN>
+  static __device__ __forceinline__ void begin(const Params&, const Product&, const EpiContext&) {}
+  template <int BN, class Release>
+  static __device__ __forceinline__ void drain(const Params& ep, const Product& p, const EpiContext& c, float* sums, Release release) {
+    const int row = c.m0 + c.row, row0 = c.m0 + (c.row & ~31);
+    float scale = ep.scale;
+    if (ep.factor) {
+      const float f = __ldg(ep.factor + c.batch);
+      scale *= f;
+      scale *= f;
+    }
+    for_chunks<BN, kSplit>(c, sums, release, [&](int chunk, float (&v)[32]) {
+      const int n0 = c.n0 + chunk * 32;
+      if (n0 > row0 || row0 >= p.M) return;      // above the diagonal (both are multiples of 32), or below the matrix
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] *= scale;
+      if (ep.a.hi) {
+        if (row < p.M) {
+          const __half* at = ep.a.hi + c.batch * ep.a.batch_stride + static_cast<int64_t>(row) * ep.a.ld + n0;
+          add_halves(v, at, ep.on_a);
+          if (kSplit) add_halves(v, at + ep.a.low, ep.on_a);
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (n0 + i == row) v[i] += ep.on_diagonal;
+      }
+      __half* base = ep.out.hi + c.batch * ep.out.batch_stride;
+#pragma unroll 1
+      for (int part = 0; part < (kSplit ? 2 : 1); ++part) {
+        if (n0 < row0) {
+          const Out out{base, ep.out.ld, 0, kF16, 1};
+          store_rows(out, 0, p.M, static_cast<int>(ep.out.ld), row0, n0, v, c.tail->staging + c.warp * kStageOutBytes, c.lane);
+        } else if (row < p.M) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (n0 + i <= row) base[static_cast<int64_t>(row) * ep.out.ld + n0 + i] = __float2half_rn(v[i]);
+        }
+        // the mirror image: a warp's 32 rows of a column are neighbours there
+        if (row < p.M) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (n0 + i < row) base[static_cast<int64_t>(n0 + i) * ep.out.ld + row] = __float2half_rn(v[i]);
+        }
+        if (kSplit) {
+          take_half(v);
+          base += ep.out.low;
+        }
+      }
+    });
+  }
+};
+
+// X <- B X as operands of the next step, or as the result.
+template <bool kSplit>
+struct UpdateOut {
+  static constexpr bool kInt8 = false, kMnMajorB = true, kGrouped = kSplit;
+  static constexpr int kClusterCtas = 0;
+  struct Params {
+    Planes x;               // the next X; hi null: the result
+    Out out;
+    int32_t flip;           // the result is transposed
+    const float* factor;    // of the first step
+    float scale;
+  };
+  template <int BN>
+  static __device__ __forceinline__ void begin(const Params&, const Product&, const EpiContext&) {}
+  template <int BN, class Release>
+  static __device__ __forceinline__ void drain(const Params& ep, const Product& p, const EpiContext& c, float* sums, Release release) {
+    const int row = c.m0 + c.row, row0 = c.m0 + (c.row & ~31);
+    const float scale = ep.factor ? ep.scale * __ldg(ep.factor + c.batch) : ep.scale;
+    uint8_t* staging = c.tail->staging + c.warp * kStageOutBytes;
+    for_chunks<BN, kSplit>(c, sums, release, [&](int chunk, float (&v)[32]) {
+      const int n0 = c.n0 + chunk * 32;
+      if (n0 >= p.N || row0 >= p.M) return;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] *= scale;
+      if (ep.x.hi) {
+        const Out out{ep.x.hi, ep.x.ld, ep.x.batch_stride, kF16, 1};
+        store_rows(out, c.batch, p.M, static_cast<int>(ep.x.ld), row0, n0, v, staging, c.lane);
+        if (kSplit) {
+          take_half(v);
+          const Out low{ep.x.hi + ep.x.low, ep.x.ld, ep.x.batch_stride, kF16, 1};
+          store_rows(low, c.batch, p.M, static_cast<int>(ep.x.ld), row0, n0, v, staging, c.lane);
+        }
+      } else if (!ep.flip) {
+        store_rows(ep.out, c.batch, p.M, p.N, row0, n0, v, staging, c.lane);
+      } else if (row < p.M) {
+        const int64_t at = c.batch * ep.out.batch_stride + row;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          if (n0 + i >= p.N) break;
+          const int64_t to = at + static_cast<int64_t>(n0 + i) * ep.out.ld;
+          if (ep.out.type == kF32) static_cast<float*>(ep.out.base)[to] = v[i];
+          else if (ep.out.type == kBF16) static_cast<__nv_bfloat16*>(ep.out.base)[to] = __float2bfloat16_rn(v[i]);
+          else static_cast<__half*>(ep.out.base)[to] = __float2half_rn(v[i]);
+        }
+      }
+    });
+  }
+};
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+int64_t up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
+
+struct Layout {
+  int64_t s, l, sp, lp;           // sides, and the pitches of rows of them
+  int64_t x_bytes, a_bytes;       // one buffer of X, of A or B (all batches and planes)
+  int64_t total;
+};
+Layout layout_of(int64_t batch, int64_t rows, int64_t cols, bool split) {
+  Layout r{};
+  r.s = rows < cols ? rows : cols;
+  r.l = rows < cols ? cols : rows;
+  r.sp = up(r.s, 64);
+  r.lp = up(r.l, 64);
+  const int64_t planes = split ? 2 : 1;
+  r.x_bytes = up(batch * planes * r.s * r.lp * 2, 256);
+  r.a_bytes = up(batch * planes * r.s * r.sp * 2, 256);
+  r.total = 2 * r.x_bytes + 2 * r.a_bytes + up(batch * 4, 256) + up(batch * kMostPartials * 8, 256);
+  return r;
+}
+
+// Tiles of a symmetric product whose columns begin before their rows end.
+int64_t lower_tiles(int64_t s, int bn) {
+  const int64_t tm = (s + kPairRows - 1) / kPairRows, tn = (s + bn - 1) / bn, per = kPairRows / bn;
+  int64_t n = 0;
+  for (int64_t i = 0; i < tm; ++i) n += (i + 1) * per < tn ? (i + 1) * per : tn;
+  return n;
+}
+
+// The width whose rounds of tiles take least, as for the 8-bit products.
+template <typename Count>
+int columns_for(const int* widths, int n, int pairs, Count tiles) {
+  int best = widths[0];
+  int64_t least = INT64_MAX;
+  for (int i = 0; i < n; ++i) {
+    const int64_t cost = (tiles(widths[i]) + pairs - 1) / pairs * (widths[i] + 24);
+    if (cost < least) {
+      least = cost;
+      best = widths[i];
+    }
+  }
+  return best;
+}
+
+template <int BN, class Epi>
+hb_status launch(Product p, const typename Epi::Params& ep, cudaStream_t s) {
+  p.group = kGroup;
+  static std::atomic<int> held[64];
+  int pairs = 0;
+  auto kernel = gemm_kernel<BN, Epi>;
+  if (const hb_status st = max_clusters(kernel, 2, kThreads, smem_bytes<BN>(), held, &pairs)) return st;
+  p.tiles_m = static_cast<int32_t>((p.M + kPairRows - 1) / kPairRows);
+  p.tiles_n = static_cast<int32_t>((p.N + BN - 1) / BN);
+  const int64_t tiles = p.batches * (p.lower ? lower_tiles(p.M, BN) : static_cast<int64_t>(p.tiles_m) * p.tiles_n);
+  if (tiles > 0x7FFFFFFF) {
+    hb::set_error("hb_orthogonalize: too large for one launch");
+    return HB_ERR_TOO_LARGE;
+  }
+  p.num_tiles = static_cast<int32_t>(tiles);
+  const int clusters = p.num_tiles < pairs ? p.num_tiles : pairs;
+  HB_CUDA_TRY(launch_clusters(kernel, clusters, 2, kThreads, smem_bytes<BN>(), s, p, ep));
+  return HB_OK;
+}
+
+}  // namespace
+}  // namespace dense
+
+extern "C" int64_t hb_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols, int32_t split) {
+  if (batch < 0 || rows < 0 || cols < 0) return -1;
+  return dense::layout_of(batch, rows, cols, split != 0).total;
+}
+
+extern "C" hb_status hb_orthogonalize(const void* update, int32_t type, int64_t batch, int64_t rows, int64_t cols, int64_t pitch,
+                                      int64_t batch_stride, int32_t steps, const double* coefficients, double eps, int32_t split, void* out,
+                                      int64_t out_pitch, int64_t out_batch_stride, void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace dense;
+  const char* name = "hb_orthogonalize";
+  if (batch < 0 || rows < 0 || cols < 0 || type < HB_F32 || type > HB_F16 || pitch < cols || out_pitch < cols || steps < 1 || steps > 100 ||
+      !coefficients || !(eps >= 0.0) || !std::isfinite(eps)) {
+    hb::set_error("%s: sizes must not be negative, pitches at least cols, steps 1 to 100, eps finite and not negative", name);
+    return HB_ERR_INVALID_ARGUMENT;
+  }
+  const double a = coefficients[0], b = coefficients[1], c = coefficients[2];
+  // The largest singular value any step can leave, from at most one on: the maximum of |x (a + b x^2 + c x^4)| over what the
+  // step before can leave; and the largest of B.  Stored operands are scaled by 2^8 and end at 65,504; A has the squares.
+  double most = 1.0, most_b = 0.0;
+  for (int i = 0; i < steps && most <= 12.0 && most_b <= 250.0; ++i) {
+    double next = 0.0;
+    for (int k = 0; k <= 4096; ++k) {
+      const double x = most * k / 4096, y = std::fabs(a + x * x * (b + c * x * x));
+      if (!(y <= 1e9)) most_b = 1e9;
+      if (y > most_b) most_b = y;
+      if (x * y > next) next = x * y;
+    }
+    most = next * 1.001;
+  }
+  if (!(most <= 12.0) || !(most_b <= 250.0)) {
+    hb::set_error("%s: with these coefficients the singular values grow beyond 12, or a factor beyond 250", name);
+    return HB_ERR_INVALID_ARGUMENT;
+  }
+  int32_t* status = nullptr;
+  if (const hb_status st = begin_call(name, &status)) return st;
+  if (batch == 0 || rows == 0 || cols == 0) return HB_OK;
+  if (!update || !out) {
+    hb::set_error("%s: NULL argument", name);
+    return HB_ERR_INVALID_ARGUMENT;
+  }
+  if (rows > (1 << 24) || cols > (1 << 24) || batch > 65535 || batch * 2 > 0x7FFFFFFF) {
+    hb::set_error("%s: at most 65,535 matrices of sides up to 2^24", name);
+    return HB_ERR_TOO_LARGE;
+  }
+  const Layout lay = layout_of(batch, rows, cols, split != 0);
+  if (!workspace || workspace_bytes < lay.total || reinterpret_cast<uintptr_t>(workspace) % 256) {
+    hb::set_error("%s: the workspace has to have %lld bytes, on a 256-byte boundary", name, static_cast<long long>(lay.total));
+    return HB_ERR_INVALID_ARGUMENT;
+  }
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  __half* x[2] = {reinterpret_cast<__half*>(ws), reinterpret_cast<__half*>(ws + lay.x_bytes)};
+  __half* A = reinterpret_cast<__half*>(ws + 2 * lay.x_bytes);
+  __half* B = reinterpret_cast<__half*>(ws + 2 * lay.x_bytes + lay.a_bytes);
+  float* factor = reinterpret_cast<float*>(ws + 2 * lay.x_bytes + 2 * lay.a_bytes);
+  double* partials = reinterpret_cast<double*>(reinterpret_cast<uint8_t*>(factor) + up(batch * 4, 256));
+  const int flip = rows > cols ? 1 : 0;
+  const int64_t planes = split ? 2 : 1;
+  const int64_t x_matrix = lay.s * lay.lp, a_matrix = lay.s * lay.sp;
+  auto x_planes = [&](int i) { return Planes{x[i], lay.lp, x_matrix, split ? batch * x_matrix : 0}; };
+  const Planes a_planes{A, lay.sp, a_matrix, split ? batch * a_matrix : 0}, b_planes{B, lay.sp, a_matrix, split ? batch * a_matrix : 0};
+
+  const Source g{update, pitch, batch_stride, type, static_cast<int32_t>(rows), static_cast<int32_t>(cols)};
+  int64_t n_partials = up(rows * cols, kNormThreads * 16) / (kNormThreads * 16);
+  if (n_partials > kMostPartials) n_partials = kMostPartials;
+  HB_CUDA_TRY(hb::launch_overlapped(norm_kernel, dim3(static_cast<unsigned>(n_partials), static_cast<unsigned>(batch)), dim3(kNormThreads), 0, st,
+                                    g, partials));
+  const dim3 grid(static_cast<unsigned>((lay.l + 31) / 32), static_cast<unsigned>((lay.s + 31) / 32), static_cast<unsigned>(batch));
+  if (grid.y > 65535) {
+    hb::set_error("%s: the shorter side is at most 2,097,120", name);
+    return HB_ERR_TOO_LARGE;
+  }
+  HB_CUDA_TRY(hb::launch_overlapped(operand_kernel, grid, dim3(256), 0, st, g, static_cast<const double*>(partials), static_cast<int>(n_partials), eps,
+                                    flip, x_planes(0), factor));
+
+  int sms = 0;
+  if (const hb_status e = sm_count(&sms)) return e;
+  const int pairs = sms / 2;
+  constexpr int kSym[3] = {256, 128, 64}, kUpd[2] = {256, 128};
+  const int bn_sym = columns_for(kSym, 3, pairs, [&](int bn) { return batch * lower_tiles(lay.s, bn); });
+  const int bn_upd = columns_for(kUpd, 2, pairs, [&](int bn) {
+    return batch * ((lay.s + kPairRows - 1) / kPairRows) * ((lay.l + bn - 1) / bn);
+  });
+  CUtensorMap x_rows[2], x_cols[2], x_k[2], a_rows, a_cols, b_rows;
+  for (int i = 0; i < (steps > 1 ? 2 : 1); ++i) {
+    HB_CUDA_TRY(encode_planes(&x_rows[i], x[i], 2, lay.l, lay.s, batch * planes, lay.lp, x_matrix, kCtaRows));
+    HB_CUDA_TRY(encode_planes(&x_cols[i], x[i], 2, lay.l, lay.s, batch * planes, lay.lp, x_matrix, bn_sym / 2));
+    HB_CUDA_TRY(encode_planes(&x_k[i], x[i], 2, lay.l, lay.s, batch * planes, lay.lp, x_matrix, 64));
+  }
+  HB_CUDA_TRY(encode_planes(&a_rows, A, 2, lay.s, lay.s, batch * planes, lay.sp, a_matrix, kCtaRows));
+  HB_CUDA_TRY(encode_planes(&a_cols, A, 2, lay.s, lay.s, batch * planes, lay.sp, a_matrix, bn_sym / 2));
+  HB_CUDA_TRY(encode_planes(&b_rows, B, 2, lay.s, lay.s, batch * planes, lay.sp, a_matrix, kCtaRows));
+
+  const int out_per = type == HB_F32 ? 4 : 8;
+  const bool out_vec = reinterpret_cast<uintptr_t>(out) % 16 == 0 && out_pitch % out_per == 0 && (batch == 1 || out_batch_stride % out_per == 0);
+  auto run = [&](auto is_split) -> hb_status {
+    constexpr bool kSplit = decltype(is_split)::value;
+    using Sym = SymmetricOut<kSplit>;
+    using Upd = UpdateOut<kSplit>;
+    auto product = [&](const CUtensorMap& ma, const CUtensorMap& mb, int64_t N, int64_t K) {
+      Product p{};
+      p.a = ma;
+      p.b = mb;
+      p.M = static_cast<int32_t>(lay.s);
+      p.N = static_cast<int32_t>(N);
+      p.kblocks = static_cast<int32_t>((K + 63) / 64);
+      p.segments = kSplit ? 3 : 1;
+      p.batches = static_cast<int32_t>(batch);
+      p.status = status;
+      return p;
+    };
+    auto symmetric = [&](const CUtensorMap& ma, const CUtensorMap& mb, int64_t K, const typename Sym::Params& ep) {
+      Product p = product(ma, mb, lay.s, K);
+      p.lower = 1;
+      return bn_sym == 256 ? launch<256, Sym>(p, ep, st) : bn_sym == 128 ? launch<128, Sym>(p, ep, st) : launch<64, Sym>(p, ep, st);
+    };
+    for (int i = 0; i < steps; ++i) {
+      const int from = i & 1, to = from ^ 1;
+      const bool first = i == 0, last = i == steps - 1;
+      const typename Sym::Params gram{a_planes, Planes{}, first ? factor : nullptr, first ? kScale : 1.0f / kScale, 0.0f, 0.0f};
+      if (const hb_status e = symmetric(x_rows[from], x_cols[from], lay.l, gram)) return e;
+      // B 2^8 = b (A 2^8) + (c / 2^8) (A 2^8)^2 + a 2^8 I
+      const typename Sym::Params poly{b_planes, a_planes, nullptr, static_cast<float>(c / kScale), static_cast<float>(b), static_cast<float>(a * kScale)};
+      if (const hb_status e = symmetric(a_rows, a_cols, lay.s, poly)) return e;
+      // (B 2^8)(X 2^8 or X0) -> X 2^8, or X
+      const float scale = (first ? 1.0f : 1.0f / kScale) * (last ? 1.0f : kScale) / kScale;
+      const typename Upd::Params ep{last ? Planes{} : x_planes(to), Out{out, out_pitch, out_batch_stride, type, out_vec}, flip, first ? factor : nullptr, scale};
+      const Product p = product(b_rows, x_k[from], lay.l, lay.s);
+      if (const hb_status e = bn_upd == 256 ? launch<256, Upd>(p, ep, st) : launch<128, Upd>(p, ep, st)) return e;
+    }
+    return HB_OK;
+  };
+  return split ? run(std::true_type{}) : run(std::false_type{});
+}

@@ -467,6 +467,57 @@ hb_status hb_partials_sum_allreduce(hb_peer* handle, const double* partials, int
  * single GPU, where kernels must not wait for one another. */
 hb_status hb_peer_allreduce(hb_peer* handle, double* values, int32_t n, int32_t phase, void* stream);
 
+/* ------------------------------------------------------------------------ */
+/* Dense layers in 8-bit integers, orthogonalised updates                   */
+/* ------------------------------------------------------------------------ */
+
+/* Element types of the calls below. */
+enum { HB_F32 = 0, HB_BF16 = 1, HB_F16 = 2 };
+
+/* Rows quantised to 8-bit integers with one scale each (nothing in the reference; the 8-bit form of its predictors'
+ * layers, analyzer/habitat/analysis/mlp/mlp.py:17-31).  In float32 arithmetic: amax = max |x|, q = rint(x * (127 / amax)), ties to
+ * even, scale = amax / 127.  amax below 2^-119: zeros, scale 0.  A row with an infinity or a NaN: zeros, scale NaN.
+ * x [rows][cols] of x_type, rows x_pitch elements apart; q rows q_pitch bytes apart. */
+hb_status hb_quantize_rows(const void* x, int32_t x_type, int64_t rows, int64_t cols, int64_t x_pitch, int8_t* q,
+                           int64_t q_pitch, float* scales, void* stream);
+
+/* out[m][n] = act((float(sum_k q[m][k] w[n][k]) * w_scales[n]) * q_scales[m] + bias[n]): exact integer sums, then float32,
+ * every operation rounded, act = max(x, 0) with relu (NaN stays), the result rounded once to out_type.  bias may be NULL.
+ * 1 <= K <= 131071.  Operands whose rows do not start on 16-byte boundaries are copied to the workspace first. */
+hb_status hb_int8_matmul(const int8_t* q, int64_t q_pitch, const float* q_scales, const int8_t* w, int64_t w_pitch,
+                         const float* w_scales, const float* bias, int32_t relu, int64_t M, int64_t N, int64_t K, void* out,
+                         int32_t out_type, int64_t out_pitch, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The same followed by hb_quantize_rows of the float32 result, which does not go through memory for N <= 1024.  out's rows
+ * have to start on 16-byte boundaries. */
+hb_status hb_int8_matmul_quantized(const int8_t* q, int64_t q_pitch, const float* q_scales, const int8_t* w, int64_t w_pitch,
+                                   const float* w_scales, const float* bias, int32_t relu, int64_t M, int64_t N, int64_t K,
+                                   int8_t* out, int64_t out_pitch, float* out_scales, void* workspace, int64_t workspace_bytes,
+                                   void* stream);
+
+/* Workspace of the two calls above for these operands (0 when they start on 16-byte boundaries; `quantized` for the second
+ * one), -1 for invalid sizes.  A workspace starts on a 256-byte boundary and belongs to one call at a time. */
+int64_t hb_int8_workspace_bytes(const int8_t* q, int64_t q_pitch, const int8_t* w, int64_t w_pitch, int64_t M, int64_t N,
+                                int64_t K, int32_t quantized);
+
+/* The update of a weight matrix with its singular values driven towards one by Newton-Schulz steps (nothing in the reference,
+ * whose training loop, mlp.py:148-250, steps along plain gradients): X = G / (|G|_F + eps), then `steps` times
+ * X <- (a I + b A + c A^2) X with A = X X^T (on G^T where rows > cols).  coefficients = {a, b, c} must keep the singular
+ * values of X below 12 and those of the factor below 250.  G [batch][rows][cols], rows `pitch` and matrices `batch_stride` elements apart, out in the same type.
+ * split: every product in three half-precision parts (22-bit operands), for float32 accuracy; otherwise one (11 bits, float32
+ * sums).  Elements of the result smaller than 2^-32 are lost.  A norm that is not finite gives NaN everywhere. */
+hb_status hb_orthogonalize(const void* update, int32_t type, int64_t batch, int64_t rows, int64_t cols, int64_t pitch,
+                           int64_t batch_stride, int32_t steps, const double* coefficients, double eps, int32_t split,
+                           void* out, int64_t out_pitch, int64_t out_batch_stride, void* workspace, int64_t workspace_bytes,
+                           void* stream);
+int64_t hb_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols, int32_t split);
+
+/* Synchronises the current GPU and reports whether one of the launches above gave up on a bounded device wait (reported
+ * once; without this call the next one of them on that GPU reports it). */
+hb_status hb_dense_status(int32_t* device_status);
+/* Writes that word from the host (tests of the error path). */
+hb_status hb_dense_inject_status(int32_t device_status);
+
 /* Builds made with -DHB_BOUNDS_CHECK compare every table and element index of the
  * wave-scaling kernels with its bound; the first violation is recorded in a device
  * word (site << 24 | index, top bit set) and the access redirected, nothing traps.
