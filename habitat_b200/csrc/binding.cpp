@@ -46,6 +46,12 @@ struct Api {
   decltype(&hb_mlp_poll_status) mlp_poll_status = nullptr;
   decltype(&hb_special_scale_grid) special_scale_grid = nullptr;
   decltype(&hb_iteration_totals) iteration_totals = nullptr;
+  decltype(&hb_quantize_rows) quantize_rows = nullptr;
+  decltype(&hb_int8_matmul) int8_matmul = nullptr;
+  decltype(&hb_int8_matmul_quantized) int8_matmul_quantized = nullptr;
+  decltype(&hb_int8_workspace_bytes) int8_workspace_bytes = nullptr;
+  decltype(&hb_orthogonalize) orthogonalize = nullptr;
+  decltype(&hb_orthogonalize_workspace_bytes) orthogonalize_workspace_bytes = nullptr;
 } api;
 
 PyObject* g_row_of = nullptr;       // device_table.row_of
@@ -1524,6 +1530,139 @@ PyObject* iteration_totals(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
+// -- dense layers (habitat_b200/dense.py) --------------------------------------
+
+// HB_F32, HB_BF16, HB_F16; -1 for other types.
+int element_type(at::ScalarType t) { return t == at::kFloat ? HB_F32 : t == at::kBFloat16 ? HB_BF16 : t == at::kHalf ? HB_F16 : -1; }
+at::ScalarType scalar_type(long t) { return t == HB_F32 ? at::kFloat : t == HB_BF16 ? at::kBFloat16 : at::kHalf; }
+
+// A CUDA matrix with contiguous rows that do not overlap, or null.
+struct Matrix {
+  const at::Tensor* t = nullptr;
+  int64_t rows = 0, cols = 0, pitch = 0;
+  explicit Matrix(PyObject* o) {
+    if (!o || !THPVariable_Check(o)) return;
+    const at::Tensor& x = THPVariable_Unpack(o);
+    if (!x.is_cuda() || x.dim() != 2) return;
+    rows = x.size(0);
+    cols = x.size(1);
+    if (cols > 1 && x.stride(1) != 1) return;
+    pitch = rows > 1 ? x.stride(0) : cols;
+    if (pitch < cols) return;
+    t = &x;
+  }
+};
+// A contiguous float32 vector of n values on `dev`.
+bool vector_of(PyObject* o, int64_t n, const at::Device& dev, const float** p) {
+  const at::Tensor* t = tensor(o, at::kFloat);
+  if (!t || t->dim() != 1 || t->size(0) != n || t->device() != dev) return false;
+  *p = static_cast<const float*>(data(t));
+  return true;
+}
+int64_t pitch_of(int64_t cols) { return (cols + 15) / 16 * 16; }
+// [rows, cols] int8 whose rows start on 16-byte boundaries; beside other tensors, with their device current.
+at::Tensor byte_rows(int64_t rows, int64_t cols, const at::Device& dev) {
+  const int64_t all[2] = {rows, pitch_of(cols)};
+  at::Tensor t = empty_beside(all, at::kChar, dev, true);
+  const int64_t sizes[2] = {rows, cols}, strides[2] = {pitch_of(cols), 1};
+  t.unsafeGetTensorImpl()->set_sizes_and_strides(sizes, strides);
+  return t;
+}
+at::Tensor float_vector(int64_t n, const at::Device& dev) {
+  const int64_t sizes[1] = {n};
+  return empty_beside(sizes, at::kFloat, dev, true);
+}
+PyObject* pair_of(at::Tensor q, at::Tensor scales) {
+  PyObject* r = PyTuple_New(2);
+  if (!r) return nullptr;
+  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(q)));
+  PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(std::move(scales)));
+  return r;
+}
+
+// quantize_rows(x)
+PyObject* quantize_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 1) Py_RETURN_NONE;
+  const Matrix x(a[0]);
+  if (!x.t || x.cols < 1 || element_type(x.t->scalar_type()) < 0) Py_RETURN_NONE;
+  const at::Device dev = x.t->device();
+  const c10::cuda::CUDAGuard guard(dev);
+  at::Tensor q = byte_rows(x.rows, x.cols, dev), scales = float_vector(x.rows, dev);
+  if (failed(api.quantize_rows(x.t->const_data_ptr(), element_type(x.t->scalar_type()), x.rows, x.cols, x.pitch,
+                               static_cast<int8_t*>(q.mutable_data_ptr()), pitch_of(x.cols), static_cast<float*>(scales.mutable_data_ptr()),
+                               c10::cuda::getCurrentCUDAStream(dev.index()).stream())))
+    return nullptr;
+  return pair_of(std::move(q), std::move(scales));
+  END_HANDLE_TH_ERRORS
+}
+
+// int8_product(q, scales, weight, weight_scales, bias or None, relu, out type, or -1 for quantised rows)
+PyObject* int8_product(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 7) Py_RETURN_NONE;
+  const Matrix q(a[0]), w(a[2]);
+  if (!q.t || !w.t || q.t->scalar_type() != at::kChar || w.t->scalar_type() != at::kChar || q.cols != w.cols || q.cols < 1 || q.cols > 131071)
+    Py_RETURN_NONE;
+  const at::Device dev = q.t->device();
+  const float *scales, *w_scales, *bias = nullptr;
+  if (w.t->device() != dev || !vector_of(a[1], q.rows, dev, &scales) || !vector_of(a[3], w.rows, dev, &w_scales) ||
+      (a[4] != Py_None && !vector_of(a[4], w.rows, dev, &bias)))
+    Py_RETURN_NONE;
+  const int relu = PyObject_IsTrue(a[5]);
+  const long type = PyLong_AsLong(a[6]);
+  if (relu < 0 || (type == -1 && PyErr_Occurred())) return nullptr;
+  if (type < 0 && w.rows < 1) Py_RETURN_NONE;
+  const c10::cuda::CUDAGuard guard(dev);
+  cudaStream_t s = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+  const int8_t *qp = static_cast<const int8_t*>(q.t->const_data_ptr()), *wp = static_cast<const int8_t*>(w.t->const_data_ptr());
+  const int64_t M = q.rows, N = w.rows, K = q.cols, ws_bytes = api.int8_workspace_bytes(qp, q.pitch, wp, w.pitch, M, N, K, type < 0);
+  c10::DataPtr ws;   // goes back to torch's allocator behind the call, on its stream
+  if (ws_bytes > 0) ws = c10::cuda::CUDACachingAllocator::get()->allocate(static_cast<size_t>(ws_bytes));
+  if (type < 0) {
+    at::Tensor out = byte_rows(M, N, dev), out_scales = float_vector(M, dev);
+    if (failed(api.int8_matmul_quantized(qp, q.pitch, scales, wp, w.pitch, w_scales, bias, relu, M, N, K, static_cast<int8_t*>(out.mutable_data_ptr()),
+                                         pitch_of(N), static_cast<float*>(out_scales.mutable_data_ptr()), ws.get(), ws_bytes, s)))
+      return nullptr;
+    return pair_of(std::move(out), std::move(out_scales));
+  }
+  const int64_t sizes[2] = {M, N};
+  at::Tensor out = empty_beside(sizes, scalar_type(type), dev, true);
+  if (failed(api.int8_matmul(qp, q.pitch, scales, wp, w.pitch, w_scales, bias, relu, M, N, K, out.mutable_data_ptr(), static_cast<int32_t>(type), N,
+                             ws.get(), ws_bytes, s)))
+    return nullptr;
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// orthogonalize(update, steps, a, b, c, eps)
+PyObject* orthogonalize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6 || !THPVariable_Check(a[0])) Py_RETURN_NONE;
+  const at::Tensor& u = THPVariable_Unpack(a[0]);
+  const int type = element_type(u.scalar_type());
+  if (!u.is_cuda() || type < 0 || u.dim() < 2 || !u.is_contiguous()) Py_RETURN_NONE;
+  const long steps = PyLong_AsLong(a[1]);
+  const double c[3] = {PyFloat_AsDouble(a[2]), PyFloat_AsDouble(a[3]), PyFloat_AsDouble(a[4])}, eps = PyFloat_AsDouble(a[5]);
+  if (PyErr_Occurred()) return nullptr;
+  const at::Device dev = u.device();
+  const c10::cuda::CUDAGuard guard(dev);
+  const int64_t rows = u.size(-2), cols = u.size(-1);
+  int64_t batch = 1;
+  for (int64_t i = 0; i < u.dim() - 2; ++i) batch *= u.size(i);
+  const int split = u.scalar_type() != at::kBFloat16;   // three products of high and low parts, for all but the 8-bit mantissas
+  at::Tensor out = empty_beside(u.sizes(), u.scalar_type(), dev, true);
+  const int64_t ws_bytes = api.orthogonalize_workspace_bytes(batch, rows, cols, split);
+  c10::DataPtr ws;
+  if (ws_bytes > 0) ws = c10::cuda::CUDACachingAllocator::get()->allocate(static_cast<size_t>(ws_bytes));
+  if (failed(api.orthogonalize(u.const_data_ptr(), type, batch, rows, cols, cols, rows * cols, steps < 0 || steps > 1000 ? -1 : static_cast<int32_t>(steps),
+                               c, eps, split, out.mutable_data_ptr(), cols, rows * cols, ws.get(), ws_bytes,
+                               c10::cuda::getCurrentCUDAStream(dev.index()).stream())))
+    return nullptr;
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
 // setup(addresses by name, row_of, check, WaveResult, DeviceProperties)
 PyObject* setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 5 || !PyDict_Check(a[0])) {
@@ -1543,7 +1682,10 @@ PyObject* setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
       !load(api.segment_sum_planes, "hb_segment_sum_planes") ||
       !load(api.mlp_predict_grid, "hb_mlp_predict_grid") || !load(api.mlp_poll_status, "hb_mlp_poll_status") ||
       !load(api.special_scale_grid, "hb_special_scale_grid") ||
-      !load(api.iteration_totals, "hb_iteration_totals")) {
+      !load(api.iteration_totals, "hb_iteration_totals") || !load(api.quantize_rows, "hb_quantize_rows") ||
+      !load(api.int8_matmul, "hb_int8_matmul") || !load(api.int8_matmul_quantized, "hb_int8_matmul_quantized") ||
+      !load(api.int8_workspace_bytes, "hb_int8_workspace_bytes") || !load(api.orthogonalize, "hb_orthogonalize") ||
+      !load(api.orthogonalize_workspace_bytes, "hb_orthogonalize_workspace_bytes")) {
     if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, "an entry point is missing");
     return nullptr;
   }
@@ -1562,7 +1704,7 @@ PyObject* set_generation(PyObject*, PyObject* v) {
 
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(setup), FAST(wave_scale), FAST(wave_scale_host), FAST(submit_wave), FAST(host_block), FAST(release_host_blocks), FAST(mlp_predict), FAST(mlp_predict_one), FAST(flatten_trace), FAST(start_kinds), FAST(run_group), FAST(iteration_totals), FAST(partials_sum), FAST(group_sum),
-                         FAST(plane_sum), FAST(segment_sum),
+                         FAST(plane_sum), FAST(segment_sum), FAST(quantize_rows), FAST(int8_product), FAST(orthogonalize),
                          {"set_generation", set_generation, METH_O, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -7,6 +7,7 @@
 // definition, give the same bits.  A row whose amax is below 2^-119 counts as zeros (127 / amax would overflow); a row with
 // an infinity or a NaN gets zeros and the scale NaN, so that its results are NaN and not finite numbers that look like some.
 #include <atomic>
+#include <type_traits>
 
 #include "dense_gemm.cuh"
 #include "dense_host.h"
@@ -50,7 +51,6 @@ template <>
 __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 
 constexpr int kQuantThreads = 256;
-constexpr int kQuantVecs = 8;           // 16-byte pieces of a row per thread
 
 // The largest value over the TPR threads that share a row, for all of them.
 template <int TPR>
@@ -66,63 +66,56 @@ __device__ __forceinline__ float row_max(float v, float* scratch) {
   return v;
 }
 
-// Bound by memory: a row is read once, into registers (TPR threads x eight pieces of 16 bytes: 4 KB with a warp per row, 32 KB
-// with a block), and written from there.
-template <typename T, int TPR>
+// Bound by memory: a row is read once, into registers (TPR threads x VECS pieces of VB bytes: up to 4 KB with a warp per row,
+// 32 KB with a block), and written from there.
+template <typename T, int VB, int TPR, int VECS>
 __global__ void __launch_bounds__(kQuantThreads)
-quantize_vec_kernel(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t pitch, int8_t* __restrict__ q, int64_t q_pitch,
+quantize_vec_kernel(const T* __restrict__ x, int64_t rows, int cols, int64_t pitch, int8_t* __restrict__ q, int64_t q_pitch,
                     float* __restrict__ scales) {
-  constexpr int kPer = 16 / static_cast<int>(sizeof(T));
+  constexpr int kPer = VB / static_cast<int>(sizeof(T));
+  using Piece = typename std::conditional<VB == 16, uint4, uint2>::type;
+  using Bytes = typename std::conditional<kPer == 8, uint2, typename std::conditional<kPer == 4, uint32_t, uint16_t>::type>::type;
   __shared__ float scratch[kQuantThreads / 32];
   hb_grid_dependency_wait();
   const int64_t row = static_cast<int64_t>(blockIdx.x) * (kQuantThreads / TPR) + threadIdx.x / TPR;
   if (row >= rows) return;   // whole warps, and with TPR = 256 whole blocks
   const int t = static_cast<int>(threadIdx.x) % TPR;
   const T* xr = x + row * pitch;
-  union Piece {
-    uint4 u;
+  union {
+    Piece u;
     T e[kPer];
-  };
-  Piece v[kQuantVecs];
+  } v[VECS];
+#pragma unroll
+  for (int i = 0; i < VECS; ++i) {
+    const int at = (i * TPR + t) * kPer;
+    v[i].u = Piece{};
+    if (at < cols) v[i].u = *reinterpret_cast<const Piece*>(xr + at);
+  }
   float amax = 0.0f;
 #pragma unroll
-  for (int i = 0; i < kQuantVecs; ++i) {
-    const int64_t at = (static_cast<int64_t>(i) * TPR + t) * kPer;
-    v[i].u = make_uint4(0, 0, 0, 0);
-    if (at + kPer <= cols) {
-      v[i].u = *reinterpret_cast<const uint4*>(xr + at);
-    } else {
-#pragma unroll
-      for (int j = 0; j < kPer; ++j)
-        if (at + j < cols) v[i].e[j] = xr[at + j];
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < kQuantVecs; ++i)
+  for (int i = 0; i < VECS; ++i)
 #pragma unroll
     for (int j = 0; j < kPer; ++j) amax = max_nan(amax, fabsf(to_float(v[i].e[j])));
   const RowScale s = row_scale(row_max<TPR>(amax, scratch));
   if (t == 0) scales[row] = s.scale;
   int8_t* qr = q + row * q_pitch;
 #pragma unroll
-  for (int i = 0; i < kQuantVecs; ++i) {
-    const int64_t at = (static_cast<int64_t>(i) * TPR + t) * kPer;
-    if (at >= cols) break;
-    uint32_t w[kPer / 4];
+  for (int i = 0; i < VECS; ++i) {
+    const int at = (i * TPR + t) * kPer;
+    uint32_t b[8];
 #pragma unroll
-    for (int j = 0; j < kPer / 4; ++j) {
-      w[j] = low_bytes(quantized(to_float(v[i].e[4 * j]), s.inverse), quantized(to_float(v[i].e[4 * j + 1]), s.inverse),
-                       quantized(to_float(v[i].e[4 * j + 2]), s.inverse), quantized(to_float(v[i].e[4 * j + 3]), s.inverse));
-      if (s.bad) w[j] = 0;
-    }
-    if (at + kPer <= cols) {
-#pragma unroll
-      for (int j = 0; j < kPer / 4; ++j) reinterpret_cast<uint32_t*>(qr + at)[j] = w[j];
+    for (int j = 0; j < kPer; ++j) b[j] = s.bad ? 0 : quantized(to_float(v[i].e[j]), s.inverse);
+    union {
+      Bytes u;
+      uint32_t w[2];
+    } o;
+    if constexpr (kPer == 2) {
+      o.w[0] = __byte_perm(b[0], b[1], 0x0040);
     } else {
 #pragma unroll
-      for (int j = 0; j < kPer; ++j)
-        if (at + j < cols) qr[at + j] = static_cast<int8_t>(w[j / 4] >> (8 * (j % 4)));
+      for (int j = 0; j < kPer / 4; ++j) o.w[j] = low_bytes(b[4 * j], b[4 * j + 1], b[4 * j + 2], b[4 * j + 3]);
     }
+    if (at < cols) *reinterpret_cast<Bytes*>(qr + at) = o.u;
   }
 }
 
@@ -148,21 +141,40 @@ quantize_any_kernel(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t
     q[row * q_pitch + i] = s.bad ? 0 : static_cast<int8_t>(quantized(to_float(xr[i]), s.inverse));
 }
 
+template <typename T, int VB>
+auto pick_vec(int64_t cols) -> decltype(&quantize_vec_kernel<T, VB, 32, 2>) {
+  constexpr int64_t kPer = VB / sizeof(T);
+  if (cols <= 32 * 2 * kPer) return quantize_vec_kernel<T, VB, 32, 2>;
+  if (cols <= 32 * 4 * kPer) return quantize_vec_kernel<T, VB, 32, 4>;
+  if (cols <= 32 * 8 * kPer) return quantize_vec_kernel<T, VB, 32, 8>;
+  if (cols <= kQuantThreads * 2 * kPer) return quantize_vec_kernel<T, VB, kQuantThreads, 2>;
+  if (cols <= kQuantThreads * 4 * kPer) return quantize_vec_kernel<T, VB, kQuantThreads, 4>;
+  if (cols <= kQuantThreads * 8 * kPer) return quantize_vec_kernel<T, VB, kQuantThreads, 8>;
+  return nullptr;
+}
+
 template <typename T>
 cudaError_t launch_quantize(const void* x, int64_t rows, int64_t cols, int64_t pitch, int8_t* q, int64_t q_pitch, float* scales,
                             cudaStream_t s) {
-  constexpr int64_t kPer = 16 / sizeof(T);
-  const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && pitch % kPer == 0 && reinterpret_cast<uintptr_t>(q) % 4 == 0 &&
-                   q_pitch % 4 == 0;
   const T* xt = static_cast<const T*>(x);
-  constexpr int64_t kWarpRow = 32 * kQuantVecs * kPer, kBlockRow = kQuantThreads * kQuantVecs * kPer;
-  // a warp per row while its registers hold one, and for single elements up to 512 of them
-  const bool warp_row = cols <= (vec ? kWarpRow : 512);
-  const int64_t per = warp_row ? kQuantThreads / 32 : 1;
-  const dim3 grid(static_cast<unsigned>((rows + per - 1) / per));
-  auto kernel = vec && cols <= kBlockRow ? (warp_row ? quantize_vec_kernel<T, 32> : quantize_vec_kernel<T, kQuantThreads>)
-                                         : (warp_row ? quantize_any_kernel<T, 32> : quantize_any_kernel<T, kQuantThreads>);
-  return hb::launch_overlapped(kernel, grid, dim3(kQuantThreads), 0, s, xt, rows, cols, pitch, q, q_pitch, scales);
+  // pieces of 16 or 8 bytes that every row starts on and consists of
+  auto whole = [&](int bytes) {
+    const int64_t per = bytes / static_cast<int64_t>(sizeof(T));
+    return reinterpret_cast<uintptr_t>(x) % bytes == 0 && (pitch % per == 0 || rows == 1) && cols % per == 0 &&
+           reinterpret_cast<uintptr_t>(q) % per == 0 && (q_pitch % per == 0 || rows == 1);
+  };
+  auto vec = whole(16) ? pick_vec<T, 16>(cols) : whole(8) ? pick_vec<T, 8>(cols) : nullptr;
+  if (vec) {
+    const bool warp_row = cols <= 32 * 8 * (whole(16) ? 16 : 8) / static_cast<int64_t>(sizeof(T));
+    const int64_t per = warp_row ? kQuantThreads / 32 : 1;
+    return hb::launch_overlapped(vec, dim3(static_cast<unsigned>((rows + per - 1) / per)), dim3(kQuantThreads), 0, s, xt, rows,
+                                 static_cast<int>(cols), pitch, q, q_pitch, scales);
+  }
+  // single elements: a warp per row up to 512 of them
+  const int64_t per = cols <= 512 ? kQuantThreads / 32 : 1;
+  return hb::launch_overlapped(cols <= 512 ? quantize_any_kernel<T, 32> : quantize_any_kernel<T, kQuantThreads>,
+                               dim3(static_cast<unsigned>((rows + per - 1) / per)), dim3(kQuantThreads), 0, s, xt, rows, cols, pitch, q,
+                               q_pitch, scales);
 }
 
 // Rows of bytes that start anywhere -> rows that start on 16 bytes (TMA reads nothing else).

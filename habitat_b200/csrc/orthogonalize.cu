@@ -23,6 +23,7 @@ namespace {
 constexpr float kScale = 256.0f;          // of stored X, A and B
 constexpr int kNormThreads = 256;
 constexpr int kMostPartials = 64;
+constexpr int kSideBlocks = 2;            // blocks of 64 columns per CTA that a cluster is made wider for
 constexpr int kGroup = 4;                 // slots of K (256 values, 16 additions) per accumulation, with `split`
 
 template <typename T>
@@ -36,6 +37,14 @@ struct Source {
   int64_t ld, batch_stride;
   int32_t type, rows, cols;
 };
+
+}  // namespace
+}  // namespace dense
+
+#include "orthogonalize_small.cuh"
+
+namespace dense {
+namespace {
 
 // Sums of squares of G's elements, one per block.
 __global__ void __launch_bounds__(kNormThreads) norm_kernel(Source g, double* partials) {
@@ -347,6 +356,50 @@ hb_status launch(Product p, const typename Epi::Params& ep, cudaStream_t s) {
   return HB_OK;
 }
 
+// The cluster that holds a matrix whose shorter side is at most 128: its CTAs, and blocks of 64 columns per CTA; 0 when it
+// does not fit.
+struct SidePlan {
+  int ctas, blocks, R;
+};
+SidePlan side_plan(int64_t rows, int64_t cols, bool split) {
+  const int64_t s = rows < cols ? rows : cols, l = rows < cols ? cols : rows;
+  SidePlan r{0, 0, static_cast<int>(up(s, 16))};
+  if (s < 1 || s > kSideRows || l > (1 << 20)) return r;
+  const int64_t n = (l + kSideColumns - 1) / kSideColumns;
+  for (const int ctas : {1, 2, 4, 8, 16}) {
+    const int blocks = static_cast<int>((n + ctas - 1) / ctas);
+    if (side_layout(r.R, blocks, split).total + 1024 > kSideSmem || (blocks > kSideBlocks && ctas < 16)) continue;
+    if (split && (blocks + 3) / 4 * r.R > 512) continue;      // accumulators of the share of A
+    r.ctas = ctas;
+    r.blocks = blocks;
+    break;
+  }
+  return r;
+}
+
+template <bool kSplit>
+hb_status launch_side(const SidePlan& plan, int64_t batch, const SideParams& p, bool* launched, cudaStream_t s) {
+  static std::atomic<int> held[64];
+  static std::atomic<int> widest[64];      // of the clusters that the GPU holds: 16, or 8 which every one does
+  auto kernel = small_side_kernel<kSplit>;
+  int dev = 0, n = 0;
+  HB_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) return HB_OK;
+  if (widest[dev].load() == 0) {
+    HB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    const bool wide = max_clusters(kernel, 16, kSideThreads, kSideSmem, held, &n) == HB_OK;
+    if (!wide) {
+      cudaGetLastError();
+      if (const hb_status st = max_clusters(kernel, 8, kSideThreads, kSideSmem, held, &n)) return st;
+    }
+    widest[dev].store(wide ? 16 : 8);
+  }
+  if (plan.ctas > widest[dev].load() || batch * plan.ctas > 0x7FFFFFFF) return HB_OK;
+  HB_CUDA_TRY(launch_clusters(kernel, static_cast<int>(batch), plan.ctas, kSideThreads, kSideSmem, s, p));
+  *launched = true;
+  return HB_OK;
+}
+
 }  // namespace
 }  // namespace dense
 
@@ -399,20 +452,39 @@ extern "C" hb_status hb_orthogonalize(const void* update, int32_t type, int64_t 
     hb::set_error("%s: the workspace has to have %lld bytes, on a 256-byte boundary", name, static_cast<long long>(lay.total));
     return HB_ERR_INVALID_ARGUMENT;
   }
+  const int flip = rows > cols ? 1 : 0;
+  const Source g{update, pitch, batch_stride, type, static_cast<int32_t>(rows), static_cast<int32_t>(cols)};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (const SidePlan plan = side_plan(rows, cols, split != 0); plan.ctas) {
+    SideParams p{};
+    p.g = g;
+    p.out = Out{out, out_pitch, out_batch_stride, type, 0};
+    p.s = static_cast<int32_t>(rows < cols ? rows : cols);
+    p.l = static_cast<int32_t>(rows < cols ? cols : rows);
+    p.R = plan.R;
+    p.blocks = plan.blocks;
+    p.flip = flip;
+    p.steps = steps;
+    p.a = static_cast<float>(a);
+    p.b = static_cast<float>(b);
+    p.c = static_cast<float>(c);
+    p.eps = eps;
+    p.status = status;
+    bool launched = false;
+    if (const hb_status e = split ? launch_side<true>(plan, batch, p, &launched, st) : launch_side<false>(plan, batch, p, &launched, st)) return e;
+    if (launched) return HB_OK;
+  }
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   __half* x[2] = {reinterpret_cast<__half*>(ws), reinterpret_cast<__half*>(ws + lay.x_bytes)};
   __half* A = reinterpret_cast<__half*>(ws + 2 * lay.x_bytes);
   __half* B = reinterpret_cast<__half*>(ws + 2 * lay.x_bytes + lay.a_bytes);
   float* factor = reinterpret_cast<float*>(ws + 2 * lay.x_bytes + 2 * lay.a_bytes);
   double* partials = reinterpret_cast<double*>(reinterpret_cast<uint8_t*>(factor) + up(batch * 4, 256));
-  const int flip = rows > cols ? 1 : 0;
   const int64_t planes = split ? 2 : 1;
   const int64_t x_matrix = lay.s * lay.lp, a_matrix = lay.s * lay.sp;
   auto x_planes = [&](int i) { return Planes{x[i], lay.lp, x_matrix, split ? batch * x_matrix : 0}; };
   const Planes a_planes{A, lay.sp, a_matrix, split ? batch * a_matrix : 0}, b_planes{B, lay.sp, a_matrix, split ? batch * a_matrix : 0};
 
-  const Source g{update, pitch, batch_stride, type, static_cast<int32_t>(rows), static_cast<int32_t>(cols)};
   int64_t n_partials = up(rows * cols, kNormThreads * 16) / (kNormThreads * 16);
   if (n_partials > kMostPartials) n_partials = kMostPartials;
   HB_CUDA_TRY(hb::launch_overlapped(norm_kernel, dim3(static_cast<unsigned>(n_partials), static_cast<unsigned>(batch)), dim3(kNormThreads), 0, st,
