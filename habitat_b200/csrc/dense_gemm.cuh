@@ -2,7 +2,7 @@
 //
 // A pair of CTAs (cta_group::2) computes tiles of 256 x BN: each CTA brings its 128 rows of A and its BN / 2 rows of B
 // into a ring of 128-byte-wide slots by TMA (128-byte swizzle, no multicast), the even CTA's elected lane issues the MMAs for
-// both, and the accumulators (32-bit) lie in TMEM twice, so that eight epilogue warps per CTA drain one tile while the
+// both, and the accumulators (32-bit) lie in TMEM twice, so that the epilogue warps of each CTA drain one tile while the
 // next one is multiplied.  Per slot the pair moves 2 (128 + BN / 2) x 128 bytes for 4 MMAs; with BN = 256 that is 64
 // bytes per clock and SM, half of what two separate SMs with 128 x 256 tiles would need of L2.  A slot is 128 bytes of K
 // whatever the type, 128 8-bit integers or 64 half-precision values, so both share the ring and the issue loop.
@@ -17,10 +17,9 @@ namespace dense {
 constexpr int kPairRows = 256;             // rows of a pair's tile
 constexpr int kCtaRows = 128;
 constexpr int kSlotK = 128;                // bytes of K per slot
-constexpr int kThreads = 384;              // warps: 0 TMA, 1 MMA, 2 TMEM, 3 none, 4-11 epilogue
-constexpr int kEpiWarp0 = 4;
-constexpr int kEpiWarps = 8;
-constexpr int kStageOutBytes = 32 * 128;   // an epilogue warp's staging: 32 rows x 128 bytes
+constexpr int kEpiWarp0 = 4;               // warps: 0 TMA, 1 MMA, 2 TMEM, 3 none, from 4 on epilogue
+constexpr int kMostEpiWarps = 16;
+constexpr int kStageOutBytes = 32 * 64;    // an epilogue warp's staging: 32 rows x 64 bytes
 
 enum OutType : int32_t { kF32 = 0, kBF16 = 1, kF16 = 2 };
 
@@ -30,14 +29,20 @@ struct Shape {
   static constexpr int kSlotBytes = (kCtaRows + kBRows) * kSlotK;     // per CTA
   static constexpr int kSlots = BN == 256 ? 5 : BN == 128 ? 7 : 8;
   static constexpr int kTmemCols = 2 * BN;
+  // Epilogue warps: what they do per tile is a chain of loads and conversions that two warps per scheduler cannot fill (28 %
+  // of the issue slots, 12,600 cycles per tile of 256 x 256 against 4,096 of MMAs at K = 1,024).
+  static constexpr int kEpiWarps = BN == 64 ? 8 : 16;
+  static constexpr int kThreads = 32 * (kEpiWarp0 + kEpiWarps);
+  static constexpr int kParts = kEpiWarps / 4;       // of the columns
+  static constexpr int kCols = BN / kParts;          // a warp's: 64, 32, 32
 };
 
 // Shared memory behind the ring: staging, channel scales and biases, row maxima of other CTAs, barriers.
 struct Tail {
-  uint8_t staging[kEpiWarps * kStageOutBytes];
+  uint8_t staging[kMostEpiWarps * kStageOutBytes];
   float scale[2][256];
   float bias[2][256];
-  float row_max[2][4][2][kCtaRows];
+  float row_max[2][4][4][kCtaRows];
   uint64_t full[8], empty[8], acc_full[2], acc_empty[2], exchange[2], drain;
   uint32_t tmem;
   int abort;
@@ -47,7 +52,7 @@ template <int BN>
 constexpr int smem_bytes() { return Shape<BN>::kSlots * Shape<BN>::kSlotBytes + static_cast<int>(sizeof(Tail)) + 1024; }
 
 // What a launch multiplies: `batches` products of M x N with kblocks slots of K each.  With `segments` 3 the operands are
-// pairs of planes, high and low parts (the low ones lie `batches` matrices behind), and the sum is hi hi + hi lo + lo hi.
+// pairs of planes, high and low parts (the low ones lie `batches` matrices behind), and the sum is hi lo + lo hi + hi hi.
 struct Product {
   CUtensorMap a, b;        // [matrices][rows][K], boxes of 128 (a) and BN / 2 (b) rows x 128 bytes; b K-major or MN-major
   int32_t M, N, kblocks, segments, batches;
@@ -122,6 +127,17 @@ __device__ __forceinline__ void mma_pair(uint32_t d_tmem, uint64_t a_desc, uint6
         "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+// "Read out": nothing but tensor memory is handed over, so the arrival need not wait for this thread's stores to memory, as
+// one with release semantics in the cluster does.
+__device__ __forceinline__ void arrive_remote_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// A value for another CTA's shared memory, counted in bytes on a barrier there.
+__device__ __forceinline__ void st_async_f32(uint32_t cluster_addr, float v, uint32_t cluster_mbar) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(cluster_addr),
+               "r"(__float_as_uint(v)), "r"(cluster_mbar)
+               : "memory");
+}
 // 32 lanes x 32 columns without the wait (tc_wait_ld follows).
 __device__ __forceinline__ void tc_ld32_async(uint32_t taddr, uint32_t* r) {
   asm volatile(
@@ -161,29 +177,34 @@ struct Out {
 };
 
 // Stores a warp's 32 x 32 results: lane `lane` has row m0 + lane, columns n0 .. n0 + 31 in v.  Through the warp's staging
-// the rows leave in whole 64- or 128-byte pieces: 16-byte stores of 32 different rows fill half a sector each.
+// the rows leave in pieces of 64 bytes: 16-byte stores of 32 different rows fill half a sector each.
 __device__ __forceinline__ void store_rows(const Out& out, int batch, int M, int N, int m0, int n0, const float (&v)[32],
                                            uint8_t* staging, int lane) {
   __syncwarp();   // the last chunk's reads of the staging are done
   if (out.type == kF32) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      *reinterpret_cast<float4*>(staging + lane * 128 + ((j ^ (lane & 7)) << 4)) =
-          make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-    __syncwarp();
     float* base = static_cast<float*>(out.base) + batch * out.batch_stride;
-    if (out.vec && n0 + 32 <= N) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = 4 * i + (lane >> 3), c = lane & 7;
-        const float4 x = *reinterpret_cast<const float4*>(staging + r * 128 + ((c ^ (r & 7)) << 4));
-        if (m0 + r < M) *reinterpret_cast<float4*>(base + static_cast<int64_t>(m0 + r) * out.ld + n0 + 4 * c) = x;
-      }
-    } else if (n0 + lane < N) {
+    for (int h = 0; h < 2; ++h) {
+      if (h) __syncwarp();
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<float4*>(staging + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) =
+            make_float4(v[16 * h + 4 * j], v[16 * h + 4 * j + 1], v[16 * h + 4 * j + 2], v[16 * h + 4 * j + 3]);
+      __syncwarp();
+      const int n = n0 + 16 * h;
+      if (out.vec && n + 16 <= N) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = 8 * i + (lane >> 2), c = lane & 3;
+          const float4 x = *reinterpret_cast<const float4*>(staging + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+          if (m0 + r < M) *reinterpret_cast<float4*>(base + static_cast<int64_t>(m0 + r) * out.ld + n + 4 * c) = x;
+        }
+      } else if (n + (lane & 15) < N) {
 #pragma unroll 4
-      for (int r = 0; r < 32 && m0 + r < M; ++r)
-        base[static_cast<int64_t>(m0 + r) * out.ld + n0 + lane] =
-            *reinterpret_cast<const float*>(staging + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + 4 * (lane & 3));
+        for (int r = lane >> 4; r < 32 && m0 + r < M; r += 2)
+          base[static_cast<int64_t>(m0 + r) * out.ld + n + (lane & 15)] =
+              *reinterpret_cast<const float*>(staging + r * 64 + ((((lane & 15) >> 2) ^ ((r >> 1) & 3)) << 4) + 4 * (lane & 3));
+      }
     }
   } else {
     uint32_t w[16];
@@ -219,10 +240,10 @@ __device__ __forceinline__ void store_rows(const Out& out, int batch, int M, int
 // What a tile's epilogue may use.
 struct EpiContext {
   Tail* tail;
-  uint32_t tmem;          // this warp's lanes and first column of its half of the tile
-  int warp, lane, half;   // epilogue warp 0 .. 7, its half of the columns
+  uint32_t tmem;          // this warp's lanes and first column of its part of the tile
+  int warp, lane, part;   // epilogue warp, its part of the columns
   int row;                // row of the CTA's 128 that the lane has
-  int m0, n0;             // first row of the CTA and first column of the warp's half, in the matrix
+  int m0, n0;             // first row of the CTA and first column of the warp's part, in the matrix
   int batch;
   uint32_t n_tile;        // how many tiles the CTA has drained before
   bool first, last;       // group of the tile
@@ -232,13 +253,14 @@ struct EpiContext {
 
 // Adds a group's accumulators to a lane's sums.
 template <int BN, class Release>
-__device__ __forceinline__ void add_group(const EpiContext& c, float (&sums)[BN / 2], Release release) {
+__device__ __forceinline__ void add_group(const EpiContext& c, float* sums, Release release) {
+  constexpr int kChunks = Shape<BN>::kCols / 32;
 #pragma unroll
-  for (int chunk = 0; chunk < BN / 64; ++chunk) {
+  for (int chunk = 0; chunk < kChunks; ++chunk) {
     uint32_t acc[32];
     tc_ld32_async(c.tmem + chunk * 32, acc);
     tc_wait_ld();
-    if (chunk == BN / 64 - 1) release();
+    if (chunk == kChunks - 1) release();
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
       const float x = __uint_as_float(acc[i]);
@@ -253,9 +275,10 @@ __device__ __forceinline__ void add_group(const EpiContext& c, float (&sums)[BN 
 //   static void drain(const Params&, const Product&, EpiContext&, sums, release)   calls release() once the accumulators are read
 // kGrouped: the tensor core adds 16 products of K at a time to its float32 sums and cuts what does not fit, which over
 // long K is off by as many units as there are additions, all to the same side.  So a tile's K goes to the accumulators in
-// groups, and drain() adds the groups in registers (sums), rounded to nearest; it acts on the last one.
+// groups (the small products of high and low parts are one), and drain() adds the groups in registers (sums), rounded to
+// nearest; it acts on the last one.
 template <int BN, class Epi>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
 gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ typename Epi::Params ep) {
   using S = Shape<BN>;
   extern __shared__ uint8_t smem_raw[];
@@ -277,8 +300,8 @@ gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ typename 
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(acc_full + 8 * s, 1);
-      mbar_init(acc_empty + 8 * s, 2 * kEpiWarps);
-      mbar_init(smem_u32(&tail->exchange[s]), kEpiWarps * (kCluster / 2));
+      mbar_init(acc_empty + 8 * s, 2 * S::kEpiWarps);
+      mbar_init(smem_u32(&tail->exchange[s]), 1);
     }
     mbar_init(smem_u32(&tail->drain), 1);
     tail->abort = 0;
@@ -305,7 +328,12 @@ gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ typename 
     return tile_of<BN>(p, t);
   };
   const int total_kb = p.kblocks * p.segments;
-  const int group = Epi::kGrouped ? p.group : total_kb;
+  // end of the group of K slots that begins at kb
+  auto group_end = [&](int kb) {
+    if (!Epi::kGrouped) return total_kb;
+    const int small = p.kblocks * (p.segments - 1);
+    return kb < small ? small : min(kb + p.group, total_kb);
+  };
 
   if (warp == 0) {
     // ------------------------------ copies ------------------------------
@@ -316,7 +344,7 @@ gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ typename 
       for (int t = worker; t < p.num_tiles && ok; t += workers) {
         const Tile tile = locate(t);
         for (int seg = 0; seg < p.segments && ok; ++seg) {
-          const int za = tile.batch + (seg == 2 ? p.batches : 0), zb = tile.batch + (seg == 1 ? p.batches : 0);
+          const int za = tile.batch + (seg == 1 ? p.batches : 0), zb = tile.batch + (p.segments > 1 && seg == 0 ? p.batches : 0);
           for (int kb = 0; kb < p.kblocks; ++kb) {
             ok = mbar_wait(empty + 8 * s, ph, abort_flag, p.status, 0x511);
             if (!ok) break;
@@ -356,14 +384,14 @@ gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ typename 
       uint32_t s = 0, ph = 0, n = 0;
       bool ok = true;
       for (int t = worker; t < p.num_tiles && ok; t += workers) {
-        for (int kb0 = 0; kb0 < total_kb && ok; kb0 += group, ++n) {
+        for (int kb0 = 0, kb1; kb0 < total_kb && ok; kb0 = kb1, ++n) {
+          kb1 = group_end(kb0);
           const uint32_t st = n & 1u;
-          ok = mbar_wait_cluster(acc_empty + 8 * st, ((n >> 1) & 1u) ^ 1u, abort_flag, p.status, 0x521);
+          ok = mbar_wait(acc_empty + 8 * st, ((n >> 1) & 1u) ^ 1u, abort_flag, p.status, 0x521);
           tc_fence_after();
           const uint32_t d = tmem + st * BN;
-          const int kb1 = min(kb0 + group, total_kb);
           for (int kb = kb0; kb < kb1 && ok; ++kb) {
-            ok = mbar_wait_cluster(full + 8 * s, ph, abort_flag, p.status, 0x522);
+            ok = mbar_wait(full + 8 * s, ph, abort_flag, p.status, 0x522);
             if (!ok) break;
             tc_fence_after();
             const uint32_t a_lo = a0 + s * (S::kSlotBytes >> 4);
@@ -384,22 +412,23 @@ gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ typename 
     const int quad = warp & 3;
     bool ok = true;
     EpiContext c;
-    c.tail = tail; c.warp = w; c.lane = lane; c.half = w >> 2; c.row = quad * 32 + lane; c.rank = rank; c.ok = &ok;
+    c.tail = tail; c.warp = w; c.lane = lane; c.part = w >> 2; c.row = quad * 32 + lane; c.rank = rank; c.ok = &ok;
     uint32_t n = 0;
     const uint32_t acc_empty_leader = map_to_cta(acc_empty, leader);
-    float sums[Epi::kGrouped ? BN / 2 : 1];
+    float sums[Epi::kGrouped ? S::kCols : 1];
     c.n_tile = 0;
     for (int t = worker; t < p.num_tiles && ok; t += workers, ++c.n_tile) {
       const Tile tile = locate(t);
       c.m0 = tile.m0 + static_cast<int>(side) * kCtaRows;
-      c.n0 = tile.n0 + c.half * (BN / 2);
+      c.n0 = tile.n0 + c.part * S::kCols;
       c.batch = tile.batch;
       Epi::template begin<BN>(ep, p, c);
-      for (int kb0 = 0; kb0 < total_kb && ok; kb0 += group, ++n) {
+      for (int kb0 = 0, kb1; kb0 < total_kb && ok; kb0 = kb1, ++n) {
+        kb1 = group_end(kb0);
         const uint32_t st = n & 1u;
-        c.tmem = tmem + (static_cast<uint32_t>(quad * 32) << 16) + st * BN + static_cast<uint32_t>(c.half * (BN / 2));
+        c.tmem = tmem + (static_cast<uint32_t>(quad * 32) << 16) + st * BN + static_cast<uint32_t>(c.part * S::kCols);
         c.first = kb0 == 0;
-        c.last = kb0 + group >= total_kb;
+        c.last = kb1 == total_kb;
         if (!mbar_wait(acc_full + 8 * st, (n >> 1) & 1u, abort_flag, p.status, 0x531)) { ok = false; break; }
         tc_fence_after();
         Epi::template drain<BN>(ep, p, c, sums, [&] {
@@ -407,7 +436,7 @@ gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ typename 
           __syncwarp();
           if (lane == 0) {
             if (side == 0) mbar_arrive(acc_empty + 8 * st);
-            else mbar_arrive_remote(acc_empty_leader + 8 * st);
+            else arrive_remote_relaxed(acc_empty_leader + 8 * st);
           }
         });
       }

@@ -212,17 +212,18 @@ struct LayerScales {
   int32_t relu;
 };
 
-// Channel scales and biases of a warp group's half of the tile into shared memory (zeros outside the matrix).
+// Channel scales and biases of a part's columns into shared memory (zeros outside the matrix), by its four warps.
 template <int BN>
 __device__ __forceinline__ void load_channels(const LayerScales& s, const Product& p, const EpiContext& c) {
-  const int i = (c.warp & 3) * 32 + c.lane;   // 0 .. 127 among the half's warps
+  constexpr int kCols = Shape<BN>::kCols;
+  const int i = (c.warp & 3) * 32 + c.lane;
   const uint32_t buf = c.n_tile & 1u;
-  if (i < BN / 2) {
+  if (i < kCols) {
     const int n = c.n0 + i;
-    c.tail->scale[buf][c.half * (BN / 2) + i] = n < p.N ? s.channel[n] : 0.0f;
-    c.tail->bias[buf][c.half * (BN / 2) + i] = n < p.N && s.bias ? s.bias[n] : 0.0f;
+    c.tail->scale[buf][c.part * kCols + i] = n < p.N ? s.channel[n] : 0.0f;
+    c.tail->bias[buf][c.part * kCols + i] = n < p.N && s.bias ? s.bias[n] : 0.0f;
   }
-  asm volatile("bar.sync %0, 128;" ::"r"(1 + c.half) : "memory");
+  asm volatile("bar.sync %0, 128;" ::"r"(1 + c.part) : "memory");
 }
 
 // 32 accumulators of a row -> results.
@@ -230,8 +231,9 @@ template <int BN>
 __device__ __forceinline__ void finish(const LayerScales& s, const EpiContext& c, float row_scale, int chunk, const uint32_t* acc,
                                        float* v) {
   const uint32_t buf = c.n_tile & 1u;
-  const float4* sc = reinterpret_cast<const float4*>(&c.tail->scale[buf][c.half * (BN / 2) + chunk * 32]);
-  const float4* bi = reinterpret_cast<const float4*>(&c.tail->bias[buf][c.half * (BN / 2) + chunk * 32]);
+  const int at = c.part * Shape<BN>::kCols + chunk * 32;
+  const float4* sc = reinterpret_cast<const float4*>(&c.tail->scale[buf][at]);
+  const float4* bi = reinterpret_cast<const float4*>(&c.tail->bias[buf][at]);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const float4 w = sc[j], b = bi[j];
@@ -260,12 +262,12 @@ struct FloatOut {
     const int row = c.m0 + c.row;
     const float rs = row < p.M ? __ldg(ep.s.row + row) : 0.0f;
 #pragma unroll 1
-    for (int chunk = 0; chunk < BN / 64; ++chunk) {
+    for (int chunk = 0; chunk < Shape<BN>::kCols / 32; ++chunk) {
       uint32_t acc[32];
       float v[32];
       tc_ld32_async(c.tmem + chunk * 32, acc);
       tc_wait_ld();
-      if (chunk == BN / 64 - 1) release();
+      if (chunk == Shape<BN>::kCols / 32 - 1) release();
       finish<BN>(ep.s, c, rs, chunk, acc, v);
       store_rows(ep.out, 0, p.M, p.N, c.m0 + (c.row & ~31), c.n0 + chunk * 32, v, c.tail->staging + c.warp * kStageOutBytes, c.lane);
     }
@@ -273,9 +275,9 @@ struct FloatOut {
 };
 
 // The result as quantised rows.  The CTAs of a cluster hold whole rows between them (one pair per 256 columns): every lane
-// keeps its 128 results in registers, sends their largest magnitude to all CTAs of its row half through distributed shared
-// memory, and quantises when the others' are there.  The accumulators are free before the exchange, so the next tile's
-// MMAs run during it.
+// keeps its 64 results in registers, sends their largest magnitude to all CTAs of its row half through distributed shared
+// memory (counted in bytes there: nobody waits for a store to be acknowledged), and quantises when the others' are there.  The
+// accumulators are free before the exchange, so the next tile's MMAs run during it.
 template <int kCtas>
 struct QuantOut {
   static constexpr bool kInt8 = true, kMnMajorB = false, kGrouped = false;
@@ -288,45 +290,46 @@ struct QuantOut {
   };
   template <int BN>
   static __device__ __forceinline__ void begin(const Params& ep, const Product& p, const EpiContext& c) {
+    if (c.warp == 0 && c.lane == 0)
+      mbar_expect_tx(smem_u32(&c.tail->exchange[c.n_tile & 1u]), kCtas / 2 * Shape<BN>::kParts * kCtaRows * 4);
     load_channels<BN>(ep.s, p, c);
   }
   template <int BN, class Release>
   static __device__ __forceinline__ void drain(const Params& ep, const Product& p, const EpiContext& c, float (&)[1], Release release) {
-    static_assert(BN == 256, "128 columns per lane");
+    static_assert(BN == 256 && Shape<BN>::kCols == 64, "64 columns per lane");
     const int row = c.m0 + c.row;
     const float rs = row < p.M ? __ldg(ep.s.row + row) : 0.0f;
-    float v[128];
+    float v[64];
     float amax = 0.0f;
 #pragma unroll
-    for (int chunk = 0; chunk < 4; ++chunk) {
+    for (int chunk = 0; chunk < 2; ++chunk) {
       uint32_t acc[32];
       tc_ld32_async(c.tmem + chunk * 32, acc);
       tc_wait_ld();
+      if (chunk == 1) release();
       finish<BN>(ep.s, c, rs, chunk, acc, v + 32 * chunk);
 #pragma unroll
       for (int i = 0; i < 32; ++i) amax = max_nan(amax, fabsf(v[32 * chunk + i]));
     }
-    release();
     const uint32_t buf = c.n_tile & 1u, side = c.rank & 1u;
     const uint32_t bar = smem_u32(&c.tail->exchange[buf]);
-    const uint32_t mine = smem_u32(&c.tail->row_max[buf][c.rank >> 1][c.half][c.row]);
+    const uint32_t mine = smem_u32(&c.tail->row_max[buf][c.rank >> 1][c.part][c.row]);
 #pragma unroll
-    for (int i = 0; i < kCtas / 2; ++i) st_cluster_f32(map_to_cta(mine, 2 * i + side), amax);
-    __syncwarp();
-    if (c.lane < kCtas / 2) mbar_arrive_remote(map_to_cta(bar, 2 * c.lane + side));
+    for (int i = 0; i < kCtas / 2; ++i) st_async_f32(map_to_cta(mine, 2 * i + side), amax, map_to_cta(bar, 2 * i + side));
     if (!mbar_wait_cluster(bar, (c.n_tile >> 1) & 1u, &c.tail->abort, p.status, 0x541)) {
       *c.ok = false;
       return;
     }
 #pragma unroll
     for (int i = 0; i < kCtas / 2; ++i)
-      amax = max_nan(amax, max_nan(c.tail->row_max[buf][i][0][c.row], c.tail->row_max[buf][i][1][c.row]));
+#pragma unroll
+      for (int j = 0; j < Shape<BN>::kParts; ++j) amax = max_nan(amax, c.tail->row_max[buf][i][j][c.row]);
     const RowScale s = row_scale(amax);
-    if (c.rank < 2 && c.half == 0 && row < p.M) ep.scales[row] = s.scale;
+    if (c.rank < 2 && c.part == 0 && row < p.M) ep.scales[row] = s.scale;
     uint8_t* staging = c.tail->staging + c.warp * kStageOutBytes;
     __syncwarp();
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < 4; ++j) {
       uint32_t w[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -334,14 +337,14 @@ struct QuantOut {
         w[i] = low_bytes(quantized(x[0], s.inverse), quantized(x[1], s.inverse), quantized(x[2], s.inverse), quantized(x[3], s.inverse));
         if (s.bad) w[i] = 0;
       }
-      *reinterpret_cast<uint4*>(staging + c.lane * 128 + ((j ^ (c.lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+      *reinterpret_cast<uint4*>(staging + c.lane * 64 + ((j ^ ((c.lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
     }
     __syncwarp();
     const int m0 = c.m0 + (c.row & ~31);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = 4 * i + (c.lane >> 3), ch = c.lane & 7;
-      const uint8_t* at = staging + r * 128 + ((ch ^ (r & 7)) << 4);
+    for (int i = 0; i < 4; ++i) {
+      const int r = 8 * i + (c.lane >> 2), ch = c.lane & 3;
+      const uint8_t* at = staging + r * 64 + ((ch ^ ((r >> 1) & 3)) << 4);
       const int n = c.n0 + 16 * ch;
       if (m0 + r >= p.M) continue;
       int8_t* to = ep.q + static_cast<int64_t>(m0 + r) * ep.pitch + n;
@@ -431,7 +434,7 @@ hb_status launch_float(const Operands& o, int64_t M, int64_t N, int64_t K, const
   static std::atomic<int> held[64];
   int pairs = 0;
   auto kernel = gemm_kernel<BN, FloatOut>;
-  if (const hb_status st = max_clusters(kernel, 2, kThreads, smem_bytes<BN>(), held, &pairs)) return st;
+  if (const hb_status st = max_clusters(kernel, 2, Shape<BN>::kThreads, smem_bytes<BN>(), held, &pairs)) return st;
   Product p{};
   if (const hb_status st = describe(&p, o, M, N, K, BN, status)) return st;
   const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
@@ -441,7 +444,7 @@ hb_status launch_float(const Operands& o, int64_t M, int64_t N, int64_t K, const
   }
   p.num_tiles = static_cast<int32_t>(tiles);
   const int clusters = p.num_tiles < pairs ? p.num_tiles : pairs;
-  HB_CUDA_TRY(launch_clusters(kernel, clusters, 2, kThreads, smem_bytes<BN>(), s, p, ep));
+  HB_CUDA_TRY(launch_clusters(kernel, clusters, 2, Shape<BN>::kThreads, smem_bytes<BN>(), s, p, ep));
   return HB_OK;
 }
 
@@ -451,12 +454,12 @@ hb_status launch_quant(const Operands& o, int64_t M, int64_t N, int64_t K, const
   static std::atomic<int> held[64];
   int clusters = 0;
   auto kernel = gemm_kernel<256, QuantOut<kCtas>>;
-  if (const hb_status st = max_clusters(kernel, kCtas, kThreads, smem_bytes<256>(), held, &clusters)) return st;
+  if (const hb_status st = max_clusters(kernel, kCtas, Shape<256>::kThreads, smem_bytes<256>(), held, &clusters)) return st;
   Product p{};
   if (const hb_status st = describe(&p, o, M, N, K, 256, status)) return st;
   p.num_tiles = p.tiles_m;
   if (p.num_tiles < clusters) clusters = p.num_tiles;
-  HB_CUDA_TRY(launch_clusters(kernel, clusters, kCtas, kThreads, smem_bytes<256>(), s, p, ep));
+  HB_CUDA_TRY(launch_clusters(kernel, clusters, kCtas, Shape<256>::kThreads, smem_bytes<256>(), s, p, ep));
   return HB_OK;
 }
 

@@ -24,7 +24,7 @@ constexpr float kScale = 256.0f;          // of stored X, A and B
 constexpr int kNormThreads = 256;
 constexpr int kMostPartials = 64;
 constexpr int kSideBlocks = 2;            // blocks of 64 columns per CTA that a cluster is made wider for
-constexpr int kGroup = 4;                 // slots of K (256 values, 16 additions) per accumulation, with `split`
+constexpr int kGroup = 2;                 // slots of K (128 values, 8 additions) per accumulation, with `split`
 
 template <typename T>
 __device__ __forceinline__ float element(const void* base, int64_t at) { return static_cast<float>(static_cast<const T*>(base)[at]); }
@@ -138,10 +138,10 @@ __device__ __forceinline__ void take_half(float (&v)[32]) {
 template <int BN, bool kGrouped, class Release, class Work>
 __device__ __forceinline__ void for_chunks(const EpiContext& c, float* sums, Release release, Work work) {
   if constexpr (kGrouped) {
-    add_group<BN>(c, *reinterpret_cast<float(*)[BN / 2]>(sums), release);
+    add_group<BN>(c, sums, release);
     if (!c.last) return;
 #pragma unroll
-    for (int chunk = 0; chunk < BN / 64; ++chunk) {
+    for (int chunk = 0; chunk < Shape<BN>::kCols / 32; ++chunk) {
       float v[32];
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] = sums[32 * chunk + i];
@@ -149,12 +149,12 @@ __device__ __forceinline__ void for_chunks(const EpiContext& c, float* sums, Rel
     }
   } else {
 #pragma unroll 1
-    for (int chunk = 0; chunk < BN / 64; ++chunk) {
+    for (int chunk = 0; chunk < Shape<BN>::kCols / 32; ++chunk) {
       uint32_t acc[32];
       float v[32];
       tc_ld32_async(c.tmem + chunk * 32, acc);
       tc_wait_ld();
-      if (chunk == BN / 64 - 1) release();
+      if (chunk == Shape<BN>::kCols / 32 - 1) release();
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(acc[i]);
       work(chunk, v);
@@ -342,7 +342,7 @@ hb_status launch(Product p, const typename Epi::Params& ep, cudaStream_t s) {
   static std::atomic<int> held[64];
   int pairs = 0;
   auto kernel = gemm_kernel<BN, Epi>;
-  if (const hb_status st = max_clusters(kernel, 2, kThreads, smem_bytes<BN>(), held, &pairs)) return st;
+  if (const hb_status st = max_clusters(kernel, 2, Shape<BN>::kThreads, smem_bytes<BN>(), held, &pairs)) return st;
   p.tiles_m = static_cast<int32_t>((p.M + kPairRows - 1) / kPairRows);
   p.tiles_n = static_cast<int32_t>((p.N + BN - 1) / BN);
   const int64_t tiles = p.batches * (p.lower ? lower_tiles(p.M, BN) : static_cast<int64_t>(p.tiles_m) * p.tiles_n);
@@ -352,7 +352,7 @@ hb_status launch(Product p, const typename Epi::Params& ep, cudaStream_t s) {
   }
   p.num_tiles = static_cast<int32_t>(tiles);
   const int clusters = p.num_tiles < pairs ? p.num_tiles : pairs;
-  HB_CUDA_TRY(launch_clusters(kernel, clusters, 2, kThreads, smem_bytes<BN>(), s, p, ep));
+  HB_CUDA_TRY(launch_clusters(kernel, clusters, 2, Shape<BN>::kThreads, smem_bytes<BN>(), s, p, ep));
   return HB_OK;
 }
 
@@ -369,7 +369,7 @@ SidePlan side_plan(int64_t rows, int64_t cols, bool split) {
   for (const int ctas : {1, 2, 4, 8, 16}) {
     const int blocks = static_cast<int>((n + ctas - 1) / ctas);
     if (side_layout(r.R, blocks, split).total + 1024 > kSideSmem || (blocks > kSideBlocks && ctas < 16)) continue;
-    if (split && (blocks + 3) / 4 * r.R > 512) continue;      // accumulators of the share of A
+    if (split && (blocks + 1) / 2 * r.R > 512) continue;      // accumulators of the share of A
     r.ctas = ctas;
     r.blocks = blocks;
     break;

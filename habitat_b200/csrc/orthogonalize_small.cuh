@@ -213,8 +213,8 @@ __global__ void __launch_bounds__(kSideThreads, 1) small_side_kernel(const __gri
   const int quad = warp & 3, part = warp >> 2, row = quad * 32 + lane;
   const bool rows_here = quad * 32 < R;                                    // warps beyond have no rows of D
   const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16);
-  // sums of four blocks' products at most per accumulator (see kGrouped); without low parts one takes all
-  const int groups = kSplit ? (nb + 3) / 4 : 1, per_group = kSplit ? 4 : nb;
+  // sums of two blocks' products at most per accumulator (see kGrouped); without low parts one takes all
+  const int groups = kSplit ? (nb + 1) / 2 : 1, per_group = kSplit ? 2 : nb;
 
   for (int step = 0; step < p.steps; ++step) {
     const bool first = step == 0, last = step == p.steps - 1;
