@@ -27,7 +27,7 @@ template <int BN>
 struct Shape {
   static constexpr int kBRows = BN / 2;                               // rows of B (columns of D) per CTA
   static constexpr int kSlotBytes = (kCtaRows + kBRows) * kSlotK;     // per CTA
-  static constexpr int kSlots = BN == 256 ? 5 : BN == 128 ? 7 : 8;
+  static constexpr int kSlots = BN == 256 ? 5 : BN == 128 ? 6 : 8;
   static constexpr int kTmemCols = 2 * BN;
   // Epilogue warps: what they do per tile is a chain of loads and conversions that two warps per scheduler cannot fill (28 %
   // of the issue slots, 12,600 cycles per tile of 256 x 256 against 4,096 of MMAs at K = 1,024).
@@ -40,8 +40,7 @@ struct Shape {
 // Shared memory behind the ring: staging, channel scales and biases, row maxima of other CTAs, barriers.
 struct Tail {
   uint8_t staging[kMostEpiWarps * kStageOutBytes];
-  float scale[2][256];
-  float bias[2][256];
+  float scales[kMostEpiWarps][160];        // an epilogue warp's: 64 channel scales, 64 biases, 32 row scales
   float row_max[2][4][4][kCtaRows];
   uint64_t full[8], empty[8], acc_full[2], acc_empty[2], exchange[2], drain;
   uint32_t tmem;
@@ -49,7 +48,11 @@ struct Tail {
 };
 
 template <int BN>
-constexpr int smem_bytes() { return Shape<BN>::kSlots * Shape<BN>::kSlotBytes + static_cast<int>(sizeof(Tail)) + 1024; }
+constexpr int smem_bytes() {
+  constexpr int bytes = Shape<BN>::kSlots * Shape<BN>::kSlotBytes + static_cast<int>(sizeof(Tail)) + 1024;
+  static_assert(bytes <= 232448, "more than a block may have");
+  return bytes;
+}
 
 // What a launch multiplies: `batches` products of M x N with kblocks slots of K each.  With `segments` 3 the operands are
 // pairs of planes, high and low parts (the low ones lie `batches` matrices behind), and the sum is hi lo + lo hi + hi hi.
@@ -58,22 +61,44 @@ struct Product {
   int32_t M, N, kblocks, segments, batches;
   int32_t tiles_m, tiles_n, num_tiles;   // num_tiles: over all batches
   int32_t lower;           // 1: D is symmetric, only tiles that reach its lower triangle are computed
+  int32_t per_batch;       // tiles of a batch, and its and a tile group's reciprocal (set_tiles)
+  uint32_t per_batch_inv, per_group_inv;
   int32_t group;           // slots of K that one accumulator takes before it is drained; several groups: see Epi::kGrouped
   int32_t* status;
 };
+
+constexpr int kTileGroup = 8;      // row blocks that tiles go through together
 
 struct Tile {
   int batch, m0, n0;
 };
 
+// n / d and, in n, the remainder, for 0 <= n < 2^31.  m is 2^32 / d rounded down (reciprocal_of): the estimate is at most two too
+// small.
+__device__ __forceinline__ int divide(int& n, int d, uint32_t m) {
+  int q = static_cast<int>(__umulhi(static_cast<uint32_t>(n), m));
+  n -= q * d;
+  while (n >= d) {
+    n -= d;
+    ++q;
+  }
+  return q;
+}
+inline uint32_t reciprocal_of(int64_t d) { return d <= 1 ? 0xFFFFFFFFu : static_cast<uint32_t>((int64_t{1} << 32) / d); }
+
+inline void set_tiles(Product* p, int64_t per_batch) {
+  p->per_batch = static_cast<int32_t>(per_batch);
+  p->num_tiles = static_cast<int32_t>(per_batch * p->batches);
+  p->per_batch_inv = reciprocal_of(per_batch);
+  p->per_group_inv = reciprocal_of(static_cast<int64_t>(kTileGroup) * p->tiles_n);
+}
+
 // Tile `t` of a launch.  Full products go through groups of eight row blocks, column by column, so that the tiles in
 // flight share rows and columns in L2.
 template <int BN>
 __device__ __forceinline__ Tile tile_of(const Product& p, int t) {
-  const int per_batch = p.num_tiles / p.batches;
   Tile r;
-  r.batch = t / per_batch;
-  t -= r.batch * per_batch;
+  r.batch = divide(t, p.per_batch, p.per_batch_inv);
   int mt, nt;
   if (p.lower) {
     constexpr int kPer = kPairRows / BN;
@@ -86,13 +111,10 @@ __device__ __forceinline__ Tile tile_of(const Product& p, int t) {
       ++mt;
     }
   } else {
-    constexpr int kGroup = 8;
-    const int per_group = kGroup * p.tiles_n;
-    const int g = t / per_group;
-    const int rows = min(kGroup, p.tiles_m - g * kGroup);
-    const int in = t - g * per_group;
-    mt = g * kGroup + in % rows;
-    nt = in / rows;
+    const int g = divide(t, kTileGroup * p.tiles_n, p.per_group_inv);
+    const int rows = min(kTileGroup, p.tiles_m - g * kTileGroup);
+    nt = rows == kTileGroup ? t / kTileGroup : t / rows;
+    mt = g * kTileGroup + t - nt * rows;
   }
   r.m0 = mt * kPairRows;
   r.n0 = nt * BN;
@@ -168,13 +190,20 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&p);
 }
 
-// Where results go: rows of `ld` elements, matrices `batch_stride` elements apart; `vec`: every row starts on 16 bytes.
+// Where results go: rows of `ld` elements, matrices `batch_stride` elements apart; `vec`: the bytes, up to 16, that every row
+// starts on a multiple of.
 struct Out {
   void* base;
   int64_t ld, batch_stride;
   int32_t type;
   int32_t vec;
 };
+
+inline int32_t row_alignment(const void* base, int64_t ld, int64_t batch_stride, int elem_bytes) {
+  const uint64_t x = static_cast<uint64_t>(reinterpret_cast<uintptr_t>(base)) | static_cast<uint64_t>(ld * elem_bytes) |
+                     static_cast<uint64_t>(batch_stride * elem_bytes) | 16u;
+  return static_cast<int32_t>(x & (~x + 1));
+}
 
 // Stores a warp's 32 x 32 results: lane `lane` has row m0 + lane, columns n0 .. n0 + 31 in v.  Through the warp's staging
 // the rows leave in pieces of 64 bytes: 16-byte stores of 32 different rows fill half a sector each.
@@ -192,7 +221,7 @@ __device__ __forceinline__ void store_rows(const Out& out, int batch, int M, int
             make_float4(v[16 * h + 4 * j], v[16 * h + 4 * j + 1], v[16 * h + 4 * j + 2], v[16 * h + 4 * j + 3]);
       __syncwarp();
       const int n = n0 + 16 * h;
-      if (out.vec && n + 16 <= N) {
+      if (out.vec == 16 && n + 16 <= N) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int r = 8 * i + (lane >> 2), c = lane & 3;
@@ -221,7 +250,7 @@ __device__ __forceinline__ void store_rows(const Out& out, int batch, int M, int
           make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
     __syncwarp();
     uint16_t* base = static_cast<uint16_t*>(out.base) + batch * out.batch_stride;
-    if (out.vec && n0 + 32 <= N) {
+    if (out.vec == 16 && n0 + 32 <= N) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int r = 8 * i + (lane >> 2), c = lane & 3;
@@ -242,12 +271,13 @@ struct EpiContext {
   Tail* tail;
   uint32_t tmem;          // this warp's lanes and first column of its part of the tile
   int warp, lane, part;   // epilogue warp, its part of the columns
-  int row;                // row of the CTA's 128 that the lane has
-  int m0, n0;             // first row of the CTA and first column of the warp's part, in the matrix
+  int row;                // the warp's first row among the CTA's 128
+  int row0, n0;           // its first row and the first column of its part, in the matrix
   int batch;
   uint32_t n_tile;        // how many tiles the CTA has drained before
   bool first, last;       // group of the tile
   uint32_t rank;          // in the cluster
+  int next_row0, next_n0; // of the next tile; next_row0 < 0: there is none
   bool* ok;
 };
 
@@ -271,8 +301,10 @@ __device__ __forceinline__ void add_group(const EpiContext& c, float* sums, Rele
 
 // The kernel.  Epilogue: a policy with `Params`, static kInt8, kMnMajorB, kGrouped, kClusterCtas (0: a pair; else the CTAs of a
 // cluster that share rows, one pair per BN columns) and
-//   static void begin(const Params&, const Product&, EpiContext&)                  before the accumulators are waited for (tables)
-//   static void drain(const Params&, const Product&, EpiContext&, sums, release)   calls release() once the accumulators are read
+//   static void begin(EpiContext&)                                              before a tile's accumulators are waited for
+//   static void fetch(const Params&, const Product&, EpiContext&, row0, n0)     requests what a tile's results need, a tile ahead
+//   static void drain(const Params&, const Product&, EpiContext&, sums, release)   calls release() once the accumulators are read,
+//                                                                                  and c.fetch_next() once that is used
 // kGrouped: the tensor core adds 16 products of K at a time to its float32 sums and cuts what does not fit, which over
 // long K is off by as many units as there are additions, all to the same side.  So a tile's K goes to the accumulators in
 // groups (the small products of high and low parts are one), and drain() adds the groups in registers (sums), rounded to
@@ -412,17 +444,28 @@ gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ typename 
     const int quad = warp & 3;
     bool ok = true;
     EpiContext c;
-    c.tail = tail; c.warp = w; c.lane = lane; c.part = w >> 2; c.row = quad * 32 + lane; c.rank = rank; c.ok = &ok;
+    c.tail = tail; c.warp = w; c.lane = lane; c.part = w >> 2; c.row = quad * 32; c.rank = rank; c.ok = &ok;
     uint32_t n = 0;
     const uint32_t acc_empty_leader = map_to_cta(acc_empty, leader);
     float sums[Epi::kGrouped ? S::kCols : 1];
     c.n_tile = 0;
+    Tile tile{}, next{};
+    auto look_ahead = [&](int t) {
+      c.next_row0 = -1;
+      if (t >= p.num_tiles) return;
+      next = locate(t);
+      c.next_row0 = next.m0 + static_cast<int>(side) * kCtaRows + c.row;
+      c.next_n0 = next.n0 + c.part * S::kCols;
+    };
+    look_ahead(worker);
+    if (c.next_row0 >= 0) Epi::template fetch<BN>(ep, p, c, c.next_row0, c.next_n0);
     for (int t = worker; t < p.num_tiles && ok; t += workers, ++c.n_tile) {
-      const Tile tile = locate(t);
-      c.m0 = tile.m0 + static_cast<int>(side) * kCtaRows;
-      c.n0 = tile.n0 + c.part * S::kCols;
+      tile = next;
+      c.row0 = c.next_row0;
+      c.n0 = c.next_n0;
       c.batch = tile.batch;
-      Epi::template begin<BN>(ep, p, c);
+      look_ahead(t + workers);
+      Epi::template begin<BN>(c);
       for (int kb0 = 0, kb1; kb0 < total_kb && ok; kb0 = kb1, ++n) {
         kb1 = group_end(kb0);
         const uint32_t st = n & 1u;

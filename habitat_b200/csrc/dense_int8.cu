@@ -7,6 +7,7 @@
 // definition, give the same bits.  A row whose amax is below 2^-119 counts as zeros (127 / amax would overflow); a row with
 // an infinity or a NaN gets zeros and the scale NaN, so that its results are NaN and not finite numbers that look like some.
 #include <atomic>
+#include <cmath>
 #include <type_traits>
 
 #include "dense_gemm.cuh"
@@ -209,41 +210,116 @@ struct LayerScales {
   const float* row;
   const float* channel;
   const float* bias;     // or null
-  int32_t relu;
+  float floor;           // 0 with ReLU, else -infinity: the larger of a value and it
 };
 
-// Channel scales and biases of a part's columns into shared memory (zeros outside the matrix), by its four warps.
-template <int BN>
-__device__ __forceinline__ void load_channels(const LayerScales& s, const Product& p, const EpiContext& c) {
-  constexpr int kCols = Shape<BN>::kCols;
-  const int i = (c.warp & 3) * 32 + c.lane;
-  const uint32_t buf = c.n_tile & 1u;
-  if (i < kCols) {
-    const int n = c.n0 + i;
-    c.tail->scale[buf][c.part * kCols + i] = n < p.N ? s.channel[n] : 0.0f;
-    c.tail->bias[buf][c.part * kCols + i] = n < p.N && s.bias ? s.bias[n] : 0.0f;
-  }
-  asm volatile("bar.sync %0, 128;" ::"r"(1 + c.part) : "memory");
+// Accumulators are read as 16 x 256-bit fragments: of 16 rows lane l gets rows l / 4 and l / 4 + 8, and of every eight
+// columns 2 (l mod 4) and the next.  A lane then has 4 rows and a quarter of its warp's columns; with whole rows per lane
+// (32 x 32 bits) every lane loads the scale and bias of every column from shared memory, which the MMAs' operands go
+// through as well (65,536 x 1024 x 1024: quantised rows 84 us, 67 without those loads).
+template <int COLS>
+__device__ __forceinline__ void load_fragment(uint32_t taddr, uint32_t* r);
+template <>
+__device__ __forceinline__ void load_fragment<64>(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+template <>
+__device__ __forceinline__ void load_fragment<32>(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
 }
 
-// 32 accumulators of a row -> results.
+// A float from memory to shared memory, zero where there is none, without a register on the way: scales that were loaded a
+// tile ahead into registers were spilled, which waits for them.
+__device__ __forceinline__ void copy_float(const float* to, const float* from, bool there) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(there ? 4 : 0) : "memory");
+}
 template <int BN>
-__device__ __forceinline__ void finish(const LayerScales& s, const EpiContext& c, float row_scale, int chunk, const uint32_t* acc,
-                                       float* v) {
-  const uint32_t buf = c.n_tile & 1u;
-  const int at = c.part * Shape<BN>::kCols + chunk * 32;
-  const float4* sc = reinterpret_cast<const float4*>(&c.tail->scale[buf][at]);
-  const float4* bi = reinterpret_cast<const float4*>(&c.tail->bias[buf][at]);
+__device__ __forceinline__ void fetch_scales(const LayerScales& s, const Product& p, const EpiContext& c, int row0, int n0) {
+  float* to = c.tail->scales[c.warp];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float4 w = sc[j], b = bi[j];
-    const float ws[4] = {w.x, w.y, w.z, w.w}, bs[4] = {b.x, b.y, b.z, b.w};
+  for (int i = 0; i < Shape<BN>::kCols; i += 32) {
+    const bool there = n0 + i + c.lane < p.N;
+    const int n = there ? n0 + i + c.lane : 0;
+    copy_float(to + i + c.lane, s.channel + n, there);
+    copy_float(to + 64 + i + c.lane, (s.bias ? s.bias : s.channel) + n, there && s.bias);
+  }
+  const bool there = row0 + c.lane < p.M;
+  copy_float(to + 128 + c.lane, s.row + (there ? row0 + c.lane : 0), there);
+}
+
+// Two products.  (The sums behind them stay single: a packed sum of packed products is merged into a multiply-add, which
+// rounds once instead of twice, whatever the instructions' rounding says.)
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+
+// The warp's part of the tile as results: v[j][i] are columns 8 j + 2 (lane mod 4) and the next of row 8 i + lane / 4.
+template <int BN, class Release>
+__device__ __forceinline__ void finish(const LayerScales& s, const Product& p, const EpiContext& c, float2 (&v)[Shape<BN>::kCols / 8][4],
+                                       Release release) {
+  constexpr int kCols = Shape<BN>::kCols;
+  uint32_t acc[2][kCols / 2];
+  load_fragment<kCols>(c.tmem, acc[0]);
+  load_fragment<kCols>(c.tmem + (16u << 16), acc[1]);
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncwarp();
+  const float* at = c.tail->scales[c.warp];
+  const float2* sc = reinterpret_cast<const float2*>(at) + (c.lane & 3);
+  float row[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) row[i] = at[128 + 8 * i + (c.lane >> 2)];
+  tc_wait_ld();
+  release();
+#pragma unroll
+  for (int j = 0; j < kCols / 8; ++j) {
+    const float2 w = sc[4 * j], b = sc[32 + 4 * j];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float y = __fadd_rn(__fmul_rn(__fmul_rn(__int2float_rn(static_cast<int>(acc[4 * j + i])), ws[i]), row_scale), bs[i]);
-      v[4 * j + i] = s.relu ? relu_nan(y) : y;
+      const uint32_t* a = &acc[i >> 1][4 * j + 2 * (i & 1)];
+      const float2 x = make_float2(__int2float_rn(static_cast<int>(a[0])), __int2float_rn(static_cast<int>(a[1])));
+      const float2 y = mul2(mul2(x, w), make_float2(row[i], row[i]));
+      v[j][i] = make_float2(max_nan(__fadd_rn(y.x, b.x), s.floor), max_nan(__fadd_rn(y.y, b.y), s.floor));
     }
   }
+  __syncwarp();
+  if (c.next_row0 >= 0) fetch_scales<BN>(s, p, c, c.next_row0, c.next_n0);
+}
+
+// Fragments to rows: stores four 8 x 8 matrices of 16-bit elements, w[j] to the 16-byte column j of rows 8 i .. 8 i + 7 of a
+// warp's staging (64 bytes per row, columns permuted by the row so that eight rows fill all banks); and the 16 bytes of row
+// r and column c.
+__device__ __forceinline__ void store_fragment(uint32_t staging, int i, const uint32_t (&w)[4], int lane) {
+  const int r = 8 * i + (lane & 7), j = lane >> 3;
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(staging + r * 64 + ((j ^ ((r >> 1) & 3)) << 4)),
+               "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+               : "memory");
+}
+__device__ __forceinline__ uint4 staged_row(const uint8_t* staging, int r, int c) {
+  return *reinterpret_cast<const uint4*>(staging + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+}
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 
 struct FloatOut {
@@ -254,30 +330,92 @@ struct FloatOut {
     Out out;
   };
   template <int BN>
-  static __device__ __forceinline__ void begin(const Params& ep, const Product& p, const EpiContext& c) {
-    load_channels<BN>(ep.s, p, c);
+  static __device__ __forceinline__ void fetch(const Params& ep, const Product& p, const EpiContext& c, int row0, int n0) {
+    fetch_scales<BN>(ep.s, p, c, row0, n0);
   }
+  template <int BN>
+  static __device__ __forceinline__ void begin(const EpiContext&) {}
   template <int BN, class Release>
   static __device__ __forceinline__ void drain(const Params& ep, const Product& p, const EpiContext& c, float (&)[1], Release release) {
-    const int row = c.m0 + c.row;
-    const float rs = row < p.M ? __ldg(ep.s.row + row) : 0.0f;
-#pragma unroll 1
-    for (int chunk = 0; chunk < Shape<BN>::kCols / 32; ++chunk) {
-      uint32_t acc[32];
-      float v[32];
-      tc_ld32_async(c.tmem + chunk * 32, acc);
-      tc_wait_ld();
-      if (chunk == Shape<BN>::kCols / 32 - 1) release();
-      finish<BN>(ep.s, c, rs, chunk, acc, v);
-      store_rows(ep.out, 0, p.M, p.N, c.m0 + (c.row & ~31), c.n0 + chunk * 32, v, c.tail->staging + c.warp * kStageOutBytes, c.lane);
+    constexpr int kBlocks = Shape<BN>::kCols / 8;
+    float2 v[kBlocks][4];
+    finish<BN>(ep.s, p, c, v, release);
+    const int row0 = c.row0 + (c.lane >> 2);
+    if (ep.out.type == kF32) {
+      // four lanes fill a sector
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (row0 + 8 * i >= p.M) continue;
+        float* to = static_cast<float*>(ep.out.base) + static_cast<int64_t>(row0 + 8 * i) * ep.out.ld + c.n0 + 2 * (c.lane & 3);
+        const int left = p.N - c.n0 - 2 * (c.lane & 3);
+        if (ep.out.vec >= 8) {
+#pragma unroll
+          for (int j = 0; j < kBlocks; ++j) {
+            if (8 * j + 2 <= left) *reinterpret_cast<float2*>(to + 8 * j) = v[j][i];
+            else if (8 * j < left) to[8 * j] = v[j][i].x;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < kBlocks; ++j) {
+            if (8 * j < left) to[8 * j] = v[j][i].x;
+            if (8 * j + 1 < left) to[8 * j + 1] = v[j][i].y;
+          }
+        }
+      }
+      return;
+    }
+    uint8_t* staging = c.tail->staging + c.warp * kStageOutBytes;
+#pragma unroll
+    for (int g = 0; g < kBlocks; g += 4) {         // 32 columns, 64 bytes, at a time
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = ep.out.type == kBF16 ? pack_bf16(v[g + j][i].x, v[g + j][i].y) : pack_f16(v[g + j][i].x, v[g + j][i].y);
+        store_fragment(smem_u32(staging), i, w, c.lane);
+      }
+      __syncwarp();
+      uint16_t* out = static_cast<uint16_t*>(ep.out.base) + c.n0 + 8 * g;
+      const int left = p.N - c.n0 - 8 * g;
+      if (ep.out.vec >= 4) {
+        const int n = 8 * (c.lane & 3);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (row0 + 8 * i >= p.M) continue;
+          const uint4 x = staged_row(staging, 8 * i + (c.lane >> 2), c.lane & 3);
+          uint16_t* to = out + static_cast<int64_t>(row0 + 8 * i) * ep.out.ld + n;
+          const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+          if (n + 8 > left) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (n + e < left) to[e] = static_cast<uint16_t>(xs[e >> 1] >> (16 * (e & 1)));
+          } else if (ep.out.vec == 16) {
+            *reinterpret_cast<uint4*>(to) = x;
+          } else if (ep.out.vec == 8) {
+            reinterpret_cast<uint2*>(to)[0] = make_uint2(x.x, x.y);
+            reinterpret_cast<uint2*>(to)[1] = make_uint2(x.z, x.w);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) reinterpret_cast<uint32_t*>(to)[e] = xs[e];
+          }
+        }
+      } else if (c.lane < left) {
+        // rows that start on any element: a row of 32 at a time
+#pragma unroll 8
+        for (int r = 0; r < 32; ++r)
+          if (c.row0 + r < p.M)
+            out[static_cast<int64_t>(c.row0 + r) * ep.out.ld + c.lane] =
+                *reinterpret_cast<const uint16_t*>(staging + r * 64 + (((c.lane >> 3) ^ ((r >> 1) & 3)) << 4) + 2 * (c.lane & 7));
+      }
     }
   }
 };
 
 // The result as quantised rows.  The CTAs of a cluster hold whole rows between them (one pair per 256 columns): every lane
-// keeps its 64 results in registers, sends their largest magnitude to all CTAs of its row half through distributed shared
-// memory (counted in bytes there: nobody waits for a store to be acknowledged), and quantises when the others' are there.  The
-// accumulators are free before the exchange, so the next tile's MMAs run during it.
+// keeps its 64 results in registers, a warp sends its rows' largest magnitudes to all CTAs of its row half through distributed
+// shared memory (counted in bytes there: nobody waits for a store to be acknowledged), and quantises when the others' are
+// there.  The accumulators are free before the exchange, so the next tile's MMAs run during it.
 template <int kCtas>
 struct QuantOut {
   static constexpr bool kInt8 = true, kMnMajorB = false, kGrouped = false;
@@ -289,33 +427,36 @@ struct QuantOut {
     float* scales;
   };
   template <int BN>
-  static __device__ __forceinline__ void begin(const Params& ep, const Product& p, const EpiContext& c) {
+  static __device__ __forceinline__ void fetch(const Params& ep, const Product& p, const EpiContext& c, int row0, int n0) {
+    fetch_scales<BN>(ep.s, p, c, row0, n0);
+  }
+  template <int BN>
+  static __device__ __forceinline__ void begin(const EpiContext& c) {
     if (c.warp == 0 && c.lane == 0)
       mbar_expect_tx(smem_u32(&c.tail->exchange[c.n_tile & 1u]), kCtas / 2 * Shape<BN>::kParts * kCtaRows * 4);
-    load_channels<BN>(ep.s, p, c);
   }
   template <int BN, class Release>
   static __device__ __forceinline__ void drain(const Params& ep, const Product& p, const EpiContext& c, float (&)[1], Release release) {
-    static_assert(BN == 256 && Shape<BN>::kCols == 64, "64 columns per lane");
-    const int row = c.m0 + c.row;
-    const float rs = row < p.M ? __ldg(ep.s.row + row) : 0.0f;
-    float v[64];
+    constexpr int kBlocks = Shape<BN>::kCols / 8, kParts = Shape<BN>::kParts;
+    float2 v[kBlocks][4];
+    finish<BN>(ep.s, p, c, v, release);
+    // the largest magnitude of each of the 32 rows; lane l goes on with row 8 (l mod 4) + l / 4
     float amax = 0.0f;
 #pragma unroll
-    for (int chunk = 0; chunk < 2; ++chunk) {
-      uint32_t acc[32];
-      tc_ld32_async(c.tmem + chunk * 32, acc);
-      tc_wait_ld();
-      if (chunk == 1) release();
-      finish<BN>(ep.s, c, rs, chunk, acc, v + 32 * chunk);
+    for (int i = 0; i < 4; ++i) {
+      float m = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) amax = max_nan(amax, fabsf(v[32 * chunk + i]));
+      for (int j = 0; j < kBlocks; ++j) m = max3_abs(m, v[j][i].x, v[j][i].y);
+      m = max_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+      m = max_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
+      if ((c.lane & 3) == i) amax = m;
     }
+    const int mine = c.row + 8 * (c.lane & 3) + (c.lane >> 2);       // among the CTA's rows
     const uint32_t buf = c.n_tile & 1u, side = c.rank & 1u;
     const uint32_t bar = smem_u32(&c.tail->exchange[buf]);
-    const uint32_t mine = smem_u32(&c.tail->row_max[buf][c.rank >> 1][c.part][c.row]);
+    const uint32_t at = smem_u32(&c.tail->row_max[buf][c.rank >> 1][c.part][mine]);
 #pragma unroll
-    for (int i = 0; i < kCtas / 2; ++i) st_async_f32(map_to_cta(mine, 2 * i + side), amax, map_to_cta(bar, 2 * i + side));
+    for (int i = 0; i < kCtas / 2; ++i) st_async_f32(map_to_cta(at, 2 * i + side), amax, map_to_cta(bar, 2 * i + side));
     if (!mbar_wait_cluster(bar, (c.n_tile >> 1) & 1u, &c.tail->abort, p.status, 0x541)) {
       *c.ok = false;
       return;
@@ -323,35 +464,42 @@ struct QuantOut {
 #pragma unroll
     for (int i = 0; i < kCtas / 2; ++i)
 #pragma unroll
-      for (int j = 0; j < Shape<BN>::kParts; ++j) amax = max_nan(amax, c.tail->row_max[buf][i][j][c.row]);
+      for (int j = 0; j < kParts; ++j) amax = max_nan(amax, c.tail->row_max[buf][i][j][mine]);
     const RowScale s = row_scale(amax);
+    const int row = c.row0 + 8 * (c.lane & 3) + (c.lane >> 2);
     if (c.rank < 2 && c.part == 0 && row < p.M) ep.scales[row] = s.scale;
+    const unsigned bad = __ballot_sync(0xFFFFFFFFu, s.bad);
     uint8_t* staging = c.tail->staging + c.warp * kStageOutBytes;
     __syncwarp();
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t w[4];
+    for (int i = 0; i < 4; ++i) {
+      const int from = (c.lane & ~3) | i;                             // the lane that has row 8 i + lane / 4
+      const float inverse = __shfl_sync(0xFFFFFFFFu, s.inverse, from);
+      uint32_t w[4];                            // the lane's two columns of blocks 2 j and 2 j + 1
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float* x = v + 16 * j + 4 * i;
-        w[i] = low_bytes(quantized(x[0], s.inverse), quantized(x[1], s.inverse), quantized(x[2], s.inverse), quantized(x[3], s.inverse));
-        if (s.bad) w[i] = 0;
-      }
-      *reinterpret_cast<uint4*>(staging + c.lane * 64 + ((j ^ ((c.lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+      for (int j = 0; j < 4; ++j)
+        w[j] = low_bytes(quantized(v[2 * j][i].x, inverse), quantized(v[2 * j][i].y, inverse), quantized(v[2 * j + 1][i].x, inverse),
+                         quantized(v[2 * j + 1][i].y, inverse));
+      store_fragment(smem_u32(staging), i, w, c.lane);
     }
     __syncwarp();
-    const int m0 = c.m0 + (c.row & ~31);
+    const int n = c.n0 + 16 * (c.lane & 3);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int r = 8 * i + (c.lane >> 2), ch = c.lane & 3;
-      const uint8_t* at = staging + r * 64 + ((ch ^ ((r >> 1) & 3)) << 4);
-      const int n = c.n0 + 16 * ch;
-      if (m0 + r >= p.M) continue;
-      int8_t* to = ep.q + static_cast<int64_t>(m0 + r) * ep.pitch + n;
+      const int r = c.row0 + 8 * i + (c.lane >> 2);
+      if (r >= p.M) continue;
+      const uint4 w = staged_row(staging, 8 * i + (c.lane >> 2), c.lane & 3);     // pairs of columns of two blocks in turn
+      uint4 x = make_uint4(__byte_perm(w.x, w.y, 0x5410), __byte_perm(w.z, w.w, 0x5410), __byte_perm(w.x, w.y, 0x7632),
+                           __byte_perm(w.z, w.w, 0x7632));
+      if (bad >> ((c.lane & ~3) | i) & 1u) x = make_uint4(0, 0, 0, 0);
+      int8_t* to = ep.q + static_cast<int64_t>(r) * ep.pitch + n;
       if (n + 16 <= p.N) {
-        *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(at);
+        *reinterpret_cast<uint4*>(to) = x;
       } else {
-        for (int e = 0; n + e < p.N && e < 16; ++e) to[e] = static_cast<int8_t>(at[e]);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (n + e < p.N) to[e] = static_cast<int8_t>(xs[e >> 2] >> (8 * (e & 3)));
       }
     }
   }
@@ -438,11 +586,11 @@ hb_status launch_float(const Operands& o, int64_t M, int64_t N, int64_t K, const
   Product p{};
   if (const hb_status st = describe(&p, o, M, N, K, BN, status)) return st;
   const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
-  if (tiles > 0x7FFFFFFF) {
+  if (tiles * kTileGroup > 0x7FFFFFFF) {
     hb::set_error("hb_int8_matmul: M x N too large for one launch");
     return HB_ERR_TOO_LARGE;
   }
-  p.num_tiles = static_cast<int32_t>(tiles);
+  set_tiles(&p, tiles);
   const int clusters = p.num_tiles < pairs ? p.num_tiles : pairs;
   HB_CUDA_TRY(launch_clusters(kernel, clusters, 2, Shape<BN>::kThreads, smem_bytes<BN>(), s, p, ep));
   return HB_OK;
@@ -457,7 +605,7 @@ hb_status launch_quant(const Operands& o, int64_t M, int64_t N, int64_t K, const
   if (const hb_status st = max_clusters(kernel, kCtas, Shape<256>::kThreads, smem_bytes<256>(), held, &clusters)) return st;
   Product p{};
   if (const hb_status st = describe(&p, o, M, N, K, 256, status)) return st;
-  p.num_tiles = p.tiles_m;
+  set_tiles(&p, p.tiles_m);
   if (p.num_tiles < clusters) clusters = p.num_tiles;
   HB_CUDA_TRY(launch_clusters(kernel, clusters, kCtas, Shape<256>::kThreads, smem_bytes<256>(), s, p, ep));
   return HB_OK;
@@ -622,9 +770,8 @@ extern "C" hb_status hb_int8_matmul(const int8_t* q, int64_t q_pitch, const floa
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   Operands o{q, q_pitch, w, w_pitch};
   if (const hb_status st = align_operands(name, &o, M, N, K, static_cast<uint8_t*>(workspace), workspace_bytes, 0, s)) return st;
-  const int per = out_type == HB_F32 ? 4 : 8;
-  FloatOut::Params ep{{q_scales, w_scales, bias, relu}, {out, out_pitch, 0, out_type, 0}};
-  ep.out.vec = reinterpret_cast<uintptr_t>(out) % 16 == 0 && out_pitch % per == 0;
+  FloatOut::Params ep{{q_scales, w_scales, bias, relu ? 0.0f : -INFINITY}, {out, out_pitch, 0, out_type, 0}};
+  ep.out.vec = row_alignment(out, out_pitch, 0, out_type == HB_F32 ? 4 : 2);
   int sms = 0;
   if (const hb_status st = sm_count(&sms)) return st;
   switch (tile_columns(M, N, sms / 2)) {
@@ -665,7 +812,7 @@ extern "C" hb_status hb_int8_matmul_quantized(const int8_t* q, int64_t q_pitch, 
     return hb_quantize_rows(y, HB_F32, M, N, pitch, out, out_pitch, out_scales, stream);
   }
   if (const hb_status st = align_operands(name, &o, M, N, K, ws, workspace_bytes, 0, s)) return st;
-  const LayerScales scales{q_scales, w_scales, bias, relu};
+  const LayerScales scales{q_scales, w_scales, bias, relu ? 0.0f : -INFINITY};
   switch ((N + 255) / 256) {
     case 1: return launch_quant<2>(o, M, N, K, {scales, out, out_pitch, out_scales}, status, s);
     case 2: return launch_quant<4>(o, M, N, K, {scales, out, out_pitch, out_scales}, status, s);

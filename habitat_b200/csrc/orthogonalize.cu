@@ -190,10 +190,12 @@ struct SymmetricOut {
     float on_a, on_diagonal;
   };
   template <int BN>
-  static __device__ __forceinline__ void begin(const Params&, const Product&, const EpiContext&) {}
+  static __device__ __forceinline__ void fetch(const Params&, const Product&, const EpiContext&, int, int) {}
+  template <int BN>
+  static __device__ __forceinline__ void begin(const EpiContext&) {}
   template <int BN, class Release>
   static __device__ __forceinline__ void drain(const Params& ep, const Product& p, const EpiContext& c, float* sums, Release release) {
-    const int row = c.m0 + c.row, row0 = c.m0 + (c.row & ~31);
+    const int row0 = c.row0, row = row0 + c.lane;
     float scale = ep.scale;
     if (ep.factor) {
       const float f = __ldg(ep.factor + c.batch);
@@ -219,7 +221,7 @@ struct SymmetricOut {
 #pragma unroll 1
       for (int part = 0; part < (kSplit ? 2 : 1); ++part) {
         if (n0 < row0) {
-          const Out out{base, ep.out.ld, 0, kF16, 1};
+          const Out out{base, ep.out.ld, 0, kF16, 16};
           store_rows(out, 0, p.M, static_cast<int>(ep.out.ld), row0, n0, v, c.tail->staging + c.warp * kStageOutBytes, c.lane);
         } else if (row < p.M) {
 #pragma unroll
@@ -254,10 +256,12 @@ struct UpdateOut {
     float scale;
   };
   template <int BN>
-  static __device__ __forceinline__ void begin(const Params&, const Product&, const EpiContext&) {}
+  static __device__ __forceinline__ void fetch(const Params&, const Product&, const EpiContext&, int, int) {}
+  template <int BN>
+  static __device__ __forceinline__ void begin(const EpiContext&) {}
   template <int BN, class Release>
   static __device__ __forceinline__ void drain(const Params& ep, const Product& p, const EpiContext& c, float* sums, Release release) {
-    const int row = c.m0 + c.row, row0 = c.m0 + (c.row & ~31);
+    const int row0 = c.row0, row = row0 + c.lane;
     const float scale = ep.factor ? ep.scale * __ldg(ep.factor + c.batch) : ep.scale;
     uint8_t* staging = c.tail->staging + c.warp * kStageOutBytes;
     for_chunks<BN, kSplit>(c, sums, release, [&](int chunk, float (&v)[32]) {
@@ -266,11 +270,11 @@ struct UpdateOut {
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] *= scale;
       if (ep.x.hi) {
-        const Out out{ep.x.hi, ep.x.ld, ep.x.batch_stride, kF16, 1};
+        const Out out{ep.x.hi, ep.x.ld, ep.x.batch_stride, kF16, 16};
         store_rows(out, c.batch, p.M, static_cast<int>(ep.x.ld), row0, n0, v, staging, c.lane);
         if (kSplit) {
           take_half(v);
-          const Out low{ep.x.hi + ep.x.low, ep.x.ld, ep.x.batch_stride, kF16, 1};
+          const Out low{ep.x.hi + ep.x.low, ep.x.ld, ep.x.batch_stride, kF16, 16};
           store_rows(low, c.batch, p.M, static_cast<int>(ep.x.ld), row0, n0, v, staging, c.lane);
         }
       } else if (!ep.flip) {
@@ -345,12 +349,12 @@ hb_status launch(Product p, const typename Epi::Params& ep, cudaStream_t s) {
   if (const hb_status st = max_clusters(kernel, 2, Shape<BN>::kThreads, smem_bytes<BN>(), held, &pairs)) return st;
   p.tiles_m = static_cast<int32_t>((p.M + kPairRows - 1) / kPairRows);
   p.tiles_n = static_cast<int32_t>((p.N + BN - 1) / BN);
-  const int64_t tiles = p.batches * (p.lower ? lower_tiles(p.M, BN) : static_cast<int64_t>(p.tiles_m) * p.tiles_n);
-  if (tiles > 0x7FFFFFFF) {
+  const int64_t tiles = p.lower ? lower_tiles(p.M, BN) : static_cast<int64_t>(p.tiles_m) * p.tiles_n;
+  if (tiles * p.batches * kTileGroup > 0x7FFFFFFF) {
     hb::set_error("hb_orthogonalize: too large for one launch");
     return HB_ERR_TOO_LARGE;
   }
-  p.num_tiles = static_cast<int32_t>(tiles);
+  set_tiles(&p, tiles);
   const int clusters = p.num_tiles < pairs ? p.num_tiles : pairs;
   HB_CUDA_TRY(launch_clusters(kernel, clusters, 2, Shape<BN>::kThreads, smem_bytes<BN>(), s, p, ep));
   return HB_OK;
@@ -515,8 +519,7 @@ extern "C" hb_status hb_orthogonalize(const void* update, int32_t type, int64_t 
   HB_CUDA_TRY(encode_planes(&a_cols, A, 2, lay.s, lay.s, batch * planes, lay.sp, a_matrix, bn_sym / 2));
   HB_CUDA_TRY(encode_planes(&b_rows, B, 2, lay.s, lay.s, batch * planes, lay.sp, a_matrix, kCtaRows));
 
-  const int out_per = type == HB_F32 ? 4 : 8;
-  const bool out_vec = reinterpret_cast<uintptr_t>(out) % 16 == 0 && out_pitch % out_per == 0 && (batch == 1 || out_batch_stride % out_per == 0);
+  const int32_t out_vec = row_alignment(out, out_pitch, batch > 1 ? out_batch_stride : 0, type == HB_F32 ? 4 : 2);
   auto run = [&](auto is_split) -> hb_status {
     constexpr bool kSplit = decltype(is_split)::value;
     using Sym = SymmetricOut<kSplit>;
