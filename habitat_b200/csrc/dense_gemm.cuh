@@ -2,13 +2,15 @@
 //
 // A pair of CTAs (cta_group::2) computes tiles of 256 x BN: each CTA brings its 128 rows of A and its BN / 2 rows of B
 // into a ring of 128-byte-wide slots by TMA (128-byte swizzle, no multicast), the even CTA's elected lane issues the MMAs for
-// both, and the accumulators (32-bit) lie in TMEM twice, so that the epilogue warps of each CTA drain one tile while the
-// next one is multiplied.  Per slot the pair moves 2 (128 + BN / 2) x 128 bytes for 4 MMAs; with BN = 256 that is 64
+// both, and the accumulators (32-bit) lie in TMEM two to four times, so that the epilogue warps of each CTA drain one tile
+// while the next one is multiplied.  Per slot the pair moves 2 (128 + BN / 2) x 128 bytes for 4 MMAs; with BN = 256 that is 64
 // bytes per clock and SM, half of what two separate SMs with 128 x 256 tiles would need of L2.  A slot is 128 bytes of K
 // whatever the type, 128 8-bit integers or 64 half-precision values, so both share the ring and the issue loop.
 #pragma once
 
 #include <cuda_fp16.h>
+
+#include <initializer_list>
 
 #include "mlp_common.cuh"
 
@@ -28,7 +30,8 @@ struct Shape {
   static constexpr int kBRows = BN / 2;                               // rows of B (columns of D) per CTA
   static constexpr int kSlotBytes = (kCtaRows + kBRows) * kSlotK;     // per CTA
   static constexpr int kSlots = BN == 256 ? 5 : BN == 128 ? 6 : 8;
-  static constexpr int kTmemCols = 2 * BN;
+  static constexpr int kAccs = BN == 256 ? 2 : 4;                     // accumulators
+  static constexpr int kTmemCols = kAccs * BN;
   // Epilogue warps: what they do per tile is a chain of loads and conversions that two warps per scheduler cannot fill (28 %
   // of the issue slots, 12,600 cycles per tile of 256 x 256 against 4,096 of MMAs at K = 1,024).
   static constexpr int kEpiWarps = BN == 64 ? 8 : 16;
@@ -42,7 +45,7 @@ struct Tail {
   uint8_t staging[kMostEpiWarps * kStageOutBytes];
   float scales[kMostEpiWarps][160];        // an epilogue warp's: 64 channel scales, 64 biases, 32 row scales
   float row_max[2][4][4][kCtaRows];
-  uint64_t full[8], empty[8], acc_full[2], acc_empty[2], exchange[2], drain;
+  uint64_t full[8], empty[8], acc_full[4], acc_empty[4], exchange[2], drain;
   uint32_t tmem;
   int abort;
 };
@@ -283,20 +286,33 @@ struct EpiContext {
 
 // Adds a group's accumulators to a lane's sums.
 template <int BN, class Release>
-__device__ __forceinline__ void add_group(const EpiContext& c, float* sums, Release release) {
-  constexpr int kChunks = Shape<BN>::kCols / 32;
+__device__ __forceinline__ void add_group(const EpiContext& c, float (&sums)[Shape<BN>::kCols], Release release) {
+  static_assert(Shape<BN>::kCols == 32, "one load");
+  uint32_t acc[32];
+  tc_ld32_async(c.tmem, acc);
+  tc_wait_ld();
+  release();
 #pragma unroll
-  for (int chunk = 0; chunk < kChunks; ++chunk) {
-    uint32_t acc[32];
-    tc_ld32_async(c.tmem + chunk * 32, acc);
-    tc_wait_ld();
-    if (chunk == kChunks - 1) release();
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const float x = __uint_as_float(acc[i]);
-      sums[32 * chunk + i] = c.first ? x : sums[32 * chunk + i] + x;
+  for (int i = 0; i < 32; ++i) {
+    const float x = __uint_as_float(acc[i]);
+    sums[i] = c.first ? x : sums[i] + x;
+  }
+}
+
+// The width of a tile whose rounds take least.  A round of MMAs takes 64 cycles per 16 values of K (32 in 8 bits) for up to
+// 128 columns and 128 for 256, and its epilogue and start about as long as 24 columns and a quarter of its own.
+template <class Count>
+inline int tile_columns(std::initializer_list<int> widths, int pairs, Count tiles) {
+  int best = 0;
+  int64_t least = INT64_MAX;
+  for (const int bn : widths) {
+    const int64_t cost = (tiles(bn) + pairs - 1) / pairs * (4 * (bn > 128 ? bn : 128) + bn + 96);
+    if (cost < least) {
+      least = cost;
+      best = bn;
     }
   }
+  return best;
 }
 
 // The kernel.  Epilogue: a policy with `Params`, static kInt8, kMnMajorB, kGrouped, kClusterCtas (0: a pair; else the CTAs of a
@@ -330,11 +346,11 @@ gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ typename 
       mbar_init(full + 8 * s, 1);       // the leader's: its producer's expect_tx; both CTAs' copies count there
       mbar_init(empty + 8 * s, 1);
     }
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < S::kAccs; ++s) {
       mbar_init(acc_full + 8 * s, 1);
       mbar_init(acc_empty + 8 * s, 2 * S::kEpiWarps);
-      mbar_init(smem_u32(&tail->exchange[s]), 1);
     }
+    for (int s = 0; s < 2; ++s) mbar_init(smem_u32(&tail->exchange[s]), 1);
     mbar_init(smem_u32(&tail->drain), 1);
     tail->abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -418,8 +434,8 @@ gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ typename 
       for (int t = worker; t < p.num_tiles && ok; t += workers) {
         for (int kb0 = 0, kb1; kb0 < total_kb && ok; kb0 = kb1, ++n) {
           kb1 = group_end(kb0);
-          const uint32_t st = n & 1u;
-          ok = mbar_wait(acc_empty + 8 * st, ((n >> 1) & 1u) ^ 1u, abort_flag, p.status, 0x521);
+          const uint32_t st = n % S::kAccs, turn = n / S::kAccs & 1u;
+          ok = mbar_wait(acc_empty + 8 * st, turn ^ 1u, abort_flag, p.status, 0x521);
           tc_fence_after();
           const uint32_t d = tmem + st * BN;
           for (int kb = kb0; kb < kb1 && ok; ++kb) {
@@ -468,11 +484,11 @@ gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ typename 
       Epi::template begin<BN>(c);
       for (int kb0 = 0, kb1; kb0 < total_kb && ok; kb0 = kb1, ++n) {
         kb1 = group_end(kb0);
-        const uint32_t st = n & 1u;
+        const uint32_t st = n % S::kAccs, turn = n / S::kAccs & 1u;
         c.tmem = tmem + (static_cast<uint32_t>(quad * 32) << 16) + st * BN + static_cast<uint32_t>(c.part * S::kCols);
         c.first = kb0 == 0;
         c.last = kb1 == total_kb;
-        if (!mbar_wait(acc_full + 8 * st, (n >> 1) & 1u, abort_flag, p.status, 0x531)) { ok = false; break; }
+        if (!mbar_wait(acc_full + 8 * st, turn, abort_flag, p.status, 0x531)) { ok = false; break; }
         tc_fence_after();
         Epi::template drain<BN>(ep, p, c, sums, [&] {
           tc_fence_before();

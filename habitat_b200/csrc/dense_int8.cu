@@ -611,21 +611,6 @@ hb_status launch_quant(const Operands& o, int64_t M, int64_t N, int64_t K, const
   return HB_OK;
 }
 
-// The tile width whose rounds of tiles take least: a round costs its columns and about 24 columns' time beside.
-int tile_columns(int64_t M, int64_t N, int pairs) {
-  int best = 256;
-  int64_t least = INT64_MAX;
-  for (const int bn : {256, 128, 64}) {
-    const int64_t tiles = ((M + kPairRows - 1) / kPairRows) * ((N + bn - 1) / bn);
-    const int64_t cost = (tiles + pairs - 1) / pairs * (bn + 24);
-    if (cost < least) {
-      least = cost;
-      best = bn;
-    }
-  }
-  return best;
-}
-
 }  // namespace
 
 hb_status sm_count(int* sms) {
@@ -774,7 +759,7 @@ extern "C" hb_status hb_int8_matmul(const int8_t* q, int64_t q_pitch, const floa
   ep.out.vec = row_alignment(out, out_pitch, 0, out_type == HB_F32 ? 4 : 2);
   int sms = 0;
   if (const hb_status st = sm_count(&sms)) return st;
-  switch (tile_columns(M, N, sms / 2)) {
+  switch (tile_columns({256, 128, 64}, sms / 2, [&](int bn) { return ((M + kPairRows - 1) / kPairRows) * ((N + bn - 1) / bn); })) {
     case 256: return launch_float<256>(o, M, N, K, ep, status, s);
     case 128: return launch_float<128>(o, M, N, K, ep, status, s);
     default: return launch_float<64>(o, M, N, K, ep, status, s);

@@ -136,17 +136,10 @@ __device__ __forceinline__ void take_half(float (&v)[32]) {
 // Calls work(chunk, values) for the lane's 32-column chunks: as they leave the accumulators, or, where K comes in groups, from
 // the sums behind the last group.
 template <int BN, bool kGrouped, class Release, class Work>
-__device__ __forceinline__ void for_chunks(const EpiContext& c, float* sums, Release release, Work work) {
+__device__ __forceinline__ void for_chunks(const EpiContext& c, float (&sums)[kGrouped ? Shape<BN>::kCols : 1], Release release, Work work) {
   if constexpr (kGrouped) {
     add_group<BN>(c, sums, release);
-    if (!c.last) return;
-#pragma unroll
-    for (int chunk = 0; chunk < Shape<BN>::kCols / 32; ++chunk) {
-      float v[32];
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = sums[32 * chunk + i];
-      work(chunk, v);
-    }
+    if (c.last) work(0, sums);
   } else {
 #pragma unroll 1
     for (int chunk = 0; chunk < Shape<BN>::kCols / 32; ++chunk) {
@@ -194,7 +187,7 @@ struct SymmetricOut {
   template <int BN>
   static __device__ __forceinline__ void begin(const EpiContext&) {}
   template <int BN, class Release>
-  static __device__ __forceinline__ void drain(const Params& ep, const Product& p, const EpiContext& c, float* sums, Release release) {
+  static __device__ __forceinline__ void drain(const Params& ep, const Product& p, const EpiContext& c, float (&sums)[kGrouped ? Shape<BN>::kCols : 1], Release release) {
     const int row0 = c.row0, row = row0 + c.lane;
     float scale = ep.scale;
     if (ep.factor) {
@@ -260,7 +253,7 @@ struct UpdateOut {
   template <int BN>
   static __device__ __forceinline__ void begin(const EpiContext&) {}
   template <int BN, class Release>
-  static __device__ __forceinline__ void drain(const Params& ep, const Product& p, const EpiContext& c, float* sums, Release release) {
+  static __device__ __forceinline__ void drain(const Params& ep, const Product& p, const EpiContext& c, float (&sums)[kGrouped ? Shape<BN>::kCols : 1], Release release) {
     const int row0 = c.row0, row = row0 + c.lane;
     const float scale = ep.factor ? ep.scale * __ldg(ep.factor + c.batch) : ep.scale;
     uint8_t* staging = c.tail->staging + c.warp * kStageOutBytes;
@@ -323,21 +316,6 @@ int64_t lower_tiles(int64_t s, int bn) {
   int64_t n = 0;
   for (int64_t i = 0; i < tm; ++i) n += (i + 1) * per < tn ? (i + 1) * per : tn;
   return n;
-}
-
-// The width whose rounds of tiles take least, as for the 8-bit products.
-template <typename Count>
-int columns_for(const int* widths, int n, int pairs, Count tiles) {
-  int best = widths[0];
-  int64_t least = INT64_MAX;
-  for (int i = 0; i < n; ++i) {
-    const int64_t cost = (tiles(widths[i]) + pairs - 1) / pairs * (widths[i] + 24);
-    if (cost < least) {
-      least = cost;
-      best = widths[i];
-    }
-  }
-  return best;
 }
 
 template <int BN, class Epi>
@@ -504,11 +482,11 @@ extern "C" hb_status hb_orthogonalize(const void* update, int32_t type, int64_t 
   int sms = 0;
   if (const hb_status e = sm_count(&sms)) return e;
   const int pairs = sms / 2;
-  constexpr int kSym[3] = {256, 128, 64}, kUpd[2] = {256, 128};
-  const int bn_sym = columns_for(kSym, 3, pairs, [&](int bn) { return batch * lower_tiles(lay.s, bn); });
-  const int bn_upd = columns_for(kUpd, 2, pairs, [&](int bn) {
-    return batch * ((lay.s + kPairRows - 1) / kPairRows) * ((lay.l + bn - 1) / bn);
-  });
+  auto sym_tiles = [&](int bn) { return batch * lower_tiles(lay.s, bn); };
+  auto upd_tiles = [&](int bn) { return batch * ((lay.s + kPairRows - 1) / kPairRows) * ((lay.l + bn - 1) / bn); };
+  // groups' sums are kept for 32 columns per epilogue lane, which is 128 for the tile
+  const int bn_sym = split ? tile_columns({128, 64}, pairs, sym_tiles) : tile_columns({256, 128, 64}, pairs, sym_tiles);
+  const int bn_upd = split ? 128 : tile_columns({256, 128}, pairs, upd_tiles);
   CUtensorMap x_rows[2], x_cols[2], x_k[2], a_rows, a_cols, b_rows;
   for (int i = 0; i < (steps > 1 ? 2 : 1); ++i) {
     HB_CUDA_TRY(encode_planes(&x_rows[i], x[i], 2, lay.l, lay.s, batch * planes, lay.lp, x_matrix, kCtaRows));
@@ -539,7 +517,9 @@ extern "C" hb_status hb_orthogonalize(const void* update, int32_t type, int64_t 
     auto symmetric = [&](const CUtensorMap& ma, const CUtensorMap& mb, int64_t K, const typename Sym::Params& ep) {
       Product p = product(ma, mb, lay.s, K);
       p.lower = 1;
-      return bn_sym == 256 ? launch<256, Sym>(p, ep, st) : bn_sym == 128 ? launch<128, Sym>(p, ep, st) : launch<64, Sym>(p, ep, st);
+      if constexpr (!kSplit)
+        if (bn_sym == 256) return launch<256, Sym>(p, ep, st);
+      return bn_sym == 128 ? launch<128, Sym>(p, ep, st) : launch<64, Sym>(p, ep, st);
     };
     for (int i = 0; i < steps; ++i) {
       const int from = i & 1, to = from ^ 1;
@@ -553,7 +533,10 @@ extern "C" hb_status hb_orthogonalize(const void* update, int32_t type, int64_t 
       const float scale = (first ? 1.0f : 1.0f / kScale) * (last ? 1.0f : kScale) / kScale;
       const typename Upd::Params ep{last ? Planes{} : x_planes(to), Out{out, out_pitch, out_batch_stride, type, out_vec}, flip, first ? factor : nullptr, scale};
       const Product p = product(b_rows, x_k[from], lay.l, lay.s);
-      if (const hb_status e = bn_upd == 256 ? launch<256, Upd>(p, ep, st) : launch<128, Upd>(p, ep, st)) return e;
+      hb_status e = HB_OK;
+      if constexpr (kSplit) e = launch<128, Upd>(p, ep, st);
+      else e = bn_upd == 256 ? launch<256, Upd>(p, ep, st) : launch<128, Upd>(p, ep, st);
+      if (e) return e;
     }
     return HB_OK;
   };
