@@ -359,24 +359,55 @@ SidePlan side_plan(int64_t rows, int64_t cols, bool split) {
   return r;
 }
 
-template <bool kSplit>
-hb_status launch_side(const SidePlan& plan, int64_t batch, const SideParams& p, bool* launched, cudaStream_t s) {
-  static std::atomic<int> held[64];
-  static std::atomic<int> widest[64];      // of the clusters that the GPU holds: 16, or 8 which every one does
-  auto kernel = small_side_kernel<kSplit>;
+// The widest clusters of `kernel` (its shared memory `smem`) that the current GPU holds: 16, or 8 which every one does.
+template <typename... KArgs>
+hb_status widest_cluster(void (*kernel)(KArgs...), int threads, int smem, std::atomic<int>* held, std::atomic<int>* widest, int* out) {
   int dev = 0, n = 0;
   HB_CUDA_TRY(cudaGetDevice(&dev));
-  if (dev < 0 || dev >= 64) return HB_OK;
+  if (dev < 0 || dev >= 64) {
+    hb::set_error("device ordinal %d out of range", dev);
+    return HB_ERR_UNSUPPORTED;
+  }
   if (widest[dev].load() == 0) {
-    HB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    const bool wide = max_clusters(kernel, 16, kSideThreads, kSideSmem, held, &n) == HB_OK;
+    HB_CUDA_TRY(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    const bool wide = max_clusters(kernel, 16, threads, smem, held, &n) == HB_OK;
     if (!wide) {
       cudaGetLastError();
-      if (const hb_status st = max_clusters(kernel, 8, kSideThreads, kSideSmem, held, &n)) return st;
+      if (const hb_status st = max_clusters(kernel, 8, threads, smem, held, &n)) return st;
     }
     widest[dev].store(wide ? 16 : 8);
   }
-  if (plan.ctas > widest[dev].load() || batch * plan.ctas > 0x7FFFFFFF) return HB_OK;
+  *out = widest[dev].load();
+  return HB_OK;
+}
+
+// Matrices with a shorter side of at most 32: CTAs of a cluster, columns of each, shared memory; ctas 0 when they do not fit.
+struct GramPlan {
+  int ctas, columns, smem;
+};
+GramPlan gram_plan(int64_t s, int64_t l, int widest) {
+  GramPlan r{0, 0, 0};
+  if (s < 1 || s > kGramSide) return r;
+  const int s4 = static_cast<int>(up(s, 4));
+  for (int ctas = 1; ctas <= widest; ctas *= 2) {
+    const int64_t columns = (l + ctas - 1) / ctas, smem = gram_smem(s4, columns);
+    if (smem > kSideSmem || (columns > 128 && ctas < widest)) continue;
+    r.ctas = ctas;
+    r.columns = static_cast<int>(columns);
+    r.smem = static_cast<int>(smem);
+    break;
+  }
+  return r;
+}
+
+template <bool kSplit>
+hb_status launch_side(const SidePlan& plan, int64_t batch, const SideParams& p, bool* launched, cudaStream_t s) {
+  static std::atomic<int> held[64];
+  static std::atomic<int> widest[64];
+  auto kernel = small_side_kernel<kSplit>;
+  int most = 0;
+  if (const hb_status st = widest_cluster(kernel, kSideThreads, kSideSmem, held, widest, &most)) return st;
+  if (plan.ctas > most || batch * plan.ctas > 0x7FFFFFFF) return HB_OK;
   HB_CUDA_TRY(launch_clusters(kernel, static_cast<int>(batch), plan.ctas, kSideThreads, kSideSmem, s, p));
   *launched = true;
   return HB_OK;
@@ -437,6 +468,30 @@ extern "C" hb_status hb_orthogonalize(const void* update, int32_t type, int64_t 
   const int flip = rows > cols ? 1 : 0;
   const Source g{update, pitch, batch_stride, type, static_cast<int32_t>(rows), static_cast<int32_t>(cols)};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  {
+    static std::atomic<int> held[64], widest[64];
+    int most = 0;
+    if (const hb_status e = widest_cluster(gram_side_kernel, kGramThreads, kSideSmem, held, widest, &most)) return e;
+    const int64_t s = rows < cols ? rows : cols, l = rows < cols ? cols : rows;
+    const GramPlan plan = gram_plan(s, l, most);
+    if (plan.ctas && batch * plan.ctas <= 0x7FFFFFFF) {
+      GramParams p{};
+      p.g = g;
+      p.out = Out{out, out_pitch, out_batch_stride, type, 0};
+      p.s = static_cast<int32_t>(s);
+      p.l = static_cast<int32_t>(l);
+      p.s4 = static_cast<int32_t>(up(s, 4));
+      p.columns = plan.columns;
+      p.flip = flip;
+      p.steps = steps;
+      p.a = a;
+      p.b = b;
+      p.c = c;
+      p.eps = eps;
+      HB_CUDA_TRY(launch_clusters(gram_side_kernel, static_cast<int>(batch), plan.ctas, kGramThreads, plan.smem, st, p));
+      return HB_OK;
+    }
+  }
   if (const SidePlan plan = side_plan(rows, cols, split != 0); plan.ctas) {
     SideParams p{};
     p.g = g;

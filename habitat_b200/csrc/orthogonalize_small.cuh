@@ -71,8 +71,8 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ void st_cluster_u4(uint32_t addr, uint4 v) {
-  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+__device__ __forceinline__ void st_cluster_u2(uint32_t addr, uint32_t a, uint32_t b) {
+  asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(a), "r"(b) : "memory");
 }
 __device__ __forceinline__ void st_cluster_f64(uint32_t addr, double v) {
   asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory");
@@ -102,6 +102,35 @@ __device__ __forceinline__ uint4 halves(float (&v)[8]) {
   }
   r.x = w[0]; r.y = w[1]; r.z = w[2]; r.w = w[3];
   return r;
+}
+
+// A from the shares of all CTAs (added in the order of the ranks), as operands in every CTA's shared memory.  All loads of a
+// piece are on their way at once: one after the other they took 9 us a step with eight CTAs and 128 rows.
+template <bool kSplit, int kCtas>
+__device__ __forceinline__ void add_shares(uint32_t share, uint32_t operand, int block, int low, int R, int rank, int tid) {
+  const int per_row = R / 4, pieces = R * per_row;
+  for (int u = rank * kSideThreads + tid; u < pieces; u += kCtas * kSideThreads) {
+    const int r = u / per_row, c = (u - r * per_row) * 4;
+    const uint32_t at = share + (r * (R + 4) + c) * 4;
+    float4 x[kCtas];
+#pragma unroll
+    for (int i = 0; i < kCtas; ++i) x[i] = ld_cluster_f4(map_to_cta(at, static_cast<uint32_t>(i)));
+    float4 v = x[0];
+#pragma unroll
+    for (int i = 1; i < kCtas; ++i) {
+      v.x += x[i].x; v.y += x[i].y; v.z += x[i].z; v.w += x[i].w;
+    }
+    const uint32_t to = operand + (c >> 6) * block + block_at(r, c & 63);
+    const uint32_t h0 = pack_f16(v.x, v.y), h1 = pack_f16(v.z, v.w);
+    const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&h0)), f1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+    const uint32_t l0 = pack_f16(v.x - f0.x, v.y - f0.y), l1 = pack_f16(v.z - f1.x, v.w - f1.y);
+#pragma unroll
+    for (int i = 0; i < kCtas; ++i) {
+      const uint32_t there = map_to_cta(to, static_cast<uint32_t>(i));
+      st_cluster_u2(there, h0, h1);
+      if (kSplit) st_cluster_u2(there + low, l0, l1);
+    }
+  }
 }
 
 template <bool kSplit>
@@ -137,33 +166,38 @@ __global__ void __launch_bounds__(kSideThreads, 1) small_side_kernel(const __gri
   const int64_t g0 = matrix * p.g.batch_stride;
   const int c0 = rank * nb * kSideColumns;                              // this CTA's columns of X
   const int cols = min(max(p.l - c0, 0), nb * kSideColumns);
-  const int n_el = p.s * cols;
-  // walks the elements along G's rows: work(row of X, column of this CTA, value)
-  auto for_elements = [&](auto work) {
-    const int inner = p.flip ? p.s : cols;
-    if (inner >= 32) {
-      const int outer = p.flip ? cols : p.s;
-      for (int o = warp; o < outer; o += kSideThreads / 32) {
-        const int64_t row = g0 + static_cast<int64_t>(p.flip ? c0 + o : o) * p.g.ld + (p.flip ? 0 : c0);
-#pragma unroll 4
-        for (int i = lane; i < inner; i += 32) {
-          const float x = load_element(p.g.base, p.g.type, row + i);
-          if (p.flip) work(i, o, x);
-          else work(o, i, x);
-        }
-      }
+  // Eight columns of a row per thread: kept as they are in the 32 bytes that their high and low parts will take (16-bit
+  // updates without low parts: in 16 bytes, unrounded as they have 8 bits).
+  const int per_row = (cols + 7) / 8, units = p.s * per_row;
+  auto unit_at = [&](int u, int& r, int& c) {
+    if (p.flip) {
+      c = u / p.s;
+      r = u - c * p.s;
     } else {
-#pragma unroll 4
-      for (int e = tid; e < n_el; e += kSideThreads) {
-        const int o = e / inner, i = e - o * inner;
-        const float x = load_element(p.g.base, p.g.type, g0 + static_cast<int64_t>(p.flip ? c0 + o : o) * p.g.ld + (p.flip ? 0 : c0) + i);
-        if (p.flip) work(i, o, x);
-        else work(o, i, x);
-      }
+      r = u / per_row;
+      c = u - r * per_row;
     }
+    c *= 8;
+    return base + (c >> 6) * lay.block + block_at(r, c & 63);
   };
   double sum = 0.0;
-  for_elements([&](int, int, float x) { sum += static_cast<double>(x) * x; });
+  for (int u = tid; u < units; u += kSideThreads) {
+    int r, c;
+    uint8_t* at = unit_at(u, r, c);
+    const int64_t from = g0 + (p.flip ? static_cast<int64_t>(c0 + c) * p.g.ld + r : static_cast<int64_t>(r) * p.g.ld + c0 + c);
+    const int64_t step = p.flip ? p.g.ld : 1;
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? load_element(p.g.base, p.g.type, from + i * step) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += static_cast<double>(v[i]) * v[i];
+    if (kSplit) {
+      *reinterpret_cast<float4*>(at) = make_float4(v[0], v[1], v[2], v[3]);
+      *reinterpret_cast<float4*>(at + x_low) = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      *reinterpret_cast<uint4*>(at) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+    }
+  }
 #pragma unroll
   for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
   if (lane == 0) tail->warp_sums[warp] = sum;
@@ -184,13 +218,24 @@ __global__ void __launch_bounds__(kSideThreads, 1) small_side_kernel(const __gri
   const float factor = fine ? static_cast<float>(1.0 / ((norm + p.eps) * ldexp(1.0, e))) : __int_as_float(0x7FFFFFFF);
 
   // ---- X0 = G 2^e ----
-  for_elements([&](int r, int c, float x) {
-    const float v = x * power;
-    uint8_t* at = base + (c >> 6) * lay.block + block_at(r, c & 63);
-    const __half hi = __float2half_rn(v);
-    *reinterpret_cast<__half*>(at) = hi;
-    if (kSplit) *reinterpret_cast<__half*>(at + x_low) = __float2half_rn(v - __half2float(hi));
-  });
+  for (int u = tid; u < units; u += kSideThreads) {
+    int r, c;
+    uint8_t* at = unit_at(u, r, c);
+    float v[8];
+    if (kSplit) {
+      const float4 x = *reinterpret_cast<const float4*>(at), y = *reinterpret_cast<const float4*>(at + x_low);
+      v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
+    } else {
+      const uint4 x = *reinterpret_cast<const uint4*>(at);
+      const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(i & 1 ? xs[i >> 1] & 0xFFFF0000u : xs[i >> 1] << 16);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= power;
+    *reinterpret_cast<uint4*>(at) = halves(v);
+    if (kSplit) *reinterpret_cast<uint4*>(at + x_low) = halves(v);
+  }
   fence_proxy_async();
   tc_fence_before();
   __syncthreads();
@@ -264,29 +309,15 @@ __global__ void __launch_bounds__(kSideThreads, 1) small_side_kernel(const __gri
     }
     __syncwarp();
     cluster_sync_all();
-    // ---- A: pieces of eight columns, each added up by one thread of the cluster and handed to all CTAs ----
-    {
-      const int pieces = R * R / 8, per_row = R / 8;
-      for (int u = rank * kSideThreads + tid; u < pieces; u += ctas * kSideThreads) {
-        const int r = u / per_row, c = (u - r * per_row) * 8;
-        const uint32_t at = sb + lay.share + (r * (R + 4) + c) * 4;
-        float v[8] = {};
-        for (int i = 0; i < ctas; ++i) {
-          const uint32_t from = map_to_cta(at, static_cast<uint32_t>(i));
-          const float4 x = ld_cluster_f4(from), y = ld_cluster_f4(from + 16);
-          v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
-          v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
-        }
-        const uint32_t to = sb + lay.operand + (c >> 6) * lay.block + block_at(r, c & 63);
-        const uint4 hi = halves(v);
-        for (int i = 0; i < ctas; ++i) st_cluster_u4(map_to_cta(to, static_cast<uint32_t>(i)), hi);
-        if (kSplit) {
-          const uint4 lo = halves(v);
-          for (int i = 0; i < ctas; ++i) st_cluster_u4(map_to_cta(to + op_low, static_cast<uint32_t>(i)), lo);
-        }
-      }
-      asm volatile("fence.proxy.async;" ::: "memory");
+    // ---- A: pieces of four columns, each added up by one thread of the cluster and handed to all CTAs ----
+    switch (ctas) {
+      case 1: add_shares<kSplit, 1>(sb + lay.share, sb + lay.operand, lay.block, op_low, R, rank, tid); break;
+      case 2: add_shares<kSplit, 2>(sb + lay.share, sb + lay.operand, lay.block, op_low, R, rank, tid); break;
+      case 4: add_shares<kSplit, 4>(sb + lay.share, sb + lay.operand, lay.block, op_low, R, rank, tid); break;
+      case 8: add_shares<kSplit, 8>(sb + lay.share, sb + lay.operand, lay.block, op_low, R, rank, tid); break;
+      default: add_shares<kSplit, 16>(sb + lay.share, sb + lay.operand, lay.block, op_low, R, rank, tid); break;
     }
+    asm volatile("fence.proxy.async;" ::: "memory");
     __syncwarp();
     cluster_sync_all();
     // ---- B = a I + b A + c A^2, in A's place ----
@@ -411,6 +442,196 @@ __global__ void __launch_bounds__(kSideThreads, 1) small_side_kernel(const __gri
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
   }
+}
+
+// ---------------------------------------------------------------------------
+// Shorter side at most 32: everything but the two ends happens on s x s matrices.  All factors B are polynomials of the first
+// A = X0 X0^T and commute, so with P the product of the B so far, X = P X0 and the next A is A B^2.  X is read once,
+// multiplied to A0 (whose trace is the squared norm), and once more, from shared memory, to P X0.  What that costs is precision:
+// A has the squares of the singular values, and P amplifies small ones by up to a^steps; so it is done in float64 on the
+// ordinary cores (64 multiply-adds per cycle and SM: 32^3 of them take 512 cycles), and rounded once at the end.
+// 1024 x 12: 47 us as steps on the tensor cores (two cluster barriers and three dependent rounds of MMAs each).
+constexpr int kGramSide = 32;
+constexpr int kGramThreads = 256;
+
+struct GramParams {
+  Source g;
+  Out out;
+  int32_t s, l, s4, columns, flip, steps;   // s4: s rounded up to 4; columns: of X, per CTA
+  double a, b, c, eps;
+};
+
+constexpr int kGramMatrix = kGramSide * (kGramSide + 1);     // doubles
+constexpr int kGramFixed = (4 * kGramMatrix + kGramThreads * 16) * 8;
+inline int64_t gram_smem(int s4, int64_t columns) { return kGramFixed + columns * (s4 + 1) * 8; }
+
+__device__ __forceinline__ double2 ld_cluster_d2(uint32_t addr) {
+  double2 v;
+  asm volatile("ld.shared::cluster.v2.f64 {%0, %1}, [%2];" : "=d"(v.x), "=d"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+
+__global__ void __launch_bounds__(kGramThreads) gram_side_kernel(const __grid_constant__ GramParams p) {
+  extern __shared__ double smem_d[];
+  const int tid = static_cast<int>(threadIdx.x);
+  const int rank = static_cast<int>(cluster_ctarank()), ctas = static_cast<int>(cluster_size());
+  const int matrix = static_cast<int>(blockIdx.x) / ctas;
+  const int s = p.s, s4 = p.s4, pitch = s4 + 1;
+  constexpr int kPitch = kGramSide + 1;
+  double* part = smem_d;                               // sums of threads; [256][16]
+  double* share = part + kGramThreads * 16;            // this CTA's share of A, then A
+  double* mat[3] = {share + kGramMatrix, share + 2 * kGramMatrix, share + 3 * kGramMatrix};
+  double* x = share + 4 * kGramMatrix;                 // [column][pitch]
+  hb_grid_dependency_wait();
+
+  // ---- this CTA's columns of X ----
+  const int c0 = rank * p.columns, cols = min(max(p.l - c0, 0), p.columns);
+  const int64_t g0 = matrix * p.g.batch_stride;
+  if (p.flip) {
+    // rows of G are columns of X
+#pragma unroll 8
+    for (int e = tid; e < cols * s4; e += kGramThreads) {
+      const int c = e / s4, r = e - c * s4;
+      x[c * pitch + r] = r < s ? static_cast<double>(load_element(p.g.base, p.g.type, g0 + static_cast<int64_t>(c0 + c) * p.g.ld + r)) : 0.0;
+    }
+  } else {
+    const int lane = tid & 31, warp = tid >> 5;
+    for (int r = warp; r < s4; r += kGramThreads / 32)
+#pragma unroll 4
+      for (int c = lane; c < cols; c += 32)
+        x[c * pitch + r] = r < s ? static_cast<double>(load_element(p.g.base, p.g.type, g0 + static_cast<int64_t>(r) * p.g.ld + c0 + c)) : 0.0;
+  }
+  __syncthreads();
+
+  // ---- its share of A: 4 x 4 elements per thread and slice of the columns ----
+  const int side = s4 / 4, tiles = side * side, slices = kGramThreads / tiles;
+  {
+    double v[16] = {};
+    const int tile = tid % tiles, slice = tid / tiles;
+    if (slice < slices) {
+      const int i0 = tile / side * 4, j0 = tile % side * 4;
+#pragma unroll 2
+      for (int c = slice; c < cols; c += slices) {
+        const double* xc = x + c * pitch;
+        double xi[4], xj[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          xi[k] = xc[i0 + k];
+          xj[k] = xc[j0 + k];
+        }
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[k] = fma(xi[k >> 2], xj[k & 3], v[k]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 16; ++k) part[k * kGramThreads + tid] = v[k];
+  }
+  __syncthreads();
+  for (int e = tid; e < tiles * 16; e += kGramThreads) {
+    const int tile = e % tiles, k = e / tiles;
+    double sum = 0.0;
+    for (int i = 0; i < slices; ++i) sum += part[k * kGramThreads + i * tiles + tile];
+    share[(tile / side * 4 + (k >> 2)) * s4 + tile % side * 4 + (k & 3)] = sum;
+  }
+  cluster_sync_all();
+  // ---- A0: the shares of all CTAs, in the order of the ranks ----
+  double* A = mat[0];
+  for (int e = 2 * tid; e < s4 * s4; e += 2 * kGramThreads) {
+    const uint32_t at = smem_u32(share + e);
+    double2 sum = make_double2(0.0, 0.0);
+#pragma unroll 8
+    for (int i = 0; i < ctas; ++i) {
+      const double2 y = ld_cluster_d2(map_to_cta(at, static_cast<uint32_t>(i)));
+      sum.x += y.x;
+      sum.y += y.y;
+    }
+    const int r = e / s4, c = e - r * s4;
+    A[r * kPitch + c] = sum.x;
+    A[r * kPitch + c + 1] = sum.y;
+  }
+  __syncthreads();
+  double trace = 0.0;
+  for (int i = 0; i < s; ++i) trace += A[i * kPitch + i];
+  const double norm = sqrt(trace);
+  const double scale = norm < static_cast<double>(INFINITY) ? 1.0 / (norm + p.eps) : __longlong_as_double(0x7FFFFFFFFFFFFFFFll);
+  __syncthreads();
+  for (int e = tid; e < s4 * s4; e += kGramThreads) A[e / s4 * kPitch + e % s4] *= scale * scale;
+  __syncthreads();
+
+  // ---- P = the product of the steps' factors ----
+  // 2 x 2 elements per thread; out = f(A-like u times v) written through `put`
+  const int half = s4 / 2, r2 = tid / half * 2, c2 = tid % half * 2;
+  const bool mine = r2 < s4;
+  auto product = [&](const double* u, const double* v, double (&o)[4]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] = 0.0;
+    if (!mine) return;
+#pragma unroll 4
+    for (int k = 0; k < s4; ++k) {
+      const double u0 = u[r2 * kPitch + k], u1 = u[(r2 + 1) * kPitch + k], v0 = v[k * kPitch + c2], v1 = v[k * kPitch + c2 + 1];
+      o[0] = fma(u0, v0, o[0]);
+      o[1] = fma(u0, v1, o[1]);
+      o[2] = fma(u1, v0, o[2]);
+      o[3] = fma(u1, v1, o[3]);
+    }
+  };
+  auto put = [&](double* to, const double (&o)[4]) {
+    if (!mine) return;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) to[(r2 + (k >> 1)) * kPitch + c2 + (k & 1)] = o[k];
+  };
+  double *B = mat[1], *P = mat[2], *T = part;          // the threads' sums are used up
+  for (int step = 0; step < p.steps; ++step) {
+    double o[4], q[4];
+    product(A, A, o);
+    if (mine) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int r = r2 + (k >> 1), c = c2 + (k & 1);
+        o[k] = fma(p.c, o[k], fma(p.b, A[r * kPitch + c], r == c ? p.a : 0.0));
+      }
+    }
+    put(B, o);
+    if (step == 0) put(P, o);
+    __syncthreads();
+    const bool last = step == p.steps - 1;
+    if (step > 0) product(B, P, o);
+    if (!last) product(B, A, q);
+    __syncthreads();
+    if (step > 0) put(P, o);
+    if (!last) put(T, q);
+    __syncthreads();
+    if (!last) {
+      product(T, B, q);
+      put(A, q);
+      __syncthreads();
+    }
+  }
+
+  // ---- X = P X0 ----
+  const int64_t o0 = matrix * p.out.batch_stride;
+  auto store = [&](int r, int c, double v) {
+    const int64_t to = o0 + (p.flip ? static_cast<int64_t>(c0 + c) * p.out.ld + r : static_cast<int64_t>(r) * p.out.ld + c0 + c);
+    const float f = static_cast<float>(v * scale);
+    if (p.out.type == kF32) static_cast<float*>(p.out.base)[to] = f;
+    else if (p.out.type == kBF16) static_cast<__nv_bfloat16*>(p.out.base)[to] = __float2bfloat16_rn(f);
+    else static_cast<__half*>(p.out.base)[to] = __float2half_rn(f);
+  };
+  // four rows of a column per thread; neighbouring threads have neighbouring elements of the result's rows
+  for (int e = tid; e < side * cols; e += kGramThreads) {
+    const int c = p.flip ? e / side : e % cols, r = (p.flip ? e % side : e / cols) * 4;
+    double v[4] = {};
+#pragma unroll 4
+    for (int k = 0; k < s; ++k) {
+      const double y = x[c * pitch + k];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = fma(P[(r + i) * kPitch + k], y, v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (r + i < s) store(r + i, c, v[i]);
+  }
+  cluster_sync_all();       // no CTA leaves while another may still read its share
 }
 
 }  // namespace
