@@ -62,6 +62,7 @@ constexpr int smem_bytes() {
 struct Product {
   CUtensorMap a, b;        // [matrices][rows][K], boxes of 128 (a) and BN / 2 (b) rows x 128 bytes; b K-major or MN-major
   int32_t M, N, kblocks, segments, batches;
+  int32_t splits;          // of K: every tile is made that many times, with a share of the slots each
   int32_t tiles_m, tiles_n, num_tiles;   // num_tiles: over all batches
   int32_t lower;           // 1: D is symmetric, only tiles that reach its lower triangle are computed
   int32_t per_batch;       // tiles of a batch, and its and a tile group's reciprocal (set_tiles)
@@ -73,7 +74,7 @@ struct Product {
 constexpr int kTileGroup = 8;      // row blocks that tiles go through together
 
 struct Tile {
-  int batch, m0, n0;
+  int batch, m0, n0, split;
 };
 
 // n / d and, in n, the remainder, for 0 <= n < 2^31.  m is 2^32 / d rounded down (reciprocal_of): the estimate is at most two too
@@ -91,7 +92,7 @@ inline uint32_t reciprocal_of(int64_t d) { return d <= 1 ? 0xFFFFFFFFu : static_
 
 inline void set_tiles(Product* p, int64_t per_batch) {
   p->per_batch = static_cast<int32_t>(per_batch);
-  p->num_tiles = static_cast<int32_t>(per_batch * p->batches);
+  p->num_tiles = static_cast<int32_t>(per_batch * p->batches * p->splits);
   p->per_batch_inv = reciprocal_of(per_batch);
   p->per_group_inv = reciprocal_of(static_cast<int64_t>(kTileGroup) * p->tiles_n);
 }
@@ -102,6 +103,11 @@ template <int BN>
 __device__ __forceinline__ Tile tile_of(const Product& p, int t) {
   Tile r;
   r.batch = divide(t, p.per_batch, p.per_batch_inv);
+  r.split = 0;
+  if (p.splits > 1) {
+    r.split = r.batch % p.splits;
+    r.batch /= p.splits;
+  }
   int mt, nt;
   if (p.lower) {
     constexpr int kPer = kPairRows / BN;
@@ -276,7 +282,7 @@ struct EpiContext {
   int warp, lane, part;   // epilogue warp, its part of the columns
   int row;                // the warp's first row among the CTA's 128
   int row0, n0;           // its first row and the first column of its part, in the matrix
-  int batch;
+  int batch, t;           // and the tile's number
   uint32_t n_tile;        // how many tiles the CTA has drained before
   bool first, last;       // group of the tile
   uint32_t rank;          // in the cluster
@@ -372,15 +378,17 @@ gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ typename 
   const int workers = static_cast<int>(gridDim.x) / kCluster * (Epi::kClusterCtas ? 1 : kCluster / 2);
   const int worker = static_cast<int>(blockIdx.x) / (Epi::kClusterCtas ? kCluster : 2);
   auto locate = [&](int t) {
-    if (Epi::kClusterCtas) return Tile{0, t * kPairRows, static_cast<int>(pair) * BN};
+    if (Epi::kClusterCtas) return Tile{0, t * kPairRows, static_cast<int>(pair) * BN, 0};
     return tile_of<BN>(p, t);
   };
-  const int total_kb = p.kblocks * p.segments;
+  // slots of K of a share, and where it begins
+  const int most_kb = p.splits > 1 ? (p.kblocks + p.splits - 1) / p.splits : p.kblocks;
+  auto slots_of = [&](int split) { return p.splits > 1 ? max(0, min(most_kb, p.kblocks - split * most_kb)) : most_kb; };
   // end of the group of K slots that begins at kb
-  auto group_end = [&](int kb) {
-    if (!Epi::kGrouped) return total_kb;
-    const int small = p.kblocks * (p.segments - 1);
-    return kb < small ? small : min(kb + p.group, total_kb);
+  auto group_end = [&](int kb, int slots) {
+    if (!Epi::kGrouped) return slots * p.segments;
+    const int small = slots * (p.segments - 1);
+    return kb < small ? small : min(kb + p.group, slots * p.segments);
   };
 
   if (warp == 0) {
@@ -393,7 +401,8 @@ gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ typename 
         const Tile tile = locate(t);
         for (int seg = 0; seg < p.segments && ok; ++seg) {
           const int za = tile.batch + (seg == 1 ? p.batches : 0), zb = tile.batch + (p.segments > 1 && seg == 0 ? p.batches : 0);
-          for (int kb = 0; kb < p.kblocks; ++kb) {
+          const int kb0 = tile.split * most_kb, kb1 = kb0 + slots_of(tile.split);
+          for (int kb = kb0; kb < kb1; ++kb) {
             ok = mbar_wait(empty + 8 * s, ph, abort_flag, p.status, 0x511);
             if (!ok) break;
             const uint32_t bar = map_to_cta(full + 8 * s, leader);
@@ -432,8 +441,9 @@ gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ typename 
       uint32_t s = 0, ph = 0, n = 0;
       bool ok = true;
       for (int t = worker; t < p.num_tiles && ok; t += workers) {
+        const int slots = slots_of(p.splits > 1 ? locate(t).split : 0), total_kb = slots * p.segments;
         for (int kb0 = 0, kb1; kb0 < total_kb && ok; kb0 = kb1, ++n) {
-          kb1 = group_end(kb0);
+          kb1 = group_end(kb0, slots);
           const uint32_t st = n % S::kAccs, turn = n / S::kAccs & 1u;
           ok = mbar_wait(acc_empty + 8 * st, turn ^ 1u, abort_flag, p.status, 0x521);
           tc_fence_after();
@@ -482,8 +492,10 @@ gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ typename 
       c.batch = tile.batch;
       look_ahead(t + workers);
       Epi::template begin<BN>(c);
+      c.t = t;
+      const int slots = slots_of(tile.split), total_kb = slots * p.segments;
       for (int kb0 = 0, kb1; kb0 < total_kb && ok; kb0 = kb1, ++n) {
-        kb1 = group_end(kb0);
+        kb1 = group_end(kb0, slots);
         const uint32_t st = n % S::kAccs, turn = n / S::kAccs & 1u;
         c.tmem = tmem + (static_cast<uint32_t>(quad * 32) << 16) + st * BN + static_cast<uint32_t>(c.part * S::kCols);
         c.first = kb0 == 0;

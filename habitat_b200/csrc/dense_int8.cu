@@ -178,40 +178,35 @@ cudaError_t launch_quantize(const void* x, int64_t rows, int64_t cols, int64_t p
                                q_pitch, scales);
 }
 
-// Rows of bytes that start anywhere -> rows that start on 16 bytes (TMA reads nothing else).
-__global__ void __launch_bounds__(256) align_rows_kernel(const int8_t* __restrict__ x, int64_t cols, int64_t pitch, int8_t* __restrict__ out,
-                                                         int64_t out_pitch) {
-  hb_grid_dependency_wait();
-  const int8_t* xr = x + static_cast<int64_t>(blockIdx.x) * pitch;
-  uint32_t* o = reinterpret_cast<uint32_t*>(out + static_cast<int64_t>(blockIdx.x) * out_pitch);
-  const uintptr_t start = reinterpret_cast<uintptr_t>(xr);
-  const uint32_t shift = static_cast<uint32_t>(start & 3u) * 8u;
-  const uint32_t* xw = reinterpret_cast<const uint32_t*>(start & ~static_cast<uintptr_t>(3));
-  for (int64_t i = threadIdx.x; 4 * i < cols; i += blockDim.x) {
-    // whole words inside the row are loaded as such; its last bytes one by one
-    uint32_t w = 0;
-    if (4 * i + 8 <= cols) {
-      w = shift ? __funnelshift_r(xw[i], xw[i + 1], shift) : xw[i];
-      if (i == 0 && shift) {
-        w = 0;
-        for (int j = 0; j < 4; ++j) w |= static_cast<uint32_t>(static_cast<uint8_t>(xr[j])) << (8 * j);
-      }
-    } else {
-      for (int j = 0; j < 4 && 4 * i + j < cols; ++j) w |= static_cast<uint32_t>(static_cast<uint8_t>(xr[4 * i + j])) << (8 * j);
-    }
-    o[i] = w;
-  }
-}
-
-// ---------------------------------------------------------------------------
-// Epilogues
-// ---------------------------------------------------------------------------
 struct LayerScales {
   const float* row;
   const float* channel;
   const float* bias;     // or null
   float floor;           // 0 with ReLU, else -infinity: the larger of a value and it
 };
+
+}  // namespace
+}  // namespace dense
+
+#include "dense_few.cuh"
+
+namespace dense {
+namespace {
+
+// Rows of bytes that start anywhere -> rows that start on 16 bytes (TMA reads nothing else), 16 bytes per thread; see load_piece.
+__global__ void __launch_bounds__(256) align_rows_kernel(const int8_t* __restrict__ x, int rows, int K, int64_t pitch, int8_t* __restrict__ out,
+                                                         int pieces) {
+  hb_grid_dependency_wait();
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= static_cast<int64_t>(rows) * pieces) return;
+  const int64_t r = i / pieces;
+  const int k = static_cast<int>(i - r * pieces) * 16;
+  reinterpret_cast<uint4*>(out)[i] = load_piece<false>(x + r * pitch, k, K);
+}
+
+// ---------------------------------------------------------------------------
+// Epilogues
+// ---------------------------------------------------------------------------
 
 // Accumulators are read as 16 x 256-bit fragments: of 16 rows lane l gets rows l / 4 and l / 4 + 8, and of every eight
 // columns 2 (l mod 4) and the next.  A lane then has 4 rows and a quarter of its warp's columns; with whole rows per lane
@@ -537,6 +532,10 @@ hb_status check_product(const char* name, const int8_t* q, int64_t q_pitch, cons
 
 int64_t align_bytes(int64_t rows, int64_t K, bool aligned) { return aligned ? 0 : round_up(rows * round_up(K, 16), 256); }
 
+// Quantised results that take two launches: rows wider than a cluster of eight holds, and few rows with so many columns that
+// eight SMs cannot read the weights in the time (1 x 1024 x 8192: 20 us in one launch, 7 in two).
+bool through_memory(int64_t M, int64_t N, int64_t K) { return N > 1024 || (M <= kFewRows && K > 2048); }
+
 // Operands that TMA can read: as they are, or copied to the workspace.
 hb_status align_operands(const char* name, Operands* o, int64_t M, int64_t N, int64_t K, uint8_t* workspace, int64_t workspace_bytes,
                          int64_t more, cudaStream_t s) {
@@ -548,8 +547,13 @@ hb_status align_operands(const char* name, Operands* o, int64_t M, int64_t N, in
   }
   const int64_t pitch = round_up(K, 16);
   auto copy = [&](const int8_t** x, int64_t* x_pitch, int64_t rows) -> hb_status {
-    HB_CUDA_TRY(hb::launch_overlapped(align_rows_kernel, dim3(static_cast<unsigned>(rows)), dim3(K > 512 ? 256 : 64), 0, s, *x, K, *x_pitch,
-                                      reinterpret_cast<int8_t*>(workspace), pitch));
+    const int64_t pieces = pitch / 16, blocks = (rows * pieces + 255) / 256;
+    if (blocks > 0x7FFFFFFF) {
+      hb::set_error("%s: too large to be copied to aligned rows", name);
+      return HB_ERR_TOO_LARGE;
+    }
+    HB_CUDA_TRY(hb::launch_overlapped(align_rows_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, *x, static_cast<int>(rows),
+                                      static_cast<int>(K), *x_pitch, reinterpret_cast<int8_t*>(workspace), static_cast<int>(pieces)));
     *x = reinterpret_cast<const int8_t*>(workspace);
     *x_pitch = pitch;
     workspace += align_bytes(rows, K, false);
@@ -557,7 +561,7 @@ hb_status align_operands(const char* name, Operands* o, int64_t M, int64_t N, in
   };
   if (!q_ok)
     if (const hb_status st = copy(&o->q, &o->q_pitch, M)) return st;
-  if (!w_ok)
+  if (!w_ok && M > kFewRows)       // few rows' kernel reads them as they are
     if (const hb_status st = copy(&o->w, &o->w_pitch, N)) return st;
   return HB_OK;
 }
@@ -570,6 +574,7 @@ hb_status describe(Product* p, const Operands& o, int64_t M, int64_t N, int64_t 
   p->kblocks = static_cast<int32_t>((K + kSlotK - 1) / kSlotK);
   p->segments = 1;
   p->batches = 1;
+  p->splits = 1;
   p->tiles_m = static_cast<int32_t>((M + kPairRows - 1) / kPairRows);
   p->tiles_n = static_cast<int32_t>((N + bn - 1) / bn);
   p->lower = 0;
@@ -735,7 +740,7 @@ extern "C" int64_t hb_int8_workspace_bytes(const int8_t* q, int64_t q_pitch, con
                                            int64_t K, int32_t quantized) {
   if (M < 0 || N < 0 || K < 1) return -1;
   int64_t bytes = dense::align_bytes(M, K, dense::tma_rows(q, q_pitch)) + dense::align_bytes(N, K, dense::tma_rows(w, w_pitch));
-  if (quantized && N > 1024) bytes += dense::round_up(M * dense::round_up(N, 4) * 4, 256);
+  if (quantized && dense::through_memory(M, N, K)) bytes += dense::round_up(M * dense::round_up(N, 4) * 4, 256);
   return bytes;
 }
 
@@ -757,6 +762,11 @@ extern "C" hb_status hb_int8_matmul(const int8_t* q, int64_t q_pitch, const floa
   if (const hb_status st = align_operands(name, &o, M, N, K, static_cast<uint8_t*>(workspace), workspace_bytes, 0, s)) return st;
   FloatOut::Params ep{{q_scales, w_scales, bias, relu ? 0.0f : -INFINITY}, {out, out_pitch, 0, out_type, 0}};
   ep.out.vec = row_alignment(out, out_pitch, 0, out_type == HB_F32 ? 4 : 2);
+  if (M <= kFewRows) {
+    FewParams few{o.q, o.w, o.q_pitch, o.w_pitch, ep.s, static_cast<int32_t>(M), static_cast<int32_t>(N), static_cast<int32_t>(K), ep.out, nullptr, 0,
+                  nullptr, status};
+    return launch_few(few, s);
+  }
   int sms = 0;
   if (const hb_status st = sm_count(&sms)) return st;
   switch (tile_columns({256, 128, 64}, sms / 2, [&](int bn) { return ((M + kPairRows - 1) / kPairRows) * ((N + bn - 1) / bn); })) {
@@ -783,8 +793,7 @@ extern "C" hb_status hb_int8_matmul_quantized(const int8_t* q, int64_t q_pitch, 
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   Operands o{q, q_pitch, w, w_pitch};
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  if (N > 1024) {
-    // wider rows than a cluster of eight holds: through memory, in float32
+  if (through_memory(M, N, K)) {
     const int64_t pitch = round_up(N, 4), bytes = round_up(M * pitch * 4, 256);
     const int64_t before = align_bytes(M, K, tma_rows(q, q_pitch)) + align_bytes(N, K, tma_rows(w, w_pitch));
     if (!ws || workspace_bytes < before + bytes || reinterpret_cast<uintptr_t>(ws) % 256) {
@@ -798,6 +807,11 @@ extern "C" hb_status hb_int8_matmul_quantized(const int8_t* q, int64_t q_pitch, 
   }
   if (const hb_status st = align_operands(name, &o, M, N, K, ws, workspace_bytes, 0, s)) return st;
   const LayerScales scales{q_scales, w_scales, bias, relu ? 0.0f : -INFINITY};
+  if (M <= kFewRows) {
+    FewParams few{o.q, o.w, o.q_pitch, o.w_pitch, scales, static_cast<int32_t>(M), static_cast<int32_t>(N), static_cast<int32_t>(K), Out{}, out,
+                  out_pitch, out_scales, status};
+    return launch_few(few, s);
+  }
   switch ((N + 255) / 256) {
     case 1: return launch_quant<2>(o, M, N, K, {scales, out, out_pitch, out_scales}, status, s);
     case 2: return launch_quant<4>(o, M, N, K, {scales, out, out_pitch, out_scales}, status, s);

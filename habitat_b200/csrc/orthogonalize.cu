@@ -170,18 +170,103 @@ __device__ __forceinline__ void add_halves(float (&v)[32], const __half* at, flo
   }
 }
 
+// What a symmetric product becomes: A = X X^T, or B = a I + b A + c A^2.
+struct Symmetric {
+  Planes out;
+  Planes a;               // of B: A; else hi is null
+  const float* factor;    // of the first A: X = X0 * factor; else null
+  float scale;            // of the accumulators
+  float on_a, on_diagonal;
+};
+__device__ __forceinline__ float symmetric_scale(const Symmetric& e, int batch) {
+  float scale = e.scale;
+  if (e.factor) {
+    const float f = __ldg(e.factor + batch);
+    scale *= f;
+    scale *= f;
+  }
+  return scale;
+}
+
+// Symmetric products with few tiles and a long K are split along it; the shares go to memory as they are, tile by tile, and
+// symmetric_sum_kernel adds them.
+struct ShareOut {
+  static constexpr bool kInt8 = false, kMnMajorB = false, kGrouped = true;
+  static constexpr int kClusterCtas = 0;
+  struct Params {
+    float* shares;          // [tile and split][256][BN]
+  };
+  template <int BN>
+  static __device__ __forceinline__ void fetch(const Params&, const Product&, const EpiContext&, int, int) {}
+  template <int BN>
+  static __device__ __forceinline__ void begin(const EpiContext&) {}
+  template <int BN, class Release>
+  static __device__ __forceinline__ void drain(const Params& ep, const Product&, const EpiContext& c, float (&sums)[Shape<BN>::kCols], Release release) {
+    for_chunks<BN, true>(c, sums, release, [&](int, float (&v)[32]) {
+      const Out out{ep.shares + static_cast<int64_t>(c.t) * kPairRows * BN, BN, 0, kF32, 16};
+      store_rows(out, 0, kPairRows, BN, static_cast<int>(c.rank & 1u) * kCtaRows + c.row, c.part * Shape<BN>::kCols, v,
+                 c.tail->staging + c.warp * kStageOutBytes, c.lane);
+    });
+  }
+};
+
+template <int BN>
+__global__ void __launch_bounds__(256) symmetric_sum_kernel(const __grid_constant__ Product p, const __grid_constant__ Symmetric e, const float* shares) {
+  __shared__ float turned[32][33];
+  hb_grid_dependency_wait();
+  constexpr int kAcross = BN / 32, kPieces = kPairRows / 32 * kAcross;
+  const int t = static_cast<int>(blockIdx.x) / kPieces, piece = static_cast<int>(blockIdx.x) % kPieces;
+  // tile t of all batches, as with one split
+  Product one = p;
+  one.splits = 1;
+  const Tile tile = tile_of<BN>(one, t);
+  const int row0 = tile.m0 + piece / kAcross * 32, n0 = tile.n0 + piece % kAcross * 32;
+  if (n0 > row0 || row0 >= p.M) return;
+  const int tx = static_cast<int>(threadIdx.x) & 31, ty = static_cast<int>(threadIdx.x) >> 5;
+  const int in_batch = t - tile.batch * p.per_batch;
+  const float scale = symmetric_scale(e, tile.batch);
+  __half* out = e.out.hi + tile.batch * e.out.batch_stride;
+#pragma unroll
+  for (int i = 0; i < 32; i += 8) {
+    const int r = row0 + ty + i, c = n0 + tx;
+    float v = 0.0f;
+    for (int k = 0; k < p.splits; ++k)
+      v += shares[(static_cast<int64_t>(tile.batch * p.splits + k) * p.per_batch + in_batch) * kPairRows * BN + (piece / kAcross * 32 + ty + i) * BN +
+                  piece % kAcross * 32 + tx];
+    v *= scale;
+    if (r < p.M && c <= r) {
+      if (e.a.hi) {
+        const __half* at = e.a.hi + tile.batch * e.a.batch_stride + static_cast<int64_t>(r) * e.a.ld + c;
+        v = fmaf(e.on_a, __half2float(*at), v);
+        if (e.a.low) v = fmaf(e.on_a, __half2float(at[e.a.low]), v);
+        if (r == c) v += e.on_diagonal;
+      }
+      const __half hi = __float2half_rn(v);
+      __half* to = out + static_cast<int64_t>(r) * e.out.ld + c;
+      *to = hi;
+      if (e.out.low) to[e.out.low] = __float2half_rn(v - __half2float(hi));
+    }
+    turned[ty + i][tx] = v;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 32; i += 8) {
+    const int c = n0 + ty + i, r = row0 + tx;
+    if (r >= p.M || c >= r) continue;
+    const float v = turned[tx][ty + i];
+    const __half hi = __float2half_rn(v);
+    __half* to = out + static_cast<int64_t>(c) * e.out.ld + r;
+    *to = hi;
+    if (e.out.low) to[e.out.low] = __float2half_rn(v - __half2float(hi));
+  }
+}
+
 // Symmetric results: A = X X^T, or B = a I + b A + c A^2, as half-precision operands (kSplit: high and low parts).
 template <bool kSplit>
 struct SymmetricOut {
   static constexpr bool kInt8 = false, kMnMajorB = false, kGrouped = kSplit;
   static constexpr int kClusterCtas = 0;
-  struct Params {
-    Planes out;
-    Planes a;               // of B: A; else hi is null
-    const float* factor;    // of the first A: X = X0 * factor; else null
-    float scale;            // of the accumulators
-    float on_a, on_diagonal;
-  };
+  using Params = Symmetric;
   template <int BN>
   static __device__ __forceinline__ void fetch(const Params&, const Product&, const EpiContext&, int, int) {}
   template <int BN>
@@ -189,12 +274,7 @@ struct SymmetricOut {
   template <int BN, class Release>
   static __device__ __forceinline__ void drain(const Params& ep, const Product& p, const EpiContext& c, float (&sums)[kGrouped ? Shape<BN>::kCols : 1], Release release) {
     const int row0 = c.row0, row = row0 + c.lane;
-    float scale = ep.scale;
-    if (ep.factor) {
-      const float f = __ldg(ep.factor + c.batch);
-      scale *= f;
-      scale *= f;
-    }
+    const float scale = symmetric_scale(ep, c.batch);
     for_chunks<BN, kSplit>(c, sums, release, [&](int chunk, float (&v)[32]) {
       const int n0 = c.n0 + chunk * 32;
       if (n0 > row0 || row0 >= p.M) return;      // above the diagonal (both are multiples of 32), or below the matrix
@@ -292,9 +372,20 @@ struct UpdateOut {
 // ---------------------------------------------------------------------------
 int64_t up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
+// Tiles of a symmetric product whose columns begin before their rows end.
+int64_t lower_tiles(int64_t s, int bn) {
+  const int64_t tm = (s + kPairRows - 1) / kPairRows, tn = (s + bn - 1) / bn, per = kPairRows / bn;
+  int64_t n = 0;
+  for (int64_t i = 0; i < tm; ++i) n += (i + 1) * per < tn ? (i + 1) * per : tn;
+  return n;
+}
+
+constexpr int kMostPairs = 128;
+
 struct Layout {
   int64_t s, l, sp, lp;           // sides, and the pitches of rows of them
   int64_t x_bytes, a_bytes;       // one buffer of X, of A or B (all batches and planes)
+  int64_t shares;                 // of products that are split along K
   int64_t total;
 };
 Layout layout_of(int64_t batch, int64_t rows, int64_t cols, bool split) {
@@ -306,20 +397,14 @@ Layout layout_of(int64_t batch, int64_t rows, int64_t cols, bool split) {
   const int64_t planes = split ? 2 : 1;
   r.x_bytes = up(batch * planes * r.s * r.lp * 2, 256);
   r.a_bytes = up(batch * planes * r.s * r.sp * 2, 256);
-  r.total = 2 * r.x_bytes + 2 * r.a_bytes + up(batch * 4, 256) + up(batch * kMostPartials * 8, 256);
+  // splits never make more tiles than there are SM pairs, of which a GPU has at most 128
+  r.shares = lower_tiles(r.s, 128) * batch <= kMostPairs / 2 ? static_cast<int64_t>(kMostPairs) * kPairRows * 128 * 4 : 0;
+  r.total = 2 * r.x_bytes + 2 * r.a_bytes + up(batch * 4, 256) + up(batch * kMostPartials * 8, 256) + r.shares;
   return r;
 }
 
-// Tiles of a symmetric product whose columns begin before their rows end.
-int64_t lower_tiles(int64_t s, int bn) {
-  const int64_t tm = (s + kPairRows - 1) / kPairRows, tn = (s + bn - 1) / bn, per = kPairRows / bn;
-  int64_t n = 0;
-  for (int64_t i = 0; i < tm; ++i) n += (i + 1) * per < tn ? (i + 1) * per : tn;
-  return n;
-}
-
 template <int BN, class Epi>
-hb_status launch(Product p, const typename Epi::Params& ep, cudaStream_t s) {
+hb_status launch(Product p, const typename Epi::Params& ep, cudaStream_t s, Product* as_launched = nullptr) {
   p.group = kGroup;
   static std::atomic<int> held[64];
   int pairs = 0;
@@ -328,14 +413,27 @@ hb_status launch(Product p, const typename Epi::Params& ep, cudaStream_t s) {
   p.tiles_m = static_cast<int32_t>((p.M + kPairRows - 1) / kPairRows);
   p.tiles_n = static_cast<int32_t>((p.N + BN - 1) / BN);
   const int64_t tiles = p.lower ? lower_tiles(p.M, BN) : static_cast<int64_t>(p.tiles_m) * p.tiles_n;
-  if (tiles * p.batches * kTileGroup > 0x7FFFFFFF) {
+  if (tiles * p.batches * p.splits * kTileGroup > 0x7FFFFFFF) {
     hb::set_error("hb_orthogonalize: too large for one launch");
     return HB_ERR_TOO_LARGE;
   }
   set_tiles(&p, tiles);
   const int clusters = p.num_tiles < pairs ? p.num_tiles : pairs;
   HB_CUDA_TRY(launch_clusters(kernel, clusters, 2, Shape<BN>::kThreads, smem_bytes<BN>(), s, p, ep));
+  if (as_launched) *as_launched = p;
   return HB_OK;
+}
+
+// How many ways K of a symmetric product is split: as many as there are SM pairs for the tiles, of at least four slots; one
+// unless that saves 24 slots' time (about 3 us, what the second launch takes).
+int splits_of(int64_t batch, int64_t s, int64_t K, bool split, int pairs) {
+  const int64_t tiles = batch * lower_tiles(s, 128), slots = (K + 63) / 64;
+  int64_t n = pairs / tiles;
+  if (n > slots / 4) n = slots / 4;
+  if (n < 2) return 1;
+  const int64_t each = (slots + n - 1) / n;
+  if ((slots - each) * (split ? 3 : 1) < 24) return 1;
+  return static_cast<int>((slots + each - 1) / each);      // none without slots
 }
 
 // The cluster that holds a matrix whose shorter side is at most 128: its CTAs, and blocks of 64 columns per CTA; 0 when it
@@ -436,13 +534,22 @@ extern "C" hb_status hb_orthogonalize(const void* update, int32_t type, int64_t 
   // step before can leave; and the largest of B.  Stored operands are scaled by 2^8 and end at 65,504; A has the squares.
   double most = 1.0, most_b = 0.0;
   for (int i = 0; i < steps && most <= 12.0 && most_b <= 250.0; ++i) {
+    const double top = most * most;
     double next = 0.0;
-    for (int k = 0; k <= 4096; ++k) {
-      const double x = most * k / 4096, y = std::fabs(a + x * x * (b + c * x * x));
-      if (!(y <= 1e9)) most_b = 1e9;
-      if (y > most_b) most_b = y;
-      if (x * y > next) next = x * y;
-    }
+    auto look = [&](double t) {          // t = x^2
+      if (!(t >= 0.0 && t <= top)) return;
+      const double y = std::fabs(a + t * (b + c * t)), x = std::sqrt(t);
+      most_b = y <= 1e9 ? std::fmax(most_b, y) : 1e9;
+      next = std::fmax(next, x * y);
+    };
+    // the ends, the factor's extremum, and those of x times it: a + 3 b t + 5 c t^2 = 0
+    look(0.0);
+    look(top);
+    look(-b / (2.0 * c));
+    const double root = std::sqrt(9.0 * b * b - 20.0 * a * c);
+    look((-3.0 * b + root) / (10.0 * c));
+    look((-3.0 * b - root) / (10.0 * c));
+    look(-a / (3.0 * b));
     most = next * 1.001;
   }
   if (!(most <= 12.0) || !(most_b <= 250.0)) {
@@ -517,6 +624,7 @@ extern "C" hb_status hb_orthogonalize(const void* update, int32_t type, int64_t 
   __half* B = reinterpret_cast<__half*>(ws + 2 * lay.x_bytes + lay.a_bytes);
   float* factor = reinterpret_cast<float*>(ws + 2 * lay.x_bytes + 2 * lay.a_bytes);
   double* partials = reinterpret_cast<double*>(reinterpret_cast<uint8_t*>(factor) + up(batch * 4, 256));
+  float* shares = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(partials) + up(batch * kMostPartials * 8, 256));
   const int64_t planes = split ? 2 : 1;
   const int64_t x_matrix = lay.s * lay.lp, a_matrix = lay.s * lay.sp;
   auto x_planes = [&](int i) { return Planes{x[i], lay.lp, x_matrix, split ? batch * x_matrix : 0}; };
@@ -536,7 +644,7 @@ extern "C" hb_status hb_orthogonalize(const void* update, int32_t type, int64_t 
 
   int sms = 0;
   if (const hb_status e = sm_count(&sms)) return e;
-  const int pairs = sms / 2;
+  const int pairs = sms / 2 < kMostPairs ? sms / 2 : kMostPairs;
   auto sym_tiles = [&](int bn) { return batch * lower_tiles(lay.s, bn); };
   auto upd_tiles = [&](int bn) { return batch * ((lay.s + kPairRows - 1) / kPairRows) * ((lay.l + bn - 1) / bn); };
   // groups' sums are kept for 32 columns per epilogue lane, which is 128 for the tile
@@ -545,11 +653,11 @@ extern "C" hb_status hb_orthogonalize(const void* update, int32_t type, int64_t 
   CUtensorMap x_rows[2], x_cols[2], x_k[2], a_rows, a_cols, b_rows;
   for (int i = 0; i < (steps > 1 ? 2 : 1); ++i) {
     HB_CUDA_TRY(encode_planes(&x_rows[i], x[i], 2, lay.l, lay.s, batch * planes, lay.lp, x_matrix, kCtaRows));
-    HB_CUDA_TRY(encode_planes(&x_cols[i], x[i], 2, lay.l, lay.s, batch * planes, lay.lp, x_matrix, bn_sym / 2));
+    HB_CUDA_TRY(encode_planes(&x_cols[i], x[i], 2, lay.l, lay.s, batch * planes, lay.lp, x_matrix, (splits_of(batch, lay.s, lay.l, split != 0, pairs) > 1 ? 128 : bn_sym) / 2));
     HB_CUDA_TRY(encode_planes(&x_k[i], x[i], 2, lay.l, lay.s, batch * planes, lay.lp, x_matrix, 64));
   }
   HB_CUDA_TRY(encode_planes(&a_rows, A, 2, lay.s, lay.s, batch * planes, lay.sp, a_matrix, kCtaRows));
-  HB_CUDA_TRY(encode_planes(&a_cols, A, 2, lay.s, lay.s, batch * planes, lay.sp, a_matrix, bn_sym / 2));
+  HB_CUDA_TRY(encode_planes(&a_cols, A, 2, lay.s, lay.s, batch * planes, lay.sp, a_matrix, (splits_of(batch, lay.s, lay.s, split != 0, pairs) > 1 ? 128 : bn_sym) / 2));
   HB_CUDA_TRY(encode_planes(&b_rows, B, 2, lay.s, lay.s, batch * planes, lay.sp, a_matrix, kCtaRows));
 
   const int32_t out_vec = row_alignment(out, out_pitch, batch > 1 ? out_batch_stride : 0, type == HB_F32 ? 4 : 2);
@@ -566,12 +674,20 @@ extern "C" hb_status hb_orthogonalize(const void* update, int32_t type, int64_t 
       p.kblocks = static_cast<int32_t>((K + 63) / 64);
       p.segments = kSplit ? 3 : 1;
       p.batches = static_cast<int32_t>(batch);
+      p.splits = 1;
       p.status = status;
       return p;
     };
-    auto symmetric = [&](const CUtensorMap& ma, const CUtensorMap& mb, int64_t K, const typename Sym::Params& ep) {
+    auto symmetric = [&](const CUtensorMap& ma, const CUtensorMap& mb, int64_t K, const typename Sym::Params& ep) -> hb_status {
       Product p = product(ma, mb, lay.s, K);
       p.lower = 1;
+      p.splits = splits_of(batch, lay.s, K, kSplit, pairs);
+      if (p.splits > 1) {
+        if (const hb_status e = launch<128, ShareOut>(p, {shares}, st, &p)) return e;
+        HB_CUDA_TRY(hb::launch_overlapped(symmetric_sum_kernel<128>, dim3(static_cast<unsigned>(p.num_tiles / p.splits * (kPairRows / 32) * 4)), dim3(256), 0,
+                                          st, p, ep, static_cast<const float*>(shares)));
+        return HB_OK;
+      }
       if constexpr (!kSplit)
         if (bn_sym == 256) return launch<256, Sym>(p, ep, st);
       return bn_sym == 128 ? launch<128, Sym>(p, ep, st) : launch<64, Sym>(p, ep, st);
