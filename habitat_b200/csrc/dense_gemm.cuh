@@ -25,11 +25,10 @@ constexpr int kStageOutBytes = 32 * 64;    // an epilogue warp's staging: 32 row
 
 enum OutType : int32_t { kF32 = 0, kBF16 = 1, kF16 = 2 };
 
+// What goes by the tile's width alone.
 template <int BN>
 struct Shape {
   static constexpr int kBRows = BN / 2;                               // rows of B (columns of D) per CTA
-  static constexpr int kSlotBytes = (kCtaRows + kBRows) * kSlotK;     // per CTA
-  static constexpr int kSlots = BN == 256 ? 5 : BN == 128 ? 6 : 8;
   static constexpr int kAccs = BN == 256 ? 2 : 4;                     // accumulators
   static constexpr int kTmemCols = kAccs * BN;
   // Epilogue warps: what they do per tile is a chain of loads and conversions that two warps per scheduler cannot fill (28 %
@@ -40,34 +39,39 @@ struct Shape {
   static constexpr int kCols = BN / kParts;          // a warp's: 64, 32, 32
 };
 
-// Shared memory behind the ring: staging, channel scales and biases, row maxima of other CTAs, barriers.
+// Shared memory behind the ring: staging, barriers; 8-bit layers: scales and row maxima of the cluster's CTAs.
 struct Tail {
   uint8_t staging[kMostEpiWarps * kStageOutBytes];
-  float scales[kMostEpiWarps][160];        // an epilogue warp's: 64 channel scales, 64 biases, 32 row scales
-  float row_max[2][4][4][kCtaRows];
   uint64_t full[8], empty[8], acc_full[4], acc_empty[4], exchange[2], drain;
   uint32_t tmem;
   int abort;
 };
+struct LayerTail {
+  float scales[kMostEpiWarps][160];        // an epilogue warp's: 64 channel scales, 64 biases, 32 row scales
+  float row_max[2][4][4][kCtaRows];
+};
 
-template <int BN>
-constexpr int smem_bytes() {
-  constexpr int bytes = Shape<BN>::kSlots * Shape<BN>::kSlotBytes + static_cast<int>(sizeof(Tail)) + 1024;
-  static_assert(bytes <= 232448, "more than a block may have");
-  return bytes;
-}
+// The ring.  kSplit: a slot has the high and the low parts of both operands.
+template <int BN, class Epi>
+struct Ring {
+  static constexpr int kOperands = (kCtaRows + Shape<BN>::kBRows) * kSlotK;     // per CTA
+  static constexpr int kSlotBytes = kOperands * (Epi::kSplit ? 2 : 1);
+  static constexpr int kSlots = Epi::kSplit ? (BN == 256 ? 3 : 4) : Epi::kInt8 ? (BN == 256 ? 5 : BN == 128 ? 6 : 8) : BN == 256 ? 6 : 8;
+  static constexpr int kSmem = kSlots * kSlotBytes + static_cast<int>(sizeof(Tail)) + (Epi::kInt8 ? static_cast<int>(sizeof(LayerTail)) : 0) + 1024;
+  static_assert(kSmem <= 232448, "more than a block may have");
+};
 
-// What a launch multiplies: `batches` products of M x N with kblocks slots of K each.  With `segments` 3 the operands are
-// pairs of planes, high and low parts (the low ones lie `batches` matrices behind), and the sum is hi lo + lo hi + hi hi.
+// What a launch multiplies: `batches` products of M x N with kblocks slots of K each.  With Epi::kSplit the operands are pairs of
+// planes, high and low parts (the low ones lie `batches` matrices behind), and the sum is hi lo + lo hi + hi hi: a slot has
+// four operands for three products.
 struct Product {
   CUtensorMap a, b;        // [matrices][rows][K], boxes of 128 (a) and BN / 2 (b) rows x 128 bytes; b K-major or MN-major
-  int32_t M, N, kblocks, segments, batches;
+  int32_t M, N, kblocks, batches;
   int32_t splits;          // of K: every tile is made that many times, with a share of the slots each
   int32_t tiles_m, tiles_n, num_tiles;   // num_tiles: over all batches
   int32_t lower;           // 1: D is symmetric, only tiles that reach its lower triangle are computed
   int32_t per_batch;       // tiles of a batch, and its and a tile group's reciprocal (set_tiles)
   uint32_t per_batch_inv, per_group_inv;
-  int32_t group;           // slots of K that one accumulator takes before it is drained; several groups: see Epi::kGrouped
   int32_t* status;
 };
 
@@ -169,10 +173,16 @@ __device__ __forceinline__ void st_async_f32(uint32_t cluster_addr, float v, uin
                "r"(__float_as_uint(v)), "r"(cluster_mbar)
                : "memory");
 }
-// 32 lanes x 32 columns without the wait (tc_wait_ld follows).
-__device__ __forceinline__ void tc_ld32_async(uint32_t taddr, uint32_t* r) {
+// Accumulators are read as 16 x 256-bit fragments: of 16 rows lane l gets rows l / 4 and l / 4 + 8, and of every eight
+// columns 2 (l mod 4) and the next.  A lane then has 4 rows and a quarter of its warp's columns; with whole rows per lane
+// (32 x 32 bits) every lane loads the scale and bias of every column from shared memory, which the MMAs' operands go
+// through as well (65,536 x 1024 x 1024: quantised rows 84 us, 67 without those loads).
+template <int COLS>
+__device__ __forceinline__ void load_fragment(uint32_t taddr, uint32_t* r);
+template <>
+__device__ __forceinline__ void load_fragment<64>(uint32_t taddr, uint32_t* r) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
       "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
       "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
@@ -182,6 +192,17 @@ __device__ __forceinline__ void tc_ld32_async(uint32_t taddr, uint32_t* r) {
       : "r"(taddr)
       : "memory");
 }
+template <>
+__device__ __forceinline__ void load_fragment<32>(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -214,95 +235,86 @@ inline int32_t row_alignment(const void* base, int64_t ld, int64_t batch_stride,
   return static_cast<int32_t>(x & (~x + 1));
 }
 
-// Stores a warp's 32 x 32 results: lane `lane` has row m0 + lane, columns n0 .. n0 + 31 in v.  Through the warp's staging
-// the rows leave in pieces of 64 bytes: 16-byte stores of 32 different rows fill half a sector each.
-__device__ __forceinline__ void store_rows(const Out& out, int batch, int M, int N, int m0, int n0, const float (&v)[32],
-                                           uint8_t* staging, int lane) {
-  __syncwarp();   // the last chunk's reads of the staging are done
-  if (out.type == kF32) {
-    float* base = static_cast<float*>(out.base) + batch * out.batch_stride;
+// Fragments to rows: stores four 8 x 8 matrices of 16-bit elements, w[j] to the 16-byte column j of rows 8 i .. 8 i + 7 of a
+// warp's staging (64 bytes per row, columns permuted by the row so that eight rows fill all banks); and the 16 bytes of row
+// r and column c.
+__device__ __forceinline__ void store_fragment(uint32_t staging, int i, const uint32_t (&w)[4], int lane) {
+  const int r = 8 * i + (lane & 7), j = lane >> 3;
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(staging + r * 64 + ((j ^ ((r >> 1) & 3)) << 4)),
+               "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+               : "memory");
+}
+__device__ __forceinline__ uint4 staged_row(const uint8_t* staging, int r, int c) {
+  return *reinterpret_cast<const uint4*>(staging + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+}
+// The same with rows and columns exchanged: w[i] to the 16-byte column i of rows 8 j .. 8 j + 7, which are columns of the results.
+__device__ __forceinline__ void store_fragment_turned(uint32_t staging, int j, const uint32_t (&w)[4], int lane) {
+  const int r = 8 * j + (lane & 7), i = lane >> 3;
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(staging + r * 64 + ((i ^ ((r >> 1) & 3)) << 4)),
+               "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+               : "memory");
+}
+// A warp's staging of 32 x 32 16-bit elements to rows of `ld` elements from `to` on, of which rows_left and cols_left are there.
+__device__ __forceinline__ void store_staged(const uint8_t* staging, uint16_t* to, int64_t ld, int vec, int rows_left, int cols_left, int lane) {
+  if (vec >= 4) {
+    const int n = 8 * (lane & 3);
+    uint16_t* at = to + (lane >> 2) * ld + n;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (h) __syncwarp();
+    for (int i = 0; i < 4; ++i, at += 8 * ld) {
+      if (8 * i + (lane >> 2) >= rows_left) continue;
+      const uint4 x = staged_row(staging, 8 * i + (lane >> 2), lane & 3);
+      const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+      if (n + 8 > cols_left) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        *reinterpret_cast<float4*>(staging + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) =
-            make_float4(v[16 * h + 4 * j], v[16 * h + 4 * j + 1], v[16 * h + 4 * j + 2], v[16 * h + 4 * j + 3]);
-      __syncwarp();
-      const int n = n0 + 16 * h;
-      if (out.vec == 16 && n + 16 <= N) {
+        for (int e = 0; e < 8; ++e)
+          if (n + e < cols_left) at[e] = static_cast<uint16_t>(xs[e >> 1] >> (16 * (e & 1)));
+      } else if (vec == 16) {
+        *reinterpret_cast<uint4*>(at) = x;
+      } else if (vec == 8) {
+        reinterpret_cast<uint2*>(at)[0] = make_uint2(x.x, x.y);
+        reinterpret_cast<uint2*>(at)[1] = make_uint2(x.z, x.w);
+      } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = 8 * i + (lane >> 2), c = lane & 3;
-          const float4 x = *reinterpret_cast<const float4*>(staging + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
-          if (m0 + r < M) *reinterpret_cast<float4*>(base + static_cast<int64_t>(m0 + r) * out.ld + n + 4 * c) = x;
-        }
-      } else if (n + (lane & 15) < N) {
-#pragma unroll 4
-        for (int r = lane >> 4; r < 32 && m0 + r < M; r += 2)
-          base[static_cast<int64_t>(m0 + r) * out.ld + n + (lane & 15)] =
-              *reinterpret_cast<const float*>(staging + r * 64 + ((((lane & 15) >> 2) ^ ((r >> 1) & 3)) << 4) + 4 * (lane & 3));
+        for (int e = 0; e < 4; ++e) reinterpret_cast<uint32_t*>(at)[e] = xs[e];
       }
     }
-  } else {
-    uint32_t w[16];
-    if (out.type == kBF16) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) w[i] = pack_f16(v[2 * i], v[2 * i + 1]);
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      *reinterpret_cast<uint4*>(staging + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) =
-          make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
-    __syncwarp();
-    uint16_t* base = static_cast<uint16_t*>(out.base) + batch * out.batch_stride;
-    if (out.vec == 16 && n0 + 32 <= N) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = 8 * i + (lane >> 2), c = lane & 3;
-        const uint4 x = *reinterpret_cast<const uint4*>(staging + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
-        if (m0 + r < M) *reinterpret_cast<uint4*>(base + static_cast<int64_t>(m0 + r) * out.ld + n0 + 8 * c) = x;
-      }
-    } else if (n0 + lane < N) {
-#pragma unroll 4
-      for (int r = 0; r < 32 && m0 + r < M; ++r)
-        base[static_cast<int64_t>(m0 + r) * out.ld + n0 + lane] =
-            *reinterpret_cast<const uint16_t*>(staging + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + 2 * (lane & 7));
-    }
+  } else if (lane < cols_left) {
+    // rows that start on any element: a row of 32 at a time
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r)
+      if (r < rows_left)
+        to[r * ld + lane] = *reinterpret_cast<const uint16_t*>(staging + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + 2 * (lane & 7));
   }
 }
 
 // What a tile's epilogue may use.
 struct EpiContext {
   Tail* tail;
+  LayerTail* layer;       // 8-bit layers'
   uint32_t tmem;          // this warp's lanes and first column of its part of the tile
   int warp, lane, part;   // epilogue warp, its part of the columns
   int row;                // the warp's first row among the CTA's 128
   int row0, n0;           // its first row and the first column of its part, in the matrix
   int batch, t;           // and the tile's number
   uint32_t n_tile;        // how many tiles the CTA has drained before
-  bool first, last;       // group of the tile
+  bool first, last;       // accumulation of the tile (kSplit)
   uint32_t rank;          // in the cluster
   int next_row0, next_n0; // of the next tile; next_row0 < 0: there is none
   bool* ok;
 };
 
-// Adds a group's accumulators to a lane's sums.
-template <int BN, class Release>
-__device__ __forceinline__ void add_group(const EpiContext& c, float (&sums)[Shape<BN>::kCols], Release release) {
-  static_assert(Shape<BN>::kCols == 32, "one load");
-  uint32_t acc[32];
-  tc_ld32_async(c.tmem, acc);
+// 32 columns of a warp's part as float fragments: v[j][i] are columns 8 j + 2 (lane mod 4) and the next of row 8 i + lane / 4.
+using Block = float2[4][4];
+template <class Use>
+__device__ __forceinline__ void load_block(uint32_t tmem, Use use) {
+  uint32_t acc[2][16];
+  load_fragment<32>(tmem, acc[0]);
+  load_fragment<32>(tmem + (16u << 16), acc[1]);
   tc_wait_ld();
-  release();
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    const float x = __uint_as_float(acc[i]);
-    sums[i] = c.first ? x : sums[i] + x;
-  }
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) use(j, i, make_float2(__uint_as_float(acc[i >> 1][4 * j + 2 * (i & 1)]), __uint_as_float(acc[i >> 1][4 * j + 2 * (i & 1) + 1])));
 }
 
 // The width of a tile whose rounds take least.  A round of MMAs takes 64 cycles per 16 values of K (32 in 8 bits) for up to
@@ -321,23 +333,24 @@ inline int tile_columns(std::initializer_list<int> widths, int pairs, Count tile
   return best;
 }
 
-// The kernel.  Epilogue: a policy with `Params`, static kInt8, kMnMajorB, kGrouped, kClusterCtas (0: a pair; else the CTAs of a
+// The kernel.  Epilogue: a policy with `Params`, static kInt8, kMnMajorB, kSplit, kClusterCtas (0: a pair; else the CTAs of a
 // cluster that share rows, one pair per BN columns) and
 //   static void begin(EpiContext&)                                              before a tile's accumulators are waited for
 //   static void fetch(const Params&, const Product&, EpiContext&, row0, n0)     requests what a tile's results need, a tile ahead
 //   static void drain(const Params&, const Product&, EpiContext&, sums, release)   calls release() once the accumulators are read,
 //                                                                                  and c.fetch_next() once that is used
-// kGrouped: the tensor core adds 16 products of K at a time to its float32 sums and cuts what does not fit, which over
-// long K is off by as many units as there are additions, all to the same side.  So a tile's K goes to the accumulators in
-// groups (the small products of high and low parts are one), and drain() adds the groups in registers (sums), rounded to
-// nearest; it acts on the last one.
+// kSplit: the tensor core adds 16 products of K at a time to its float32 sums and cuts what does not fit, which over long K is
+// off by as many units as there are additions, all to the same side (1024 x 1024 float32 updates: 3.7e-5).  So every
+// slot has an accumulation of its own, the small products of high and low parts first, and drain() adds them in
+// registers (sums), rounded to nearest (2.1e-6); it acts on the last one.
 template <int BN, class Epi>
 __global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
 gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ typename Epi::Params ep) {
   using S = Shape<BN>;
+  using R = Ring<BN, Epi>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  Tail* tail = reinterpret_cast<Tail*>(ring + S::kSlots * S::kSlotBytes);
+  Tail* tail = reinterpret_cast<Tail*>(ring + R::kSlots * R::kSlotBytes);
   const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31);
   const uint32_t rank = cluster_ctarank();
   const uint32_t side = rank & 1u, pair = rank >> 1;
@@ -348,7 +361,7 @@ gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ typename 
                  acc_empty = smem_u32(tail->acc_empty);
 
   if (threadIdx.x == 32) {
-    for (int s = 0; s < S::kSlots; ++s) {
+    for (int s = 0; s < R::kSlots; ++s) {
       mbar_init(full + 8 * s, 1);       // the leader's: its producer's expect_tx; both CTAs' copies count there
       mbar_init(empty + 8 * s, 1);
     }
@@ -384,12 +397,6 @@ gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ typename 
   // slots of K of a share, and where it begins
   const int most_kb = p.splits > 1 ? (p.kblocks + p.splits - 1) / p.splits : p.kblocks;
   auto slots_of = [&](int split) { return p.splits > 1 ? max(0, min(most_kb, p.kblocks - split * most_kb)) : most_kb; };
-  // end of the group of K slots that begins at kb
-  auto group_end = [&](int kb, int slots) {
-    if (!Epi::kGrouped) return slots * p.segments;
-    const int small = slots * (p.segments - 1);
-    return kb < small ? small : min(kb + p.group, slots * p.segments);
-  };
 
   if (warp == 0) {
     // ------------------------------ copies ------------------------------
@@ -399,28 +406,29 @@ gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ typename 
       bool ok = true;
       for (int t = worker; t < p.num_tiles && ok; t += workers) {
         const Tile tile = locate(t);
-        for (int seg = 0; seg < p.segments && ok; ++seg) {
-          const int za = tile.batch + (seg == 1 ? p.batches : 0), zb = tile.batch + (p.segments > 1 && seg == 0 ? p.batches : 0);
-          const int kb0 = tile.split * most_kb, kb1 = kb0 + slots_of(tile.split);
-          for (int kb = kb0; kb < kb1; ++kb) {
-            ok = mbar_wait(empty + 8 * s, ph, abort_flag, p.status, 0x511);
-            if (!ok) break;
-            const uint32_t bar = map_to_cta(full + 8 * s, leader);
-            if (side == 0) mbar_expect_tx(full + 8 * s, 2 * S::kSlotBytes);
-            const uint32_t dst = ring_addr + s * S::kSlotBytes;
-            constexpr int kElems = Epi::kInt8 ? kSlotK : kSlotK / 2;
-            tma_3d_2sm(dst, &p.a, kb * kElems, tile.m0 + static_cast<int>(side) * kCtaRows, za, bar);
-            const int n = tile.n0 + static_cast<int>(side) * S::kBRows;
+        const int kb0 = tile.split * most_kb, kb1 = kb0 + slots_of(tile.split);
+        const int m = tile.m0 + static_cast<int>(side) * kCtaRows, n = tile.n0 + static_cast<int>(side) * S::kBRows;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          ok = mbar_wait(empty + 8 * s, ph, abort_flag, p.status, 0x511);
+          if (!ok) break;
+          const uint32_t bar = map_to_cta(full + 8 * s, leader);
+          if (side == 0) mbar_expect_tx(full + 8 * s, 2 * R::kSlotBytes);
+          constexpr int kElems = Epi::kInt8 ? kSlotK : kSlotK / 2;
+#pragma unroll
+          for (int part = 0; part < (Epi::kSplit ? 2 : 1); ++part) {
+            const uint32_t dst = ring_addr + s * R::kSlotBytes + part * R::kOperands;
+            const int z = tile.batch + part * p.batches;
+            tma_3d_2sm(dst, &p.a, kb * kElems, m, z, bar);
             if (Epi::kMnMajorB) {
               // [64 rows of K][64 columns] per slab
 #pragma unroll
               for (int j = 0; j < S::kBRows / 64; ++j)
-                tma_3d_2sm(dst + kCtaRows * kSlotK + j * 8192, &p.b, n + 64 * j, kb * kElems, zb, bar);
+                tma_3d_2sm(dst + kCtaRows * kSlotK + j * 8192, &p.b, n + 64 * j, kb * kElems, z, bar);
             } else {
-              tma_3d_2sm(dst + kCtaRows * kSlotK, &p.b, kb * kElems, n, zb, bar);
+              tma_3d_2sm(dst + kCtaRows * kSlotK, &p.b, kb * kElems, n, z, bar);
             }
-            if (++s == S::kSlots) { s = 0; ph ^= 1u; }
           }
+          if (++s == R::kSlots) { s = 0; ph ^= 1u; }
         }
       }
     }
@@ -441,24 +449,32 @@ gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ typename 
       uint32_t s = 0, ph = 0, n = 0;
       bool ok = true;
       for (int t = worker; t < p.num_tiles && ok; t += workers) {
-        const int slots = slots_of(p.splits > 1 ? locate(t).split : 0), total_kb = slots * p.segments;
-        for (int kb0 = 0, kb1; kb0 < total_kb && ok; kb0 = kb1, ++n) {
-          kb1 = group_end(kb0, slots);
+        const int slots = slots_of(p.splits > 1 ? locate(t).split : 0);
+        for (int kb = 0; kb < slots && ok;) {
           const uint32_t st = n % S::kAccs, turn = n / S::kAccs & 1u;
+          ++n;
           ok = mbar_wait(acc_empty + 8 * st, turn ^ 1u, abort_flag, p.status, 0x521);
           tc_fence_after();
           const uint32_t d = tmem + st * BN;
-          for (int kb = kb0; kb < kb1 && ok; ++kb) {
+          uint32_t more = 0;
+          for (const int end = Epi::kSplit ? kb + 1 : slots; kb < end && ok; ++kb) {
             ok = mbar_wait(full + 8 * s, ph, abort_flag, p.status, 0x522);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t a_lo = a0 + s * (S::kSlotBytes >> 4);
+            const uint32_t a_lo = a0 + s * (R::kSlotBytes >> 4);
             const uint32_t b_lo = a_lo + (kCtaRows * kSlotK >> 4);
+            constexpr uint32_t kLow = R::kOperands >> 4;      // from a high part to its low one
+            if (Epi::kSplit) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              mma_pair<Epi::kInt8>(d, a_hi | (a_lo + 2 * k), b_hi | (b_lo + b_step * k), idesc, (kb != kb0 || k) ? 1u : 0u);
+              for (int k = 0; k < 4; ++k) mma_pair<Epi::kInt8>(d, a_hi | (a_lo + 2 * k), b_hi | (b_lo + kLow + b_step * k), idesc, k ? 1u : 0u);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) mma_pair<Epi::kInt8>(d, a_hi | (a_lo + kLow + 2 * k), b_hi | (b_lo + b_step * k), idesc, 1u);
+              more = 1;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k, more = 1) mma_pair<Epi::kInt8>(d, a_hi | (a_lo + 2 * k), b_hi | (b_lo + b_step * k), idesc, more);
             commit_pair(empty + 8 * s, pair);
-            if (++s == S::kSlots) { s = 0; ph ^= 1u; }
+            if (++s == R::kSlots) { s = 0; ph ^= 1u; }
           }
           if (ok) commit_pair(acc_full + 8 * st, pair);
         }
@@ -470,10 +486,10 @@ gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ typename 
     const int quad = warp & 3;
     bool ok = true;
     EpiContext c;
-    c.tail = tail; c.warp = w; c.lane = lane; c.part = w >> 2; c.row = quad * 32; c.rank = rank; c.ok = &ok;
+    c.tail = tail; c.layer = reinterpret_cast<LayerTail*>(tail + 1); c.warp = w; c.lane = lane; c.part = w >> 2; c.row = quad * 32; c.rank = rank; c.ok = &ok;
     uint32_t n = 0;
     const uint32_t acc_empty_leader = map_to_cta(acc_empty, leader);
-    float sums[Epi::kGrouped ? S::kCols : 1];
+    Block sums;
     c.n_tile = 0;
     Tile tile{}, next{};
     auto look_ahead = [&](int t) {
@@ -493,13 +509,12 @@ gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ typename 
       look_ahead(t + workers);
       Epi::template begin<BN>(c);
       c.t = t;
-      const int slots = slots_of(tile.split), total_kb = slots * p.segments;
-      for (int kb0 = 0, kb1; kb0 < total_kb && ok; kb0 = kb1, ++n) {
-        kb1 = group_end(kb0, slots);
+      const int rounds = Epi::kSplit ? slots_of(tile.split) : 1;
+      for (int i = 0; i < rounds && ok; ++i, ++n) {
         const uint32_t st = n % S::kAccs, turn = n / S::kAccs & 1u;
         c.tmem = tmem + (static_cast<uint32_t>(quad * 32) << 16) + st * BN + static_cast<uint32_t>(c.part * S::kCols);
-        c.first = kb0 == 0;
-        c.last = kb1 == total_kb;
+        c.first = i == 0;
+        c.last = i == rounds - 1;
         if (!mbar_wait(acc_full + 8 * st, turn, abort_flag, p.status, 0x531)) { ok = false; break; }
         tc_fence_after();
         Epi::template drain<BN>(ep, p, c, sums, [&] {

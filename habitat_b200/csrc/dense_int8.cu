@@ -208,36 +208,6 @@ __global__ void __launch_bounds__(256) align_rows_kernel(const int8_t* __restric
 // Epilogues
 // ---------------------------------------------------------------------------
 
-// Accumulators are read as 16 x 256-bit fragments: of 16 rows lane l gets rows l / 4 and l / 4 + 8, and of every eight
-// columns 2 (l mod 4) and the next.  A lane then has 4 rows and a quarter of its warp's columns; with whole rows per lane
-// (32 x 32 bits) every lane loads the scale and bias of every column from shared memory, which the MMAs' operands go
-// through as well (65,536 x 1024 x 1024: quantised rows 84 us, 67 without those loads).
-template <int COLS>
-__device__ __forceinline__ void load_fragment(uint32_t taddr, uint32_t* r);
-template <>
-__device__ __forceinline__ void load_fragment<64>(uint32_t taddr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr)
-      : "memory");
-}
-template <>
-__device__ __forceinline__ void load_fragment<32>(uint32_t taddr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr)
-      : "memory");
-}
-
 // A float from memory to shared memory, zero where there is none, without a register on the way: scales that were loaded a
 // tile ahead into registers were spilled, which waits for them.
 __device__ __forceinline__ void copy_float(const float* to, const float* from, bool there) {
@@ -245,7 +215,7 @@ __device__ __forceinline__ void copy_float(const float* to, const float* from, b
 }
 template <int BN>
 __device__ __forceinline__ void fetch_scales(const LayerScales& s, const Product& p, const EpiContext& c, int row0, int n0) {
-  float* to = c.tail->scales[c.warp];
+  float* to = c.layer->scales[c.warp];
 #pragma unroll
   for (int i = 0; i < Shape<BN>::kCols; i += 32) {
     const bool there = n0 + i + c.lane < p.N;
@@ -277,7 +247,7 @@ __device__ __forceinline__ void finish(const LayerScales& s, const Product& p, c
   load_fragment<kCols>(c.tmem + (16u << 16), acc[1]);
   asm volatile("cp.async.wait_all;" ::: "memory");
   __syncwarp();
-  const float* at = c.tail->scales[c.warp];
+  const float* at = c.layer->scales[c.warp];
   const float2* sc = reinterpret_cast<const float2*>(at) + (c.lane & 3);
   float row[4];
 #pragma unroll
@@ -299,18 +269,6 @@ __device__ __forceinline__ void finish(const LayerScales& s, const Product& p, c
   if (c.next_row0 >= 0) fetch_scales<BN>(s, p, c, c.next_row0, c.next_n0);
 }
 
-// Fragments to rows: stores four 8 x 8 matrices of 16-bit elements, w[j] to the 16-byte column j of rows 8 i .. 8 i + 7 of a
-// warp's staging (64 bytes per row, columns permuted by the row so that eight rows fill all banks); and the 16 bytes of row
-// r and column c.
-__device__ __forceinline__ void store_fragment(uint32_t staging, int i, const uint32_t (&w)[4], int lane) {
-  const int r = 8 * i + (lane & 7), j = lane >> 3;
-  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(staging + r * 64 + ((j ^ ((r >> 1) & 3)) << 4)),
-               "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
-               : "memory");
-}
-__device__ __forceinline__ uint4 staged_row(const uint8_t* staging, int r, int c) {
-  return *reinterpret_cast<const uint4*>(staging + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
-}
 __device__ __forceinline__ float max3_abs(float a, float b, float c) {
   float r;
   asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -318,7 +276,7 @@ __device__ __forceinline__ float max3_abs(float a, float b, float c) {
 }
 
 struct FloatOut {
-  static constexpr bool kInt8 = true, kMnMajorB = false, kGrouped = false;
+  static constexpr bool kInt8 = true, kMnMajorB = false, kSplit = false;
   static constexpr int kClusterCtas = 0;
   struct Params {
     LayerScales s;
@@ -331,7 +289,7 @@ struct FloatOut {
   template <int BN>
   static __device__ __forceinline__ void begin(const EpiContext&) {}
   template <int BN, class Release>
-  static __device__ __forceinline__ void drain(const Params& ep, const Product& p, const EpiContext& c, float (&)[1], Release release) {
+  static __device__ __forceinline__ void drain(const Params& ep, const Product& p, const EpiContext& c, Block&, Release release) {
     constexpr int kBlocks = Shape<BN>::kCols / 8;
     float2 v[kBlocks][4];
     finish<BN>(ep.s, p, c, v, release);
@@ -371,38 +329,8 @@ struct FloatOut {
         store_fragment(smem_u32(staging), i, w, c.lane);
       }
       __syncwarp();
-      uint16_t* out = static_cast<uint16_t*>(ep.out.base) + c.n0 + 8 * g;
-      const int left = p.N - c.n0 - 8 * g;
-      if (ep.out.vec >= 4) {
-        const int n = 8 * (c.lane & 3);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (row0 + 8 * i >= p.M) continue;
-          const uint4 x = staged_row(staging, 8 * i + (c.lane >> 2), c.lane & 3);
-          uint16_t* to = out + static_cast<int64_t>(row0 + 8 * i) * ep.out.ld + n;
-          const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
-          if (n + 8 > left) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (n + e < left) to[e] = static_cast<uint16_t>(xs[e >> 1] >> (16 * (e & 1)));
-          } else if (ep.out.vec == 16) {
-            *reinterpret_cast<uint4*>(to) = x;
-          } else if (ep.out.vec == 8) {
-            reinterpret_cast<uint2*>(to)[0] = make_uint2(x.x, x.y);
-            reinterpret_cast<uint2*>(to)[1] = make_uint2(x.z, x.w);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) reinterpret_cast<uint32_t*>(to)[e] = xs[e];
-          }
-        }
-      } else if (c.lane < left) {
-        // rows that start on any element: a row of 32 at a time
-#pragma unroll 8
-        for (int r = 0; r < 32; ++r)
-          if (c.row0 + r < p.M)
-            out[static_cast<int64_t>(c.row0 + r) * ep.out.ld + c.lane] =
-                *reinterpret_cast<const uint16_t*>(staging + r * 64 + (((c.lane >> 3) ^ ((r >> 1) & 3)) << 4) + 2 * (c.lane & 7));
-      }
+      store_staged(staging, static_cast<uint16_t*>(ep.out.base) + static_cast<int64_t>(c.row0) * ep.out.ld + c.n0 + 8 * g, ep.out.ld, ep.out.vec,
+                   p.M - c.row0, p.N - c.n0 - 8 * g, c.lane);
     }
   }
 };
@@ -413,7 +341,7 @@ struct FloatOut {
 // there.  The accumulators are free before the exchange, so the next tile's MMAs run during it.
 template <int kCtas>
 struct QuantOut {
-  static constexpr bool kInt8 = true, kMnMajorB = false, kGrouped = false;
+  static constexpr bool kInt8 = true, kMnMajorB = false, kSplit = false;
   static constexpr int kClusterCtas = kCtas;
   struct Params {
     LayerScales s;
@@ -431,7 +359,7 @@ struct QuantOut {
       mbar_expect_tx(smem_u32(&c.tail->exchange[c.n_tile & 1u]), kCtas / 2 * Shape<BN>::kParts * kCtaRows * 4);
   }
   template <int BN, class Release>
-  static __device__ __forceinline__ void drain(const Params& ep, const Product& p, const EpiContext& c, float (&)[1], Release release) {
+  static __device__ __forceinline__ void drain(const Params& ep, const Product& p, const EpiContext& c, Block&, Release release) {
     constexpr int kBlocks = Shape<BN>::kCols / 8, kParts = Shape<BN>::kParts;
     float2 v[kBlocks][4];
     finish<BN>(ep.s, p, c, v, release);
@@ -449,7 +377,7 @@ struct QuantOut {
     const int mine = c.row + 8 * (c.lane & 3) + (c.lane >> 2);       // among the CTA's rows
     const uint32_t buf = c.n_tile & 1u, side = c.rank & 1u;
     const uint32_t bar = smem_u32(&c.tail->exchange[buf]);
-    const uint32_t at = smem_u32(&c.tail->row_max[buf][c.rank >> 1][c.part][mine]);
+    const uint32_t at = smem_u32(&c.layer->row_max[buf][c.rank >> 1][c.part][mine]);
 #pragma unroll
     for (int i = 0; i < kCtas / 2; ++i) st_async_f32(map_to_cta(at, 2 * i + side), amax, map_to_cta(bar, 2 * i + side));
     if (!mbar_wait_cluster(bar, (c.n_tile >> 1) & 1u, &c.tail->abort, p.status, 0x541)) {
@@ -459,7 +387,7 @@ struct QuantOut {
 #pragma unroll
     for (int i = 0; i < kCtas / 2; ++i)
 #pragma unroll
-      for (int j = 0; j < kParts; ++j) amax = max_nan(amax, c.tail->row_max[buf][i][j][mine]);
+      for (int j = 0; j < kParts; ++j) amax = max_nan(amax, c.layer->row_max[buf][i][j][mine]);
     const RowScale s = row_scale(amax);
     const int row = c.row0 + 8 * (c.lane & 3) + (c.lane >> 2);
     if (c.rank < 2 && c.part == 0 && row < p.M) ep.scales[row] = s.scale;
@@ -572,7 +500,6 @@ hb_status describe(Product* p, const Operands& o, int64_t M, int64_t N, int64_t 
   p->M = static_cast<int32_t>(M);
   p->N = static_cast<int32_t>(N);
   p->kblocks = static_cast<int32_t>((K + kSlotK - 1) / kSlotK);
-  p->segments = 1;
   p->batches = 1;
   p->splits = 1;
   p->tiles_m = static_cast<int32_t>((M + kPairRows - 1) / kPairRows);
@@ -587,7 +514,7 @@ hb_status launch_float(const Operands& o, int64_t M, int64_t N, int64_t K, const
   static std::atomic<int> held[64];
   int pairs = 0;
   auto kernel = gemm_kernel<BN, FloatOut>;
-  if (const hb_status st = max_clusters(kernel, 2, Shape<BN>::kThreads, smem_bytes<BN>(), held, &pairs)) return st;
+  if (const hb_status st = max_clusters(kernel, 2, Shape<BN>::kThreads, Ring<BN, FloatOut>::kSmem, held, &pairs)) return st;
   Product p{};
   if (const hb_status st = describe(&p, o, M, N, K, BN, status)) return st;
   const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
@@ -597,7 +524,7 @@ hb_status launch_float(const Operands& o, int64_t M, int64_t N, int64_t K, const
   }
   set_tiles(&p, tiles);
   const int clusters = p.num_tiles < pairs ? p.num_tiles : pairs;
-  HB_CUDA_TRY(launch_clusters(kernel, clusters, 2, Shape<BN>::kThreads, smem_bytes<BN>(), s, p, ep));
+  HB_CUDA_TRY(launch_clusters(kernel, clusters, 2, Shape<BN>::kThreads, Ring<BN, FloatOut>::kSmem, s, p, ep));
   return HB_OK;
 }
 
@@ -607,12 +534,12 @@ hb_status launch_quant(const Operands& o, int64_t M, int64_t N, int64_t K, const
   static std::atomic<int> held[64];
   int clusters = 0;
   auto kernel = gemm_kernel<256, QuantOut<kCtas>>;
-  if (const hb_status st = max_clusters(kernel, kCtas, Shape<256>::kThreads, smem_bytes<256>(), held, &clusters)) return st;
+  if (const hb_status st = max_clusters(kernel, kCtas, Shape<256>::kThreads, Ring<256, QuantOut<kCtas>>::kSmem, held, &clusters)) return st;
   Product p{};
   if (const hb_status st = describe(&p, o, M, N, K, 256, status)) return st;
   set_tiles(&p, p.tiles_m);
   if (p.num_tiles < clusters) clusters = p.num_tiles;
-  HB_CUDA_TRY(launch_clusters(kernel, clusters, kCtas, Shape<256>::kThreads, smem_bytes<256>(), s, p, ep));
+  HB_CUDA_TRY(launch_clusters(kernel, clusters, kCtas, Shape<256>::kThreads, Ring<256, QuantOut<kCtas>>::kSmem, s, p, ep));
   return HB_OK;
 }
 

@@ -24,7 +24,6 @@ constexpr float kScale = 256.0f;          // of stored X, A and B
 constexpr int kNormThreads = 256;
 constexpr int kMostPartials = 64;
 constexpr int kSideBlocks = 2;            // blocks of 64 columns per CTA that a cluster is made wider for
-constexpr int kGroup = 2;                 // slots of K (128 values, 8 additions) per accumulation, with `split`
 
 template <typename T>
 __device__ __forceinline__ float element(const void* base, int64_t at) { return static_cast<float>(static_cast<const T*>(base)[at]); }
@@ -127,45 +126,60 @@ __global__ void __launch_bounds__(256) operand_kernel(Source g, const double* pa
   }
 }
 
-// float32 values -> what their half-precision parts leave.
-__device__ __forceinline__ void take_half(float (&v)[32]) {
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] -= __half2float(__float2half_rn(v[i]));
-}
-
-// Calls work(chunk, values) for the lane's 32-column chunks: as they leave the accumulators, or, where K comes in groups, from
-// the sums behind the last group.
-template <int BN, bool kGrouped, class Release, class Work>
-__device__ __forceinline__ void for_chunks(const EpiContext& c, float (&sums)[kGrouped ? Shape<BN>::kCols : 1], Release release, Work work) {
-  if constexpr (kGrouped) {
-    add_group<BN>(c, sums, release);
+// Calls work(chunk, values) for the 32-column chunks of a warp's part: as they leave the accumulators, or, with kSplit (one chunk),
+// from the sums behind the last accumulation.
+template <int BN, bool kSplit, class Release, class Work>
+__device__ __forceinline__ void for_chunks(const EpiContext& c, Block& sums, Release release, Work work) {
+  constexpr int kChunks = Shape<BN>::kCols / 32;
+  if constexpr (kSplit) {
+    static_assert(kChunks == 1, "sums of 64 columns do not fit the registers");
+    load_block(c.tmem, [&](int j, int i, float2 x) {
+      sums[j][i] = c.first ? x : make_float2(sums[j][i].x + x.x, sums[j][i].y + x.y);
+    });
+    release();
     if (c.last) work(0, sums);
   } else {
 #pragma unroll 1
-    for (int chunk = 0; chunk < Shape<BN>::kCols / 32; ++chunk) {
-      uint32_t acc[32];
-      float v[32];
-      tc_ld32_async(c.tmem + chunk * 32, acc);
-      tc_wait_ld();
-      if (chunk == Shape<BN>::kCols / 32 - 1) release();
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(acc[i]);
+    for (int chunk = 0; chunk < kChunks; ++chunk) {
+      Block v;
+      load_block(c.tmem + chunk * 32, [&](int j, int i, float2 x) { v[j][i] = x; });
+      if (chunk == kChunks - 1) release();
       work(chunk, v);
     }
   }
 }
 
-// v += factor * 32 half-precision values
-__device__ __forceinline__ void add_halves(float (&v)[32], const __half* at, float factor) {
+// A block as half-precision operands at `to` (rows of `ld`) and, with rows and columns exchanged, at `turned`, and with kSplit what
+// that leaves, `low` elements behind.
+template <bool kSplit>
+__device__ __forceinline__ void store_operands(Block& v, __half* to, __half* turned, int64_t ld, int64_t low, int rows_left, uint8_t* staging, int lane) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint4 x = *reinterpret_cast<const uint4*>(at + 8 * j);
-    const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+  for (int part = 0; part < (kSplit ? 2 : 1); ++part) {
+    uint32_t w[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        w[j][i] = pack_f16(v[j][i].x, v[j][i].y);
+        if (kSplit && part == 0) {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j][i]));
+          v[j][i] = make_float2(v[j][i].x - f.x, v[j][i].y - f.y);
+        }
+      }
+    __syncwarp();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&xs[i]));
-      v[8 * j + 2 * i] = fmaf(factor, f.x, v[8 * j + 2 * i]);
-      v[8 * j + 2 * i + 1] = fmaf(factor, f.y, v[8 * j + 2 * i + 1]);
+      const uint32_t x[4] = {w[0][i], w[1][i], w[2][i], w[3][i]};
+      store_fragment(smem_u32(staging), i, x, lane);
+    }
+    __syncwarp();
+    store_staged(staging, reinterpret_cast<uint16_t*>(to + part * low), ld, 16, rows_left, 32, lane);
+    if (turned) {
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < 4; ++j) store_fragment_turned(smem_u32(staging), j, w[j], lane);
+      __syncwarp();
+      store_staged(staging, reinterpret_cast<uint16_t*>(turned + part * low), ld, 16, 32, 32, lane);
     }
   }
 }
@@ -190,8 +204,10 @@ __device__ __forceinline__ float symmetric_scale(const Symmetric& e, int batch) 
 
 // Symmetric products with few tiles and a long K are split along it; the shares go to memory as they are, tile by tile, and
 // symmetric_sum_kernel adds them.
+template <bool kLow>
 struct ShareOut {
-  static constexpr bool kInt8 = false, kMnMajorB = false, kGrouped = true;
+  static constexpr bool kSplit = kLow;
+  static constexpr bool kInt8 = false, kMnMajorB = false;
   static constexpr int kClusterCtas = 0;
   struct Params {
     float* shares;          // [tile and split][256][BN]
@@ -201,11 +217,14 @@ struct ShareOut {
   template <int BN>
   static __device__ __forceinline__ void begin(const EpiContext&) {}
   template <int BN, class Release>
-  static __device__ __forceinline__ void drain(const Params& ep, const Product&, const EpiContext& c, float (&sums)[Shape<BN>::kCols], Release release) {
-    for_chunks<BN, true>(c, sums, release, [&](int, float (&v)[32]) {
-      const Out out{ep.shares + static_cast<int64_t>(c.t) * kPairRows * BN, BN, 0, kF32, 16};
-      store_rows(out, 0, kPairRows, BN, static_cast<int>(c.rank & 1u) * kCtaRows + c.row, c.part * Shape<BN>::kCols, v,
-                 c.tail->staging + c.warp * kStageOutBytes, c.lane);
+  static __device__ __forceinline__ void drain(const Params& ep, const Product&, const EpiContext& c, Block& sums, Release release) {
+    for_chunks<BN, kSplit>(c, sums, release, [&](int chunk, Block& v) {
+      float* to = ep.shares + (static_cast<int64_t>(c.t) * kPairRows + static_cast<int>(c.rank & 1u) * kCtaRows + c.row + (c.lane >> 2)) * BN +
+                  c.part * Shape<BN>::kCols + 32 * chunk + 2 * (c.lane & 3);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) *reinterpret_cast<float2*>(to + 8 * i * BN + 8 * j) = v[j][i];
     });
   }
 };
@@ -262,9 +281,10 @@ __global__ void __launch_bounds__(256) symmetric_sum_kernel(const __grid_constan
 }
 
 // Symmetric results: A = X X^T, or B = a I + b A + c A^2, as half-precision operands (kSplit: high and low parts).
-template <bool kSplit>
+template <bool kLow>
 struct SymmetricOut {
-  static constexpr bool kInt8 = false, kMnMajorB = false, kGrouped = kSplit;
+  static constexpr bool kSplit = kLow;
+  static constexpr bool kInt8 = false, kMnMajorB = false;
   static constexpr int kClusterCtas = 0;
   using Params = Symmetric;
   template <int BN>
@@ -272,54 +292,51 @@ struct SymmetricOut {
   template <int BN>
   static __device__ __forceinline__ void begin(const EpiContext&) {}
   template <int BN, class Release>
-  static __device__ __forceinline__ void drain(const Params& ep, const Product& p, const EpiContext& c, float (&sums)[kGrouped ? Shape<BN>::kCols : 1], Release release) {
-    const int row0 = c.row0, row = row0 + c.lane;
+  static __device__ __forceinline__ void drain(const Params& ep, const Product& p, const EpiContext& c, Block& sums, Release release) {
+    const int row0 = c.row0;
     const float scale = symmetric_scale(ep, c.batch);
-    for_chunks<BN, kSplit>(c, sums, release, [&](int chunk, float (&v)[32]) {
+    for_chunks<BN, kSplit>(c, sums, release, [&](int chunk, Block& v) {
       const int n0 = c.n0 + chunk * 32;
       if (n0 > row0 || row0 >= p.M) return;      // above the diagonal (both are multiples of 32), or below the matrix
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] *= scale;
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[j][i] = make_float2(v[j][i].x * scale, v[j][i].y * scale);
+      const int r = c.lane >> 2, n = 2 * (c.lane & 3);
       if (ep.a.hi) {
-        if (row < p.M) {
-          const __half* at = ep.a.hi + c.batch * ep.a.batch_stride + static_cast<int64_t>(row) * ep.a.ld + n0;
-          add_halves(v, at, ep.on_a);
-          if (kSplit) add_halves(v, at + ep.a.low, ep.on_a);
-        }
+        const __half* at = ep.a.hi + c.batch * ep.a.batch_stride + static_cast<int64_t>(row0 + r) * ep.a.ld + n0 + n;
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (n0 + i == row) v[i] += ep.on_diagonal;
+        for (int part = 0; part < (kSplit ? 2 : 1); ++part)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (row0 + r + 8 * i >= p.M) continue;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(at + part * ep.a.low + 8 * i * ep.a.ld + 8 * j));
+              v[j][i] = make_float2(fmaf(ep.on_a, f.x, v[j][i].x), fmaf(ep.on_a, f.y, v[j][i].y));
+            }
+          }
+        if (n0 == row0) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (n == r) v[j][j].x += ep.on_diagonal;
+            if (n + 1 == r) v[j][j].y += ep.on_diagonal;
+          }
+        }
       }
+      // blocks below the diagonal also to their mirror image
       __half* base = ep.out.hi + c.batch * ep.out.batch_stride;
-#pragma unroll 1
-      for (int part = 0; part < (kSplit ? 2 : 1); ++part) {
-        if (n0 < row0) {
-          const Out out{base, ep.out.ld, 0, kF16, 16};
-          store_rows(out, 0, p.M, static_cast<int>(ep.out.ld), row0, n0, v, c.tail->staging + c.warp * kStageOutBytes, c.lane);
-        } else if (row < p.M) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (n0 + i <= row) base[static_cast<int64_t>(row) * ep.out.ld + n0 + i] = __float2half_rn(v[i]);
-        }
-        // the mirror image: a warp's 32 rows of a column are neighbours there
-        if (row < p.M) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (n0 + i < row) base[static_cast<int64_t>(n0 + i) * ep.out.ld + row] = __float2half_rn(v[i]);
-        }
-        if (kSplit) {
-          take_half(v);
-          base += ep.out.low;
-        }
-      }
+      store_operands<kSplit>(v, base + static_cast<int64_t>(row0) * ep.out.ld + n0, n0 < row0 ? base + static_cast<int64_t>(n0) * ep.out.ld + row0 : nullptr,
+                             ep.out.ld, ep.out.low, p.M - row0, c.tail->staging + c.warp * kStageOutBytes, c.lane);
     });
   }
 };
 
 // X <- B X as operands of the next step, or as the result.
-template <bool kSplit>
+template <bool kLow>
 struct UpdateOut {
-  static constexpr bool kInt8 = false, kMnMajorB = true, kGrouped = kSplit;
+  static constexpr bool kSplit = kLow;
+  static constexpr bool kInt8 = false, kMnMajorB = true;
   static constexpr int kClusterCtas = 0;
   struct Params {
     Planes x;               // the next X; hi null: the result
@@ -333,36 +350,60 @@ struct UpdateOut {
   template <int BN>
   static __device__ __forceinline__ void begin(const EpiContext&) {}
   template <int BN, class Release>
-  static __device__ __forceinline__ void drain(const Params& ep, const Product& p, const EpiContext& c, float (&sums)[kGrouped ? Shape<BN>::kCols : 1], Release release) {
-    const int row0 = c.row0, row = row0 + c.lane;
+  static __device__ __forceinline__ void drain(const Params& ep, const Product& p, const EpiContext& c, Block& sums, Release release) {
+    const int row0 = c.row0;
     const float scale = ep.factor ? ep.scale * __ldg(ep.factor + c.batch) : ep.scale;
     uint8_t* staging = c.tail->staging + c.warp * kStageOutBytes;
-    for_chunks<BN, kSplit>(c, sums, release, [&](int chunk, float (&v)[32]) {
+    for_chunks<BN, kSplit>(c, sums, release, [&](int chunk, Block& v) {
       const int n0 = c.n0 + chunk * 32;
       if (n0 >= p.N || row0 >= p.M) return;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] *= scale;
-      if (ep.x.hi) {
-        const Out out{ep.x.hi, ep.x.ld, ep.x.batch_stride, kF16, 16};
-        store_rows(out, c.batch, p.M, static_cast<int>(ep.x.ld), row0, n0, v, staging, c.lane);
-        if (kSplit) {
-          take_half(v);
-          const Out low{ep.x.hi + ep.x.low, ep.x.ld, ep.x.batch_stride, kF16, 16};
-          store_rows(low, c.batch, p.M, static_cast<int>(ep.x.ld), row0, n0, v, staging, c.lane);
-        }
-      } else if (!ep.flip) {
-        store_rows(ep.out, c.batch, p.M, p.N, row0, n0, v, staging, c.lane);
-      } else if (row < p.M) {
-        const int64_t at = c.batch * ep.out.batch_stride + row;
+      for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          if (n0 + i >= p.N) break;
-          const int64_t to = at + static_cast<int64_t>(n0 + i) * ep.out.ld;
-          if (ep.out.type == kF32) static_cast<float*>(ep.out.base)[to] = v[i];
-          else if (ep.out.type == kBF16) static_cast<__nv_bfloat16*>(ep.out.base)[to] = __float2bfloat16_rn(v[i]);
-          else static_cast<__half*>(ep.out.base)[to] = __float2half_rn(v[i]);
-        }
+        for (int i = 0; i < 4; ++i) v[j][i] = make_float2(v[j][i].x * scale, v[j][i].y * scale);
+      if (ep.x.hi) {
+        store_operands<kSplit>(v, ep.x.hi + c.batch * ep.x.batch_stride + static_cast<int64_t>(row0) * ep.x.ld + n0, nullptr, ep.x.ld, ep.x.low, p.M - row0,
+                               staging, c.lane);
+        return;
       }
+      // rows and columns of the result from here on
+      const int64_t first = c.batch * ep.out.batch_stride + (ep.flip ? static_cast<int64_t>(n0) * ep.out.ld + row0 : static_cast<int64_t>(row0) * ep.out.ld + n0);
+      const int rows_left = p.M - row0, cols_left = p.N - n0;
+      if (ep.out.type == kF32) {
+        const int r = c.lane >> 2, n = 2 * (c.lane & 3);
+        float* to = static_cast<float*>(ep.out.base) + first;
+        const int64_t down = ep.flip ? 1 : ep.out.ld, across = ep.flip ? ep.out.ld : 1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (8 * i + r >= rows_left) continue;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float* at = to + (8 * i + r) * down + (8 * j + n) * across;
+            if (!ep.flip && ep.out.vec >= 8 && 8 * j + n + 1 < cols_left) {
+              *reinterpret_cast<float2*>(at) = v[j][i];
+            } else {
+              if (8 * j + n < cols_left) at[0] = v[j][i].x;
+              if (8 * j + n + 1 < cols_left) at[across] = v[j][i].y;
+            }
+          }
+        }
+        return;
+      }
+      __syncwarp();
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        uint32_t w[4];
+#pragma unroll
+        for (int l = 0; l < 4; ++l) {
+          const float2 x = ep.flip ? v[k][l] : v[l][k];
+          w[l] = ep.out.type == kBF16 ? pack_bf16(x.x, x.y) : pack_f16(x.x, x.y);
+        }
+        if (ep.flip) store_fragment_turned(smem_u32(staging), k, w, c.lane);
+        else store_fragment(smem_u32(staging), k, w, c.lane);
+      }
+      __syncwarp();
+      store_staged(staging, static_cast<uint16_t*>(ep.out.base) + first, ep.out.ld, ep.out.vec, ep.flip ? cols_left : rows_left,
+                   ep.flip ? rows_left : cols_left, c.lane);
     });
   }
 };
@@ -405,11 +446,10 @@ Layout layout_of(int64_t batch, int64_t rows, int64_t cols, bool split) {
 
 template <int BN, class Epi>
 hb_status launch(Product p, const typename Epi::Params& ep, cudaStream_t s, Product* as_launched = nullptr) {
-  p.group = kGroup;
   static std::atomic<int> held[64];
   int pairs = 0;
   auto kernel = gemm_kernel<BN, Epi>;
-  if (const hb_status st = max_clusters(kernel, 2, Shape<BN>::kThreads, smem_bytes<BN>(), held, &pairs)) return st;
+  if (const hb_status st = max_clusters(kernel, 2, Shape<BN>::kThreads, Ring<BN, Epi>::kSmem, held, &pairs)) return st;
   p.tiles_m = static_cast<int32_t>((p.M + kPairRows - 1) / kPairRows);
   p.tiles_n = static_cast<int32_t>((p.N + BN - 1) / BN);
   const int64_t tiles = p.lower ? lower_tiles(p.M, BN) : static_cast<int64_t>(p.tiles_m) * p.tiles_n;
@@ -419,7 +459,7 @@ hb_status launch(Product p, const typename Epi::Params& ep, cudaStream_t s, Prod
   }
   set_tiles(&p, tiles);
   const int clusters = p.num_tiles < pairs ? p.num_tiles : pairs;
-  HB_CUDA_TRY(launch_clusters(kernel, clusters, 2, Shape<BN>::kThreads, smem_bytes<BN>(), s, p, ep));
+  HB_CUDA_TRY(launch_clusters(kernel, clusters, 2, Shape<BN>::kThreads, Ring<BN, Epi>::kSmem, s, p, ep));
   if (as_launched) *as_launched = p;
   return HB_OK;
 }
@@ -647,7 +687,7 @@ extern "C" hb_status hb_orthogonalize(const void* update, int32_t type, int64_t 
   const int pairs = sms / 2 < kMostPairs ? sms / 2 : kMostPairs;
   auto sym_tiles = [&](int bn) { return batch * lower_tiles(lay.s, bn); };
   auto upd_tiles = [&](int bn) { return batch * ((lay.s + kPairRows - 1) / kPairRows) * ((lay.l + bn - 1) / bn); };
-  // groups' sums are kept for 32 columns per epilogue lane, which is 128 for the tile
+  // sums for 64 columns per epilogue lane, a tile of 256, do not fit its registers (8192 x 4096 float32: 13.1 ms)
   const int bn_sym = split ? tile_columns({128, 64}, pairs, sym_tiles) : tile_columns({256, 128, 64}, pairs, sym_tiles);
   const int bn_upd = split ? 128 : tile_columns({256, 128}, pairs, upd_tiles);
   CUtensorMap x_rows[2], x_cols[2], x_k[2], a_rows, a_cols, b_rows;
@@ -672,7 +712,6 @@ extern "C" hb_status hb_orthogonalize(const void* update, int32_t type, int64_t 
       p.M = static_cast<int32_t>(lay.s);
       p.N = static_cast<int32_t>(N);
       p.kblocks = static_cast<int32_t>((K + 63) / 64);
-      p.segments = kSplit ? 3 : 1;
       p.batches = static_cast<int32_t>(batch);
       p.splits = 1;
       p.status = status;
@@ -683,7 +722,7 @@ extern "C" hb_status hb_orthogonalize(const void* update, int32_t type, int64_t 
       p.lower = 1;
       p.splits = splits_of(batch, lay.s, K, kSplit, pairs);
       if (p.splits > 1) {
-        if (const hb_status e = launch<128, ShareOut>(p, {shares}, st, &p)) return e;
+        if (const hb_status e = launch<128, ShareOut<kSplit>>(p, {shares}, st, &p)) return e;
         HB_CUDA_TRY(hb::launch_overlapped(symmetric_sum_kernel<128>, dim3(static_cast<unsigned>(p.num_tiles / p.splits * (kPairRows / 32) * 4)), dim3(256), 0,
                                           st, p, ep, static_cast<const float*>(shares)));
         return HB_OK;
