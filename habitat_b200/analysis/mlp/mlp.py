@@ -5,8 +5,12 @@ reference's attribute names (fc1, mlp.layers.{0,2,...}, fc2, features) so its
 checkpoints ({"mu", "sigma", "model": state_dict}, mlp.py:133-146) load
 unchanged.  The modules only hold parameters: inference runs in the fused
 sm_100a kernel (habitat_b200/csrc/mlp_chain.cu) through `predict_batch`, and
-`predict` is that path with one query.  Training is out of scope.
+`predict` is that path with one query.  The reference's training loop
+(mlp.py:148-250) is not here; `update_hidden` is the step of the hidden layers for a loop of
+the caller's.
 """
+import functools
+
 import numpy as np
 import torch
 import torch.nn as nn
@@ -86,7 +90,9 @@ def state_to_arrays(model):
 
 
 class RuntimePredictor:
-    """mlp.py:112-146, 252-267: same constructor, attributes and predict()."""
+    """mlp.py:112-146, 252-267: same constructor, attributes and predict().
+
+    precision: "bf16", "bf16x3" (batched.MLPHandle) or "int8" (batched.Int8MLPHandle)."""
 
     def __init__(self, model_name, layers, layer_size, model_path=None, precision="bf16"):
         self.model_name = model_name
@@ -99,6 +105,7 @@ class RuntimePredictor:
         self.precision = precision
         self._handle = None
         self._device_rows = None
+        self._momentum = None
         if model_path is not None:
             self.load_state(model_path)
 
@@ -110,6 +117,7 @@ class RuntimePredictor:
         self.mu = checkpoint["mu"]
         self.sigma = checkpoint["sigma"]
         self.model.load_state_dict(checkpoint["model"])
+        self._momentum = None
         self.invalidate()
 
     def save_state(self, path):
@@ -121,11 +129,37 @@ class RuntimePredictor:
         self._handle = None
         self._device_rows = None
 
+    # -- retraining ---------------------------------------------------------
+    def update_hidden(self, lr, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5):
+        """Steps the hidden layers' weights along orthogonalised updates, from the gradients that a backward pass has left in
+        `model` (on a GPU, in float32; the reference's training loop does that with mlp.py:148-250): with g the gradients
+        and m the kept momentum, m <- momentum m + g, the update is g + momentum m (nesterov) or m, made nearly orthogonal
+        by `steps` Newton-Schulz steps (dense.orthogonalize, all layers in one call), and
+        w <- (1 - lr weight_decay) w - lr update.  Biases, fc1 and fc2 are left to the caller's optimizer.
+        The next prediction packs the new weights (`invalidate`)."""
+        from habitat_b200 import dense
+        weights = [block.weight for block in self.model.mlp.layers if isinstance(block, nn.Linear)]
+        if any(w.grad is None for w in weights):
+            raise RuntimeError("update_hidden needs the gradients of all hidden layers (run a backward pass first)")
+        if any(not w.is_cuda or w.dtype != torch.float32 for w in weights):
+            raise RuntimeError("update_hidden needs the model on a GPU, in float32")
+        with torch.no_grad():
+            g = torch.stack([w.grad for w in weights])
+            if self._momentum is None or self._momentum.shape != g.shape or self._momentum.device != g.device:
+                self._momentum = torch.zeros_like(g)
+            self._momentum.mul_(momentum).add_(g)
+            update = torch.add(g, self._momentum, alpha=momentum) if nesterov else self._momentum
+            step = dense.orthogonalize(update, steps=steps)
+            if weight_decay:
+                torch._foreach_mul_(weights, 1.0 - lr * weight_decay)
+            torch._foreach_add_(weights, list(step.unbind(0)), alpha=-lr)
+        self.invalidate()
+
     # -- inference ----------------------------------------------------------
     def _ensure_handle(self):
         if self._handle is not None:
             return
-        from habitat_b200.batched import MLPHandle
+        from habitat_b200.batched import Int8MLPHandle, MLPHandle
         if self.mu is None or self.sigma is None:
             raise RuntimeError("RuntimePredictor has no mu/sigma (load a checkpoint first)")
         devices = get_all_devices(self.device_params)
@@ -133,9 +167,9 @@ class RuntimePredictor:
         self._device_rows = {name: i for i, name in enumerate(names)}
         table = np.array([devices[n] for n in names], dtype=np.float64)
         arrays = state_to_arrays(self.model)
-        self._handle = MLPHandle(len(self.model.features), mu=np.asarray(self.mu, np.float64),
-                                 sigma=np.asarray(self.sigma, np.float64), device_features=table,
-                                 precision=self.precision, **arrays)
+        made = Int8MLPHandle if self.precision == "int8" else functools.partial(MLPHandle, precision=self.precision)
+        self._handle = made(len(self.model.features), mu=np.asarray(self.mu, np.float64),
+                            sigma=np.asarray(self.sigma, np.float64), device_features=table, **arrays)
 
     def device_row(self, device_name):
         self._ensure_handle()

@@ -374,11 +374,12 @@ class Predictor:
             kernel_metadata_file = default if os.path.exists(default) else None
         self._kernel_metadata = MetadataManager(kernel_metadata_file)
         self._wave_scaling_strategy = wave_scaling_strategy
-        # "bf16" (2e-2 relative against the float32 reference) or "bf16x3" (1e-4); the environment
-        # variable HABITAT_B200_PRECISION chooses for callers that keep the reference's constructor call
+        # "bf16" (2e-2 relative against the float32 reference), "bf16x3" (1e-4) or "int8" (large batches; see
+        # batched.Int8MLPHandle); the environment variable HABITAT_B200_PRECISION chooses for callers that keep the reference's
+        # constructor call
         self._precision = precision or os.environ.get("HABITAT_B200_PRECISION", "bf16")
-        if self._precision not in ("bf16", "bf16x3"):
-            raise ValueError("precision must be 'bf16' or 'bf16x3', got %r" % (self._precision,))
+        if self._precision not in ("bf16", "bf16x3", "int8"):
+            raise ValueError("precision must be 'bf16', 'bf16x3' or 'int8', got %r" % (self._precision,))
         self._model_paths = dict(model_paths or {})
         self._predictors = {}
 
@@ -496,7 +497,9 @@ class Predictor:
 
     @staticmethod
     def _is_plain(pred):
-        return getattr(pred.predict_batch, "__func__", None) is RuntimePredictor.predict_batch
+        # one of the fused kernels': 8-bit predictors are several launches and go through predict_batch
+        return (getattr(pred.predict_batch, "__func__", None) is RuntimePredictor.predict_batch
+                and getattr(pred, "precision", None) != "int8")
 
     def _has_registers(self):
         return self._kernel_metadata is not None and not getattr(self._kernel_metadata, "empty", False)

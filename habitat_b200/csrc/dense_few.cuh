@@ -9,6 +9,7 @@
 
 #include "dense_gemm.cuh"
 #include "dense_host.h"
+#include "dense_quant.cuh"
 
 namespace dense {
 namespace {

@@ -500,6 +500,19 @@ hb_status hb_int8_matmul_quantized(const int8_t* q, int64_t q_pitch, const float
 int64_t hb_int8_workspace_bytes(const int8_t* q, int64_t q_pitch, const int8_t* w, int64_t w_pitch, int64_t M, int64_t N,
                                 int64_t K, int32_t quantized);
 
+/* The two ends of a runtime predictor whose hidden layers are 8-bit (hb_mlp_create's network; the hidden layers are
+ * hb_int8_matmul_quantized calls).  hb_int8_mlp_input: queries as hb_mlp_predict takes them, normalised in float64, through fc1
+ * (w [width][F+4], b [width], float32 multiply-adds in the order of the inputs) and ReLU, as quantised rows.
+ * hb_int8_mlp_output: fc2 of quantised rows, out[i] = scales[i] * sum_k q[i][k] w[k] + b.  All pointers are DEVICE pointers;
+ * device_features is [n_device_rows][4], mu and sigma have F + 4 entries; a device_row beyond the table reads its last row.
+ * 1 <= F <= 8, 1 <= width <= 1024, rows of q on 16-byte boundaries. */
+hb_status hb_int8_mlp_input(const float* op_features, int32_t n_op_features, const uint8_t* device_row,
+                            const double* device_features, int32_t n_device_rows, const double* mu, const double* sigma,
+                            const float* w, const float* b, int64_t Q, int32_t width, int8_t* q, int64_t q_pitch, float* scales,
+                            void* stream);
+hb_status hb_int8_mlp_output(const int8_t* q, int64_t q_pitch, const float* scales, const float* w, const float* b, int64_t Q,
+                             int32_t width, float* out, void* stream);
+
 /* The update of a weight matrix with its singular values driven towards one by Newton-Schulz steps (nothing in the reference,
  * whose training loop, mlp.py:148-250, steps along plain gradients): X = G / (|G|_F + eps), then `steps` times
  * X <- (a I + b A + c A^2) X with A = X X^T (on G^T where rows > cols).  coefficients = {a, b, c} must keep the singular
