@@ -364,7 +364,7 @@ class Int8MLPHandle:
     error is that of 8-bit rows, about 1 % of a layer's spread per layer.  A call is one launch per layer, so batches of up to a few
     thousand queries are quicker in bf16.  Queries go through in pieces of `chunk`, whose rows are allocated through torch."""
 
-    chunk = 65536
+    chunk = 131072
 
     def __init__(self, n_op_features, fc1_w, fc1_b, hidden_w, hidden_b, fc2_w, fc2_b, mu, sigma, device_features):
         from habitat_b200 import dense

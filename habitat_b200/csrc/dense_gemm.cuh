@@ -380,11 +380,15 @@ gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ typename 
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
-  hb_grid_dependency_wait();   // the set-up above overlaps the end of the launch before it on the stream
+  if (threadIdx.x == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&p.a)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&p.b)) : "memory");
+  }
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();
   tc_fence_after();
+  hb_grid_dependency_wait();   // the set-up above overlaps the end of the launch before it on the stream
   const uint32_t tmem = tail->tmem;
 
   // a tile of the list per pair, or, where a cluster shares rows, per cluster (its pairs take neighbouring columns)

@@ -7,73 +7,117 @@ namespace {
 
 constexpr int kInputThreads = 256;       // four features each: up to 1,024
 constexpr int kInputQueries = 8;         // at a time
+constexpr int kInputDevices = 256;
+
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z, d;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 d, x, y, z;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
 
 // fc1 has at most 12 inputs: a thread keeps the weights of its four features in registers and walks over queries, eight between
-// barriers.  12 multiply-adds per result on the ordinary cores are 22 us for 65,536 queries, and the rows' 67 MB 10 us.
-__global__ void __launch_bounds__(kInputThreads)
+// barriers, while the next eight are loaded and normalised.  12 multiply-adds per result on the ordinary cores, in pairs, are
+// 11 us for 65,536 queries of 12 inputs, and the rows' 67 MB 10 us.
+__global__ void __launch_bounds__(kInputThreads, 2)
 mlp_input_kernel(const float* __restrict__ features, int n_op_feat, const uint8_t* __restrict__ device_row, const double* __restrict__ device_features,
                  int n_dev, const double* __restrict__ mu, const double* __restrict__ sigma, const float* __restrict__ w, const float* __restrict__ b,
                  int64_t Q, int width, int8_t* __restrict__ q, int64_t q_pitch, float* __restrict__ scales) {
-  __shared__ float x[kInputQueries][kMaxInFeat];
-  __shared__ float peak[kInputThreads / 32][kInputQueries];
+  __shared__ __align__(16) float x[2][kInputQueries][kMaxInFeat];
+  __shared__ __align__(16) float peak[2][kInputQueries][kInputThreads / 32];
+  static_assert(kInputQueries == 8 && kInputThreads == 256, "eight queries by eight warps");
+  __shared__ float devices[kInputDevices][4];                 // normalised
   const int tid = static_cast<int>(threadIdx.x), warp = tid >> 5, lane = tid & 31;
   const int inputs = n_op_feat + 4;
   hb_grid_dependency_wait();
-  float wr[4][kMaxInFeat], br[4];
+  float2 wr[2][kMaxInFeat], br[2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int f = 4 * tid + i;
-    br[i] = f < width ? b[f] : 0.0f;
+  for (int i = 0; i < 2; ++i) {
+    const int f = 4 * tid + 2 * i;
+    br[i] = make_float2(f < width ? b[f] : 0.0f, f + 1 < width ? b[f + 1] : 0.0f);
 #pragma unroll
-    for (int c = 0; c < kMaxInFeat; ++c) wr[i][c] = f < width && c < inputs ? w[f * inputs + c] : 0.0f;
+    for (int c = 0; c < kMaxInFeat; ++c)
+      wr[i][c] = make_float2(f < width && c < inputs ? w[f * inputs + c] : 0.0f, f + 1 < width && c < inputs ? w[(f + 1) * inputs + c] : 0.0f);
   }
-  for (int64_t q0 = static_cast<int64_t>(blockIdx.x) * kInputQueries; q0 < Q; q0 += static_cast<int64_t>(gridDim.x) * kInputQueries) {
-    __syncthreads();                     // the last queries' x and peak have been read
-    for (int e = tid; e < kInputQueries * kMaxInFeat; e += kInputThreads) {
-      const int k = e / kMaxInFeat, c = e - k * kMaxInFeat;
-      float v = 0.0f;
-      if (q0 + k < Q && c < inputs) {
-        int row = device_row[q0 + k];
-        row = row < n_dev ? row : n_dev - 1;
-        const double y = c < n_op_feat ? static_cast<double>(features[(q0 + k) * n_op_feat + c]) : device_features[row * 4 + c - n_op_feat];
-        v = static_cast<float>((y - mu[c]) / sigma[c]);
-      }
-      x[k][c] = v;
-    }
-    __syncthreads();
-    float y[kInputQueries][4];
+  for (int e = tid; e < 4 * n_dev; e += kInputThreads) {
+    const int c = n_op_feat + (e & 3);
+    devices[e >> 2][e & 3] = static_cast<float>((device_features[e] - mu[c]) / sigma[c]);
+  }
+  // thread e of the first 96 brings input e mod 12 of query e / 12
+  const int mine_k = tid / kMaxInFeat, mine_c = tid - mine_k * kMaxInFeat;
+  const bool brings = tid < kInputQueries * kMaxInFeat && mine_c < inputs;
+  const double mine_mu = brings ? mu[mine_c] : 0.0, mine_sigma = brings ? sigma[mine_c] : 1.0;
+  float raw = 0.0f;
+  int row = 0;
+  auto request = [&](int64_t q0) {
+    if (!brings || q0 + mine_k >= Q) return;
+    if (mine_c < n_op_feat) raw = features[(q0 + mine_k) * n_op_feat + mine_c];
+    else row = device_row[q0 + mine_k];
+  };
+  auto put = [&](int buf) {
+    if (!brings) return;
+    x[buf][mine_k][mine_c] = mine_c < n_op_feat ? static_cast<float>((static_cast<double>(raw) - mine_mu) / mine_sigma)
+                                                : devices[row < n_dev ? row : n_dev - 1][mine_c - n_op_feat];
+  };
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kInputQueries;
+  int64_t q0 = static_cast<int64_t>(blockIdx.x) * kInputQueries;
+  request(q0);
+  __syncthreads();                       // the devices
+  put(0);
+  __syncthreads();
+  for (int buf = 0; q0 < Q; q0 += step, buf ^= 1) {
+    request(q0 + step);
+    float2 y[kInputQueries][2];
+    float tops[kInputQueries];
 #pragma unroll
     for (int k = 0; k < kInputQueries; ++k) {
+      y[k][0] = br[0];
+      y[k][1] = br[1];
+      float xs[kMaxInFeat];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) y[k][i] = br[i];
+      for (int c = 0; c < kMaxInFeat; c += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(&x[buf][k][c]);
+        xs[c] = v.x; xs[c + 1] = v.y; xs[c + 2] = v.z; xs[c + 3] = v.w;
+      }
 #pragma unroll
       for (int c = 0; c < kMaxInFeat; ++c) {
-        const float v = x[k][c];
         if (c < inputs) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) y[k][i] = fmaf(wr[i][c], v, y[k][i]);
+          const float2 vv = make_float2(xs[c], xs[c]);
+          y[k][0] = fma2(wr[0][c], vv, y[k][0]);
+          y[k][1] = fma2(wr[1][c], vv, y[k][1]);
         }
       }
-      float m = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        y[k][i] = relu_nan(y[k][i]);
-        m = max_nan(m, y[k][i]);
-      }
-#pragma unroll
-      for (int d = 16; d; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
-      if (lane == 0) peak[warp][k] = m;
+      for (int i = 0; i < 2; ++i) y[k][i] = make_float2(relu_nan(y[k][i].x), relu_nan(y[k][i].y));
+      tops[k] = max_nan(max_nan(y[k][0].x, y[k][0].y), max_nan(y[k][1].x, y[k][1].y));
     }
+    // the warp's largest value of each query: halves of the queries over pairs of lanes, then what is left over all
+#pragma unroll
+    for (int n = kInputQueries / 2, d = 16; n; n /= 2, d /= 2) {
+      const bool upper = (lane & d) != 0;
+#pragma unroll
+      for (int i = 0; i < n; ++i) {
+        const float keep = upper ? tops[i + n] : tops[i], send = upper ? tops[i] : tops[i + n];
+        tops[i] = max_nan(keep, __shfl_xor_sync(0xFFFFFFFFu, send, d));
+      }
+    }
+    tops[0] = max_nan(tops[0], __shfl_xor_sync(0xFFFFFFFFu, tops[0], 2));
+    tops[0] = max_nan(tops[0], __shfl_xor_sync(0xFFFFFFFFu, tops[0], 1));
+    if ((lane & 3) == 0) peak[buf][lane >> 2][warp] = tops[0];      // lane bits 4, 3, 2 are the query's
+    put(buf ^ 1);
     __syncthreads();
+    // lane k mod 8 works out query k's scale for its warp
+    const float4 lo = *reinterpret_cast<const float4*>(peak[buf][lane & 7]), hi = *reinterpret_cast<const float4*>(&peak[buf][lane & 7][4]);
+    const RowScale s = row_scale(max_nan(max_nan(max_nan(lo.x, lo.y), max_nan(lo.z, lo.w)), max_nan(max_nan(hi.x, hi.y), max_nan(hi.z, hi.w))));
+    if (tid < kInputQueries && q0 + tid < Q) scales[q0 + tid] = s.scale;
+    const unsigned bad = __ballot_sync(0xFFFFFFFFu, s.bad);
 #pragma unroll
     for (int k = 0; k < kInputQueries; ++k) {
+      const float inverse = __shfl_sync(0xFFFFFFFFu, s.inverse, k);
       if (q0 + k >= Q) break;
-      float m = peak[0][k];
-#pragma unroll
-      for (int i = 1; i < kInputThreads / 32; ++i) m = max_nan(m, peak[i][k]);
-      const RowScale s = row_scale(m);
-      if (tid == 0) scales[q0 + k] = s.scale;
-      const uint32_t word = s.bad ? 0 : low_bytes(quantized(y[k][0], s.inverse), quantized(y[k][1], s.inverse), quantized(y[k][2], s.inverse), quantized(y[k][3], s.inverse));
+      const uint32_t word = bad >> k & 1u ? 0 : low_bytes(quantized(y[k][0].x, inverse), quantized(y[k][0].y, inverse), quantized(y[k][1].x, inverse),
+                                                          quantized(y[k][1].y, inverse));
       int8_t* to = q + (q0 + k) * q_pitch + 4 * tid;
       if (4 * tid + 4 <= width) {
         *reinterpret_cast<uint32_t*>(to) = word;
@@ -97,29 +141,45 @@ mlp_output_kernel(const int8_t* __restrict__ q, int64_t q_pitch, const float* __
     wr[i] = f < width ? w[f] : 0.0f;
   }
   const float bias = b[0];
-  for (int64_t row = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) >> 5; row < Q; row += static_cast<int64_t>(gridDim.x) * 8) {
-    float sum = 0.0f;
+  constexpr int kRows = 4;               // on their way at a time
+  for (int64_t row = ((static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) >> 5) * kRows; row < Q; row += static_cast<int64_t>(gridDim.x) * 8 * kRows) {
+    uint32_t ws[kRows][2][4];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int f = h * 512 + 16 * lane;
-      // the row's pitch is a multiple of 16; what lies behind its end has no weight, and is not read where nothing of the row is
-      if (f >= width) continue;
-      const int8_t* at = q + row * q_pitch + f;
-      uint32_t ws[4] = {0, 0, 0, 0};
-      if (f + 16 <= width) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(at));
-        ws[0] = v.x; ws[1] = v.y; ws[2] = v.z; ws[3] = v.w;
-      } else {
+    for (int r = 0; r < kRows; ++r)
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (f + i < width) ws[i >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(at[i])) << (8 * (i & 3));
+      for (int h = 0; h < 2; ++h) {
+        // the row's pitch is a multiple of 16; what lies behind its end has no weight, and is not read where nothing of the row is
+        const int f = h * 512 + 16 * lane;
+        const int8_t* at = q + (row + r) * q_pitch + f;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (row + r < Q) {
+          if (f + 16 <= width) {
+            v = __ldg(reinterpret_cast<const uint4*>(at));
+          } else if (f < width) {
+            uint32_t t[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (f + i < width) t[i >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(at[i])) << (8 * (i & 3));
+            v = make_uint4(t[0], t[1], t[2], t[3]);
+          }
+        }
+        ws[r][h][0] = v.x; ws[r][h][1] = v.y; ws[r][h][2] = v.z; ws[r][h][3] = v.w;
       }
+    float sums[kRows] = {};
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sum = fmaf(static_cast<float>(static_cast<int8_t>(ws[i >> 2] >> (8 * (i & 3)))), wr[16 * h + i], sum);
-    }
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
-    if (lane == 0) out[row] = fmaf(sum, scales[row], bias);
+      for (int i = 0; i < 16; ++i)
+#pragma unroll
+        for (int r = 0; r < kRows; ++r)
+          sums[r] = fmaf(static_cast<float>(static_cast<int8_t>(ws[r][h][i >> 2] >> (8 * (i & 3)))), wr[16 * h + i], sums[r]);
+#pragma unroll
+    for (int d = 16; d; d >>= 1)
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) sums[r] += __shfl_xor_sync(0xFFFFFFFFu, sums[r], d);
+#pragma unroll
+    for (int r = 0; r < kRows; ++r)
+      if (lane == r && row + r < Q) out[row + r] = fmaf(sums[r], scales[row + r], bias);
   }
 }
 
@@ -129,8 +189,9 @@ mlp_output_kernel(const int8_t* __restrict__ q, int64_t q_pitch, const float* __
 extern "C" hb_status hb_int8_mlp_input(const float* op_features, int32_t n_op_features, const uint8_t* device_row, const double* device_features,
                                        int32_t n_device_rows, const double* mu, const double* sigma, const float* w, const float* b, int64_t Q,
                                        int32_t width, int8_t* q, int64_t q_pitch, float* scales, void* stream) {
-  if (Q < 0 || n_op_features < 1 || n_op_features + 4 > kMaxInFeat || width < 1 || width > 1024 || n_device_rows < 1) {
-    hb::set_error("hb_int8_mlp_input: 1 <= F <= 8, 1 <= width <= 1024, at least one device row");
+  if (Q < 0 || n_op_features < 1 || n_op_features + 4 > kMaxInFeat || width < 1 || width > 1024 || n_device_rows < 1 ||
+      n_device_rows > dense::kInputDevices) {
+    hb::set_error("hb_int8_mlp_input: 1 <= F <= 8, 1 <= width <= 1024, 1 to 256 device rows");
     return HB_ERR_UNSUPPORTED;
   }
   if (Q == 0) return HB_OK;
@@ -162,7 +223,7 @@ extern "C" hb_status hb_int8_mlp_output(const int8_t* q, int64_t q_pitch, const 
   }
   int sms = 0;
   if (const hb_status st = dense::sm_count(&sms)) return st;
-  const int64_t blocks = (Q + 7) / 8 < 8 * sms ? (Q + 7) / 8 : 8 * sms;
+  const int64_t blocks = (Q + 31) / 32 < 4 * sms ? (Q + 31) / 32 : 4 * sms;
   HB_CUDA_TRY(hb::launch_overlapped(dense::mlp_output_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, static_cast<cudaStream_t>(stream), q, q_pitch,
                                     scales, w, b, Q, width, out));
   return HB_OK;

@@ -505,7 +505,7 @@ int64_t hb_int8_workspace_bytes(const int8_t* q, int64_t q_pitch, const int8_t* 
  * (w [width][F+4], b [width], float32 multiply-adds in the order of the inputs) and ReLU, as quantised rows.
  * hb_int8_mlp_output: fc2 of quantised rows, out[i] = scales[i] * sum_k q[i][k] w[k] + b.  All pointers are DEVICE pointers;
  * device_features is [n_device_rows][4], mu and sigma have F + 4 entries; a device_row beyond the table reads its last row.
- * 1 <= F <= 8, 1 <= width <= 1024, rows of q on 16-byte boundaries. */
+ * 1 <= F <= 8, 1 <= width <= 1024, at most 256 device rows, rows of q on 16-byte boundaries. */
 hb_status hb_int8_mlp_input(const float* op_features, int32_t n_op_features, const uint8_t* device_row,
                             const double* device_features, int32_t n_device_rows, const double* mu, const double* sigma,
                             const float* w, const float* b, int64_t Q, int32_t width, int8_t* q, int64_t q_pitch, float* scales,
