@@ -1547,7 +1547,8 @@ struct Matrix {
     rows = x.size(0);
     cols = x.size(1);
     if (cols > 1 && x.stride(1) != 1) return;
-    pitch = rows > 1 ? x.stride(0) : cols;
+    // one row has no pitch: any will do, and a multiple of 16 never needs a copy
+    pitch = rows > 1 ? x.stride(0) : (cols + 15) / 16 * 16;
     if (pitch < cols) return;
     t = &x;
   }

@@ -67,7 +67,7 @@ __device__ __forceinline__ uint4 load_piece(const int8_t* row, int k, int K) {
 // kAligned: the channels' rows start on 16 bytes (the tokens' always do).  kTiles: groups of eight rows; kChannels: tiles of 16 channels per block; kSplits: warps that share a tile's K.  kQuant: a cluster has
 // all channels and the result leaves as quantised rows.
 template <int kTiles, int kChannels, int kSplits, bool kQuant, bool kAligned>
-__global__ void __launch_bounds__(32 * kChannels * kSplits) few_rows_kernel(const __grid_constant__ FewParams p) {
+__global__ void __launch_bounds__(32 * kChannels * kSplits, kChannels == 1 && kTiles == 1 ? 4 : 1) few_rows_kernel(const __grid_constant__ FewParams p) {
   constexpr int kWarps = kChannels * kSplits, kRows = 8 * kTiles;
   __shared__ int sums[kSplits > 1 ? kWarps : 1][kTiles][4][32];
   __shared__ float peak[8][kRows];           // largest magnitudes of each CTA of the cluster

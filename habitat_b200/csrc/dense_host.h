@@ -21,6 +21,10 @@ hb_status begin_call(const char* name, int32_t** word);
 
 hb_status sm_count(int* sms);
 
+// Whether arrays of elements of these sizes can start at these addresses.
+inline bool starts_on(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(bytes) == 0; }
+inline int bytes_of(int32_t type) { return type == HB_F32 ? 4 : 2; }
+
 }  // namespace dense
 
 #if defined(__CUDACC__)

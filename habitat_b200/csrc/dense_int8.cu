@@ -92,8 +92,9 @@ quantize_vec_kernel(const T* __restrict__ x, int64_t rows, int cols, int64_t pit
   }
 }
 
-// Rows that start anywhere, or are longer than a block's registers: element by element, read twice (the second time from
-// cache).
+// Rows that start anywhere, or are longer than a block's registers: element by element, TPR threads per row with up to eight
+// elements each in registers; longer rows are read twice (the second time from cache).
+constexpr int kAnyElements = 8;
 template <typename T, int TPR>
 __global__ void __launch_bounds__(kQuantThreads)
 quantize_any_kernel(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t pitch, int8_t* __restrict__ q, int64_t q_pitch,
@@ -104,14 +105,27 @@ quantize_any_kernel(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t
   if (row >= rows) return;
   const int t = static_cast<int>(threadIdx.x) % TPR;
   const T* xr = x + row * pitch;
+  int8_t* qr = q + row * q_pitch;
   float amax = 0.0f;
+  if (cols <= TPR * kAnyElements) {
+    float v[kAnyElements];
+#pragma unroll
+    for (int i = 0; i < kAnyElements; ++i) v[i] = i * TPR + t < cols ? to_float(xr[i * TPR + t]) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < kAnyElements; ++i) amax = max_nan(amax, fabsf(v[i]));
+    const RowScale s = row_scale(row_max<TPR>(amax, scratch));
+    if (t == 0) scales[row] = s.scale;
+#pragma unroll
+    for (int i = 0; i < kAnyElements; ++i)
+      if (i * TPR + t < cols) qr[i * TPR + t] = s.bad ? 0 : static_cast<int8_t>(quantized(v[i], s.inverse));
+    return;
+  }
 #pragma unroll 4
   for (int64_t i = t; i < cols; i += TPR) amax = max_nan(amax, fabsf(to_float(xr[i])));
   const RowScale s = row_scale(row_max<TPR>(amax, scratch));
   if (t == 0) scales[row] = s.scale;
 #pragma unroll 4
-  for (int64_t i = t; i < cols; i += TPR)
-    q[row * q_pitch + i] = s.bad ? 0 : static_cast<int8_t>(quantized(to_float(xr[i]), s.inverse));
+  for (int64_t i = t; i < cols; i += TPR) qr[i] = s.bad ? 0 : static_cast<int8_t>(quantized(to_float(xr[i]), s.inverse));
 }
 
 template <typename T, int VB>
@@ -143,9 +157,10 @@ cudaError_t launch_quantize(const void* x, int64_t rows, int64_t cols, int64_t p
     return hb::launch_overlapped(vec, dim3(static_cast<unsigned>((rows + per - 1) / per)), dim3(kQuantThreads), 0, s, xt, rows,
                                  static_cast<int>(cols), pitch, q, q_pitch, scales);
   }
-  // single elements: a warp per row up to 512 of them
-  const int64_t per = cols <= 512 ? kQuantThreads / 32 : 1;
-  return hb::launch_overlapped(cols <= 512 ? quantize_any_kernel<T, 32> : quantize_any_kernel<T, kQuantThreads>,
+  // single elements: a warp per row while its registers hold one
+  const bool warp_row = cols <= 32 * kAnyElements;
+  const int64_t per = warp_row ? kQuantThreads / 32 : 1;
+  return hb::launch_overlapped(warp_row ? quantize_any_kernel<T, 32> : quantize_any_kernel<T, kQuantThreads>,
                                dim3(static_cast<unsigned>((rows + per - 1) / per)), dim3(kQuantThreads), 0, s, xt, rows, cols, pitch, q,
                                q_pitch, scales);
 }
@@ -414,7 +429,7 @@ struct Operands {
 };
 
 hb_status check_product(const char* name, const int8_t* q, int64_t q_pitch, const float* q_scales, const int8_t* w, int64_t w_pitch,
-                        const float* w_scales, int64_t M, int64_t N, int64_t K) {
+                        const float* w_scales, const float* bias, int64_t M, int64_t N, int64_t K) {
   if (M < 0 || N < 0 || K < 1 || q_pitch < K || w_pitch < K) {
     hb::set_error("%s: M and N must not be negative, K at least 1, pitches at least K", name);
     return HB_ERR_INVALID_ARGUMENT;
@@ -427,14 +442,20 @@ hb_status check_product(const char* name, const int8_t* q, int64_t q_pitch, cons
     hb::set_error("%s: NULL argument", name);
     return HB_ERR_INVALID_ARGUMENT;
   }
+  if (!starts_on(q_scales, 4) || !starts_on(w_scales, 4) || !starts_on(bias, 4)) {
+    hb::set_error("%s: scales and biases start on 4-byte boundaries", name);
+    return HB_ERR_INVALID_ARGUMENT;
+  }
   return HB_OK;
 }
 
 int64_t align_bytes(int64_t rows, int64_t K, bool aligned) { return aligned ? 0 : round_up(rows * round_up(K, 16), 256); }
 
-// Quantised results that take two launches: rows wider than a cluster of eight holds, and few rows with so many columns that
-// eight SMs cannot read the weights in the time (1 x 1024 x 8192: 20 us in one launch, 7 in two).
-bool through_memory(int64_t M, int64_t N, int64_t K) { return N > 1024 || (M <= kFewRows && K > 2048); }
+// Quantised results that take two launches, through float32 rows in memory: rows wider than a cluster of eight holds; few rows with
+// so many columns that eight SMs cannot read the weights in the time (1 x 1024 x 8192: 20 us in one launch, 7 in two);
+// and batches of up to two rounds of 256 rows, for which one cluster's SMs are the whole launch (127 rows through eight 1024-wide
+// layers: 63 us in one launch each, 56 in two; 1,024 rows: 66 and 67).
+bool through_memory(int64_t M, int64_t N, int64_t K) { return N > 1024 || (M <= kFewRows ? K > 2048 : M <= 512); }
 
 // Operands that TMA can read: as they are, or copied to the workspace.
 hb_status align_operands(const char* name, Operands* o, int64_t M, int64_t N, int64_t K, uint8_t* workspace, int64_t workspace_bytes,
@@ -620,8 +641,8 @@ extern "C" hb_status hb_quantize_rows(const void* x, int32_t x_type, int64_t row
     return HB_ERR_INVALID_ARGUMENT;
   }
   if (rows == 0) return HB_OK;
-  if (!x || !q || !scales) {
-    hb::set_error("hb_quantize_rows: NULL argument");
+  if (!x || !q || !scales || !dense::starts_on(x, dense::bytes_of(x_type)) || !dense::starts_on(scales, 4)) {
+    hb::set_error("hb_quantize_rows: NULL argument, or one that does not start on a boundary of its type");
     return HB_ERR_INVALID_ARGUMENT;
   }
   if (rows > dense::kMostRows) {
@@ -648,9 +669,9 @@ extern "C" hb_status hb_int8_matmul(const int8_t* q, int64_t q_pitch, const floa
                                     int32_t out_type, int64_t out_pitch, void* workspace, int64_t workspace_bytes, void* stream) {
   using namespace dense;
   const char* name = "hb_int8_matmul";
-  if (const hb_status st = check_product(name, q, q_pitch, q_scales, w, w_pitch, w_scales, M, N, K)) return st;
-  if (out_type < HB_F32 || out_type > HB_F16 || out_pitch < N || (M && N && !out)) {
-    hb::set_error("%s: out has to be given, with a pitch of at least N and a type of 0 to 2", name);
+  if (const hb_status st = check_product(name, q, q_pitch, q_scales, w, w_pitch, w_scales, bias, M, N, K)) return st;
+  if (out_type < HB_F32 || out_type > HB_F16 || out_pitch < N || (M && N && !out) || !starts_on(out, bytes_of(out_type))) {
+    hb::set_error("%s: out has to be given, on a boundary of its type (0 to 2), with a pitch of at least N", name);
     return HB_ERR_INVALID_ARGUMENT;
   }
   int32_t* status = nullptr;
@@ -681,8 +702,8 @@ extern "C" hb_status hb_int8_matmul_quantized(const int8_t* q, int64_t q_pitch, 
                                               void* stream) {
   using namespace dense;
   const char* name = "hb_int8_matmul_quantized";
-  if (const hb_status st = check_product(name, q, q_pitch, q_scales, w, w_pitch, w_scales, M, N, K)) return st;
-  if (M && (N < 1 || !out || !out_scales || !tma_rows(out, out_pitch) || out_pitch < N)) {
+  if (const hb_status st = check_product(name, q, q_pitch, q_scales, w, w_pitch, w_scales, bias, M, N, K)) return st;
+  if (M && (N < 1 || !out || !out_scales || !tma_rows(out, out_pitch) || out_pitch < N || !starts_on(out_scales, 4))) {
     hb::set_error("%s: out and out_scales have to be given, N at least 1, out's rows on 16-byte boundaries", name);
     return HB_ERR_INVALID_ARGUMENT;
   }

@@ -217,7 +217,7 @@ extern "C" hb_status hb_int8_mlp_output(const int8_t* q, int64_t q_pitch, const 
     return HB_ERR_UNSUPPORTED;
   }
   if (Q == 0) return HB_OK;
-  if (!q || !scales || !w || !b || !out || q_pitch < width || q_pitch % 16 || reinterpret_cast<uintptr_t>(q) % 16) {
+  if (!q || !scales || !w || !b || !out || !dense::starts_on(out, 4) || q_pitch < width || q_pitch % 16 || reinterpret_cast<uintptr_t>(q) % 16) {
     hb::set_error("hb_int8_mlp_output: NULL argument, or rows of q that do not start on 16-byte boundaries");
     return HB_ERR_INVALID_ARGUMENT;
   }

@@ -599,8 +599,8 @@ extern "C" hb_status hb_orthogonalize(const void* update, int32_t type, int64_t 
   int32_t* status = nullptr;
   if (const hb_status st = begin_call(name, &status)) return st;
   if (batch == 0 || rows == 0 || cols == 0) return HB_OK;
-  if (!update || !out) {
-    hb::set_error("%s: NULL argument", name);
+  if (!update || !out || !starts_on(update, bytes_of(type)) || !starts_on(out, bytes_of(type))) {
+    hb::set_error("%s: NULL argument, or one that does not start on a boundary of its type", name);
     return HB_ERR_INVALID_ARGUMENT;
   }
   if (rows > (1 << 24) || cols > (1 << 24) || batch > 65535 || batch * 2 > 0x7FFFFFFF) {

@@ -81,6 +81,33 @@ def test_orthogonalize_refuses(bad):
     assert b"hb_orthogonalize" in _native.load().hb_last_error()
 
 
+def test_misaligned_arguments_are_refused():
+    lib = _native.load()
+    assert _matmul(out=18) == _native.HB_ERR_INVALID_ARGUMENT                  # float32 on a 2-byte boundary
+    assert _matmul(out=17, out_type=1) == _native.HB_ERR_INVALID_ARGUMENT
+    for at in range(3):
+        scales, w_scales, bias = (18 if i == at else 16 for i in range(3))
+        assert lib.hb_int8_matmul(P(16), 16, P(scales), P(16), 16, P(w_scales), P(bias), 0, 4, 4, 16, P(16), 0, 4, None, 0,
+                                  None) == _native.HB_ERR_INVALID_ARGUMENT
+    assert lib.hb_quantize_rows(P(18), 0, 4, 16, 16, P(16), 16, P(16), None) == _native.HB_ERR_INVALID_ARGUMENT
+    assert lib.hb_quantize_rows(P(16), 0, 4, 16, 16, P(16), 16, P(18), None) == _native.HB_ERR_INVALID_ARGUMENT
+    for misplaced in ((P(17), P(16)), (P(16), P(17))):
+        status = lib.hb_int8_mlp_output(misplaced[0], 16, P(16), P(16), P(16), 4, 16, misplaced[1], None)
+        assert status == _native.HB_ERR_INVALID_ARGUMENT
+
+
+def test_predictor_ends_refuse():
+    lib = _native.load()
+
+    def put_in(F=4, rows=6, width=64, q=16, pitch=64, Q=3):
+        return lib.hb_int8_mlp_input(P(16), F, P(16), P(16), rows, P(16), P(16), P(16), P(16), Q, width, P(q), pitch, P(16), None)
+    for bad in (dict(F=0), dict(F=9), dict(rows=0), dict(rows=257), dict(width=0), dict(width=1025), dict(Q=-1)):
+        assert put_in(**bad) == _native.HB_ERR_UNSUPPORTED
+    for bad in (dict(q=0), dict(q=24), dict(pitch=63), dict(pitch=72)):
+        assert put_in(**bad) == _native.HB_ERR_INVALID_ARGUMENT
+    assert put_in(Q=0, q=0) == _native.HB_OK
+
+
 def test_host_tensors_are_refused():
     x = torch.zeros((4, 16))
     q, s = torch.zeros((4, 16), dtype=torch.int8), torch.zeros((4,))

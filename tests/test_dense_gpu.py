@@ -162,6 +162,32 @@ def test_int8_matmul_rows_that_start_anywhere(m):
     assert torch.equal(got.cpu(), want)
 
 
+@pytest.mark.parametrize("k", [1, 15, 16, 17, 40, 63, 64, 65, 200, 777])
+def test_int8_matmul_few_rows_of_weights_that_start_anywhere(k):
+    """The kernel for up to 16 rows reads unaligned weights as they are, in whole words: every start, every end."""
+    g = np.random.default_rng(k)
+    for m in (1, 9):
+        q, s, w, ws, b = _layer(m, 37, k, 11 + m)
+        want = torch.from_numpy(_product(q, s, w, ws, b, True))
+        for start in range(5):
+            room = torch.from_numpy(g.integers(-128, 128, size=37 * (k + 3) + 8, dtype=np.int8)).cuda()
+            view = room[start:start + 37 * (k + 3)].view(37, k + 3)[:, :k]
+            view.copy_(torch.from_numpy(w))
+            got = dense.int8_matmul(*_cuda(q, s), view, *_cuda(ws, b), relu=True)
+            assert torch.equal(got.cpu(), want), (m, start)
+            got_q, got_s = dense.int8_matmul_quantized(*_cuda(q, s), view, *_cuda(ws, b), relu=True)
+            want_q, want_s = _quantized(want.numpy())
+            assert np.array_equal(got_q.cpu().numpy(), want_q) and np.array_equal(got_s.cpu().numpy(), want_s)
+
+
+@pytest.mark.parametrize("m, k", [(1, 3000), (16, 2100), (17, 300), (512, 300), (513, 300), (300, 3000)])
+def test_int8_matmul_quantized_in_one_launch_and_in_two(m, k):
+    arrays = _layer(m, 900, k, m + k)
+    q, s = dense.int8_matmul_quantized(*_cuda(*arrays[:4]), bias=_cuda(arrays[4])[0], relu=True)
+    want_q, want_s = _quantized(_product(*arrays, True))
+    assert np.array_equal(s.cpu().numpy(), want_s) and np.array_equal(q.cpu().numpy(), want_q)
+
+
 def test_int8_matmul_of_nothing():
     q, s, w, ws, b = _cuda(*_layer(4, 6, 16, 1))
     assert dense.int8_matmul(q[:0], s[:0], w, ws, b).shape == (0, 6)
@@ -291,6 +317,15 @@ def test_orthogonalize(shape, dtype):
     _check(update, got)
 
 
+# the shorter side around what is kept on chip (32, 128), the longer one around what a cluster holds of it
+@pytest.mark.parametrize("shape", [(32, 33), (33, 32), (32, 10048), (32, 10400), (31, 30000), (1, 70000), (5, 40000), (20000, 20), (128, 129), (129, 128),
+                                   (128, 3300), (128, 6000), (9000, 100), (70, 14000), (130, 9000), (2, 160, 5000), (300, 256), (520, 700)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_orthogonalize_long_and_short_sides(shape, dtype):
+    update = _update(shape, sum(shape), dtype)
+    _check(update, dense.orthogonalize(update))
+
+
 @pytest.mark.parametrize("steps, coefficients", [(1, COEFFICIENTS), (2, COEFFICIENTS), (3, (1.5, -0.5, 0.0)), (10, (1.875, -1.25, 0.375))])
 def test_orthogonalize_steps_and_coefficients(steps, coefficients):
     for dtype in (torch.float32, torch.bfloat16):
@@ -363,6 +398,35 @@ def test_on_another_stream_and_in_a_graph():
     torch.cuda.synchronize()
     for out in outs:
         assert all(torch.equal(a, e) for a, e in zip(out, want))
+
+
+def test_first_use_of_a_kernel_inside_a_capture():
+    """One call sets up the GPU's status word; whatever kernel a later capture is the first to use may be captured."""
+    code = """
+import torch
+from habitat_b200 import dense
+w, s = torch.ones((600, 64), dtype=torch.int8, device="cuda"), torch.ones((600,), device="cuda")
+q, qs = dense.quantize_rows(torch.ones((1, 64), device="cuda"))
+dense.int8_matmul(q, qs, w, s)
+x, u, v, t = (torch.randn(n, device="cuda") for n in ((700, 64), (300, 200), (100, 90), (20, 30)))
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    a = dense.quantize_rows(x)
+    b = dense.int8_matmul_quantized(*a, w, s)
+    c = dense.int8_matmul(*a, w, s, out_dtype=torch.bfloat16)
+    d = [dense.orthogonalize(y) for y in (u, v, t)]
+g.replay()
+torch.cuda.synchronize()
+assert torch.equal(c, dense.int8_matmul(*dense.quantize_rows(x), w, s, out_dtype=torch.bfloat16))
+assert all(torch.equal(y, dense.orthogonalize(z)) for y, z in zip(d, (u, v, t)))
+assert torch.equal(b[0], dense.int8_matmul_quantized(*a, w, s)[0])
+"""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
 
 
 def test_two_streams_at_once_and_repeated_calls_agree():
