@@ -122,6 +122,12 @@ def test_predictor_precision_and_trace(monkeypatch):
     plain.mu, plain.sigma = pred.mu, pred.sigma
     value, close = pred.predict([1, 64, 512, 256], "V100"), plain.predict([1, 64, 512, 256], "V100")
     assert isinstance(value, float) and abs(value - close) <= 0.02 * abs(close)
+    # a trace: the operation's measured time by the ratio of the predictions (predictor.py:132-148 of the reference)
+    operation = MeasuredOperation("linear", Arguments(((64, 512), (256, 512), None), {}), RunTimeMeasurement(3.0, [], Device.V100), None, Device.V100)
+    there = {d: 3.0 * pred.predict([0, 64, 512, 256], d.name) / pred.predict([0, 64, 512, 256], "V100") for d in (Device.T4, Device.P100)}
+    traces = Trace(Device.V100, [operation]).to_devices(list(there), predictor)
+    for device, trace in zip(there, traces):
+        assert abs(trace.run_time_ms - there[device]) <= 1e-6 * there[device]
 
 
 def test_retrained_and_served_in_8_bits():
