@@ -188,6 +188,24 @@ def test_int8_matmul_quantized_in_one_launch_and_in_two(m, k):
     assert np.array_equal(s.cpu().numpy(), want_s) and np.array_equal(q.cpu().numpy(), want_q)
 
 
+@pytest.mark.parametrize("m, n, k", [(19000, 1000, 200), (18433, 1024, 1024), (38000, 300, 77), (76000, 200, 64)])
+def test_int8_matmul_long_batches(m, n, k):
+    """Weights that stay in shared memory for all of an SM pair's rows."""
+    arrays = _layer(m, n, k, m + n)
+    got = dense.int8_matmul(*_cuda(*arrays[:4]), bias=_cuda(arrays[4])[0], relu=True, out_dtype=torch.bfloat16)
+    dense.check_status()
+    assert torch.equal(got.cpu(), torch.from_numpy(_product(*arrays, True)).to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("m, n, k", [(15361, 1000, 200), (20000, 1024, 1024), (21000, 700, 90), (31000, 500, 64), (62000, 130, 40)])
+def test_int8_matmul_quantized_long_batches(m, n, k):
+    arrays = _layer(m, n, k, m + n)
+    q, s = dense.int8_matmul_quantized(*_cuda(*arrays[:4]), bias=_cuda(arrays[4])[0], relu=True)
+    want_q, want_s = _quantized(_product(*arrays, True))
+    dense.check_status()
+    assert np.array_equal(s.cpu().numpy(), want_s) and np.array_equal(q.cpu().numpy(), want_q)
+
+
 def test_int8_matmul_of_nothing():
     q, s, w, ws, b = _cuda(*_layer(4, 6, 16, 1))
     assert dense.int8_matmul(q[:0], s[:0], w, ws, b).shape == (0, 6)
