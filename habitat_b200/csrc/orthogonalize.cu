@@ -526,9 +526,9 @@ struct GramPlan {
 GramPlan gram_plan(int64_t s, int64_t l, int widest) {
   GramPlan r{0, 0, 0};
   if (s < 1 || s > kGramSide) return r;
-  const int s4 = static_cast<int>(up(s, 4));
+  const int S = static_cast<int>(up(s, 8));
   for (int ctas = 1; ctas <= widest; ctas *= 2) {
-    const int64_t columns = (l + ctas - 1) / ctas, smem = gram_smem(s4, columns);
+    const int64_t columns = (l + ctas - 1) / ctas, smem = gram_smem(S, columns);
     if (smem > kSideSmem || (columns > 128 && ctas < widest)) continue;
     r.ctas = ctas;
     r.columns = static_cast<int>(columns);
@@ -616,28 +616,27 @@ extern "C" hb_status hb_orthogonalize(const void* update, int32_t type, int64_t 
   const Source g{update, pitch, batch_stride, type, static_cast<int32_t>(rows), static_cast<int32_t>(cols)};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   {
-    static std::atomic<int> held[64], widest[64];
-    int most = 0;
-    if (const hb_status e = widest_cluster(gram_side_kernel, kGramThreads, kSideSmem, held, widest, &most)) return e;
     const int64_t s = rows < cols ? rows : cols, l = rows < cols ? cols : rows;
-    const GramPlan plan = gram_plan(s, l, most);
-    if (plan.ctas && batch * plan.ctas <= 0x7FFFFFFF) {
-      GramParams p{};
-      p.g = g;
-      p.out = Out{out, out_pitch, out_batch_stride, type, 0};
-      p.s = static_cast<int32_t>(s);
-      p.l = static_cast<int32_t>(l);
-      p.s4 = static_cast<int32_t>(up(s, 4));
-      p.columns = plan.columns;
-      p.flip = flip;
-      p.steps = steps;
-      p.a = a;
-      p.b = b;
-      p.c = c;
-      p.eps = eps;
-      HB_CUDA_TRY(launch_clusters(gram_side_kernel, static_cast<int>(batch), plan.ctas, kGramThreads, plan.smem, st, p));
+    bool launched = false;
+    auto gram = [&](auto size) -> hb_status {
+      constexpr int S = decltype(size)::value;
+      static std::atomic<int> held[64], widest[64];
+      int most = 0;
+      if (const hb_status e = widest_cluster(gram_side_kernel<S>, kGramThreads, kSideSmem, held, widest, &most)) return e;
+      const GramPlan plan = gram_plan(s, l, most);
+      if (!plan.ctas || batch * plan.ctas > 0x7FFFFFFF) return HB_OK;
+      const GramParams p{g, Out{out, out_pitch, out_batch_stride, type, 0}, static_cast<int32_t>(s), static_cast<int32_t>(l), plan.columns, flip, steps,
+                         a, b, c, eps};
+      HB_CUDA_TRY(launch_clusters(gram_side_kernel<S>, static_cast<int>(batch), plan.ctas, kGramThreads, plan.smem, st, p));
+      launched = true;
       return HB_OK;
-    }
+    };
+    hb_status e = HB_OK;
+    if (s <= 8) e = gram(std::integral_constant<int, 8>{});
+    else if (s <= 16) e = gram(std::integral_constant<int, 16>{});
+    else if (s <= 24) e = gram(std::integral_constant<int, 24>{});
+    else if (s <= 32) e = gram(std::integral_constant<int, 32>{});
+    if (e != HB_OK || launched) return e;
   }
   if (const SidePlan plan = side_plan(rows, cols, split != 0); plan.ctas) {
     SideParams p{};

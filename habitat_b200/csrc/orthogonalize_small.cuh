@@ -457,13 +457,14 @@ constexpr int kGramThreads = 256;
 struct GramParams {
   Source g;
   Out out;
-  int32_t s, l, s4, columns, flip, steps;   // s4: s rounded up to 4; columns: of X, per CTA
+  int32_t s, l, columns, flip, steps;       // columns: of X, per CTA
   double a, b, c, eps;
 };
 
-constexpr int kGramMatrix = kGramSide * (kGramSide + 1);     // doubles
-constexpr int kGramFixed = (4 * kGramMatrix + kGramThreads * 16) * 8;
-inline int64_t gram_smem(int s4, int64_t columns) { return kGramFixed + columns * (s4 + 1) * 8; }
+constexpr int kGramPitch = kGramSide + 2;                     // rows of doubles start on 16 bytes, eight of them in different banks
+constexpr int kGramMatrix = kGramSide * kGramPitch;           // doubles
+constexpr int kGramFixed = (5 * kGramMatrix + kGramThreads * 16) * 8;
+inline int64_t gram_smem(int S, int64_t columns) { return kGramFixed + columns * (S + 2) * 8; }
 
 __device__ __forceinline__ double2 ld_cluster_d2(uint32_t addr) {
   double2 v;
@@ -471,17 +472,22 @@ __device__ __forceinline__ double2 ld_cluster_d2(uint32_t addr) {
   return v;
 }
 
+// S: s rounded up to a multiple of eight, so that loops over it are unrolled (loads of a whole row on their way at once).
+template <int S>
 __global__ void __launch_bounds__(kGramThreads) gram_side_kernel(const __grid_constant__ GramParams p) {
   extern __shared__ double smem_d[];
-  const int tid = static_cast<int>(threadIdx.x);
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
   const int rank = static_cast<int>(cluster_ctarank()), ctas = static_cast<int>(cluster_size());
   const int matrix = static_cast<int>(blockIdx.x) / ctas;
-  const int s = p.s, s4 = p.s4, pitch = s4 + 1;
-  constexpr int kPitch = kGramSide + 1;
-  double* part = smem_d;                               // sums of threads; [256][16]
-  double* share = part + kGramThreads * 16;            // this CTA's share of A, then A
-  double* mat[3] = {share + kGramMatrix, share + 2 * kGramMatrix, share + 3 * kGramMatrix};
-  double* x = share + 4 * kGramMatrix;                 // [column][pitch]
+  const int s = p.s;
+  constexpr int kX = S + 2, kPitch = kGramPitch;
+  double* part = smem_d;                               // sums of threads; [16][256]
+  double* share = part + kGramThreads * 16;            // this CTA's share of A
+  double* A = share + kGramMatrix;
+  double* B = A + kGramMatrix;
+  double* P = B + kGramMatrix;                         // and the next one behind it
+  double* T = part;                                    // the threads' sums are used up by then
+  double* x = share + 5 * kGramMatrix;                 // [column][kX]
   hb_grid_dependency_wait();
 
   // ---- this CTA's columns of X ----
@@ -490,34 +496,36 @@ __global__ void __launch_bounds__(kGramThreads) gram_side_kernel(const __grid_co
   if (p.flip) {
     // rows of G are columns of X
 #pragma unroll 8
-    for (int e = tid; e < cols * s4; e += kGramThreads) {
-      const int c = e / s4, r = e - c * s4;
-      x[c * pitch + r] = r < s ? static_cast<double>(load_element(p.g.base, p.g.type, g0 + static_cast<int64_t>(c0 + c) * p.g.ld + r)) : 0.0;
+    for (int e = tid; e < cols * S; e += kGramThreads) {
+      const int c = e / S, r = e - c * S;
+      x[c * kX + r] = r < s ? static_cast<double>(load_element(p.g.base, p.g.type, g0 + static_cast<int64_t>(c0 + c) * p.g.ld + r)) : 0.0;
     }
   } else {
-    const int lane = tid & 31, warp = tid >> 5;
-    for (int r = warp; r < s4; r += kGramThreads / 32)
+#pragma unroll
+    for (int r0 = 0; r0 < S; r0 += kGramThreads / 32) {
+      const int r = r0 + warp;
 #pragma unroll 4
       for (int c = lane; c < cols; c += 32)
-        x[c * pitch + r] = r < s ? static_cast<double>(load_element(p.g.base, p.g.type, g0 + static_cast<int64_t>(r) * p.g.ld + c0 + c)) : 0.0;
+        x[c * kX + r] = r < s ? static_cast<double>(load_element(p.g.base, p.g.type, g0 + static_cast<int64_t>(r) * p.g.ld + c0 + c)) : 0.0;
+    }
   }
   __syncthreads();
 
   // ---- its share of A: 4 x 4 elements per thread and slice of the columns ----
-  const int side = s4 / 4, tiles = side * side, slices = kGramThreads / tiles;
+  constexpr int kSide = S / 4, kTiles = kSide * kSide, kSlices = kGramThreads / kTiles;
   {
     double v[16] = {};
-    const int tile = tid % tiles, slice = tid / tiles;
-    if (slice < slices) {
-      const int i0 = tile / side * 4, j0 = tile % side * 4;
+    const int tile = tid % kTiles, slice = tid / kTiles;
+    if (slice < kSlices) {
+      const int i0 = tile / kSide * 4, j0 = tile % kSide * 4;
 #pragma unroll 2
-      for (int c = slice; c < cols; c += slices) {
-        const double* xc = x + c * pitch;
+      for (int c = slice; c < cols; c += kSlices) {
+        const double* xc = x + c * kX;
         double xi[4], xj[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          xi[k] = xc[i0 + k];
-          xj[k] = xc[j0 + k];
+        for (int k = 0; k < 4; k += 2) {
+          const double2 a = *reinterpret_cast<const double2*>(xc + i0 + k), b = *reinterpret_cast<const double2*>(xc + j0 + k);
+          xi[k] = a.x; xi[k + 1] = a.y; xj[k] = b.x; xj[k + 1] = b.y;
         }
 #pragma unroll
         for (int k = 0; k < 16; ++k) v[k] = fma(xi[k >> 2], xj[k & 3], v[k]);
@@ -527,16 +535,16 @@ __global__ void __launch_bounds__(kGramThreads) gram_side_kernel(const __grid_co
     for (int k = 0; k < 16; ++k) part[k * kGramThreads + tid] = v[k];
   }
   __syncthreads();
-  for (int e = tid; e < tiles * 16; e += kGramThreads) {
-    const int tile = e % tiles, k = e / tiles;
+  for (int e = tid; e < kTiles * 16; e += kGramThreads) {
+    const int tile = e % kTiles, k = e / kTiles;
     double sum = 0.0;
-    for (int i = 0; i < slices; ++i) sum += part[k * kGramThreads + i * tiles + tile];
-    share[(tile / side * 4 + (k >> 2)) * s4 + tile % side * 4 + (k & 3)] = sum;
+#pragma unroll 8
+    for (int i = 0; i < kSlices; ++i) sum += part[k * kGramThreads + i * kTiles + tile];
+    share[(tile / kSide * 4 + (k >> 2)) * S + tile % kSide * 4 + (k & 3)] = sum;
   }
   cluster_sync_all();
   // ---- A0: the shares of all CTAs, in the order of the ranks ----
-  double* A = mat[0];
-  for (int e = 2 * tid; e < s4 * s4; e += 2 * kGramThreads) {
+  for (int e = 2 * tid; e < S * S; e += 2 * kGramThreads) {
     const uint32_t at = smem_u32(share + e);
     double2 sum = make_double2(0.0, 0.0);
 #pragma unroll 8
@@ -545,70 +553,95 @@ __global__ void __launch_bounds__(kGramThreads) gram_side_kernel(const __grid_co
       sum.x += y.x;
       sum.y += y.y;
     }
-    const int r = e / s4, c = e - r * s4;
-    A[r * kPitch + c] = sum.x;
-    A[r * kPitch + c + 1] = sum.y;
+    A[e / S * kPitch + e % S] = sum.x;
+    A[e / S * kPitch + e % S + 1] = sum.y;
   }
   __syncthreads();
-  double trace = 0.0;
-  for (int i = 0; i < s; ++i) trace += A[i * kPitch + i];
+  double trace = lane < S ? A[lane * kPitch + lane] : 0.0;       // every warp for itself, in the same order
+#pragma unroll
+  for (int d = 16; d; d >>= 1) trace += __shfl_xor_sync(0xFFFFFFFFu, trace, d);
   const double norm = sqrt(trace);
   const double scale = norm < static_cast<double>(INFINITY) ? 1.0 / (norm + p.eps) : __longlong_as_double(0x7FFFFFFFFFFFFFFFll);
-  __syncthreads();
-  for (int e = tid; e < s4 * s4; e += kGramThreads) A[e / s4 * kPitch + e % s4] *= scale * scale;
-  __syncthreads();
 
-  // ---- P = the product of the steps' factors ----
-  // 2 x 2 elements per thread; out = f(A-like u times v) written through `put`
-  const int half = s4 / 2, r2 = tid / half * 2, c2 = tid % half * 2;
-  const bool mine = r2 < s4;
-  auto product = [&](const double* u, const double* v, double (&o)[4]) {
+  // ---- P = the product of the steps' factors: kRows x 2 elements of each matrix per thread ----
+  // All matrices are symmetric (polynomials of A), so rows of the left one are read as columns, two doubles at a time.  With
+  // four rows three loads feed eight multiply-adds, what shared memory and the float64 pipe do in the same time; up to 16 x 16
+  // latency counts and two rows keep more threads busy.
+  constexpr int kRows = S <= 16 ? 2 : 4, kHalf = S / 2, kBatch = S <= 16 ? 8 : 4;
+  const int r4 = tid / kHalf * kRows, c2 = tid % kHalf * 2;
+  const bool mine = r4 < S;
+  using Part = double[kRows][2];
+  auto product = [&](const double* u, const double* v, Part& o) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) o[k] = 0.0;
+    for (int i = 0; i < kRows; ++i) o[i][0] = o[i][1] = 0.0;
     if (!mine) return;
-#pragma unroll 4
-    for (int k = 0; k < s4; ++k) {
-      const double u0 = u[r2 * kPitch + k], u1 = u[(r2 + 1) * kPitch + k], v0 = v[k * kPitch + c2], v1 = v[k * kPitch + c2 + 1];
-      o[0] = fma(u0, v0, o[0]);
-      o[1] = fma(u0, v1, o[1]);
-      o[2] = fma(u1, v0, o[2]);
-      o[3] = fma(u1, v1, o[3]);
+#pragma unroll
+    for (int k0 = 0; k0 < S; k0 += kBatch) {
+      double2 us[kBatch][kRows / 2], w[kBatch];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+#pragma unroll
+        for (int i = 0; i < kRows / 2; ++i) us[k][i] = *reinterpret_cast<const double2*>(u + (k0 + k) * kPitch + r4 + 2 * i);
+        w[k] = *reinterpret_cast<const double2*>(v + (k0 + k) * kPitch + c2);
+      }
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k)
+#pragma unroll
+        for (int i = 0; i < kRows / 2; ++i) {
+          o[2 * i][0] = fma(us[k][i].x, w[k].x, o[2 * i][0]);
+          o[2 * i][1] = fma(us[k][i].x, w[k].y, o[2 * i][1]);
+          o[2 * i + 1][0] = fma(us[k][i].y, w[k].x, o[2 * i + 1][0]);
+          o[2 * i + 1][1] = fma(us[k][i].y, w[k].y, o[2 * i + 1][1]);
+        }
     }
   };
-  auto put = [&](double* to, const double (&o)[4]) {
+  auto put = [&](double* to, const Part& o) {
     if (!mine) return;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) to[(r2 + (k >> 1)) * kPitch + c2 + (k & 1)] = o[k];
+    for (int i = 0; i < kRows; ++i) *reinterpret_cast<double2*>(to + (r4 + i) * kPitch + c2) = make_double2(o[i][0], o[i][1]);
   };
-  double *B = mat[1], *P = mat[2], *T = part;          // the threads' sums are used up
+  auto at = [&](int i, int j) { return (r4 + i) * kPitch + c2 + j; };
+  __syncthreads();
+  if (mine) {
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) A[at(i, j)] *= scale * scale;
+  }
+  __syncthreads();
+  int now = 0;
   for (int step = 0; step < p.steps; ++step) {
-    double o[4], q[4];
+    const bool last = step == p.steps - 1;
+    Part o;
     product(A, A, o);
     if (mine) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int r = r2 + (k >> 1), c = c2 + (k & 1);
-        o[k] = fma(p.c, o[k], fma(p.b, A[r * kPitch + c], r == c ? p.a : 0.0));
-      }
+      for (int i = 0; i < kRows; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) o[i][j] = fma(p.c, o[i][j], fma(p.b, A[at(i, j)], r4 + i == c2 + j ? p.a : 0.0));
     }
     put(B, o);
     if (step == 0) put(P, o);
     __syncthreads();
-    const bool last = step == p.steps - 1;
-    if (step > 0) product(B, P, o);
-    if (!last) product(B, A, q);
-    __syncthreads();
-    if (step > 0) put(P, o);
-    if (!last) put(T, q);
+    if (step > 0) {
+      product(B, P + now, o);
+      now = kGramMatrix - now;
+      put(P + now, o);
+    }
+    if (!last) {
+      product(B, A, o);
+      put(T, o);
+    }
     __syncthreads();
     if (!last) {
-      product(T, B, q);
-      put(A, q);
+      product(T, B, o);
+      put(A, o);
       __syncthreads();
     }
   }
+  const double* F = P + now;
 
-  // ---- X = P X0 ----
+  // ---- X = P X0: some rows of one or two columns per lane, lanes over the columns ----
   const int64_t o0 = matrix * p.out.batch_stride;
   auto store = [&](int r, int c, double v) {
     const int64_t to = o0 + (p.flip ? static_cast<int64_t>(c0 + c) * p.out.ld + r : static_cast<int64_t>(r) * p.out.ld + c0 + c);
@@ -617,19 +650,39 @@ __global__ void __launch_bounds__(kGramThreads) gram_side_kernel(const __grid_co
     else if (p.out.type == kBF16) static_cast<__nv_bfloat16*>(p.out.base)[to] = __float2bfloat16_rn(f);
     else static_cast<__half*>(p.out.base)[to] = __float2half_rn(f);
   };
-  // four rows of a column per thread; neighbouring threads have neighbouring elements of the result's rows
-  for (int e = tid; e < side * cols; e += kGramThreads) {
-    const int c = p.flip ? e / side : e % cols, r = (p.flip ? e % side : e / cols) * 4;
-    double v[4] = {};
-#pragma unroll 4
-    for (int k = 0; k < s; ++k) {
-      const double y = x[c * pitch + k];
+  constexpr int kOutRows = S <= 16 ? 4 : 8, kOutCols = S <= 16 ? 1 : 2;
+  const int chunks = (cols + 32 * kOutCols - 1) / (32 * kOutCols);
+  for (int item = warp; item < S / kOutRows * chunks; item += kGramThreads / 32) {
+    const int r = item % (S / kOutRows) * kOutRows, c = item / (S / kOutRows) * 32 * kOutCols + lane;
+    if (r >= s) continue;
+    const double* xs[kOutCols];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = fma(P[(r + i) * kPitch + k], y, v[i]);
+    for (int j = 0; j < kOutCols; ++j) xs[j] = x + min(c + 32 * j, cols - 1) * kX;      // columns beyond the last read it again
+    double v[kOutRows][kOutCols] = {};
+#pragma unroll 4
+    for (int k = 0; k < S; k += 2) {
+      double2 y[kOutCols];
+#pragma unroll
+      for (int j = 0; j < kOutCols; ++j) y[j] = *reinterpret_cast<const double2*>(xs[j] + k);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < kOutRows; i += 2) {
+          const double2 f = *reinterpret_cast<const double2*>(F + (k + h) * kPitch + r + i);
+#pragma unroll
+          for (int j = 0; j < kOutCols; ++j) {
+            v[i][j] = fma(f.x, h ? y[j].y : y[j].x, v[i][j]);
+            v[i + 1][j] = fma(f.y, h ? y[j].y : y[j].x, v[i + 1][j]);
+          }
+        }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (r + i < s) store(r + i, c, v[i]);
+    for (int i = 0; i < kOutRows; ++i) {
+      if (r + i >= s) break;
+#pragma unroll
+      for (int j = 0; j < kOutCols; ++j)
+        if (c + 32 * j < cols) store(r + i, c + 32 * j, v[i][j]);
+    }
   }
   cluster_sync_all();       // no CTA leaves while another may still read its share
 }
