@@ -19,7 +19,9 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 
 // fc1 has at most 12 inputs: a thread keeps the weights of its four features in registers and walks over queries, eight between
 // barriers, while the next eight are loaded and normalised.  12 multiply-adds per result on the ordinary cores, in pairs, are
-// 11 us for 65,536 queries of 12 inputs, and the rows' 67 MB 10 us.
+// 11 us for 65,536 queries of 12 inputs, and the rows' 67 MB 10 us; 77 us measured.  What is left is issue: per result the maximum,
+// the product with the row's factor, the rounding and the packing next to twelve half multiply-adds, and the largest value of a
+// query has to cross all eight warps before its first byte can be written.
 __global__ void __launch_bounds__(kInputThreads, 2)
 mlp_input_kernel(const float* __restrict__ features, int n_op_feat, const uint8_t* __restrict__ device_row, const double* __restrict__ device_features,
                  int n_dev, const double* __restrict__ mu, const double* __restrict__ sigma, const float* __restrict__ w, const float* __restrict__ b,
@@ -47,7 +49,7 @@ mlp_input_kernel(const float* __restrict__ features, int n_op_feat, const uint8_
   // thread e of the first 96 brings input e mod 12 of query e / 12
   const int mine_k = tid / kMaxInFeat, mine_c = tid - mine_k * kMaxInFeat;
   const bool brings = tid < kInputQueries * kMaxInFeat && mine_c < inputs;
-  const double mine_mu = brings ? mu[mine_c] : 0.0, mine_sigma = brings ? sigma[mine_c] : 1.0;
+  const double mine_mu = brings ? mu[mine_c] : 0.0, mine_per_sigma = brings ? 1.0 / sigma[mine_c] : 1.0;
   float raw = 0.0f;
   int row = 0;
   auto request = [&](int64_t q0) {
@@ -57,7 +59,7 @@ mlp_input_kernel(const float* __restrict__ features, int n_op_feat, const uint8_
   };
   auto put = [&](int buf) {
     if (!brings) return;
-    x[buf][mine_k][mine_c] = mine_c < n_op_feat ? static_cast<float>((static_cast<double>(raw) - mine_mu) / mine_sigma)
+    x[buf][mine_k][mine_c] = mine_c < n_op_feat ? static_cast<float>((static_cast<double>(raw) - mine_mu) * mine_per_sigma)
                                                 : devices[row < n_dev ? row : n_dev - 1][mine_c - n_op_feat];
   };
   const int64_t step = static_cast<int64_t>(gridDim.x) * kInputQueries;
@@ -128,7 +130,15 @@ mlp_input_kernel(const float* __restrict__ features, int n_op_feat, const uint8_
   }
 }
 
-// A warp per row, bound by the rows' bytes; a lane's 32 weights stay in registers.  The sum goes over the lanes as a fixed tree.
+// Byte i of a word of signed bytes whose signs are flipped, as a float: behind the exponent of 2^23 it counts from 128 on.  (The
+// conversion instruction takes bytes at an eighth of this rate: 28 us.)
+constexpr uint32_t kFlip = 0x80808080u;
+__device__ __forceinline__ float byte_value(uint32_t word, int i) {
+  return __uint_as_float(__byte_perm(word, 0x4B000000u, 0x7540u + i)) - 8388736.0f;
+}
+
+// A warp per row; a lane's 32 weights stay in registers.  65,536 rows of 1,024 features are 67 MB, 10 us; 22 us measured, about
+// three instructions per byte.  The sum goes over the lanes as a fixed tree.
 __global__ void __launch_bounds__(256)
 mlp_output_kernel(const int8_t* __restrict__ q, int64_t q_pitch, const float* __restrict__ scales, const float* __restrict__ w, const float* __restrict__ b,
                   int64_t Q, int width, float* __restrict__ out) {
@@ -163,7 +173,7 @@ mlp_output_kernel(const int8_t* __restrict__ q, int64_t q_pitch, const float* __
             v = make_uint4(t[0], t[1], t[2], t[3]);
           }
         }
-        ws[r][h][0] = v.x; ws[r][h][1] = v.y; ws[r][h][2] = v.z; ws[r][h][3] = v.w;
+        ws[r][h][0] = v.x ^ kFlip; ws[r][h][1] = v.y ^ kFlip; ws[r][h][2] = v.z ^ kFlip; ws[r][h][3] = v.w ^ kFlip;
       }
     float sums[kRows] = {};
 #pragma unroll
@@ -172,7 +182,7 @@ mlp_output_kernel(const int8_t* __restrict__ q, int64_t q_pitch, const float* __
       for (int i = 0; i < 16; ++i)
 #pragma unroll
         for (int r = 0; r < kRows; ++r)
-          sums[r] = fmaf(static_cast<float>(static_cast<int8_t>(ws[r][h][i >> 2] >> (8 * (i & 3)))), wr[16 * h + i], sums[r]);
+          sums[r] = fmaf(byte_value(ws[r][h][i >> 2], i & 3), wr[16 * h + i], sums[r]);
 #pragma unroll
     for (int d = 16; d; d >>= 1)
 #pragma unroll
