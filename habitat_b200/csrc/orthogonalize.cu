@@ -9,7 +9,11 @@
 // so that its Frobenius norm is in [2^13, 2^14).  The exact factor 1 / (|G| + eps) enters the first step's results in
 // float32, so a 16-bit G is multiplied unrounded.  Sums are float32, the norm float64.  With `split` every operand is a
 // pair of half-precision matrices, high and low parts (22 bits), and a product three (hi hi + hi lo + lo hi): float32
-// updates, whose results are held to float32's accuracy.
+// updates, whose results are held to float32's accuracy, and half-precision ones, whose own 11 bits would be no fewer than the
+// operands'.
+//
+// Sides.  All steps of an update with a shorter side of up to 128 run in one launch of one cluster, which keeps X on chip, and
+// with one of up to 32 in float64 on the Gram matrix alone (orthogonalize_small.cuh); larger ones take three launches per step.
 #include <atomic>
 #include <cmath>
 #include <type_traits>
@@ -152,7 +156,7 @@ __device__ __forceinline__ void for_chunks(const EpiContext& c, Block& sums, Rel
 // A block as half-precision operands at `to` (rows of `ld`) and, with rows and columns exchanged, at `turned`, and with kSplit what
 // that leaves, `low` elements behind.
 template <bool kSplit>
-__device__ __forceinline__ void store_operands(Block& v, __half* to, __half* turned, int64_t ld, int64_t low, int rows_left, uint8_t* staging, int lane) {
+__device__ __forceinline__ void store_operands(Block& v, __half* to, __half* turned, int64_t ld, int64_t low, int rows_left, int turned_left, uint8_t* staging, int lane) {
 #pragma unroll
   for (int part = 0; part < (kSplit ? 2 : 1); ++part) {
     uint32_t w[4][4];
@@ -179,9 +183,17 @@ __device__ __forceinline__ void store_operands(Block& v, __half* to, __half* tur
 #pragma unroll
       for (int j = 0; j < 4; ++j) store_fragment_turned(smem_u32(staging), j, w[j], lane);
       __syncwarp();
-      store_staged(staging, reinterpret_cast<uint16_t*>(turned + part * low), ld, 16, 32, 32, lane);
+      store_staged(staging, reinterpret_cast<uint16_t*>(turned + part * low), ld, 16, turned_left, 32, lane);
     }
   }
+}
+
+// Whether 32 x 32 results of a symmetric product from (row0, n0) on are this tile's to store, and their mirror image with them:
+// inside the matrix; of tiles of 128 columns, whose blocks lie on either side of the diagonal, all but the upper halves
+// of those on it, of others what is not above it.
+template <int BN>
+__device__ __forceinline__ bool needed(int row0, int n0, int M) {
+  return row0 < M && n0 < M && (n0 <= row0 || (BN == kCtaRows && n0 / kCtaRows != row0 / kCtaRows));
 }
 
 // What a symmetric product becomes: A = X X^T, or B = a I + b A + c A^2.
@@ -239,8 +251,9 @@ __global__ void __launch_bounds__(256) symmetric_sum_kernel(const __grid_constan
   Product one = p;
   one.splits = 1;
   const Tile tile = tile_of<BN>(one, t);
-  const int row0 = tile.m0 + piece / kAcross * 32, n0 = tile.n0 + piece % kAcross * 32;
-  if (n0 > row0 || row0 >= p.M) return;
+  const int down = piece / kAcross * 32;
+  const int row0 = down < kCtaRows ? tile.m0 + down : tile.m1 + down - kCtaRows, n0 = tile.n0 + piece % kAcross * 32;
+  if (!needed<BN>(row0, n0, p.M)) return;
   const int tx = static_cast<int>(threadIdx.x) & 31, ty = static_cast<int>(threadIdx.x) >> 5;
   const int in_batch = t - tile.batch * p.per_batch;
   const float scale = symmetric_scale(e, tile.batch);
@@ -253,7 +266,7 @@ __global__ void __launch_bounds__(256) symmetric_sum_kernel(const __grid_constan
       v += shares[(static_cast<int64_t>(tile.batch * p.splits + k) * p.per_batch + in_batch) * kPairRows * BN + (piece / kAcross * 32 + ty + i) * BN +
                   piece % kAcross * 32 + tx];
     v *= scale;
-    if (r < p.M && c <= r) {
+    if (r < p.M && c < p.M && (n0 != row0 || c <= r)) {
       if (e.a.hi) {
         const __half* at = e.a.hi + tile.batch * e.a.batch_stride + static_cast<int64_t>(r) * e.a.ld + c;
         v = fmaf(e.on_a, __half2float(*at), v);
@@ -271,7 +284,7 @@ __global__ void __launch_bounds__(256) symmetric_sum_kernel(const __grid_constan
 #pragma unroll
   for (int i = 0; i < 32; i += 8) {
     const int c = n0 + ty + i, r = row0 + tx;
-    if (r >= p.M || c >= r) continue;
+    if (r >= p.M || c >= p.M || (n0 == row0 && c >= r)) continue;
     const float v = turned[tx][ty + i];
     const __half hi = __float2half_rn(v);
     __half* to = out + static_cast<int64_t>(c) * e.out.ld + r;
@@ -297,7 +310,7 @@ struct SymmetricOut {
     const float scale = symmetric_scale(ep, c.batch);
     for_chunks<BN, kSplit>(c, sums, release, [&](int chunk, Block& v) {
       const int n0 = c.n0 + chunk * 32;
-      if (n0 > row0 || row0 >= p.M) return;      // above the diagonal (both are multiples of 32), or below the matrix
+      if (!needed<BN>(row0, n0, p.M)) return;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -324,10 +337,10 @@ struct SymmetricOut {
           }
         }
       }
-      // blocks below the diagonal also to their mirror image
+      // and those off the diagonal to their mirror image
       __half* base = ep.out.hi + c.batch * ep.out.batch_stride;
-      store_operands<kSplit>(v, base + static_cast<int64_t>(row0) * ep.out.ld + n0, n0 < row0 ? base + static_cast<int64_t>(n0) * ep.out.ld + row0 : nullptr,
-                             ep.out.ld, ep.out.low, p.M - row0, c.tail->staging + c.warp * kStageOutBytes, c.lane);
+      store_operands<kSplit>(v, base + static_cast<int64_t>(row0) * ep.out.ld + n0, n0 != row0 ? base + static_cast<int64_t>(n0) * ep.out.ld + row0 : nullptr,
+                             ep.out.ld, ep.out.low, p.M - row0, p.M - n0, c.tail->staging + c.warp * kStageOutBytes, c.lane);
     });
   }
 };
@@ -362,7 +375,7 @@ struct UpdateOut {
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[j][i] = make_float2(v[j][i].x * scale, v[j][i].y * scale);
       if (ep.x.hi) {
-        store_operands<kSplit>(v, ep.x.hi + c.batch * ep.x.batch_stride + static_cast<int64_t>(row0) * ep.x.ld + n0, nullptr, ep.x.ld, ep.x.low, p.M - row0,
+        store_operands<kSplit>(v, ep.x.hi + c.batch * ep.x.batch_stride + static_cast<int64_t>(row0) * ep.x.ld + n0, nullptr, ep.x.ld, ep.x.low, p.M - row0, 0,
                                staging, c.lane);
         return;
       }
@@ -413,8 +426,9 @@ struct UpdateOut {
 // ---------------------------------------------------------------------------
 int64_t up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
-// Tiles of a symmetric product whose columns begin before their rows end.
+// Tiles of a symmetric product: with 128 columns two blocks each, else those whose columns begin before their rows end.
 int64_t lower_tiles(int64_t s, int bn) {
+  if (bn == kCtaRows) return two_block_tiles((s + kCtaRows - 1) / kCtaRows);
   const int64_t tm = (s + kPairRows - 1) / kPairRows, tn = (s + bn - 1) / bn, per = kPairRows / bn;
   int64_t n = 0;
   for (int64_t i = 0; i < tm; ++i) n += (i + 1) * per < tn ? (i + 1) * per : tn;

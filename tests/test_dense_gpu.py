@@ -344,6 +344,17 @@ def test_orthogonalize_long_and_short_sides(shape, dtype):
     _check(update, dense.orthogonalize(update))
 
 
+# blocks of 128 rows per side, and enough matrices for tiles of two such blocks
+@pytest.mark.parametrize("blocks, batch", [(2, 40), (3, 30), (4, 20), (5, 12), (6, 10), (7, 8), (8, 8), (9, 5)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_orthogonalize_batches_of_equal_updates(blocks, batch, dtype):
+    update = _update((128 * blocks - 37, 128 * blocks - 16), blocks, dtype)
+    got = dense.orthogonalize(update.expand((batch,) + update.shape).contiguous())
+    _check(update, got[0])
+    for x in got:
+        assert torch.equal(x, got[0])
+
+
 @pytest.mark.parametrize("steps, coefficients", [(1, COEFFICIENTS), (2, COEFFICIENTS), (3, (1.5, -0.5, 0.0)), (10, (1.875, -1.25, 0.375))])
 def test_orthogonalize_steps_and_coefficients(steps, coefficients):
     for dtype in (torch.float32, torch.bfloat16):
