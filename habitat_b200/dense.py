@@ -85,7 +85,7 @@ def int8_matmul(q, scales, weight, weight_scales, bias=None, relu=False, out_dty
 
 def int8_matmul_quantized(q, scales, weight, weight_scales, bias=None, relu=False):
     """quantize_rows(int8_matmul(...)) of the float32 product, bit for bit, as (int8 rows, scales); with up to 1,024 output
-    channels the product does not go through memory."""
+    channels the product of large batches does not go through memory."""
     res = _native.binding().int8_product(q, scales, weight, weight_scales, bias, relu, -1)
     if res is None:
         _check_product(q, scales, weight, weight_scales, bias)
@@ -98,8 +98,9 @@ def orthogonalize(update, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1
     A = X X^T and (a, b, c) = coefficients.  Same shape and dtype as the update.
 
     float32 and float16 updates are multiplied in three half-precision products each (22-bit operands), bfloat16 ones in one
-    (11-bit operands, float32 sums), so that the result's own rounding is the larger error.  Elements of the result smaller than 2^-32 are lost; an update with an infinity or a NaN
-    gives NaN everywhere.  Coefficients that would let singular values grow beyond 12 are refused."""
+    (11-bit operands, float32 sums), so that the result's own rounding is the larger error; with a shorter side of up to 32 all
+    of them are multiplied in float64.  Elements of the result smaller than 2^-32 may be lost; an update with an infinity or a
+    NaN gives NaN everywhere.  Coefficients that would let singular values grow beyond 12 are refused."""
     a, b, c = coefficients
     res = _native.binding().orthogonalize(update, steps, a, b, c, eps)
     if res is None:

@@ -488,15 +488,16 @@ hb_status hb_int8_matmul(const int8_t* q, int64_t q_pitch, const float* q_scales
                          const float* w_scales, const float* bias, int32_t relu, int64_t M, int64_t N, int64_t K, void* out,
                          int32_t out_type, int64_t out_pitch, void* workspace, int64_t workspace_bytes, void* stream);
 
-/* The same followed by hb_quantize_rows of the float32 result, which does not go through memory for N <= 1024.  out's rows
- * have to start on 16-byte boundaries. */
+/* The same followed by hb_quantize_rows of the float32 result, which goes through the workspace for N > 1024 and where
+ * few rows leave most SMs without work otherwise, and stays on chip in all other cases.  out's rows have to start on
+ * 16-byte boundaries. */
 hb_status hb_int8_matmul_quantized(const int8_t* q, int64_t q_pitch, const float* q_scales, const int8_t* w, int64_t w_pitch,
                                    const float* w_scales, const float* bias, int32_t relu, int64_t M, int64_t N, int64_t K,
                                    int8_t* out, int64_t out_pitch, float* out_scales, void* workspace, int64_t workspace_bytes,
                                    void* stream);
 
-/* Workspace of the two calls above for these operands (0 when they start on 16-byte boundaries; `quantized` for the second
- * one), -1 for invalid sizes.  A workspace starts on a 256-byte boundary and belongs to one call at a time. */
+/* Workspace of the two calls above for these operands (`quantized` for the second one; 0 where nothing is copied and nothing
+ * quantised through memory), -1 for invalid sizes.  A workspace starts on a 256-byte boundary and belongs to one call at a time. */
 int64_t hb_int8_workspace_bytes(const int8_t* q, int64_t q_pitch, const int8_t* w, int64_t w_pitch, int64_t M, int64_t N,
                                 int64_t K, int32_t quantized);
 
@@ -518,7 +519,7 @@ hb_status hb_int8_mlp_output(const int8_t* q, int64_t q_pitch, const float* scal
  * X <- (a I + b A + c A^2) X with A = X X^T (on G^T where rows > cols).  coefficients = {a, b, c} must keep the singular
  * values of X below 12 and those of the factor below 250.  G [batch][rows][cols], rows `pitch` and matrices `batch_stride` elements apart, out in the same type.
  * split: every product in three half-precision parts (22-bit operands), for float32 accuracy; otherwise one (11 bits, float32
- * sums).  Elements of the result smaller than 2^-32 are lost.  A norm that is not finite gives NaN everywhere. */
+ * sums).  Elements of the result smaller than 2^-32 may be lost.  A norm that is not finite gives NaN everywhere. */
 hb_status hb_orthogonalize(const void* update, int32_t type, int64_t batch, int64_t rows, int64_t cols, int64_t pitch,
                            int64_t batch_stride, int32_t steps, const double* coefficients, double eps, int32_t split,
                            void* out, int64_t out_pitch, int64_t out_batch_stride, void* workspace, int64_t workspace_bytes,
