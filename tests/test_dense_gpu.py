@@ -344,6 +344,17 @@ def test_orthogonalize_long_and_short_sides(shape, dtype):
     _check(update, dense.orthogonalize(update))
 
 
+# read in pieces of eight elements or one by one: rows that are no multiple of eight, that start on any element, and both
+@pytest.mark.parametrize("shape", [(129, 204), (131, 260), (129, 1030), (3, 131, 204), (1030, 129), (131, 2056)])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shift", [0, 1, 4])
+def test_orthogonalize_updates_that_start_anywhere(shape, dtype, shift):
+    update = _update(shape, sum(shape), dtype)
+    flat = torch.full((shift + update.numel(),), float("nan"), dtype=dtype, device="cuda")
+    flat[shift:] = update.flatten()
+    _check(update, dense.orthogonalize(flat[shift:].view(shape)))
+
+
 # blocks of 128 rows per side, and enough matrices for tiles of two such blocks
 @pytest.mark.parametrize("blocks, batch", [(2, 40), (3, 30), (4, 20), (5, 12), (6, 10), (7, 8), (8, 8), (9, 5)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
