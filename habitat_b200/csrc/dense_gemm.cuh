@@ -105,8 +105,8 @@ inline void set_tiles(Product* p, int64_t per_batch) {
 // Of a block and its mirror image one is needed, n (n + 1) / 2 in all; a column c has those of rows c to n - 1, and every
 // other column an odd number.  Two such columns, c and c + 2, help each other out: block (c + 2, c) is computed as its mirror
 // image (c, c + 2), which leaves both with an even number, and at most one tile in all is half empty.  (Neighbouring rows in
-// every pair: 20 tiles for n = 8, not 18, so eight matrices of 1024 x 1024 take a third round of 74 pairs: five float32 steps 758 us,
-// 557 so.)
+// every pair: 20 tiles for n = 8, not 18, so eight matrices of 1024 x 1024 take a third round of 74 pairs: five float32 steps, call
+// after call, 758 us, 678 so.)
 // With r = n - 1 - c the columns r = 4 g to 4 g + 3 have 2 g + 1, 2 g + 1, 2 g + 1 and 2 g + 2 tiles, all before them
 // 4 g^2 + g.
 __host__ __device__ __forceinline__ int64_t two_block_tiles(int64_t n) {
