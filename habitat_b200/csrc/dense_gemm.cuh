@@ -338,6 +338,7 @@ struct EpiContext {
   int batch, t;           // and the tile's number
   uint32_t n_tile;        // how many tiles the CTA has drained before
   bool first, last;       // accumulation of the tile (kSplit)
+  float scale;            // a policy's
   uint32_t rank;          // in the cluster
   int next_row0, next_n0; // of the next tile; next_row0 < 0: there is none
   bool* ok;
@@ -375,7 +376,7 @@ inline int tile_columns(std::initializer_list<int> widths, int pairs, Count tile
 
 // The kernel.  Epilogue: a policy with `Params`, static kInt8, kMnMajorB, kSplit, kClusterCtas (0: a pair; else the CTAs of a
 // cluster that share rows, one pair per BN columns) and
-//   static void begin(EpiContext&)                                              before a tile's accumulators are waited for
+//   static void begin(const Params&, const Product&, EpiContext&, sums)         before a tile's accumulators are waited for
 //   static void fetch(const Params&, const Product&, EpiContext&, row0, n0)     requests what a tile's results need, a tile ahead
 //   static void drain(const Params&, const Product&, EpiContext&, sums, release)   calls release() once the accumulators are read,
 //                                                                                  and c.fetch_next() once that is used
@@ -551,7 +552,7 @@ gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ typename 
       c.n0 = c.next_n0;
       c.batch = tile.batch;
       look_ahead(t + workers);
-      Epi::template begin<BN>(c);
+      Epi::template begin<BN>(ep, p, c, sums);
       c.t = t;
       const int rounds = Epi::kSplit ? slots_of(tile.split) : 1;
       for (int i = 0; i < rounds && ok; ++i, ++n) {

@@ -274,7 +274,7 @@ struct FloatOut {
     fetch_scales<BN>(ep.s, p, c, row0, n0);
   }
   template <int BN>
-  static __device__ __forceinline__ void begin(const EpiContext&) {}
+  static __device__ __forceinline__ void begin(const Params&, const Product&, const EpiContext&, Block&) {}
   template <int BN, class Release>
   static __device__ __forceinline__ void drain(const Params& ep, const Product& p, const EpiContext& c, Block&, Release release) {
     constexpr int kBlocks = Shape<BN>::kCols / 8;
@@ -341,7 +341,7 @@ struct QuantOut {
     fetch_scales<BN>(ep.s, p, c, row0, n0);
   }
   template <int BN>
-  static __device__ __forceinline__ void begin(const EpiContext& c) {
+  static __device__ __forceinline__ void begin(const Params&, const Product&, const EpiContext& c, Block&) {
     if (c.warp == 0 && c.lane == 0)
       mbar_expect_tx(smem_u32(&c.tail->exchange[c.n_tile & 1u]), kCtas / 2 * Shape<BN>::kParts * kCtaRows * 4);
   }

@@ -309,7 +309,7 @@ struct ShareOut {
   template <int BN>
   static __device__ __forceinline__ void fetch(const Params&, const Product&, const EpiContext&, int, int) {}
   template <int BN>
-  static __device__ __forceinline__ void begin(const EpiContext&) {}
+  static __device__ __forceinline__ void begin(const Params&, const Product&, const EpiContext&, Block&) {}
   template <int BN, class Release>
   static __device__ __forceinline__ void drain(const Params& ep, const Product&, const EpiContext& c, Block& sums, Release release) {
     for_chunks<BN, kSplit>(c, sums, release, [&](int chunk, Block& v) {
@@ -340,21 +340,38 @@ __global__ void __launch_bounds__(256) symmetric_sum_kernel(const __grid_constan
   const int in_batch = t - tile.batch * p.per_batch;
   const float scale = symmetric_scale(e, tile.batch);
   __half* out = e.out.hi + tile.batch * e.out.batch_stride;
+  // A's values and up to eight shares of each of four rows are on their way at once (one after the other, 25 shares of 150 x 150
+  // results took 20 us; five steps of a 150 x 8000 update 192 us, 161 so); they are added in their order
+  float a[4], sums[4] = {};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = row0 + ty + 8 * i, c = n0 + tx;
+    a[i] = 0.0f;
+    if (e.a.hi && r < p.M && c < p.M) {
+      const __half* at = e.a.hi + tile.batch * e.a.batch_stride + static_cast<int64_t>(r) * e.a.ld + c;
+      a[i] = __half2float(*at);
+      if (e.a.low) a[i] += __half2float(at[e.a.low]);
+    }
+  }
+  const int64_t share = static_cast<int64_t>(p.per_batch) * kPairRows * BN;
+  const float* from = shares + tile.batch * p.splits * share + (static_cast<int64_t>(in_batch) * kPairRows + down + ty) * BN + piece % kAcross * 32 + tx;
+  constexpr int kAtOnce = 8;
+  for (int k0 = 0; k0 < p.splits; k0 += kAtOnce) {
+    float x[kAtOnce][4];
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[k][i] = k0 + k < p.splits ? from[(k0 + k) * share + 8 * i * BN] : 0.0f;
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sums[i] += x[k][i];
+  }
 #pragma unroll
   for (int i = 0; i < 32; i += 8) {
     const int r = row0 + ty + i, c = n0 + tx;
-    float v = 0.0f;
-    for (int k = 0; k < p.splits; ++k)
-      v += shares[(static_cast<int64_t>(tile.batch * p.splits + k) * p.per_batch + in_batch) * kPairRows * BN + (piece / kAcross * 32 + ty + i) * BN +
-                  piece % kAcross * 32 + tx];
-    v *= scale;
+    const float v = fmaf(e.on_a, a[i / 8], sums[i / 8] * scale) + (e.a.hi && r == c ? e.on_diagonal : 0.0f);
     if (r < p.M && c < p.M && (n0 != row0 || c <= r)) {
-      if (e.a.hi) {
-        const __half* at = e.a.hi + tile.batch * e.a.batch_stride + static_cast<int64_t>(r) * e.a.ld + c;
-        v = fmaf(e.on_a, __half2float(*at), v);
-        if (e.a.low) v = fmaf(e.on_a, __half2float(at[e.a.low]), v);
-        if (r == c) v += e.on_diagonal;
-      }
       const __half hi = __float2half_rn(v);
       __half* to = out + static_cast<int64_t>(r) * e.out.ld + c;
       *to = hi;
@@ -384,46 +401,80 @@ struct SymmetricOut {
   using Params = Symmetric;
   template <int BN>
   static __device__ __forceinline__ void fetch(const Params&, const Product&, const EpiContext&, int, int) {}
+  // b A + a I of the 32 x 32 results from (row0, n0) on.
+  static __device__ __forceinline__ void other_terms(const Params& ep, const Product& p, const EpiContext& c, int row0, int n0, Block& v) {
+    const int r = c.lane >> 2, n = 2 * (c.lane & 3);
+    const __half* at = ep.a.hi + c.batch * ep.a.batch_stride + static_cast<int64_t>(row0 + r) * ep.a.ld + n0 + n;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool there = row0 + r + 8 * i < p.M;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float2 f = make_float2(0.0f, 0.0f);
+        if (there) {
+          f = __half22float2(*reinterpret_cast<const __half2*>(at + 8 * i * ep.a.ld + 8 * j));
+          if (kSplit) {
+            const float2 g = __half22float2(*reinterpret_cast<const __half2*>(at + ep.a.low + 8 * i * ep.a.ld + 8 * j));
+            f = make_float2(f.x + g.x, f.y + g.y);      // 22 bits
+          }
+        }
+        v[j][i] = make_float2(ep.on_a * f.x, ep.on_a * f.y);
+      }
+    }
+    if (n0 == row0) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (n == r) v[j][j].x += ep.on_diagonal;
+        if (n + 1 == r) v[j][j].y += ep.on_diagonal;
+      }
+    }
+  }
+  // The other terms are where the sums begin, read while the first slots are on their way: behind the last accumulation they took
+  // 2,900 cycles of latency (five steps of a 200 x 200 float32 update 114 us, 103 so).
   template <int BN>
-  static __device__ __forceinline__ void begin(const EpiContext&) {}
-  template <int BN, class Release>
-  static __device__ __forceinline__ void drain(const Params& ep, const Product& p, const EpiContext& c, Block& sums, Release release) {
-    const int row0 = c.row0;
-    const float scale = symmetric_scale(ep, c.batch);
-    for_chunks<BN, kSplit>(c, sums, release, [&](int chunk, Block& v) {
-      const int n0 = c.n0 + chunk * 32;
-      if (!needed<BN>(row0, n0, p.M)) return;
+  static __device__ __forceinline__ void begin(const Params& ep, const Product& p, EpiContext& c, Block& sums) {
+    c.scale = symmetric_scale(ep, c.batch);
+    if (Shape<BN>::kCols > 32) return;
+    if (ep.a.hi && needed<BN>(c.row0, c.n0, p.M)) {
+      other_terms(ep, p, c, c.row0, c.n0, sums);
+    } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[j][i] = make_float2(v[j][i].x * scale, v[j][i].y * scale);
-      const int r = c.lane >> 2, n = 2 * (c.lane & 3);
-      if (ep.a.hi) {
-        const __half* at = ep.a.hi + c.batch * ep.a.batch_stride + static_cast<int64_t>(row0 + r) * ep.a.ld + n0 + n;
-#pragma unroll
-        for (int part = 0; part < (kSplit ? 2 : 1); ++part)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (row0 + r + 8 * i >= p.M) continue;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(at + part * ep.a.low + 8 * i * ep.a.ld + 8 * j));
-              v[j][i] = make_float2(fmaf(ep.on_a, f.x, v[j][i].x), fmaf(ep.on_a, f.y, v[j][i].y));
-            }
-          }
-        if (n0 == row0) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (n == r) v[j][j].x += ep.on_diagonal;
-            if (n + 1 == r) v[j][j].y += ep.on_diagonal;
-          }
-        }
-      }
+        for (int i = 0; i < 4; ++i) sums[j][i] = make_float2(0.0f, 0.0f);
+    }
+  }
+  template <int BN, class Release>
+  static __device__ __forceinline__ void drain(const Params& ep, const Product& p, const EpiContext& c, Block& sums, Release release) {
+    auto store = [&](int n0, Block& v) {
+      if (!needed<BN>(c.row0, n0, p.M)) return;
       // and those off the diagonal to their mirror image
       __half* base = ep.out.hi + c.batch * ep.out.batch_stride;
-      store_operands<kSplit>(v, base + static_cast<int64_t>(row0) * ep.out.ld + n0, n0 != row0 ? base + static_cast<int64_t>(n0) * ep.out.ld + row0 : nullptr,
-                             ep.out.ld, ep.out.low, p.M - row0, p.M - n0, c.tail->staging + c.warp * kStageOutBytes, c.lane);
-    });
+      store_operands<kSplit>(v, base + static_cast<int64_t>(c.row0) * ep.out.ld + n0,
+                             n0 != c.row0 ? base + static_cast<int64_t>(n0) * ep.out.ld + c.row0 : nullptr, ep.out.ld, ep.out.low, p.M - c.row0,
+                             p.M - n0, c.tail->staging + c.warp * kStageOutBytes, c.lane);
+    };
+    constexpr int kChunks = Shape<BN>::kCols / 32;
+    if constexpr (kChunks == 1) {
+      load_block(c.tmem, [&](int j, int i, float2 x) {
+        sums[j][i] = make_float2(fmaf(c.scale, x.x, sums[j][i].x), fmaf(c.scale, x.y, sums[j][i].y));
+      });
+      release();
+      if (!kSplit || c.last) store(c.n0, sums);
+    } else {
+      static_assert(!kSplit, "sums of 64 columns do not fit the registers");
+#pragma unroll 1
+      for (int chunk = 0; chunk < kChunks; ++chunk) {
+        const int n0 = c.n0 + chunk * 32;
+        Block v = {};
+        if (ep.a.hi && needed<BN>(c.row0, n0, p.M)) other_terms(ep, p, c, c.row0, n0, v);
+        load_block(c.tmem + chunk * 32, [&](int j, int i, float2 x) {
+          v[j][i] = make_float2(fmaf(c.scale, x.x, v[j][i].x), fmaf(c.scale, x.y, v[j][i].y));
+        });
+        if (chunk == kChunks - 1) release();
+        store(n0, v);
+      }
+    }
   }
 };
 
@@ -443,7 +494,7 @@ struct UpdateOut {
   template <int BN>
   static __device__ __forceinline__ void fetch(const Params&, const Product&, const EpiContext&, int, int) {}
   template <int BN>
-  static __device__ __forceinline__ void begin(const EpiContext&) {}
+  static __device__ __forceinline__ void begin(const Params&, const Product&, const EpiContext&, Block&) {}
   template <int BN, class Release>
   static __device__ __forceinline__ void drain(const Params& ep, const Product& p, const EpiContext& c, Block& sums, Release release) {
     const int row0 = c.row0;
