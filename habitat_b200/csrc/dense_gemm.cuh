@@ -56,8 +56,10 @@ template <int BN, class Epi>
 struct Ring {
   static constexpr int kOperands = (kCtaRows + Shape<BN>::kBRows) * kSlotK;     // per CTA
   static constexpr int kSlotBytes = kOperands * (Epi::kSplit ? 2 : 1);
-  static constexpr int kSlots = Epi::kSplit ? (BN == 256 ? 3 : 4) : Epi::kInt8 ? (BN == 256 ? 5 : BN == 128 ? 6 : 8) : BN == 256 ? 6 : 8;
-  static constexpr int kSmem = kSlots * kSlotBytes + static_cast<int>(sizeof(Tail)) + (Epi::kInt8 ? static_cast<int>(sizeof(LayerTail)) : 0) + 1024;
+  static constexpr int kSlots = Epi::kShares > 1 ? (Epi::kSplit ? 3 : 6) : Epi::kSplit ? (BN == 256 ? 3 : 4) : Epi::kInt8 ? (BN == 256 ? 5 : BN == 128 ? 6 : 8) : BN == 256 ? 6 : 8;
+  // what the other pairs of a cluster send of a tile: their sums of this CTA's part of the columns
+  static constexpr int kShareBytes = (Epi::kShares - 1) * (kCtaRows * BN / Epi::kShares) * 4;
+  static constexpr int kSmem = kSlots * kSlotBytes + kShareBytes + static_cast<int>(sizeof(Tail)) + (Epi::kInt8 ? static_cast<int>(sizeof(LayerTail)) : 0) + 1024;
   static_assert(kSmem <= 232448, "more than a block may have");
 };
 
@@ -374,8 +376,51 @@ inline int tile_columns(std::initializer_list<int> widths, int pairs, Count tile
   return best;
 }
 
-// The kernel.  Epilogue: a policy with `Params`, static kInt8, kMnMajorB, kSplit, kClusterCtas (0: a pair; else the CTAs of a
-// cluster that share rows, one pair per BN columns) and
+// Sums of a tile whose K is split over the kShares pairs of a cluster: every warp but one sends its 32 x 32 sums to the same warp
+// of the pair that finishes these columns, which adds them in the order of the pairs.  False: they are another pair's.
+template <int BN, class Epi>
+__device__ __forceinline__ bool join_shares(const Product& p, const EpiContext& c, Block& sums) {
+  constexpr int S = Epi::kShares;
+  static_assert(Shape<BN>::kCols == 32 && Shape<BN>::kParts % S == 0, "a block per warp, parts for every pair");
+  const int mine = static_cast<int>(c.rank >> 1), owner = c.part % S;
+  const uint32_t bar = smem_u32(&c.tail->exchange[0]);
+  const uint32_t at = smem_u32(c.tail) - Ring<BN, Epi>::kShareBytes + ((c.part / S * 4 + (c.row >> 5)) * (S - 1)) * 4096 + c.lane * 16;
+  if (mine != owner) {
+    const uint32_t there = 2 * owner + (c.rank & 1u);
+    const uint32_t to = map_to_cta(at + (mine - (mine > owner ? 1 : 0)) * 4096, there), to_bar = map_to_cta(bar, there);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float2 x = sums[k >> 1][2 * (k & 1)], y = sums[k >> 1][2 * (k & 1) + 1];
+      st_async_v4(to + 512 * k, __float_as_uint(x.x), __float_as_uint(x.y), __float_as_uint(y.x), __float_as_uint(y.y), to_bar);
+    }
+    return false;
+  }
+  if (!mbar_wait_cluster(bar, 0, &c.tail->abort, p.status, 0x542)) {
+    *c.ok = false;
+    return false;
+  }
+#pragma unroll
+  for (int from = 0; from < S - 1; ++from)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      float4 v;
+      asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at + from * 4096 + 512 * k) : "memory");
+      float2& x = sums[k >> 1][2 * (k & 1)];
+      float2& y = sums[k >> 1][2 * (k & 1) + 1];
+      x = make_float2(x.x + v.x, x.y + v.y);
+      y = make_float2(y.x + v.z, y.y + v.w);
+    }
+  return true;
+}
+
+// What this CTA will be sent.
+template <int BN, class Epi>
+__device__ __forceinline__ void expect_shares(const EpiContext& c) {
+  if (Epi::kShares > 1 && c.warp == 0 && c.lane == 0) mbar_expect_tx(smem_u32(&c.tail->exchange[0]), Ring<BN, Epi>::kShareBytes);
+}
+
+// The kernel.  Epilogue: a policy with `Params`, static kInt8, kMnMajorB, kSplit, kClusterCtas (0: pairs by themselves; else the CTAs of a
+// cluster that share rows, one pair per BN columns), kShares (above 1: the pairs of a cluster share K, a tile per cluster) and
 //   static void begin(const Params&, const Product&, EpiContext&, sums)         before a tile's accumulators are waited for
 //   static void fetch(const Params&, const Product&, EpiContext&, row0, n0)     requests what a tile's results need, a tile ahead
 //   static void drain(const Params&, const Product&, EpiContext&, sums, release)   calls release() once the accumulators are read,
@@ -391,12 +436,12 @@ gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ typename 
   using R = Ring<BN, Epi>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  Tail* tail = reinterpret_cast<Tail*>(ring + R::kSlots * R::kSlotBytes);
+  Tail* tail = reinterpret_cast<Tail*>(ring + R::kSlots * R::kSlotBytes + R::kShareBytes);
   const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31);
   const uint32_t rank = cluster_ctarank();
   const uint32_t side = rank & 1u, pair = rank >> 1;
   const uint32_t leader = rank & ~1u;
-  constexpr int kCluster = Epi::kClusterCtas ? Epi::kClusterCtas : 2;
+  constexpr int kCluster = Epi::kClusterCtas ? Epi::kClusterCtas : 2 * Epi::kShares;
   volatile int* abort_flag = &tail->abort;
   const uint32_t full = smem_u32(tail->full), empty = smem_u32(tail->empty), acc_full = smem_u32(tail->acc_full),
                  acc_empty = smem_u32(tail->acc_empty);
@@ -432,16 +477,19 @@ gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ typename 
   hb_grid_dependency_wait();   // the set-up above overlaps the end of the launch before it on the stream
   const uint32_t tmem = tail->tmem;
 
-  // a tile of the list per pair, or, where a cluster shares rows, per cluster (its pairs take neighbouring columns)
-  const int workers = static_cast<int>(gridDim.x) / kCluster * (Epi::kClusterCtas ? 1 : kCluster / 2);
-  const int worker = static_cast<int>(blockIdx.x) / (Epi::kClusterCtas ? kCluster : 2);
+  // a tile of the list per cluster; where it shares rows, its pairs take neighbouring columns
+  const int workers = static_cast<int>(gridDim.x) / kCluster;
+  const int worker = static_cast<int>(blockIdx.x) / kCluster;
   auto locate = [&](int t) {
     if (Epi::kClusterCtas) return Tile{0, t * kPairRows, t * kPairRows + kCtaRows, static_cast<int>(pair) * BN, 0};
-    return tile_of<BN>(p, t);
+    Tile r = tile_of<BN>(p, t);
+    if (Epi::kShares > 1) r.split = static_cast<int>(pair);
+    return r;
   };
   // slots of K of a share, and where it begins
-  const int most_kb = p.splits > 1 ? (p.kblocks + p.splits - 1) / p.splits : p.kblocks;
-  auto slots_of = [&](int split) { return p.splits > 1 ? max(0, min(most_kb, p.kblocks - split * most_kb)) : most_kb; };
+  const int splits = Epi::kShares > 1 ? Epi::kShares : p.splits;
+  const int most_kb = splits > 1 ? (p.kblocks + splits - 1) / splits : p.kblocks;
+  auto slots_of = [&](int split) { return splits > 1 ? max(0, min(most_kb, p.kblocks - split * most_kb)) : most_kb; };
 
   if (warp == 0) {
     // ------------------------------ copies ------------------------------
@@ -494,7 +542,7 @@ gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ typename 
       uint32_t s = 0, ph = 0, n = 0;
       bool ok = true;
       for (int t = worker; t < p.num_tiles && ok; t += workers) {
-        const int slots = slots_of(p.splits > 1 ? locate(t).split : 0);
+        const int slots = slots_of(splits > 1 ? locate(t).split : 0);
         for (int kb = 0; kb < slots && ok;) {
           const uint32_t st = n % S::kAccs, turn = n / S::kAccs & 1u;
           ++n;

@@ -264,7 +264,7 @@ __device__ __forceinline__ float max3_abs(float a, float b, float c) {
 
 struct FloatOut {
   static constexpr bool kInt8 = true, kMnMajorB = false, kSplit = false;
-  static constexpr int kClusterCtas = 0;
+  static constexpr int kClusterCtas = 0, kShares = 1;
   struct Params {
     LayerScales s;
     Out out;
@@ -329,7 +329,7 @@ struct FloatOut {
 template <int kCtas>
 struct QuantOut {
   static constexpr bool kInt8 = true, kMnMajorB = false, kSplit = false;
-  static constexpr int kClusterCtas = kCtas;
+  static constexpr int kClusterCtas = kCtas, kShares = 1;
   struct Params {
     LayerScales s;
     int8_t* q;

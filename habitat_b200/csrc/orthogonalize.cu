@@ -302,7 +302,7 @@ template <bool kLow>
 struct ShareOut {
   static constexpr bool kSplit = kLow;
   static constexpr bool kInt8 = false, kMnMajorB = false;
-  static constexpr int kClusterCtas = 0;
+  static constexpr int kClusterCtas = 0, kShares = 1;
   struct Params {
     float* shares;          // [tile and split][256][BN]
   };
@@ -393,11 +393,11 @@ __global__ void __launch_bounds__(256) symmetric_sum_kernel(const __grid_constan
 }
 
 // Symmetric results: A = X X^T, or B = a I + b A + c A^2, as half-precision operands (kSplit: high and low parts).
-template <bool kLow>
+template <bool kLow, int kPairs>
 struct SymmetricOut {
   static constexpr bool kSplit = kLow;
   static constexpr bool kInt8 = false, kMnMajorB = false;
-  static constexpr int kClusterCtas = 0;
+  static constexpr int kClusterCtas = 0, kShares = kPairs;
   using Params = Symmetric;
   template <int BN>
   static __device__ __forceinline__ void fetch(const Params&, const Product&, const EpiContext&, int, int) {}
@@ -434,8 +434,9 @@ struct SymmetricOut {
   template <int BN>
   static __device__ __forceinline__ void begin(const Params& ep, const Product& p, EpiContext& c, Block& sums) {
     c.scale = symmetric_scale(ep, c.batch);
+    expect_shares<BN, SymmetricOut>(c);
     if (Shape<BN>::kCols > 32) return;
-    if (ep.a.hi && needed<BN>(c.row0, c.n0, p.M)) {
+    if (ep.a.hi && needed<BN>(c.row0, c.n0, p.M) && (kShares == 1 || c.part % kShares == static_cast<int>(c.rank >> 1))) {
       other_terms(ep, p, c, c.row0, c.n0, sums);
     } else {
 #pragma unroll
@@ -460,7 +461,10 @@ struct SymmetricOut {
         sums[j][i] = make_float2(fmaf(c.scale, x.x, sums[j][i].x), fmaf(c.scale, x.y, sums[j][i].y));
       });
       release();
-      if (!kSplit || c.last) store(c.n0, sums);
+      if (kSplit && !c.last) return;
+      if constexpr (kShares > 1)
+        if (!join_shares<BN, SymmetricOut>(p, c, sums)) return;
+      store(c.n0, sums);
     } else {
       static_assert(!kSplit, "sums of 64 columns do not fit the registers");
 #pragma unroll 1
@@ -479,28 +483,33 @@ struct SymmetricOut {
 };
 
 // X <- B X as operands of the next step, or as the result.
-template <bool kLow>
+struct Step {
+  Planes x;               // the next X; hi null: the result
+  Out out;
+  int32_t flip;           // the result is transposed
+  const float* factor;    // of the first step
+  float scale;
+};
+template <bool kLow, int kPairs>
 struct UpdateOut {
   static constexpr bool kSplit = kLow;
   static constexpr bool kInt8 = false, kMnMajorB = true;
-  static constexpr int kClusterCtas = 0;
-  struct Params {
-    Planes x;               // the next X; hi null: the result
-    Out out;
-    int32_t flip;           // the result is transposed
-    const float* factor;    // of the first step
-    float scale;
-  };
+  static constexpr int kClusterCtas = 0, kShares = kPairs;
+  using Params = Step;
   template <int BN>
   static __device__ __forceinline__ void fetch(const Params&, const Product&, const EpiContext&, int, int) {}
   template <int BN>
-  static __device__ __forceinline__ void begin(const Params&, const Product&, const EpiContext&, Block&) {}
+  static __device__ __forceinline__ void begin(const Params&, const Product&, const EpiContext& c, Block&) {
+    expect_shares<BN, UpdateOut>(c);
+  }
   template <int BN, class Release>
   static __device__ __forceinline__ void drain(const Params& ep, const Product& p, const EpiContext& c, Block& sums, Release release) {
     const int row0 = c.row0;
     const float scale = ep.factor ? ep.scale * __ldg(ep.factor + c.batch) : ep.scale;
     uint8_t* staging = c.tail->staging + c.warp * kStageOutBytes;
     for_chunks<BN, kSplit>(c, sums, release, [&](int chunk, Block& v) {
+      if constexpr (kShares > 1)
+        if (!join_shares<BN, UpdateOut>(p, c, v)) return;
       const int n0 = c.n0 + chunk * 32;
       if (n0 >= p.N || row0 >= p.M) return;
 #pragma unroll
@@ -591,12 +600,18 @@ Layout layout_of(int64_t batch, int64_t rows, int64_t cols, bool split) {
   return r;
 }
 
+// Clusters of a product that the current GPU holds.
+template <int BN, class Epi>
+hb_status clusters_held(int* n) {
+  static std::atomic<int> held[64];
+  return max_clusters(gemm_kernel<BN, Epi>, 2 * Epi::kShares, Shape<BN>::kThreads, Ring<BN, Epi>::kSmem, held, n);
+}
+
 template <int BN, class Epi>
 hb_status launch(Product p, const typename Epi::Params& ep, cudaStream_t s, Product* as_launched = nullptr) {
-  static std::atomic<int> held[64];
-  int pairs = 0;
+  int held = 0;
   auto kernel = gemm_kernel<BN, Epi>;
-  if (const hb_status st = max_clusters(kernel, 2, Shape<BN>::kThreads, Ring<BN, Epi>::kSmem, held, &pairs)) return st;
+  if (const hb_status st = clusters_held<BN, Epi>(&held)) return st;
   p.tiles_m = static_cast<int32_t>((p.M + kPairRows - 1) / kPairRows);
   p.tiles_n = static_cast<int32_t>((p.N + BN - 1) / BN);
   const int64_t tiles = p.lower ? lower_tiles(p.M, BN) : static_cast<int64_t>(p.tiles_m) * p.tiles_n;
@@ -605,22 +620,43 @@ hb_status launch(Product p, const typename Epi::Params& ep, cudaStream_t s, Prod
     return HB_ERR_TOO_LARGE;
   }
   set_tiles(&p, tiles);
-  const int clusters = p.num_tiles < pairs ? p.num_tiles : pairs;
-  HB_CUDA_TRY(launch_clusters(kernel, clusters, 2, Shape<BN>::kThreads, Ring<BN, Epi>::kSmem, s, p, ep));
+  // pairs that share a tile have one each
+  const int clusters = p.num_tiles < held || Epi::kShares > 1 ? p.num_tiles : held;
+  HB_CUDA_TRY(launch_clusters(kernel, clusters, 2 * Epi::kShares, Shape<BN>::kThreads, Ring<BN, Epi>::kSmem, s, p, ep));
   if (as_launched) *as_launched = p;
   return HB_OK;
 }
 
-// How many ways K of a symmetric product is split: as many as there are SM pairs for the tiles, of at least four slots; one
-// unless that saves 24 slots' time (about 3 us, what the second launch takes).
+// Times in units of 240 cycles: a slot of operands with low parts takes 4, of others 1, a second launch that adds shares from
+// memory about 55, and sums that the pairs of a cluster exchange 15 and 7 (fitted to updates of 200 x 200 to 1024 x 1024).
+constexpr int kSecondLaunch = 55;
+int64_t slot_time(int64_t slots, bool split) { return slots * (split ? 4 : 1); }
+
+// How many ways K of a symmetric product is split, the shares added by a second launch: as many as there are SM pairs for the
+// tiles, of at least four slots; one unless that saves more than the launch takes.
 int splits_of(int64_t batch, int64_t s, int64_t K, bool split, int pairs) {
   const int64_t tiles = batch * lower_tiles(s, 128), slots = (K + 63) / 64;
   int64_t n = pairs / tiles;
   if (n > slots / 4) n = slots / 4;
   if (n < 2) return 1;
   const int64_t each = (slots + n - 1) / n;
-  if ((slots - each) * (split ? 3 : 1) < 24) return 1;
+  if (slot_time(slots - each, split) < kSecondLaunch) return 1;
   return static_cast<int>((slots + each - 1) / each);      // none without slots
+}
+
+// How many pairs of a cluster share K of a product with `tiles` tiles of 128 columns: as many as make it shortest, where all its
+// clusters run at once and every pair has a slot.  `alone`: what it takes otherwise.  (Five steps of a 777 x 1000 half-precision
+// update, with the sums of all products exchanged or added by second launches: 159 and 213 us; 1024 x 1024 float32 176 and 220.)
+int shares_of(int64_t tiles, int64_t K, bool split, const int (&held)[5], int64_t alone) {
+  const int64_t slots = (K + 63) / 64;
+  int best = 1;
+  for (const int n : {2, 4}) {
+    const int64_t each = (slots + n - 1) / n, cost = slot_time(each, split) + (split ? 15 : 7);
+    if (tiles > held[n] || (n - 1) * each >= slots || cost >= alone) continue;
+    alone = cost;
+    best = n;
+  }
+  return best;
 }
 
 // The cluster that holds a matrix whose shorter side is at most 128: its CTAs, and blocks of 64 columns per CTA; 0 when it
@@ -850,21 +886,34 @@ extern "C" hb_status hb_orthogonalize(const void* update, int32_t type, int64_t 
   // sums for 64 columns per epilogue lane, a tile of 256, do not fit its registers (8192 x 4096 float32: 13.1 ms)
   const int bn_sym = split ? tile_columns({128, 64}, pairs, sym_tiles) : tile_columns({256, 128, 64}, pairs, sym_tiles);
   const int bn_upd = split ? 128 : tile_columns({256, 128}, pairs, upd_tiles);
+  // pairs of a cluster that share K: of X X^T, A A and B X
+  int held[5] = {};
+  if (const hb_status e = split ? clusters_held<128, SymmetricOut<true, 2>>(&held[2]) : clusters_held<128, SymmetricOut<false, 2>>(&held[2])) return e;
+  if (const hb_status e = split ? clusters_held<128, SymmetricOut<true, 4>>(&held[4]) : clusters_held<128, SymmetricOut<false, 4>>(&held[4])) return e;
+  auto symmetric_shares = [&](int64_t K) {
+    const int64_t slots = (K + 63) / 64, each_way = splits_of(batch, lay.s, K, split != 0, pairs);
+    const int64_t alone = each_way > 1 ? slot_time((slots + each_way - 1) / each_way, split != 0) + kSecondLaunch
+                                       : slot_time(slots, split != 0) * (bn_sym == 64 ? 3 : 4) / 4;
+    return shares_of(sym_tiles(128), K, split != 0, held, alone);
+  };
+  const int gram_shares = symmetric_shares(lay.l), poly_shares = symmetric_shares(lay.s);
+  const int upd_shares = shares_of(upd_tiles(128), lay.s, split != 0, held, slot_time((lay.s + 63) / 64, split != 0) * (bn_upd == 256 ? 2 : 1));
+  auto symmetric_columns = [&](int64_t K, int shares) { return shares > 1 || splits_of(batch, lay.s, K, split != 0, pairs) > 1 ? 128 : bn_sym; };
   CUtensorMap x_rows[2], x_cols[2], x_k[2], a_rows, a_cols, b_rows;
   for (int i = 0; i < (steps > 1 ? 2 : 1); ++i) {
     HB_CUDA_TRY(encode_planes(&x_rows[i], x[i], 2, lay.l, lay.s, batch * planes, lay.lp, x_matrix, kCtaRows));
-    HB_CUDA_TRY(encode_planes(&x_cols[i], x[i], 2, lay.l, lay.s, batch * planes, lay.lp, x_matrix, (splits_of(batch, lay.s, lay.l, split != 0, pairs) > 1 ? 128 : bn_sym) / 2));
+    HB_CUDA_TRY(encode_planes(&x_cols[i], x[i], 2, lay.l, lay.s, batch * planes, lay.lp, x_matrix, symmetric_columns(lay.l, gram_shares) / 2));
     HB_CUDA_TRY(encode_planes(&x_k[i], x[i], 2, lay.l, lay.s, batch * planes, lay.lp, x_matrix, 64));
   }
   HB_CUDA_TRY(encode_planes(&a_rows, A, 2, lay.s, lay.s, batch * planes, lay.sp, a_matrix, kCtaRows));
-  HB_CUDA_TRY(encode_planes(&a_cols, A, 2, lay.s, lay.s, batch * planes, lay.sp, a_matrix, (splits_of(batch, lay.s, lay.s, split != 0, pairs) > 1 ? 128 : bn_sym) / 2));
+  HB_CUDA_TRY(encode_planes(&a_cols, A, 2, lay.s, lay.s, batch * planes, lay.sp, a_matrix, symmetric_columns(lay.s, poly_shares) / 2));
   HB_CUDA_TRY(encode_planes(&b_rows, B, 2, lay.s, lay.s, batch * planes, lay.sp, a_matrix, kCtaRows));
 
   const int32_t out_vec = row_alignment(out, out_pitch, batch > 1 ? out_batch_stride : 0, type == HB_F32 ? 4 : 2);
   auto run = [&](auto is_split) -> hb_status {
     constexpr bool kSplit = decltype(is_split)::value;
-    using Sym = SymmetricOut<kSplit>;
-    using Upd = UpdateOut<kSplit>;
+    using Sym = SymmetricOut<kSplit, 1>;
+    using Upd = UpdateOut<kSplit, 1>;
     auto product = [&](const CUtensorMap& ma, const CUtensorMap& mb, int64_t N, int64_t K) {
       Product p{};
       p.a = ma;
@@ -877,9 +926,11 @@ extern "C" hb_status hb_orthogonalize(const void* update, int32_t type, int64_t 
       p.status = status;
       return p;
     };
-    auto symmetric = [&](const CUtensorMap& ma, const CUtensorMap& mb, int64_t K, const typename Sym::Params& ep) -> hb_status {
+    auto symmetric = [&](const CUtensorMap& ma, const CUtensorMap& mb, int64_t K, int shares_of_k, const typename Sym::Params& ep) -> hb_status {
       Product p = product(ma, mb, lay.s, K);
       p.lower = 1;
+      if (shares_of_k == 2) return launch<128, SymmetricOut<kSplit, 2>>(p, ep, st);
+      if (shares_of_k == 4) return launch<128, SymmetricOut<kSplit, 4>>(p, ep, st);
       p.splits = splits_of(batch, lay.s, K, kSplit, pairs);
       if (p.splits > 1) {
         if (const hb_status e = launch<128, ShareOut<kSplit>>(p, {shares}, st, &p)) return e;
@@ -895,16 +946,18 @@ extern "C" hb_status hb_orthogonalize(const void* update, int32_t type, int64_t 
       const int from = i & 1, to = from ^ 1;
       const bool first = i == 0, last = i == steps - 1;
       const typename Sym::Params gram{a_planes, Planes{}, first ? factor : nullptr, first ? kScale : 1.0f / kScale, 0.0f, 0.0f};
-      if (const hb_status e = symmetric(x_rows[from], x_cols[from], lay.l, gram)) return e;
+      if (const hb_status e = symmetric(x_rows[from], x_cols[from], lay.l, gram_shares, gram)) return e;
       // B 2^8 = b (A 2^8) + (c / 2^8) (A 2^8)^2 + a 2^8 I
       const typename Sym::Params poly{b_planes, a_planes, nullptr, static_cast<float>(c / kScale), static_cast<float>(b), static_cast<float>(a * kScale)};
-      if (const hb_status e = symmetric(a_rows, a_cols, lay.s, poly)) return e;
+      if (const hb_status e = symmetric(a_rows, a_cols, lay.s, poly_shares, poly)) return e;
       // (B 2^8)(X 2^8 or X0) -> X 2^8, or X
       const float scale = (first ? 1.0f : 1.0f / kScale) * (last ? 1.0f : kScale) / kScale;
-      const typename Upd::Params ep{last ? Planes{} : x_planes(to), Out{out, out_pitch, out_batch_stride, type, out_vec}, flip, first ? factor : nullptr, scale};
+      const Step ep{last ? Planes{} : x_planes(to), Out{out, out_pitch, out_batch_stride, type, out_vec}, flip, first ? factor : nullptr, scale};
       const Product p = product(b_rows, x_k[from], lay.l, lay.s);
       hb_status e = HB_OK;
-      if constexpr (kSplit) e = launch<128, Upd>(p, ep, st);
+      if (upd_shares == 2) e = launch<128, UpdateOut<kSplit, 2>>(p, ep, st);
+      else if (upd_shares == 4) e = launch<128, UpdateOut<kSplit, 4>>(p, ep, st);
+      else if constexpr (kSplit) e = launch<128, Upd>(p, ep, st);
       else e = bn_upd == 256 ? launch<256, Upd>(p, ep, st) : launch<128, Upd>(p, ep, st);
       if (e) return e;
     }

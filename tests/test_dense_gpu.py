@@ -344,6 +344,18 @@ def test_orthogonalize_long_and_short_sides(shape, dtype):
     _check(update, dense.orthogonalize(update))
 
 
+# single matrices, whose products are split along K over the pairs of a cluster or over launches, with slots that do not divide by the shares
+@pytest.mark.parametrize("shape", [(400, 400), (768, 768), (777, 1000), (1000, 777), (513, 1100), (900, 900), (300, 3000), (150, 8000), (2, 650, 700),
+                                   (4, 510, 520), (1200, 1100)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_orthogonalize_single_matrices(shape, dtype):
+    update = _update(shape, sum(shape), dtype)
+    got = dense.orthogonalize(update)
+    _check(update, got)
+    for _ in range(3):
+        assert torch.equal(got, dense.orthogonalize(update))
+
+
 # read in pieces of eight elements or one by one: rows that are no multiple of eight, that start on any element, and both
 @pytest.mark.parametrize("shape", [(129, 204), (131, 260), (129, 1030), (3, 131, 204), (1030, 129), (131, 2056)])
 @pytest.mark.parametrize("dtype", DTYPES)
