@@ -134,7 +134,8 @@ __global__ void __launch_bounds__(32 * kChannels * kSplits, kChannels == 1 && kT
       for (int j = 0; j < 4; ++j) {
         const int m = 8 * i + 2 * t + (j & 1), n = n0 + g + 8 * (j >> 1);
         const float rs = m < p.M ? __ldg(p.s.row + m) : 0.0f;
-        const float y = max_nan(__fadd_rn(__fmul_rn(__fmul_rn(__int2float_rn(acc[i][j]), w[j >> 1]), rs), b[j >> 1]), p.s.floor);
+        float y = __fadd_rn(__fmul_rn(__fmul_rn(__int2float_rn(acc[i][j]), w[j >> 1]), rs), b[j >> 1]);
+        if (p.s.relu) y = relu_nan(y);
         v[i][j] = y;
         if (!kQuant && m < p.M && n < p.N) {
           const int64_t at = m * p.out.ld + n;

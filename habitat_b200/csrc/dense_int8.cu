@@ -169,7 +169,8 @@ struct LayerScales {
   const float* row;
   const float* channel;
   const float* bias;     // or null
-  float floor;           // 0 with ReLU, else -infinity: the larger of a value and it
+  int32_t relu;
+  float one;             // 1
 };
 
 }  // namespace
@@ -214,8 +215,9 @@ __device__ __forceinline__ void fetch_scales(const LayerScales& s, const Product
   copy_float(to + 128 + c.lane, s.row + (there ? row0 + c.lane : 0), there);
 }
 
-// Two products.  (The sums behind them stay single: a packed sum of packed products is merged into a multiply-add, which
-// rounds once instead of twice, whatever the instructions' rounding says.)
+// Two products, two sums.  A packed sum of packed products is merged into a multiply-add, which rounds once instead of twice,
+// whatever the instructions' rounding says; y * one + b, with a one that only the host knows, is the rounded sum and stays as it is.
+// (The epilogue is bound by its issue slots: with single sums quantised rows of 65,536 x 1024 x 1024 took CHANGED.)
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   float2 r;
   asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
@@ -223,8 +225,16 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return r;
 }
+__device__ __forceinline__ float2 add2(float2 a, float2 b, float one) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z, d;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%6, %6};\n\tmov.b64 z, {%4, %5};\n\tfma.rn.f32x2 d, x, y, z;\n\t"
+      "mov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(one));
+  return r;
+}
 
-// The warp's part of the tile as results: v[j][i] are columns 8 j + 2 (lane mod 4) and the next of row 8 i + lane / 4.
+// The warp's part of the tile as results before ReLU: v[j][i] are columns 8 j + 2 (lane mod 4) and the next of row 8 i + lane / 4.
 template <int BN, class Release>
 __device__ __forceinline__ void finish(const LayerScales& s, const Product& p, const EpiContext& c, float2 (&v)[Shape<BN>::kCols / 8][4],
                                        Release release) {
@@ -249,7 +259,7 @@ __device__ __forceinline__ void finish(const LayerScales& s, const Product& p, c
       const uint32_t* a = &acc[i >> 1][4 * j + 2 * (i & 1)];
       const float2 x = make_float2(__int2float_rn(static_cast<int>(a[0])), __int2float_rn(static_cast<int>(a[1])));
       const float2 y = mul2(mul2(x, w), make_float2(row[i], row[i]));
-      v[j][i] = make_float2(max_nan(__fadd_rn(y.x, b.x), s.floor), max_nan(__fadd_rn(y.y, b.y), s.floor));
+      v[j][i] = add2(y, b, s.one);
     }
   }
   __syncwarp();
@@ -260,6 +270,46 @@ __device__ __forceinline__ float max3_abs(float a, float b, float c) {
   float r;
   asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// quantized() of four values, packed.  With ReLU what is negative, by however much, has to become 0: the conversion instruction
+// and the packing one saturate (6 instructions for four, 9 with maxima).
+template <bool kRelu>
+__device__ __forceinline__ uint32_t quantized4(float2 a, float2 b, float inverse, float one) {
+  const float2 scale = make_float2(inverse, inverse);
+  float2 x = mul2(a, scale), y = mul2(b, scale);
+  if (kRelu) {
+    uint32_t high, r;
+    asm("cvt.pack.sat.u8.s32.b32 %0, %1, %2, %3;" : "=r"(high) : "r"(__float2int_rn(y.y)), "r"(__float2int_rn(y.x)), "r"(0));
+    asm("cvt.pack.sat.u8.s32.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(__float2int_rn(x.y)), "r"(__float2int_rn(x.x)), "r"(high));
+    return r;
+  }
+  const float2 magic = make_float2(12582912.0f, 12582912.0f);
+  x = add2(x, magic, one);
+  y = add2(y, magic, one);
+  return __byte_perm(__byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x0040), __byte_perm(__float_as_uint(y.x), __float_as_uint(y.y), 0x0040), 0x5410);
+}
+
+// Two results in 16 bits, with ReLU (NaN stays) in the conversion.
+template <bool kRelu, bool kBf16>
+__device__ __forceinline__ uint32_t pack_result(float2 x) {
+  uint32_t r;
+  if (!kRelu) return kBf16 ? pack_bf16(x.x, x.y) : pack_f16(x.x, x.y);
+  if (kBf16) asm("cvt.rn.relu.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(x.y), "f"(x.x));
+  else asm("cvt.rn.relu.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(x.y), "f"(x.x));
+  return r;
+}
+template <bool kRelu, bool kBf16>
+__device__ __forceinline__ void pack_results(const float2 (*v)[4], uint32_t (&w)[4][4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[i][j] = pack_result<kRelu, kBf16>(v[j][i]);
 }
 
 struct FloatOut {
@@ -282,6 +332,12 @@ struct FloatOut {
     finish<BN>(ep.s, p, c, v, release);
     const int row0 = c.row0 + (c.lane >> 2);
     if (ep.out.type == kF32) {
+      if (ep.s.relu) {
+#pragma unroll
+        for (int j = 0; j < kBlocks; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[j][i] = make_float2(relu_nan(v[j][i].x), relu_nan(v[j][i].y));
+      }
       // four lanes fill a sector
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -307,14 +363,17 @@ struct FloatOut {
     uint8_t* staging = c.tail->staging + c.warp * kStageOutBytes;
 #pragma unroll
     for (int g = 0; g < kBlocks; g += 4) {         // 32 columns, 64 bytes, at a time
+      uint32_t w[4][4];
+      if (ep.out.type == kBF16) {
+        if (ep.s.relu) pack_results<true, true>(v + g, w);
+        else pack_results<false, true>(v + g, w);
+      } else {
+        if (ep.s.relu) pack_results<true, false>(v + g, w);
+        else pack_results<false, false>(v + g, w);
+      }
       __syncwarp();
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t w[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = ep.out.type == kBF16 ? pack_bf16(v[g + j][i].x, v[g + j][i].y) : pack_f16(v[g + j][i].x, v[g + j][i].y);
-        store_fragment(smem_u32(staging), i, w, c.lane);
-      }
+      for (int i = 0; i < 4; ++i) store_fragment(smem_u32(staging), i, w[i], c.lane);
       __syncwarp();
       store_staged(staging, static_cast<uint16_t*>(ep.out.base) + static_cast<int64_t>(c.row0) * ep.out.ld + c.n0 + 8 * g, ep.out.ld, ep.out.vec,
                    p.M - c.row0, p.N - c.n0 - 8 * g, c.lane);
@@ -355,8 +414,13 @@ struct QuantOut {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float m = 0.0f;
+      if (ep.s.relu) {
 #pragma unroll
-      for (int j = 0; j < kBlocks; ++j) m = max3_abs(m, v[j][i].x, v[j][i].y);
+        for (int j = 0; j < kBlocks; ++j) m = max3(m, v[j][i].x, v[j][i].y);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kBlocks; ++j) m = max3_abs(m, v[j][i].x, v[j][i].y);
+      }
       m = max_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
       m = max_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
       if ((c.lane & 3) == i) amax = m;
@@ -386,10 +450,13 @@ struct QuantOut {
       const int from = (c.lane & ~3) | i;                             // the lane that has row 8 i + lane / 4
       const float inverse = __shfl_sync(0xFFFFFFFFu, s.inverse, from);
       uint32_t w[4];                            // the lane's two columns of blocks 2 j and 2 j + 1
+      if (ep.s.relu) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        w[j] = low_bytes(quantized(v[2 * j][i].x, inverse), quantized(v[2 * j][i].y, inverse), quantized(v[2 * j + 1][i].x, inverse),
-                         quantized(v[2 * j + 1][i].y, inverse));
+        for (int j = 0; j < 4; ++j) w[j] = quantized4<true>(v[2 * j][i], v[2 * j + 1][i], inverse, ep.s.one);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = quantized4<false>(v[2 * j][i], v[2 * j + 1][i], inverse, ep.s.one);
+      }
       store_fragment(smem_u32(staging), i, w, c.lane);
     }
     __syncwarp();
@@ -680,7 +747,7 @@ extern "C" hb_status hb_int8_matmul(const int8_t* q, int64_t q_pitch, const floa
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   Operands o{q, q_pitch, w, w_pitch};
   if (const hb_status st = align_operands(name, &o, M, N, K, static_cast<uint8_t*>(workspace), workspace_bytes, 0, s)) return st;
-  FloatOut::Params ep{{q_scales, w_scales, bias, relu ? 0.0f : -INFINITY}, {out, out_pitch, 0, out_type, 0}};
+  FloatOut::Params ep{{q_scales, w_scales, bias, relu ? 1 : 0, 1.0f}, {out, out_pitch, 0, out_type, 0}};
   ep.out.vec = row_alignment(out, out_pitch, 0, out_type == HB_F32 ? 4 : 2);
   if (M <= kFewRows) {
     FewParams few{o.q, o.w, o.q_pitch, o.w_pitch, ep.s, static_cast<int32_t>(M), static_cast<int32_t>(N), static_cast<int32_t>(K), ep.out, nullptr, 0,
@@ -726,7 +793,7 @@ extern "C" hb_status hb_int8_matmul_quantized(const int8_t* q, int64_t q_pitch, 
     return hb_quantize_rows(y, HB_F32, M, N, pitch, out, out_pitch, out_scales, stream);
   }
   if (const hb_status st = align_operands(name, &o, M, N, K, ws, workspace_bytes, 0, s)) return st;
-  const LayerScales scales{q_scales, w_scales, bias, relu ? 0.0f : -INFINITY};
+  const LayerScales scales{q_scales, w_scales, bias, relu ? 1 : 0, 1.0f};
   if (M <= kFewRows) {
     FewParams few{o.q, o.w, o.q_pitch, o.w_pitch, scales, static_cast<int32_t>(M), static_cast<int32_t>(N), static_cast<int32_t>(K), Out{}, out,
                   out_pitch, out_scales, status};
