@@ -42,7 +42,7 @@ struct Shape {
 // Shared memory behind the ring: staging, barriers; 8-bit layers: scales and row maxima of the cluster's CTAs.
 struct Tail {
   uint8_t staging[kMostEpiWarps * kStageOutBytes];
-  uint64_t full[8], empty[8], acc_full[4], acc_empty[4], exchange[2], drain;
+  uint64_t full[8], empty[8], acc_full[4], acc_empty[4], exchange[2][4], drain;
   uint32_t tmem;
   int abort;
 };
@@ -383,7 +383,7 @@ __device__ __forceinline__ bool join_shares(const Product& p, const EpiContext& 
   constexpr int S = Epi::kShares;
   static_assert(Shape<BN>::kCols == 32 && Shape<BN>::kParts % S == 0, "a block per warp, parts for every pair");
   const int mine = static_cast<int>(c.rank >> 1), owner = c.part % S;
-  const uint32_t bar = smem_u32(&c.tail->exchange[0]);
+  const uint32_t bar = smem_u32(&c.tail->exchange[0][0]);
   const uint32_t at = smem_u32(c.tail) - Ring<BN, Epi>::kShareBytes + ((c.part / S * 4 + (c.row >> 5)) * (S - 1)) * 4096 + c.lane * 16;
   if (mine != owner) {
     const uint32_t there = 2 * owner + (c.rank & 1u);
@@ -416,7 +416,7 @@ __device__ __forceinline__ bool join_shares(const Product& p, const EpiContext& 
 // What this CTA will be sent.
 template <int BN, class Epi>
 __device__ __forceinline__ void expect_shares(const EpiContext& c) {
-  if (Epi::kShares > 1 && c.warp == 0 && c.lane == 0) mbar_expect_tx(smem_u32(&c.tail->exchange[0]), Ring<BN, Epi>::kShareBytes);
+  if (Epi::kShares > 1 && c.warp == 0 && c.lane == 0) mbar_expect_tx(smem_u32(&c.tail->exchange[0][0]), Ring<BN, Epi>::kShareBytes);
 }
 
 // The kernel.  Epilogue: a policy with `Params`, static kInt8, kMnMajorB, kSplit, kClusterCtas (0: pairs by themselves; else the CTAs of a
@@ -455,7 +455,7 @@ gemm_kernel(const __grid_constant__ Product p, const __grid_constant__ typename 
       mbar_init(acc_full + 8 * s, 1);
       mbar_init(acc_empty + 8 * s, 2 * S::kEpiWarps);
     }
-    for (int s = 0; s < 2; ++s) mbar_init(smem_u32(&tail->exchange[s]), 1);
+    for (int s = 0; s < 8; ++s) mbar_init(smem_u32(&tail->exchange[0][0]) + 8 * s, 1);
     mbar_init(smem_u32(&tail->drain), 1);
     tail->abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");

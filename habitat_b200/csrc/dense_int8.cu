@@ -202,14 +202,16 @@ __device__ __forceinline__ void copy_float(const float* to, const float* from, b
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(there ? 4 : 0) : "memory");
 }
 template <int BN>
-__device__ __forceinline__ void fetch_scales(const LayerScales& s, const Product& p, const EpiContext& c, int row0, int n0) {
+__device__ __forceinline__ void fetch_scales(const LayerScales& s, const Product& p, const EpiContext& c, int row0, int n0, bool channels) {
   float* to = c.layer->scales[c.warp];
+  if (channels) {
 #pragma unroll
-  for (int i = 0; i < Shape<BN>::kCols; i += 32) {
-    const bool there = n0 + i + c.lane < p.N;
-    const int n = there ? n0 + i + c.lane : 0;
-    copy_float(to + i + c.lane, s.channel + n, there);
-    copy_float(to + 64 + i + c.lane, (s.bias ? s.bias : s.channel) + n, there && s.bias);
+    for (int i = 0; i < Shape<BN>::kCols; i += 32) {
+      const bool there = n0 + i + c.lane < p.N;
+      const int n = there ? n0 + i + c.lane : 0;
+      copy_float(to + i + c.lane, s.channel + n, there);
+      copy_float(to + 64 + i + c.lane, (s.bias ? s.bias : s.channel) + n, there && s.bias);
+    }
   }
   const bool there = row0 + c.lane < p.M;
   copy_float(to + 128 + c.lane, s.row + (there ? row0 + c.lane : 0), there);
@@ -217,7 +219,8 @@ __device__ __forceinline__ void fetch_scales(const LayerScales& s, const Product
 
 // Two products, two sums.  A packed sum of packed products is merged into a multiply-add, which rounds once instead of twice,
 // whatever the instructions' rounding says; y * one + b, with a one that only the host knows, is the rounded sum and stays as it is.
-// (The epilogue is bound by its issue slots: with single sums quantised rows of 65,536 x 1024 x 1024 took CHANGED.)
+// (The epilogue is bound by its issue slots: with single sums and maxima quantised rows of 65,536 x 1024 x 1024 took 69 us,
+// 63 so.)
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   float2 r;
   asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
@@ -263,7 +266,7 @@ __device__ __forceinline__ void finish(const LayerScales& s, const Product& p, c
     }
   }
   __syncwarp();
-  if (c.next_row0 >= 0) fetch_scales<BN>(s, p, c, c.next_row0, c.next_n0);
+  if (c.next_row0 >= 0) fetch_scales<BN>(s, p, c, c.next_row0, c.next_n0, c.next_n0 != c.n0);
 }
 
 __device__ __forceinline__ float max3_abs(float a, float b, float c) {
@@ -277,22 +280,21 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-// quantized() of four values, packed.  With ReLU what is negative, by however much, has to become 0: the conversion instruction
-// and the packing one saturate (6 instructions for four, 9 with maxima).
+// quantized() of four values, packed.  The conversion instruction and the packing one saturate, which with ReLU leaves 0 of what is
+// negative, by however much (6 instructions for four results, 9 with maxima and sums with 1.5 * 2^23).
 template <bool kRelu>
-__device__ __forceinline__ uint32_t quantized4(float2 a, float2 b, float inverse, float one) {
+__device__ __forceinline__ uint32_t quantized4(float2 a, float2 b, float inverse) {
   const float2 scale = make_float2(inverse, inverse);
-  float2 x = mul2(a, scale), y = mul2(b, scale);
+  const float2 x = mul2(a, scale), y = mul2(b, scale);
+  uint32_t high, r;
   if (kRelu) {
-    uint32_t high, r;
     asm("cvt.pack.sat.u8.s32.b32 %0, %1, %2, %3;" : "=r"(high) : "r"(__float2int_rn(y.y)), "r"(__float2int_rn(y.x)), "r"(0));
     asm("cvt.pack.sat.u8.s32.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(__float2int_rn(x.y)), "r"(__float2int_rn(x.x)), "r"(high));
-    return r;
+  } else {
+    asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;" : "=r"(high) : "r"(__float2int_rn(y.y)), "r"(__float2int_rn(y.x)), "r"(0));
+    asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(__float2int_rn(x.y)), "r"(__float2int_rn(x.x)), "r"(high));
   }
-  const float2 magic = make_float2(12582912.0f, 12582912.0f);
-  x = add2(x, magic, one);
-  y = add2(y, magic, one);
-  return __byte_perm(__byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x0040), __byte_perm(__float_as_uint(y.x), __float_as_uint(y.y), 0x0040), 0x5410);
+  return r;
 }
 
 // Two results in 16 bits, with ReLU (NaN stays) in the conversion.
@@ -321,7 +323,7 @@ struct FloatOut {
   };
   template <int BN>
   static __device__ __forceinline__ void fetch(const Params& ep, const Product& p, const EpiContext& c, int row0, int n0) {
-    fetch_scales<BN>(ep.s, p, c, row0, n0);
+    fetch_scales<BN>(ep.s, p, c, row0, n0, true);
   }
   template <int BN>
   static __device__ __forceinline__ void begin(const Params&, const Product&, const EpiContext&, Block&) {}
@@ -397,12 +399,12 @@ struct QuantOut {
   };
   template <int BN>
   static __device__ __forceinline__ void fetch(const Params& ep, const Product& p, const EpiContext& c, int row0, int n0) {
-    fetch_scales<BN>(ep.s, p, c, row0, n0);
+    fetch_scales<BN>(ep.s, p, c, row0, n0, true);
   }
   template <int BN>
   static __device__ __forceinline__ void begin(const Params&, const Product&, const EpiContext& c, Block&) {
-    if (c.warp == 0 && c.lane == 0)
-      mbar_expect_tx(smem_u32(&c.tail->exchange[c.n_tile & 1u]), kCtas / 2 * Shape<BN>::kParts * kCtaRows * 4);
+    if (c.part == 0 && c.lane == 0)
+      mbar_expect_tx(smem_u32(&c.tail->exchange[c.n_tile & 1u][c.row >> 5]), kCtas / 2 * Shape<BN>::kParts * 32 * 4);
   }
   template <int BN, class Release>
   static __device__ __forceinline__ void drain(const Params& ep, const Product& p, const EpiContext& c, Block&, Release release) {
@@ -427,7 +429,7 @@ struct QuantOut {
     }
     const int mine = c.row + 8 * (c.lane & 3) + (c.lane >> 2);       // among the CTA's rows
     const uint32_t buf = c.n_tile & 1u, side = c.rank & 1u;
-    const uint32_t bar = smem_u32(&c.tail->exchange[buf]);
+    const uint32_t bar = smem_u32(&c.tail->exchange[buf][c.row >> 5]);       // of the warps with the same 32 rows (one for all 128: 64 us, not 60.4)
     const uint32_t at = smem_u32(&c.layer->row_max[buf][c.rank >> 1][c.part][mine]);
 #pragma unroll
     for (int i = 0; i < kCtas / 2; ++i) st_async_f32(map_to_cta(at, 2 * i + side), amax, map_to_cta(bar, 2 * i + side));
@@ -452,10 +454,10 @@ struct QuantOut {
       uint32_t w[4];                            // the lane's two columns of blocks 2 j and 2 j + 1
       if (ep.s.relu) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = quantized4<true>(v[2 * j][i], v[2 * j + 1][i], inverse, ep.s.one);
+        for (int j = 0; j < 4; ++j) w[j] = quantized4<true>(v[2 * j][i], v[2 * j + 1][i], inverse);
       } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = quantized4<false>(v[2 * j][i], v[2 * j + 1][i], inverse, ep.s.one);
+        for (int j = 0; j < 4; ++j) w[j] = quantized4<false>(v[2 * j][i], v[2 * j + 1][i], inverse);
       }
       store_fragment(smem_u32(staging), i, w, c.lane);
     }
