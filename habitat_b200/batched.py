@@ -360,9 +360,9 @@ class Int8MLPHandle:
     """A runtime predictor whose hidden layers are 8-bit: MLPHandle's predictions from rows quantised layer by layer
     (habitat_b200.dense), the weights with one scale per output feature.  fc1 and fc2 stay float32.
 
-    For large batches: predictors of eight hidden layers of 1,024 take 0.92 of bf16's time for 65,536 queries and 0.86 for
-    262,144, and the weights half the memory; the error is that of 8-bit rows, about 1 % of a layer's spread per layer.  A call
-    is one launch per layer, so batches of up to 16,384 queries are quicker in bf16 (211 us against 226).  Queries go through in pieces of `chunk`, whose rows are allocated through torch."""
+    For large batches: predictors of eight hidden layers of 1,024 take 0.77 of bf16's time for 65,536 queries and more,
+    and the weights half the memory; the error is that of 8-bit rows, about 1 % of a layer's spread per layer.  A call is one
+    launch per layer, so batches of up to 8,192 queries are quicker in bf16 (110 us against 139).  Queries go through in pieces of `chunk`, whose rows are allocated through torch."""
 
     chunk = 131072
 

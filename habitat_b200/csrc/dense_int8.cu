@@ -217,17 +217,10 @@ __device__ __forceinline__ void fetch_scales(const LayerScales& s, const Product
   copy_float(to + 128 + c.lane, s.row + (there ? row0 + c.lane : 0), there);
 }
 
-// Two products, two sums.  A packed sum of packed products is merged into a multiply-add, which rounds once instead of twice,
+// Two sums (mul2: two products).  A packed sum of packed products is merged into a multiply-add, which rounds once instead of twice,
 // whatever the instructions' rounding says; y * one + b, with a one that only the host knows, is the rounded sum and stays as it is.
 // (The epilogue is bound by its issue slots: with single sums and maxima quantised rows of 65,536 x 1024 x 1024 took 69 us,
 // 63 so.)
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 r;
-  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
 __device__ __forceinline__ float2 add2(float2 a, float2 b, float one) {
   float2 r;
   asm("{\n\t.reg .b64 x, y, z, d;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%6, %6};\n\tmov.b64 z, {%4, %5};\n\tfma.rn.f32x2 d, x, y, z;\n\t"
@@ -274,29 +267,6 @@ __device__ __forceinline__ float max3_abs(float a, float b, float c) {
   asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-
-// quantized() of four values, packed.  The conversion instruction and the packing one saturate, which with ReLU leaves 0 of what is
-// negative, by however much (6 instructions for four results, 9 with maxima and sums with 1.5 * 2^23).
-template <bool kRelu>
-__device__ __forceinline__ uint32_t quantized4(float2 a, float2 b, float inverse) {
-  const float2 scale = make_float2(inverse, inverse);
-  const float2 x = mul2(a, scale), y = mul2(b, scale);
-  uint32_t high, r;
-  if (kRelu) {
-    asm("cvt.pack.sat.u8.s32.b32 %0, %1, %2, %3;" : "=r"(high) : "r"(__float2int_rn(y.y)), "r"(__float2int_rn(y.x)), "r"(0));
-    asm("cvt.pack.sat.u8.s32.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(__float2int_rn(x.y)), "r"(__float2int_rn(x.x)), "r"(high));
-  } else {
-    asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;" : "=r"(high) : "r"(__float2int_rn(y.y)), "r"(__float2int_rn(y.x)), "r"(0));
-    asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(__float2int_rn(x.y)), "r"(__float2int_rn(x.x)), "r"(high));
-  }
-  return r;
-}
-
 // Two results in 16 bits, with ReLU (NaN stays) in the conversion.
 template <bool kRelu, bool kBf16>
 __device__ __forceinline__ uint32_t pack_result(float2 x) {

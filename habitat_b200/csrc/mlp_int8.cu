@@ -19,9 +19,9 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 
 // fc1 has at most 12 inputs: a thread keeps the weights of its four features in registers and walks over queries, eight between
 // barriers, while the next eight are loaded and normalised.  12 multiply-adds per result on the ordinary cores, in pairs, are
-// 11 us for 65,536 queries of 12 inputs, and the rows' 67 MB 10 us; 77 us measured.  What is left is issue: per result the maximum,
-// the product with the row's factor, the rounding and the packing next to twelve half multiply-adds, and the largest value of a
-// query has to cross all eight warps before its first byte can be written.
+// 11 us for 65,536 queries of 12 inputs, and the rows' 67 MB 10 us; 73 us measured.  What is left is what happens
+// around the barrier, at which the largest value of a query crosses all eight warps before its first byte can be written: four queries at
+// a time take 83 us, one CTA per SM 91, and three CTAs of fewer registers, four queries at a time, 87.
 __global__ void __launch_bounds__(kInputThreads, 2)
 mlp_input_kernel(const float* __restrict__ features, int n_op_feat, const uint8_t* __restrict__ device_row, const double* __restrict__ device_features,
                  int n_dev, const double* __restrict__ mu, const double* __restrict__ sigma, const float* __restrict__ w, const float* __restrict__ b,
@@ -90,9 +90,8 @@ mlp_input_kernel(const float* __restrict__ features, int n_op_feat, const uint8_
           y[k][1] = fma2(wr[1][c], vv, y[k][1]);
         }
       }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) y[k][i] = make_float2(relu_nan(y[k][i].x), relu_nan(y[k][i].y));
-      tops[k] = max_nan(max_nan(y[k][0].x, y[k][0].y), max_nan(y[k][1].x, y[k][1].y));
+      // (ReLU: in the maxima, which begin at 0, and in the conversion below)
+      tops[k] = max3(max3(0.0f, y[k][0].x, y[k][0].y), y[k][1].x, y[k][1].y);
     }
     // the warp's largest value of each query: halves of the queries over pairs of lanes, then what is left over all
 #pragma unroll
@@ -111,15 +110,15 @@ mlp_input_kernel(const float* __restrict__ features, int n_op_feat, const uint8_
     __syncthreads();
     // lane k mod 8 works out query k's scale for its warp
     const float4 lo = *reinterpret_cast<const float4*>(peak[buf][lane & 7]), hi = *reinterpret_cast<const float4*>(&peak[buf][lane & 7][4]);
-    const RowScale s = row_scale(max_nan(max_nan(max_nan(lo.x, lo.y), max_nan(lo.z, lo.w)), max_nan(max_nan(hi.x, hi.y), max_nan(hi.z, hi.w))));
+    const float amax = max_nan(max_nan(max_nan(lo.x, lo.y), max_nan(lo.z, lo.w)), max_nan(max_nan(hi.x, hi.y), max_nan(hi.z, hi.w)));
+    const RowScale s = row_scale(amax);
     if (tid < kInputQueries && q0 + tid < Q) scales[q0 + tid] = s.scale;
     const unsigned bad = __ballot_sync(0xFFFFFFFFu, s.bad);
 #pragma unroll
     for (int k = 0; k < kInputQueries; ++k) {
       const float inverse = __shfl_sync(0xFFFFFFFFu, s.inverse, k);
       if (q0 + k >= Q) break;
-      const uint32_t word = bad >> k & 1u ? 0 : low_bytes(quantized(y[k][0].x, inverse), quantized(y[k][0].y, inverse), quantized(y[k][1].x, inverse),
-                                                          quantized(y[k][1].y, inverse));
+      const uint32_t word = bad >> k & 1u ? 0 : quantized4<true>(y[k][0], y[k][1], inverse);
       int8_t* to = q + (q0 + k) * q_pitch + 4 * tid;
       if (4 * tid + 4 <= width) {
         *reinterpret_cast<uint32_t*>(to) = word;
