@@ -206,6 +206,24 @@ def test_int8_matmul_quantized_long_batches(m, n, k):
     assert np.array_equal(s.cpu().numpy(), want_s) and np.array_equal(q.cpu().numpy(), want_q)
 
 
+@pytest.mark.parametrize("m", [5, 100, 700])
+@pytest.mark.parametrize("relu", [False, True])
+def test_int8_matmul_far_below_zero(m, relu):
+    """Results that ReLU drops, by however much they are below zero, and zeros of either sign, bit for bit."""
+    q, s, w, ws, b = _layer(m, 300, 96, m)
+    b[::7], b[3::11] = np.float32(-1e30), np.float32(-3e7)
+    if relu:
+        b[5::13] = -np.inf
+    q[m // 2], b[1::9] = 0, np.float32(-0.0)
+    want = _product(q, s, w, ws, b, relu)
+    got_q, got_s = dense.int8_matmul_quantized(*_cuda(q, s, w, ws, b), relu=relu)
+    want_q, want_s = _quantized(want)
+    assert np.array_equal(got_s.cpu().numpy(), want_s) and np.array_equal(got_q.cpu().numpy(), want_q)
+    for dtype, bits in ((torch.float32, torch.int32), (torch.bfloat16, torch.int16), (torch.float16, torch.int16)):
+        got = dense.int8_matmul(*_cuda(q, s, w, ws, b), relu=relu, out_dtype=dtype)
+        assert torch.equal(got.cpu().view(bits), torch.from_numpy(want + np.float32(0) if relu else want).to(dtype).view(bits))
+
+
 def test_int8_matmul_of_nothing():
     q, s, w, ws, b = _cuda(*_layer(4, 6, 16, 1))
     assert dense.int8_matmul(q[:0], s[:0], w, ws, b).shape == (0, 6)
