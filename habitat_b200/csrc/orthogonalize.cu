@@ -42,14 +42,6 @@ struct Source {
   int32_t type, rows, cols;
 };
 
-}  // namespace
-}  // namespace dense
-
-#include "orthogonalize_small.cuh"
-
-namespace dense {
-namespace {
-
 // Eight elements from a 16-byte boundary on.
 __device__ __forceinline__ void load_eight(const void* base, int type, int64_t at, float (&x)[8]) {
   if (type == kF32) {
@@ -69,6 +61,14 @@ __device__ __forceinline__ void load_eight(const void* base, int type, int64_t a
     x[2 * i + 1] = f.y;
   }
 }
+
+}  // namespace
+}  // namespace dense
+
+#include "orthogonalize_small.cuh"
+
+namespace dense {
+namespace {
 
 // Sums of squares of G's elements, one per block.  `eights`: rows follow one another and are read in pieces of eight elements
 // (figures below).
@@ -824,12 +824,13 @@ extern "C" hb_status hb_orthogonalize(const void* update, int32_t type, int64_t 
   if (const SidePlan plan = side_plan(rows, cols, split != 0); plan.ctas) {
     SideParams p{};
     p.g = g;
-    p.out = Out{out, out_pitch, out_batch_stride, type, 0};
+    p.out = Out{out, out_pitch, out_batch_stride, type, row_alignment(out, out_pitch, batch > 1 ? out_batch_stride : 0, bytes_of(type))};
     p.s = static_cast<int32_t>(rows < cols ? rows : cols);
     p.l = static_cast<int32_t>(rows < cols ? cols : rows);
     p.R = plan.R;
     p.blocks = plan.blocks;
     p.flip = flip;
+    p.eights = !flip && row_alignment(update, pitch, batch > 1 ? batch_stride : 0, bytes_of(type)) == 16 ? 1 : 0;
     p.steps = steps;
     p.a = static_cast<float>(a);
     p.b = static_cast<float>(b);

@@ -17,7 +17,8 @@
 namespace dense {
 namespace {
 
-constexpr int kSideThreads = 256;
+constexpr int kSideThreads = 512;              // between two rounds of MMAs each warp has 16 columns in four (256 threads: 64 x 64 bfloat16 25 us, 19 so)
+constexpr int kSideParts = kSideThreads / 128; // of the columns
 constexpr int kSideRows = 128;                 // the longest shorter side
 constexpr int kSideSmem = 232448;              // all of an SM's, so that no two of these blocks share its tensor memory
 constexpr int kSideColumns = 64;               // per block of X
@@ -34,6 +35,7 @@ struct SideParams {
   Source g;
   Out out;
   int32_t s, l, R, blocks, flip, steps;   // blocks: of 64 columns, per CTA
+  int32_t eights;                         // G's rows start on 16-byte boundaries and are X's
   float a, b, c;
   double eps;
   int32_t* status;
@@ -181,16 +183,23 @@ __global__ void __launch_bounds__(kSideThreads, 1) small_side_kernel(const __gri
     return base + (c >> 6) * lay.block + block_at(r, c & 63);
   };
   double sum = 0.0;
+#pragma unroll 2
   for (int u = tid; u < units; u += kSideThreads) {
     int r, c;
     uint8_t* at = unit_at(u, r, c);
     const int64_t from = g0 + (p.flip ? static_cast<int64_t>(c0 + c) * p.g.ld + r : static_cast<int64_t>(r) * p.g.ld + c0 + c);
     const int64_t step = p.flip ? p.g.ld : 1;
     float v[8];
+    if (p.eights && c + 8 <= cols) {
+      load_eight(p.g.base, p.g.type, from, v);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? load_element(p.g.base, p.g.type, from + i * step) : 0.0f;
+      for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? load_element(p.g.base, p.g.type, from + i * step) : 0.0f;
+    }
+    double some[2] = {};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum += static_cast<double>(v[i]) * v[i];
+    for (int i = 0; i < 8; ++i) some[i & 1] = fma(static_cast<double>(v[i]), static_cast<double>(v[i]), some[i & 1]);
+    sum += some[0] + some[1];
     if (kSplit) {
       *reinterpret_cast<float4*>(at) = make_float4(v[0], v[1], v[2], v[3]);
       *reinterpret_cast<float4*>(at + x_low) = make_float4(v[4], v[5], v[6], v[7]);
@@ -287,7 +296,7 @@ __global__ void __launch_bounds__(kSideThreads, 1) small_side_kernel(const __gri
         scale *= factor;
       }
       if (rows_here) {
-        for (int j = part; j < R / 16; j += 2) {
+        for (int j = part; j < R / 16; j += kSideParts) {
           __syncwarp();
           float v[16];
           tc_ld16(lanes + j * 16, v);
@@ -297,7 +306,19 @@ __global__ void __launch_bounds__(kSideThreads, 1) small_side_kernel(const __gri
 #pragma unroll
             for (int i = 0; i < 16; ++i) v[i] += w[i];
           }
-          if (row < R) {
+          if (row < R && ctas == 1) {
+            // the share is A
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int c = j * 16 + 8 * h;
+              uint8_t* at = base + lay.operand + (c >> 6) * lay.block + block_at(row, c & 63);
+              float w[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) w[i] = v[8 * h + i] * scale;
+              *reinterpret_cast<uint4*>(at) = halves(w);
+              if (kSplit) *reinterpret_cast<uint4*>(at + op_low) = halves(w);
+            }
+          } else if (row < R) {
             float* at = reinterpret_cast<float*>(base + lay.share) + row * (R + 4) + j * 16;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -307,19 +328,23 @@ __global__ void __launch_bounds__(kSideThreads, 1) small_side_kernel(const __gri
       }
       tc_fence_before();
     }
-    __syncwarp();
-    cluster_sync_all();
     // ---- A: pieces of four columns, each added up by one thread of the cluster and handed to all CTAs ----
-    switch (ctas) {
-      case 1: add_shares<kSplit, 1>(sb + lay.share, sb + lay.operand, lay.block, op_low, R, rank, tid); break;
-      case 2: add_shares<kSplit, 2>(sb + lay.share, sb + lay.operand, lay.block, op_low, R, rank, tid); break;
-      case 4: add_shares<kSplit, 4>(sb + lay.share, sb + lay.operand, lay.block, op_low, R, rank, tid); break;
-      case 8: add_shares<kSplit, 8>(sb + lay.share, sb + lay.operand, lay.block, op_low, R, rank, tid); break;
-      default: add_shares<kSplit, 16>(sb + lay.share, sb + lay.operand, lay.block, op_low, R, rank, tid); break;
+    if (ctas > 1) {
+      __syncwarp();
+      cluster_sync_all();
+      switch (ctas) {
+        case 2: add_shares<kSplit, 2>(sb + lay.share, sb + lay.operand, lay.block, op_low, R, rank, tid); break;
+        case 4: add_shares<kSplit, 4>(sb + lay.share, sb + lay.operand, lay.block, op_low, R, rank, tid); break;
+        case 8: add_shares<kSplit, 8>(sb + lay.share, sb + lay.operand, lay.block, op_low, R, rank, tid); break;
+        default: add_shares<kSplit, 16>(sb + lay.share, sb + lay.operand, lay.block, op_low, R, rank, tid); break;
+      }
+      asm volatile("fence.proxy.async;" ::: "memory");
+      __syncwarp();
+      cluster_sync_all();
+    } else {
+      fence_proxy_async();
+      __syncthreads();
     }
-    asm volatile("fence.proxy.async;" ::: "memory");
-    __syncwarp();
-    cluster_sync_all();
     // ---- B = a I + b A + c A^2, in A's place ----
     asm volatile("fence.proxy.async;" ::: "memory");
     tc_fence_after();
@@ -335,7 +360,7 @@ __global__ void __launch_bounds__(kSideThreads, 1) small_side_kernel(const __gri
     __syncwarp();
     finished();
     if (rows_here) {
-      for (int j = part; j < R / 16; j += 2) {
+      for (int j = part; j < R / 16; j += kSideParts) {
         __syncwarp();
         float v[16];
         tc_ld16(lanes + j * 16, v);
@@ -394,7 +419,7 @@ __global__ void __launch_bounds__(kSideThreads, 1) small_side_kernel(const __gri
       __syncwarp();
       finished();
       if (rows_here) {
-        for (int j = part; j < (b1 - b0) * (kSideColumns / 16); j += 2) {
+        for (int j = part; j < (b1 - b0) * (kSideColumns / 16); j += kSideParts) {
           __syncwarp();
           float v[16];
           tc_ld16(lanes + j * 16, v);
@@ -415,6 +440,22 @@ __global__ void __launch_bounds__(kSideThreads, 1) small_side_kernel(const __gri
             }
           } else if (row < p.s) {
             const int64_t m0 = matrix * p.out.batch_stride;
+            if (p.out.vec == 16 && !p.flip && c + 16 <= cols) {
+              const int64_t to = m0 + static_cast<int64_t>(row) * p.out.ld + c0 + c;
+              if (p.out.type == kF32) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  reinterpret_cast<float4*>(static_cast<float*>(p.out.base) + to)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+              } else {
+                uint32_t w[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) w[i] = p.out.type == kBF16 ? pack_bf16(v[2 * i], v[2 * i + 1]) : pack_f16(v[2 * i], v[2 * i + 1]);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                  reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out.base) + to)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+              }
+              continue;
+            }
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               if (c + i >= cols) break;
