@@ -1,8 +1,8 @@
 // Newton-Schulz steps of matrices whose shorter side is at most 128, in one launch: a cluster per matrix keeps X in shared
 // memory, columns spread over its CTAs, for all steps.
 //
-// A step on tiles in memory is three launches of a few microseconds each whatever the size; here it is two barriers of
-// the cluster.  Per step each CTA multiplies its columns to a share of A = X X^T, the shares are added slice by slice through
+// A step on tiles in memory is three launches of a few microseconds each whatever the size; here it is two barriers and
+// one exchange within the cluster.  Per step each CTA multiplies its columns to a share of A = X X^T, the shares are added slice by slice through
 // distributed shared memory (in the order of the ranks) and the sums handed to every CTA, which works out A^2 and
 // B = a I + b A + c A^2 for itself and replaces its columns by B X.  X lies as blocks of 64 columns, R rows of 128 bytes with
 // the 128-byte swizzle: K-major for A (K = columns) and MN-major for B X (N = columns) with the same bytes.
@@ -17,14 +17,14 @@
 namespace dense {
 namespace {
 
-constexpr int kSideThreads = 512;              // between two rounds of MMAs each warp has 16 columns in four (256 threads: 64 x 64 bfloat16 25 us, 19 so)
+constexpr int kSideThreads = 512;              // a warp has every fourth 16 columns (every second with 256: 64 x 64 bfloat16 25 us, 19 so)
 constexpr int kSideParts = kSideThreads / 128; // of the columns
 constexpr int kSideRows = 128;                 // the longest shorter side
 constexpr int kSideSmem = 232448;              // all of an SM's, so that no two of these blocks share its tensor memory
 constexpr int kSideColumns = 64;               // per block of X
 
 struct SideTail {
-  uint64_t done;
+  uint64_t done, arrived;
   uint32_t tmem;
   int abort;
   double sums[16];
@@ -73,9 +73,6 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ void st_cluster_u2(uint32_t addr, uint32_t a, uint32_t b) {
-  asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(a), "r"(b) : "memory");
-}
 __device__ __forceinline__ void st_cluster_f64(uint32_t addr, double v) {
   asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory");
 }
@@ -106,13 +103,13 @@ __device__ __forceinline__ uint4 halves(float (&v)[8]) {
   return r;
 }
 
-// A from the shares of all CTAs (added in the order of the ranks), as operands in every CTA's shared memory.  All loads of a
+// This CTA's rows of A, from r0 on, from the shares of all CTAs (added in the order of the ranks), as operands.  All loads of a
 // piece are on their way at once: one after the other they took 9 us a step with eight CTAs and 128 rows.
 template <bool kSplit, int kCtas>
-__device__ __forceinline__ void add_shares(uint32_t share, uint32_t operand, int block, int low, int R, int rank, int tid) {
-  const int per_row = R / 4, pieces = R * per_row;
-  for (int u = rank * kSideThreads + tid; u < pieces; u += kCtas * kSideThreads) {
-    const int r = u / per_row, c = (u - r * per_row) * 4;
+__device__ __forceinline__ void add_shares(uint32_t share, uint32_t operand, int block, int low, int R, int r0, int rows, int tid) {
+  const int per_row = R / 4, pieces = rows * per_row;
+  for (int u = tid; u < pieces; u += kSideThreads) {
+    const int r = r0 + u / per_row, c = (u - u / per_row * per_row) * 4;
     const uint32_t at = share + (r * (R + 4) + c) * 4;
     float4 x[kCtas];
 #pragma unroll
@@ -125,14 +122,17 @@ __device__ __forceinline__ void add_shares(uint32_t share, uint32_t operand, int
     const uint32_t to = operand + (c >> 6) * block + block_at(r, c & 63);
     const uint32_t h0 = pack_f16(v.x, v.y), h1 = pack_f16(v.z, v.w);
     const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&h0)), f1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
-    const uint32_t l0 = pack_f16(v.x - f0.x, v.y - f0.y), l1 = pack_f16(v.z - f1.x, v.w - f1.y);
-#pragma unroll
-    for (int i = 0; i < kCtas; ++i) {
-      const uint32_t there = map_to_cta(to, static_cast<uint32_t>(i));
-      st_cluster_u2(there, h0, h1);
-      if (kSplit) st_cluster_u2(there + low, l0, l1);
-    }
+    asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to), "r"(h0), "r"(h1) : "memory");
+    if (kSplit)
+      asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to + low), "r"(pack_f16(v.x - f0.x, v.y - f0.y)), "r"(pack_f16(v.z - f1.x, v.w - f1.y))
+                   : "memory");
   }
+}
+// Bytes of this CTA's shared memory to the same place in another's, counted on a barrier there.
+__device__ __forceinline__ void push(uint32_t at, uint32_t bytes, uint32_t bar, uint32_t rank) {
+  asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(map_to_cta(at, rank)), "r"(at),
+               "r"(bytes), "r"(map_to_cta(bar, rank))
+               : "memory");
 }
 
 template <bool kSplit>
@@ -149,10 +149,14 @@ __global__ void __launch_bounds__(kSideThreads, 1) small_side_kernel(const __gri
   const int k_blocks = (R + 63) / 64, op_low = k_blocks * lay.block;
   volatile int* abort_flag = &tail->abort;
   const uint32_t bar = smem_u32(&tail->done);
+  const uint32_t arrived = smem_u32(&tail->arrived);
+  // the rows of A that this CTA adds up
+  const int slice0 = min(R, rank * ((R + ctas - 1) / ctas)), slice = min(R, slice0 + (R + ctas - 1) / ctas) - slice0;
   uint32_t phase = 0;
 
   if (tid == 0) {
     mbar_init(bar, 1);
+    mbar_init(arrived, 1);
     tail->abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -328,19 +332,27 @@ __global__ void __launch_bounds__(kSideThreads, 1) small_side_kernel(const __gri
       }
       tc_fence_before();
     }
-    // ---- A: pieces of four columns, each added up by one thread of the cluster and handed to all CTAs ----
+    // ---- A: a slice of rows added up by each CTA, whole rows copied to the others (written piece by piece into all shared
+    // memories: 64 x 1024 float32 43.6 us, 37.9 so; 100 x 4000 91.5 and 82.5) ----
     if (ctas > 1) {
+      if (tid == 0) mbar_expect_tx(arrived, static_cast<uint32_t>((kSplit ? 2 : 1) * k_blocks * (R - slice) * 128));
       __syncwarp();
       cluster_sync_all();
       switch (ctas) {
-        case 2: add_shares<kSplit, 2>(sb + lay.share, sb + lay.operand, lay.block, op_low, R, rank, tid); break;
-        case 4: add_shares<kSplit, 4>(sb + lay.share, sb + lay.operand, lay.block, op_low, R, rank, tid); break;
-        case 8: add_shares<kSplit, 8>(sb + lay.share, sb + lay.operand, lay.block, op_low, R, rank, tid); break;
-        default: add_shares<kSplit, 16>(sb + lay.share, sb + lay.operand, lay.block, op_low, R, rank, tid); break;
+        case 2: add_shares<kSplit, 2>(sb + lay.share, sb + lay.operand, lay.block, op_low, R, slice0, slice, tid); break;
+        case 4: add_shares<kSplit, 4>(sb + lay.share, sb + lay.operand, lay.block, op_low, R, slice0, slice, tid); break;
+        case 8: add_shares<kSplit, 8>(sb + lay.share, sb + lay.operand, lay.block, op_low, R, slice0, slice, tid); break;
+        default: add_shares<kSplit, 16>(sb + lay.share, sb + lay.operand, lay.block, op_low, R, slice0, slice, tid); break;
       }
-      asm volatile("fence.proxy.async;" ::: "memory");
+      fence_proxy_async();
+      __syncthreads();
+      if (tid < ctas && tid != rank && slice > 0)
+        for (int i = 0; i < (kSplit ? 2 : 1) * k_blocks; ++i)
+          push(sb + lay.operand + i * lay.block + slice0 * 128, static_cast<uint32_t>(slice * 128), arrived, static_cast<uint32_t>(tid));
       __syncwarp();
-      cluster_sync_all();
+      mbar_wait_cluster(arrived, static_cast<uint32_t>(step & 1), abort_flag, p.status, 0x552);
+      __syncwarp();
+      asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // "have all rows": B may take the place of what was copied
     } else {
       fence_proxy_async();
       __syncthreads();
@@ -359,6 +371,8 @@ __global__ void __launch_bounds__(kSideThreads, 1) small_side_kernel(const __gri
     }
     __syncwarp();
     finished();
+    __syncwarp();
+    if (ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     if (rows_here) {
       for (int j = part; j < R / 16; j += kSideParts) {
         __syncwarp();
