@@ -454,7 +454,7 @@ __global__ void __launch_bounds__(kSideThreads, 1) small_side_kernel(const __gri
             }
           } else if (row < p.s) {
             const int64_t m0 = matrix * p.out.batch_stride;
-            if (p.out.vec == 16 && !p.flip && c + 16 <= cols) {
+            if (p.out.vec >= (p.out.type == kF32 ? 16 : 4) && !p.flip && c + 16 <= cols) {
               const int64_t to = m0 + static_cast<int64_t>(row) * p.out.ld + c0 + c;
               if (p.out.type == kF32) {
 #pragma unroll
@@ -464,9 +464,17 @@ __global__ void __launch_bounds__(kSideThreads, 1) small_side_kernel(const __gri
                 uint32_t w[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) w[i] = p.out.type == kBF16 ? pack_bf16(v[2 * i], v[2 * i + 1]) : pack_f16(v[2 * i], v[2 * i + 1]);
+                uint16_t* at = static_cast<uint16_t*>(p.out.base) + to;
+                if (p.out.vec == 16) {
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-                  reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out.base) + to)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                  for (int i = 0; i < 2; ++i) reinterpret_cast<uint4*>(at)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                } else if (p.out.vec == 8) {
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) reinterpret_cast<uint2*>(at)[i] = make_uint2(w[2 * i], w[2 * i + 1]);
+                } else {
+#pragma unroll
+                  for (int i = 0; i < 8; ++i) reinterpret_cast<uint32_t*>(at)[i] = w[i];
+                }
               }
               continue;
             }

@@ -362,6 +362,16 @@ def test_orthogonalize_long_and_short_sides(shape, dtype):
     _check(update, dense.orthogonalize(update))
 
 
+# shorter sides kept on chip, with rows that start on 16, 8, 4 and 2 bytes
+@pytest.mark.parametrize("shape", [(64, 128), (100, 100), (90, 102), (40, 101), (2, 64, 100), (3, 50, 102), (128, 1004), (60, 2002), (128, 6000), (100, 100, 44)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_orthogonalize_on_chip(shape, dtype):
+    update = _update(shape, sum(shape), dtype)
+    got = dense.orthogonalize(update)
+    _check(update, got)
+    assert torch.equal(got, dense.orthogonalize(update))
+
+
 # single matrices, whose products are split along K over the pairs of a cluster or over launches, with slots that do not divide by the shares
 @pytest.mark.parametrize("shape", [(400, 400), (768, 768), (777, 1000), (1000, 777), (513, 1100), (900, 900), (300, 3000), (150, 8000), (2, 650, 700),
                                    (4, 510, 520), (1200, 1100)])
@@ -512,6 +522,34 @@ def test_two_streams_at_once_and_repeated_calls_agree():
         torch.cuda.synchronize()
         for g in got:
             assert all(torch.equal(x, y) for x, y in zip(g, want))
+
+
+def test_clusters_of_several_calls_and_graphs_at_once():
+    updates = [_update((777, 1000), 1, torch.float16), _update((100, 4000), 2, torch.float32), _update((3, 300, 320), 3, torch.float32),
+               _update((150, 5000), 4, torch.bfloat16)]
+    layer = _cuda(*_layer(1500, 700, 300, 5))
+    run = lambda: [dense.orthogonalize(u) for u in updates] + list(dense.int8_matmul_quantized(*layer, relu=True))
+    want = run()
+    torch.cuda.synchronize()
+    graphs, results = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            results.append(run())
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    for _ in range(5):
+        for st, g in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                g.replay()
+        eager = []
+        for st in streams[2:]:
+            with torch.cuda.stream(st):
+                eager.append(run())
+        torch.cuda.synchronize()
+        for got in results + eager:
+            assert all(torch.equal(x, y) for x, y in zip(got, want))
+    dense.check_status()
 
 
 def test_a_launch_that_gave_up_is_reported():
