@@ -577,3 +577,51 @@ def test_workspaces_that_are_too_small_are_refused():
     size = lib.hb_orthogonalize_workspace_bytes(1, 4, 6, 1)
     assert lib.hb_orthogonalize(p(u), 0, 1, 4, 6, 6, 24, 5, (ctypes.c_double * 3)(*COEFFICIENTS), 1e-7, 1, p(u), 6, 24, p(room), size - 1,
                                 _native.current_stream_ptr()) == _native.HB_ERR_INVALID_ARGUMENT
+
+
+@pytest.mark.parametrize("shape", [(1, 20, 30), (3, 12, 70), (1, 100, 90), (2, 64, 200), (1, 300, 200), (2, 260, 300), (1, 900, 1000)])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("more", [1, 6, 24])
+def test_orthogonalize_rows_and_matrices_apart(shape, dtype, more):
+    """Through the C interface: pitches and strides, of which nothing else is written to."""
+    lib = _native.load()
+    batch, rows, cols = shape
+    update = _update(shape, sum(shape), dtype)
+    kind = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype]
+    pitch, stride = cols + more, rows * (cols + more) + 3 * more
+    source, out = (torch.full((batch * stride,), float("nan"), dtype=dtype, device="cuda") for _ in range(2))
+    at = torch.arange(batch, device="cuda")[:, None, None] * stride + torch.arange(rows, device="cuda")[:, None] * pitch + torch.arange(cols, device="cuda")
+    source[at] = update
+    out.fill_(7.0)
+    split = 0 if dtype == torch.bfloat16 else 1
+    size = lib.hb_orthogonalize_workspace_bytes(batch, rows, cols, split)
+    room = torch.empty(size, dtype=torch.uint8, device="cuda")
+    p = lambda t: ctypes.c_void_p(t.data_ptr())
+    assert lib.hb_orthogonalize(p(source), kind, batch, rows, cols, pitch, stride, 5, (ctypes.c_double * 3)(*COEFFICIENTS), 1e-7, split, p(out), pitch, stride,
+                                p(room), size, None) == 0
+    torch.cuda.synchronize()
+    dense.check_status()
+    got = out[at]
+    _check(update, got)
+    out[at] = 7.0
+    assert bool((out == 7.0).all())
+
+
+@pytest.mark.parametrize("m, n, k", [(3, 50, 64), (100, 70, 40), (600, 300, 100)])
+@pytest.mark.parametrize("more", [1, 4, 8, 16])
+def test_int8_matmul_rows_apart(m, n, k, more):
+    lib = _native.load()
+    arrays = _layer(m, n, k, m)
+    q, s, w, ws, b = arrays
+    wide_q, wide_w = np.full((m, k + more), 99, np.int8), np.full((n, k + more), -99, np.int8)
+    wide_q[:, :k], wide_w[:, :k] = q, w
+    dq, ds, dw, dws, db = _cuda(wide_q, s, wide_w, ws, b)
+    want = torch.from_numpy(_product(*arrays, True))
+    p = lambda t: ctypes.c_void_p(t.data_ptr())
+    size = lib.hb_int8_workspace_bytes(p(dq), k + more, p(dw), k + more, m, n, k, 0)
+    room = torch.empty(max(size, 1), dtype=torch.uint8, device="cuda")
+    for kind, dtype in enumerate((torch.float32, torch.bfloat16, torch.float16)):
+        out = torch.full((m, n + more), 7.0, dtype=dtype, device="cuda")
+        assert lib.hb_int8_matmul(p(dq), k + more, p(ds), p(dw), k + more, p(dws), p(db), 1, m, n, k, p(out), kind, n + more, p(room), size, None) == 0
+        torch.cuda.synchronize()
+        assert torch.equal(out[:, :n].cpu(), want.to(dtype)) and bool((out[:, n:] == 7.0).all())
