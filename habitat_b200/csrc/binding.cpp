@@ -1636,22 +1636,22 @@ PyObject* int8_product(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// orthogonalize(update, steps, a, b, c, eps)
+// orthogonalize(update, steps, a, b, c, eps, split: products of high and low parts)
 PyObject* orthogonalize(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 6 || !THPVariable_Check(a[0])) Py_RETURN_NONE;
+  if (n != 7 || !THPVariable_Check(a[0])) Py_RETURN_NONE;
   const at::Tensor& u = THPVariable_Unpack(a[0]);
   const int type = element_type(u.scalar_type());
   if (!u.is_cuda() || type < 0 || u.dim() < 2 || !u.is_contiguous()) Py_RETURN_NONE;
   const long steps = PyLong_AsLong(a[1]);
   const double c[3] = {PyFloat_AsDouble(a[2]), PyFloat_AsDouble(a[3]), PyFloat_AsDouble(a[4])}, eps = PyFloat_AsDouble(a[5]);
-  if (PyErr_Occurred()) return nullptr;
+  const int split = PyObject_IsTrue(a[6]);
+  if (split < 0 || PyErr_Occurred()) return nullptr;
   const at::Device dev = u.device();
   const c10::cuda::CUDAGuard guard(dev);
   const int64_t rows = u.size(-2), cols = u.size(-1);
   int64_t batch = 1;
   for (int64_t i = 0; i < u.dim() - 2; ++i) batch *= u.size(i);
-  const int split = u.scalar_type() != at::kBFloat16;   // three products of high and low parts, for all but the 8-bit mantissas
   at::Tensor out = empty_beside(u.sizes(), u.scalar_type(), dev, true);
   const int64_t ws_bytes = api.orthogonalize_workspace_bytes(batch, rows, cols, split);
   c10::DataPtr ws;

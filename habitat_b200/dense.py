@@ -92,17 +92,21 @@ def int8_matmul_quantized(q, scales, weight, weight_scales, bias=None, relu=Fals
     return res
 
 
-def orthogonalize(update, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
+def orthogonalize(update, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7, operand_bits=22):
     """The update of a weight matrix, or of a batch of equal ones ([..., rows, cols], contiguous), with its singular values driven
     towards one by Newton-Schulz steps: X = update / (|update|_F + eps), then `steps` times X <- (a I + b A + c A^2) X with
     A = X X^T and (a, b, c) = coefficients.  Same shape and dtype as the update.
 
-    float32 and float16 updates are multiplied in three half-precision products each (22-bit operands), bfloat16 ones in one
-    (11-bit operands, float32 sums), so that the result's own rounding is the larger error; with a shorter side of up to 32 all
-    of them are multiplied in float64.  Elements of the result smaller than 2^-32 may be lost; an update with an infinity or a
-    NaN gives NaN everywhere.  Coefficients that would let singular values grow beyond 12 are refused."""
+    operand_bits: what X, A and B = a I + b A + c A^2 are held in between the products.  22: as pairs of half-precision numbers, three
+    products for each one of the formula, close to float32 for updates of all three types.  11: as single ones, a third of the
+    products; bfloat16 results are then off by 2.0e-3 instead of the 1.7e-3 that their own rounding is (2-norm).  The sums are
+    float32 either way.  With a shorter side of up to 32 everything is float64, whatever operand_bits.  Elements of the result
+    smaller than 2^-32 may be lost; an update with an infinity or a NaN gives NaN everywhere.  Coefficients that would let singular
+    values grow beyond 12 are refused."""
+    if operand_bits not in (11, 22):
+        raise ValueError("operand_bits must be 22 or 11, got %r" % (operand_bits,))
     a, b, c = coefficients
-    res = _native.binding().orthogonalize(update, steps, a, b, c, eps)
+    res = _native.binding().orthogonalize(update, steps, a, b, c, eps, operand_bits == 22)
     if res is None:
         if not isinstance(update, torch.Tensor) or not update.is_cuda:
             raise TypeError("update must be a CUDA tensor")
