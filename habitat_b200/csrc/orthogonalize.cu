@@ -721,6 +721,19 @@ GramPlan gram_plan(int64_t s, int64_t l, int widest) {
   return r;
 }
 
+// How many steps the recurrence of gram_side_kernel may take between two looks at X: what rounding leaves in A, 2^-53 of its norm by
+// up to 32 terms, grows by the largest slope of t (a + b t + c t^2)^2 (at 0: a^2) per step, and has to be below 2^-24 when the last
+// factor is made from it.  top: the largest eigenvalue of A.  The slope is of degree four: 64 points find its size.
+int gram_stretch(double a, double b, double c, double top, int steps) {
+  double slope = 1.0;
+  for (int i = 0; i <= 64; ++i) {
+    const double t = top * i / 64, y = a + t * (b + c * t);
+    slope = std::fmax(slope, std::fabs(y * (y + 2.0 * t * (b + 2.0 * c * t))));
+  }
+  const double most = slope > 1.0 ? 24.0 / std::log2(slope) : steps;
+  return most < steps ? 1 + static_cast<int>(most) : steps;
+}
+
 template <bool kSplit>
 hb_status launch_side(const SidePlan& plan, int64_t batch, const SideParams& p, bool* launched, cudaStream_t s) {
   static std::atomic<int> held[64];
@@ -755,8 +768,9 @@ extern "C" hb_status hb_orthogonalize(const void* update, int32_t type, int64_t 
   const double a = coefficients[0], b = coefficients[1], c = coefficients[2];
   // The largest singular value any step can leave, from at most one on: the maximum of |x (a + b x^2 + c x^4)| over what the
   // step before can leave; and the largest of B.  Stored operands are scaled by 2^8 and end at 65,504; A has the squares.
-  double most = 1.0, most_b = 0.0;
+  double most = 1.0, most_b = 0.0, widest = 1.0;      // widest: the largest before any step
   for (int i = 0; i < steps && most <= 12.0 && most_b <= 250.0; ++i) {
+    widest = std::fmax(widest, most);
     const double top = most * most;
     double next = 0.0;
     auto look = [&](double t) {          // t = x^2
@@ -803,13 +817,13 @@ extern "C" hb_status hb_orthogonalize(const void* update, int32_t type, int64_t 
     bool launched = false;
     auto gram = [&](auto size) -> hb_status {
       constexpr int S = decltype(size)::value;
-      static std::atomic<int> held[64], widest[64];
-      int most = 0;
-      if (const hb_status e = widest_cluster(gram_side_kernel<S>, kGramThreads, kSideSmem, held, widest, &most)) return e;
-      const GramPlan plan = gram_plan(s, l, most);
+      static std::atomic<int> held[64], held_width[64];
+      int ctas = 0;
+      if (const hb_status e = widest_cluster(gram_side_kernel<S>, kGramThreads, kSideSmem, held, held_width, &ctas)) return e;
+      const GramPlan plan = gram_plan(s, l, ctas);
       if (!plan.ctas || batch * plan.ctas > 0x7FFFFFFF) return HB_OK;
       const GramParams p{g, Out{out, out_pitch, out_batch_stride, type, 0}, static_cast<int32_t>(s), static_cast<int32_t>(l), plan.columns, flip, steps,
-                         a, b, c, eps};
+                         gram_stretch(a, b, c, widest * widest, steps), a, b, c, eps};
       HB_CUDA_TRY(launch_clusters(gram_side_kernel<S>, static_cast<int>(batch), plan.ctas, kGramThreads, plan.smem, st, p));
       launched = true;
       return HB_OK;

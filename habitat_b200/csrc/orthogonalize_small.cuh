@@ -513,6 +513,9 @@ __global__ void __launch_bounds__(kSideThreads, 1) small_side_kernel(const __gri
 // multiplied to A0 (whose trace is the squared norm), and once more, from shared memory, to P X0.  What that costs is precision:
 // A has the squares of the singular values, and P amplifies small ones by up to a^steps; so it is done in float64 on the
 // ordinary cores (64 multiply-adds per cycle and SM: 32^3 of them take 512 cycles), and rounded once at the end.
+// What rounding leaves in A where an eigenvalue should be zero grows by about a^2 per step, and may be negative, which X X^T cannot
+// be and a + b A + c A^2 does not bring back.  So after `stretch` steps, before that is 2^-24 (seven steps with the default
+// coefficients), X <- P X is formed and its A is what the next steps begin with.
 // 1024 x 12: 47 us as steps on the tensor cores (two cluster barriers and three dependent rounds of MMAs each).
 constexpr int kGramSide = 32;
 constexpr int kGramThreads = 256;
@@ -520,7 +523,7 @@ constexpr int kGramThreads = 256;
 struct GramParams {
   Source g;
   Out out;
-  int32_t s, l, columns, flip, steps;       // columns: of X, per CTA
+  int32_t s, l, columns, flip, steps, stretch;       // columns: of X, per CTA; stretch: steps between two looks at X
   double a, b, c, eps;
 };
 
@@ -574,137 +577,168 @@ __global__ void __launch_bounds__(kGramThreads) gram_side_kernel(const __grid_co
   }
   __syncthreads();
 
-  // ---- its share of A: 4 x 4 elements per thread and slice of the columns ----
   constexpr int kSide = S / 4, kTiles = kSide * kSide, kSlices = kGramThreads / kTiles;
-  {
-    double v[16] = {};
-    const int tile = tid % kTiles, slice = tid / kTiles;
-    if (slice < kSlices) {
-      const int i0 = tile / kSide * 4, j0 = tile % kSide * 4;
+  double scale = 0.0;                                  // what X is still to be multiplied by
+  const double* F = nullptr;                           // and its factor
+  for (int done = 0;;) {
+    // ---- its share of A: 4 x 4 elements per thread and slice of the columns ----
+    {
+      double v[16] = {};
+      const int tile = tid % kTiles, slice = tid / kTiles;
+      if (slice < kSlices) {
+        const int i0 = tile / kSide * 4, j0 = tile % kSide * 4;
 #pragma unroll 2
-      for (int c = slice; c < cols; c += kSlices) {
-        const double* xc = x + c * kX;
-        double xi[4], xj[4];
+        for (int c = slice; c < cols; c += kSlices) {
+          const double* xc = x + c * kX;
+          double xi[4], xj[4];
 #pragma unroll
-        for (int k = 0; k < 4; k += 2) {
-          const double2 a = *reinterpret_cast<const double2*>(xc + i0 + k), b = *reinterpret_cast<const double2*>(xc + j0 + k);
-          xi[k] = a.x; xi[k + 1] = a.y; xj[k] = b.x; xj[k + 1] = b.y;
+          for (int k = 0; k < 4; k += 2) {
+            const double2 a = *reinterpret_cast<const double2*>(xc + i0 + k), b = *reinterpret_cast<const double2*>(xc + j0 + k);
+            xi[k] = a.x; xi[k + 1] = a.y; xj[k] = b.x; xj[k + 1] = b.y;
+          }
+#pragma unroll
+          for (int k = 0; k < 16; ++k) v[k] = fma(xi[k >> 2], xj[k & 3], v[k]);
         }
-#pragma unroll
-        for (int k = 0; k < 16; ++k) v[k] = fma(xi[k >> 2], xj[k & 3], v[k]);
       }
-    }
 #pragma unroll
-    for (int k = 0; k < 16; ++k) part[k * kGramThreads + tid] = v[k];
-  }
-  __syncthreads();
-  for (int e = tid; e < kTiles * 16; e += kGramThreads) {
-    const int tile = e % kTiles, k = e / kTiles;
-    double sum = 0.0;
-#pragma unroll 8
-    for (int i = 0; i < kSlices; ++i) sum += part[k * kGramThreads + i * kTiles + tile];
-    share[(tile / kSide * 4 + (k >> 2)) * S + tile % kSide * 4 + (k & 3)] = sum;
-  }
-  cluster_sync_all();
-  // ---- A0: the shares of all CTAs, in the order of the ranks ----
-  for (int e = 2 * tid; e < S * S; e += 2 * kGramThreads) {
-    const uint32_t at = smem_u32(share + e);
-    double2 sum = make_double2(0.0, 0.0);
-#pragma unroll 8
-    for (int i = 0; i < ctas; ++i) {
-      const double2 y = ld_cluster_d2(map_to_cta(at, static_cast<uint32_t>(i)));
-      sum.x += y.x;
-      sum.y += y.y;
+      for (int k = 0; k < 16; ++k) part[k * kGramThreads + tid] = v[k];
     }
-    A[e / S * kPitch + e % S] = sum.x;
-    A[e / S * kPitch + e % S + 1] = sum.y;
-  }
-  __syncthreads();
-  double trace = lane < S ? A[lane * kPitch + lane] : 0.0;       // every warp for itself, in the same order
+    __syncthreads();
+    for (int e = tid; e < kTiles * 16; e += kGramThreads) {
+      const int tile = e % kTiles, k = e / kTiles;
+      double sum = 0.0;
+#pragma unroll 8
+      for (int i = 0; i < kSlices; ++i) sum += part[k * kGramThreads + i * kTiles + tile];
+      share[(tile / kSide * 4 + (k >> 2)) * S + tile % kSide * 4 + (k & 3)] = sum;
+    }
+    cluster_sync_all();
+    // ---- A: the shares of all CTAs, in the order of the ranks ----
+    for (int e = 2 * tid; e < S * S; e += 2 * kGramThreads) {
+      const uint32_t at = smem_u32(share + e);
+      double2 sum = make_double2(0.0, 0.0);
+#pragma unroll 8
+      for (int i = 0; i < ctas; ++i) {
+        const double2 y = ld_cluster_d2(map_to_cta(at, static_cast<uint32_t>(i)));
+        sum.x += y.x;
+        sum.y += y.y;
+      }
+      A[e / S * kPitch + e % S] = sum.x;
+      A[e / S * kPitch + e % S + 1] = sum.y;
+    }
+    __syncthreads();
+    if (done == 0) {
+      double trace = lane < S ? A[lane * kPitch + lane] : 0.0;       // every warp for itself, in the same order
 #pragma unroll
-  for (int d = 16; d; d >>= 1) trace += __shfl_xor_sync(0xFFFFFFFFu, trace, d);
-  const double norm = sqrt(trace);
-  const double scale = norm < static_cast<double>(INFINITY) ? 1.0 / (norm + p.eps) : __longlong_as_double(0x7FFFFFFFFFFFFFFFll);
+      for (int d = 16; d; d >>= 1) trace += __shfl_xor_sync(0xFFFFFFFFu, trace, d);
+      const double norm = sqrt(trace);
+      scale = norm < static_cast<double>(INFINITY) ? 1.0 / (norm + p.eps) : __longlong_as_double(0x7FFFFFFFFFFFFFFFll);
+    }
 
-  // ---- P = the product of the steps' factors: kRows x 2 elements of each matrix per thread ----
-  // All matrices are symmetric (polynomials of A), so rows of the left one are read as columns, two doubles at a time.  With
-  // four rows three loads feed eight multiply-adds, what shared memory and the float64 pipe do in the same time; up to 16 x 16
-  // latency counts and two rows keep more threads busy.
-  constexpr int kRows = S <= 16 ? 2 : 4, kHalf = S / 2, kBatch = S <= 16 ? 8 : 4;
-  const int r4 = tid / kHalf * kRows, c2 = tid % kHalf * 2;
-  const bool mine = r4 < S;
-  using Part = double[kRows][2];
-  auto product = [&](const double* u, const double* v, Part& o) {
+    // ---- P = the product of the steps' factors: kRows x 2 elements of each matrix per thread ----
+    // All matrices are symmetric (polynomials of A), so rows of the left one are read as columns, two doubles at a time.  With
+    // four rows three loads feed eight multiply-adds, what shared memory and the float64 pipe do in the same time; up to 16 x 16
+    // latency counts and two rows keep more threads busy.
+    constexpr int kRows = S <= 16 ? 2 : 4, kHalf = S / 2, kBatch = S <= 16 ? 8 : 4;
+    const int r4 = tid / kHalf * kRows, c2 = tid % kHalf * 2;
+    const bool mine = r4 < S;
+    using Part = double[kRows][2];
+    auto product = [&](const double* u, const double* v, Part& o) {
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) o[i][0] = o[i][1] = 0.0;
-    if (!mine) return;
+      for (int i = 0; i < kRows; ++i) o[i][0] = o[i][1] = 0.0;
+      if (!mine) return;
 #pragma unroll
-    for (int k0 = 0; k0 < S; k0 += kBatch) {
-      double2 us[kBatch][kRows / 2], w[kBatch];
+      for (int k0 = 0; k0 < S; k0 += kBatch) {
+        double2 us[kBatch][kRows / 2], w[kBatch];
 #pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
+        for (int k = 0; k < kBatch; ++k) {
 #pragma unroll
-        for (int i = 0; i < kRows / 2; ++i) us[k][i] = *reinterpret_cast<const double2*>(u + (k0 + k) * kPitch + r4 + 2 * i);
-        w[k] = *reinterpret_cast<const double2*>(v + (k0 + k) * kPitch + c2);
-      }
-#pragma unroll
-      for (int k = 0; k < kBatch; ++k)
-#pragma unroll
-        for (int i = 0; i < kRows / 2; ++i) {
-          o[2 * i][0] = fma(us[k][i].x, w[k].x, o[2 * i][0]);
-          o[2 * i][1] = fma(us[k][i].x, w[k].y, o[2 * i][1]);
-          o[2 * i + 1][0] = fma(us[k][i].y, w[k].x, o[2 * i + 1][0]);
-          o[2 * i + 1][1] = fma(us[k][i].y, w[k].y, o[2 * i + 1][1]);
+          for (int i = 0; i < kRows / 2; ++i) us[k][i] = *reinterpret_cast<const double2*>(u + (k0 + k) * kPitch + r4 + 2 * i);
+          w[k] = *reinterpret_cast<const double2*>(v + (k0 + k) * kPitch + c2);
         }
-    }
-  };
-  auto put = [&](double* to, const Part& o) {
-    if (!mine) return;
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) *reinterpret_cast<double2*>(to + (r4 + i) * kPitch + c2) = make_double2(o[i][0], o[i][1]);
-  };
-  auto at = [&](int i, int j) { return (r4 + i) * kPitch + c2 + j; };
-  __syncthreads();
-  if (mine) {
+        for (int k = 0; k < kBatch; ++k)
 #pragma unroll
-    for (int i = 0; i < kRows; ++i)
+          for (int i = 0; i < kRows / 2; ++i) {
+            o[2 * i][0] = fma(us[k][i].x, w[k].x, o[2 * i][0]);
+            o[2 * i][1] = fma(us[k][i].x, w[k].y, o[2 * i][1]);
+            o[2 * i + 1][0] = fma(us[k][i].y, w[k].x, o[2 * i + 1][0]);
+            o[2 * i + 1][1] = fma(us[k][i].y, w[k].y, o[2 * i + 1][1]);
+          }
+      }
+    };
+    auto put = [&](double* to, const Part& o) {
+      if (!mine) return;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) A[at(i, j)] *= scale * scale;
-  }
-  __syncthreads();
-  int now = 0;
-  for (int step = 0; step < p.steps; ++step) {
-    const bool last = step == p.steps - 1;
-    Part o;
-    product(A, A, o);
+      for (int i = 0; i < kRows; ++i) *reinterpret_cast<double2*>(to + (r4 + i) * kPitch + c2) = make_double2(o[i][0], o[i][1]);
+    };
+    auto at = [&](int i, int j) { return (r4 + i) * kPitch + c2 + j; };
+    __syncthreads();
     if (mine) {
 #pragma unroll
       for (int i = 0; i < kRows; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) o[i][j] = fma(p.c, o[i][j], fma(p.b, A[at(i, j)], r4 + i == c2 + j ? p.a : 0.0));
-    }
-    put(B, o);
-    if (step == 0) put(P, o);
-    __syncthreads();
-    if (step > 0) {
-      product(B, P + now, o);
-      now = kGramMatrix - now;
-      put(P + now, o);
-    }
-    if (!last) {
-      product(B, A, o);
-      put(T, o);
+        for (int j = 0; j < 2; ++j) A[at(i, j)] *= scale * scale;
     }
     __syncthreads();
-    if (!last) {
-      product(T, B, o);
-      put(A, o);
+    int now = 0;
+    const int steps = min(p.stretch, p.steps - done);
+    for (int step = 0; step < steps; ++step) {
+      const bool last = step == steps - 1;
+      Part o;
+      product(A, A, o);
+      if (mine) {
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) o[i][j] = fma(p.c, o[i][j], fma(p.b, A[at(i, j)], r4 + i == c2 + j ? p.a : 0.0));
+      }
+      put(B, o);
+      if (step == 0) put(P, o);
       __syncthreads();
+      if (step > 0) {
+        product(B, P + now, o);
+        now = kGramMatrix - now;
+        put(P + now, o);
+      }
+      if (!last) {
+        product(B, A, o);
+        put(T, o);
+      }
+      __syncthreads();
+      if (!last) {
+        product(T, B, o);
+        put(A, o);
+        __syncthreads();
+      }
     }
-  }
-  const double* F = P + now;
+    F = P + now;
+    done += steps;
+    if (done >= p.steps) break;
 
-  // ---- X = P X0: some rows of one or two columns per lane, lanes over the columns ----
+    // ---- X <- P X, a column per thread ----
+    cluster_sync_all();       // all have read the shares
+    for (int c = tid; c < cols; c += kGramThreads) {
+      double* xc = x + c * kX;
+      double2 v[S / 2];
+#pragma unroll
+      for (int k = 0; k < S / 2; ++k) v[k] = *reinterpret_cast<const double2*>(xc + 2 * k);
+#pragma unroll 1
+      for (int r = 0; r < S; r += 2) {
+        double2 sum = make_double2(0.0, 0.0);
+#pragma unroll
+        for (int k = 0; k < S; ++k) {
+          const double2 f = *reinterpret_cast<const double2*>(F + k * kPitch + r);
+          sum.x = fma(f.x, k & 1 ? v[k >> 1].y : v[k >> 1].x, sum.x);
+          sum.y = fma(f.y, k & 1 ? v[k >> 1].y : v[k >> 1].x, sum.y);
+        }
+        *reinterpret_cast<double2*>(xc + r) = make_double2(sum.x * scale, sum.y * scale);
+      }
+    }
+    scale = 1.0;
+    __syncthreads();
+  }
+
+  // ---- the result, P X: some rows of one or two columns per lane, lanes over the columns ----
   const int64_t o0 = matrix * p.out.batch_stride;
   auto store = [&](int r, int c, double v) {
     const int64_t to = o0 + (p.flip ? static_cast<int64_t>(c0 + c) * p.out.ld + r : static_cast<int64_t>(r) * p.out.ld + c0 + c);

@@ -44,9 +44,9 @@ def steps_of(g, steps=5, coefficients=COEFFICIENTS, eps=1e-7, bits=None):
 def inner_error(g, want, operand_bits, **kwargs):
     """Relative to the result (2-norm over all matrices), see above.  operand_bits: 22, 11, or 64 for float64 matrices."""
     if operand_bits == 64:
-        # what is off grows by at most the largest slope of x (a + b x^2 + c x^4) in each step
+        # what is off grows by at most the largest slope of x (a + b x^2 + c x^4) in each step (up to 1.21, which no step here exceeds)
         a, b, c = kwargs.get("coefficients", COEFFICIENTS)
-        t = torch.linspace(0, 1.3, 1001, dtype=torch.float64)
+        t = torch.linspace(0, 1.21, 1001, dtype=torch.float64)
         slope = float((a + 3 * b * t ** 2 + 5 * c * t ** 4).abs().max())
         return 2.0 ** -52 * 32 * max(slope, 1.0) ** kwargs.get("steps", 5)
     off = steps_of(g, bits={22: 20, 11: 11}[operand_bits], **kwargs) - want

@@ -39,3 +39,54 @@ def test_operand_bits_refused():
     for bad in (0, 16, None, "22"):
         with pytest.raises(ValueError, match="operand_bits"):
             dense.orthogonalize(torch.ones((40, 50), device="cuda"), operand_bits=bad)
+
+
+# rows and columns that depend on each other, on each way an update can take
+@pytest.mark.parametrize("shape, rank", [((12, 1024), 4), ((1024, 12), 4), ((32, 600), 9), ((20, 30), 7), ((2, 8, 50), 1), ((64, 500), 20), ((100, 100), 30), ((300, 260), 90)])
+@pytest.mark.parametrize("steps", [5, 15, 30])
+def test_dependent_rows(shape, rank, steps):
+    """Where singular values are zero the formula leaves zeros, and arithmetic of finitely many bits what rounding makes of them, at
+    most the coefficients' largest value (1.21) once it has grown; the others end in their band (0.67 to 1.21)."""
+    update = ns.update(shape, steps, rank=rank).cuda()
+    got = dense.orthogonalize(update, steps=steps)
+    dense.check_status()
+    if steps == 5:
+        ns.check(got, update, 64 if min(shape[-2:]) <= 32 else 22)
+    assert bool(torch.isfinite(got).all())
+    assert float(torch.linalg.svdvals(got.double()).max()) < 1.25
+    u, s, vt = torch.linalg.svd(update.double(), full_matrices=False)
+    inside = torch.linalg.svdvals(u[..., :rank].mT @ got.double() @ vt[..., :rank, :].mT)
+    if steps > 5:
+        assert 0.6 < float(inside.min()) and float(inside.max()) < 1.25
+
+
+@pytest.mark.parametrize("shape, rank", [((12, 1024), 4), ((400, 25), 6), ((64, 500), 20), ((200, 300), 50)])
+def test_dependent_rows_and_steps_that_converge(shape, rank):
+    """(3 x - x^3) / 2 goes to one and stays: U V^T of the update's directions, and at most one elsewhere.  What a step's operands
+    (pairs: 2^-22 each, X and B) are off by is left of the last steps', towards one with the slope 0; between equal singular values nothing
+    pulls back, so in those directions steps add up: 60 of them, in squares, with sums of 2^-22 as well."""
+    update = ns.update(shape, 3, rank=rank).cuda()
+    got = dense.orthogonalize(update, steps=60, coefficients=(1.5, -0.5, 0.0)).double()
+    assert float(torch.linalg.svdvals(got).max()) < 1.0 + 1e-5
+    u, s, vt = torch.linalg.svd(update.double(), full_matrices=False)
+    u, vt = u[..., :rank], vt[..., :rank, :]
+    inside = u.mT @ got @ vt.mT
+    eye = torch.eye(rank, dtype=torch.float64, device="cuda")
+    assert float((inside - eye).norm() / rank ** 0.5) < 60 ** 0.5 * 3 * 2.0 ** -22 * 4
+
+
+@pytest.mark.parametrize("shape", [(12, 1024), (31, 31), (700, 20), (3, 24, 100)])
+@pytest.mark.parametrize("steps", [1, 2, 6, 7, 8, 9, 14, 15, 16])
+def test_steps_of_float64_matrices(shape, steps):
+    update = ns.update(shape, steps).cuda()
+    ns.check(dense.orthogonalize(update, steps=steps), update, 64, steps=steps)
+
+
+@pytest.mark.parametrize("coefficients", [(1.5, -0.5, 0.0), (1.875, -1.25, 0.375), (2.0, -1.5, 0.5), (1.0, 0.0, 0.0), (0.5, 0.25, 0.0)])
+@pytest.mark.parametrize("steps", [3, 40, 100])
+def test_coefficients_of_float64_matrices(coefficients, steps):
+    update = ns.update((16, 200), 5).cuda()
+    got = dense.orthogonalize(update, steps=steps, coefficients=coefficients)
+    want = ns.steps_of(update, steps, coefficients)
+    # slopes of at most one in the end: what is off in the first steps (a^steps of 2^-52, until values are near one) is all there is
+    assert float((got.double() - want).norm()) <= float((want.float().double() - want).norm()) * 1.01 + 1e-9 * float(want.norm())
