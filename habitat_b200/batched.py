@@ -362,7 +362,11 @@ class Int8MLPHandle:
 
     For large batches: predictors of eight hidden layers of 1,024 take 0.77 of bf16's time for 65,536 queries and more,
     and the weights half the memory; the error is that of 8-bit rows, about 1 % of a layer's spread per layer.  A call is one
-    launch per layer, so batches of up to 8,192 queries are quicker in bf16 (110 us against 139).  Queries go through in pieces of `chunk`, whose rows are allocated through torch."""
+    launch per layer, so batches of up to 8,192 queries are quicker in bf16 (110 us against 139).  Queries go through in pieces of `chunk`, whose rows are allocated through torch.
+
+    The pack lies in torch's memory, which goes back when the handle is dropped.  It is not used again before the
+    predictions that any stream has queued by then have ended; graphs that hold predictions are to be replayed only while the handle is kept,
+    as with MLPHandle, and dropping it waits for replays under way."""
 
     chunk = 131072
 
@@ -397,7 +401,28 @@ class Int8MLPHandle:
         biases = up(hidden_b, np.float32, (layers, width), "hidden bias")
         self._layers = [dense.quantize_rows(torch.from_numpy(np.ascontiguousarray(hidden_w[i])).to(self.device)) + (biases[i],)
                         for i in range(layers)]
-        torch.cuda.current_stream(self.device).synchronize()      # the pack is there for every stream
+        self._pack = [*self._fc1, *self._fc2, self._mu, self._sigma, self._devices, biases]
+        for weight, scales, _ in self._layers:
+            self._pack += [weight, scales]
+        stream = torch.cuda.current_stream(self.device)
+        self._streams, self._captured = {stream.cuda_stream}, False       # that the pack is known to be used on; in a graph
+        stream.synchronize()                                      # the pack is there for every stream
+
+    def _used_on(self, stream):
+        """Tells the allocator that the pack is used on a stream, which its memory then waits for when it is given back."""
+        if torch.cuda.is_current_stream_capturing():
+            self._captured = True               # replays may be on any stream: __del__ waits for them
+        elif stream.cuda_stream not in self._streams:
+            for t in self._pack:
+                t.record_stream(stream)
+            self._streams.add(stream.cuda_stream)
+
+    def __del__(self):
+        try:
+            if self._captured:
+                torch.cuda.synchronize(self.device)
+        except Exception:
+            pass
 
     def predict(self, op_features, device_row, out=None):
         """op_features [Q, F] float32 CUDA, device_row [Q] uint8 CUDA -> [Q] float32."""
@@ -422,6 +447,7 @@ class Int8MLPHandle:
         flat = out.view(-1)
         pitch = (self.width + 15) // 16 * 16
         with torch.cuda.device(self.device):
+            self._used_on(torch.cuda.current_stream())
             stream = _native.current_stream_ptr()
             for at in range(0, n, self.chunk):
                 m = min(self.chunk, n - at)

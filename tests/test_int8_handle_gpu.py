@@ -1,0 +1,72 @@
+"""What an 8-bit predictor owes its caller beyond the numbers: its memory, its errors, its weights' updates."""
+import numpy as np
+import pytest
+import torch
+
+from habitat_b200 import _native, batched, dense, workloads
+from habitat_b200.analysis.mlp.mlp import RuntimePredictor, state_to_arrays
+
+pytestmark = pytest.mark.gpu
+
+
+def _handle(width=256, layers=3, Q=600, op="linear", seed=1):
+    torch.manual_seed(seed)
+    w = state_to_arrays(RuntimePredictor(op, layers, width).model)
+    feats, dev = workloads.make_queries(op, Q, seed=seed)
+    mu, sigma = workloads.batch_mu_sigma(feats, dev)
+    h = batched.Int8MLPHandle(feats.shape[1], mu=mu, sigma=sigma, device_features=workloads.BENCH_DEVICE_FEATURES, **w)
+    return h, torch.from_numpy(feats).cuda(), torch.from_numpy(dev).cuda()
+
+
+def _overwrite():
+    """Takes what the allocator has free on the current stream in blocks of every size up to 4 MB, and fills it."""
+    held = []
+    for size in (512, 1024, 2048, 4096, 16384, 65536, 262144, 1048576, 4194304):
+        held += [torch.full((size,), 85, dtype=torch.uint8, device="cuda") for _ in range(40)]
+    return held
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_weights_stay_until_queued_predictions_have_ended(captured):
+    """A prediction waits on a stream of its own while the handle is dropped and its memory asked for again."""
+    h, f, d = _handle()
+    want = h.predict(f, d)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = h.predict(f, d)
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)          # some 0.1 s
+        if captured:
+            graph.replay()
+        else:
+            got = h.predict(f, d)
+    del h
+    held = _overwrite()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    del held
+
+
+def test_retrained_under_queued_predictions():
+    """The same through the predictor: an update drops the pack and the next prediction uploads another."""
+    torch.manual_seed(2)
+    pred = RuntimePredictor("linear", 2, 128, precision="int8")
+    pred.model.cuda()
+    pred.mu, pred.sigma = np.zeros(8), np.full(8, 1e4)
+    feats, dev = (torch.from_numpy(a).cuda() for a in workloads.make_queries("linear", 300, seed=4))
+    want = pred.predict_batch(feats, dev).clone()
+    pred.model(torch.randn(64, 8, device="cuda")).square().mean().backward()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)
+        got = pred.predict_batch(feats, dev)
+    pred.update_hidden(0.5)
+    new = pred.predict_batch(feats, dev)
+    held = _overwrite()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and not torch.equal(new, want)
+    del held
