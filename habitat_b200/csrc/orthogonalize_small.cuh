@@ -172,8 +172,8 @@ __global__ void __launch_bounds__(kSideThreads, 1) small_side_kernel(const __gri
   const int64_t g0 = matrix * p.g.batch_stride;
   const int c0 = rank * nb * kSideColumns;                              // this CTA's columns of X
   const int cols = min(max(p.l - c0, 0), nb * kSideColumns);
-  // Eight columns of a row per thread: kept as they are in the 32 bytes that their high and low parts will take (16-bit
-  // updates without low parts: in 16 bytes, unrounded as they have 8 bits).
+  // Eight columns of a row per thread: kept as they are in the 32 bytes that their high and low parts will take; without low parts
+  // there are 16, which take 16-bit updates, and float32 ones are read again.
   const int per_row = (cols + 7) / 8, units = p.s * per_row;
   auto unit_at = [&](int u, int& r, int& c) {
     if (p.flip) {
@@ -186,20 +186,23 @@ __global__ void __launch_bounds__(kSideThreads, 1) small_side_kernel(const __gri
     c *= 8;
     return base + (c >> 6) * lay.block + block_at(r, c & 63);
   };
-  double sum = 0.0;
-#pragma unroll 2
-  for (int u = tid; u < units; u += kSideThreads) {
-    int r, c;
-    uint8_t* at = unit_at(u, r, c);
+  auto load_unit = [&](int r, int c, float (&v)[8]) {
     const int64_t from = g0 + (p.flip ? static_cast<int64_t>(c0 + c) * p.g.ld + r : static_cast<int64_t>(r) * p.g.ld + c0 + c);
     const int64_t step = p.flip ? p.g.ld : 1;
-    float v[8];
     if (p.eights && c + 8 <= cols) {
       load_eight(p.g.base, p.g.type, from, v);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? load_element(p.g.base, p.g.type, from + i * step) : 0.0f;
     }
+  };
+  double sum = 0.0;
+#pragma unroll 2
+  for (int u = tid; u < units; u += kSideThreads) {
+    int r, c;
+    uint8_t* at = unit_at(u, r, c);
+    float v[8];
+    load_unit(r, c, v);
     double some[2] = {};
 #pragma unroll
     for (int i = 0; i < 8; ++i) some[i & 1] = fma(static_cast<double>(v[i]), static_cast<double>(v[i]), some[i & 1]);
@@ -207,8 +210,10 @@ __global__ void __launch_bounds__(kSideThreads, 1) small_side_kernel(const __gri
     if (kSplit) {
       *reinterpret_cast<float4*>(at) = make_float4(v[0], v[1], v[2], v[3]);
       *reinterpret_cast<float4*>(at + x_low) = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
+    } else if (p.g.type == kBF16) {
       *reinterpret_cast<uint4*>(at) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+    } else if (p.g.type == kF16) {
+      *reinterpret_cast<uint4*>(at) = make_uint4(pack_f16(v[0], v[1]), pack_f16(v[2], v[3]), pack_f16(v[4], v[5]), pack_f16(v[6], v[7]));
     }
   }
 #pragma unroll
@@ -238,11 +243,18 @@ __global__ void __launch_bounds__(kSideThreads, 1) small_side_kernel(const __gri
     if (kSplit) {
       const float4 x = *reinterpret_cast<const float4*>(at), y = *reinterpret_cast<const float4*>(at + x_low);
       v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
+    } else if (p.g.type == kF32) {
+      load_unit(r, c, v);
     } else {
       const uint4 x = *reinterpret_cast<const uint4*>(at);
       const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(i & 1 ? xs[i >> 1] & 0xFFFF0000u : xs[i >> 1] << 16);
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = p.g.type == kBF16 ? make_float2(__uint_as_float(xs[i] << 16), __uint_as_float(xs[i] & 0xFFFF0000u))
+                                           : __half22float2(*reinterpret_cast<const __half2*>(&xs[i]));
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+      }
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] *= power;

@@ -90,3 +90,32 @@ def test_coefficients_of_float64_matrices(coefficients, steps):
     want = ns.steps_of(update, steps, coefficients)
     # slopes of at most one in the end: what is off in the first steps (a^steps of 2^-52, until values are near one) is all there is
     assert float((got.double() - want).norm()) <= float((want.float().double() - want).norm()) * 1.01 + 1e-9 * float(want.norm())
+
+
+@pytest.mark.parametrize("shape", [(33, 40), (64, 64), (3, 70, 50), (100, 90), (128, 1000), (2000, 120), (300, 200)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_single_parts_of_wider_types(shape, dtype):
+    """11 bits of what a float32 or float16 update has, not bfloat16's 8."""
+    update = ns.update(shape, sum(shape), dtype).cuda()
+    ns.check(dense.orthogonalize(update, operand_bits=11), update, 11)
+
+
+def test_single_parts_of_the_largest_numbers():
+    update = ns.update((60, 200), 6).double()
+    update = (update * (0.99999 * torch.finfo(torch.float32).max / update.abs().max())).float().cuda()    # beyond bfloat16's largest when rounded to it
+    ns.check(dense.orthogonalize(update, operand_bits=11), update, 11)
+
+
+@pytest.mark.parametrize("rows, cols", [(64, 200), (100, 100), (300, 260)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_single_parts_through_the_c_interface(rows, cols, dtype):
+    lib = _native.load()
+    update = ns.update((rows, cols), rows, dtype).cuda()
+    out = torch.empty_like(update)
+    size = lib.hb_orthogonalize_workspace_bytes(1, rows, cols, 0)
+    room = torch.empty(size, dtype=torch.uint8, device="cuda")
+    p = lambda t: ctypes.c_void_p(t.data_ptr())
+    _native.check(lib.hb_orthogonalize(p(update), DTYPES.index(dtype), 1, rows, cols, cols, rows * cols, 5, (ctypes.c_double * 3)(*ns.COEFFICIENTS), 1e-7, 0, p(out),
+                                       cols, rows * cols, p(room), size, _native.current_stream_ptr()))
+    ns.check(out, update, 11)
+    assert torch.equal(out, dense.orthogonalize(update, operand_bits=11))
