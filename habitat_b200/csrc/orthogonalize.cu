@@ -672,7 +672,6 @@ SidePlan side_plan(int64_t rows, int64_t cols, bool split) {
   for (const int ctas : {1, 2, 4, 8, 16}) {
     const int blocks = static_cast<int>((n + ctas - 1) / ctas);
     if (side_layout(r.R, blocks, split).total + 1024 > kSideSmem || (blocks > kSideBlocks && ctas < 16)) continue;
-    if (split && (blocks + 1) / 2 * r.R > 512) continue;      // accumulators of the share of A
     r.ctas = ctas;
     r.blocks = blocks;
     break;

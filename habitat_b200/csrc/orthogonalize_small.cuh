@@ -283,28 +283,58 @@ __global__ void __launch_bounds__(kSideThreads, 1) small_side_kernel(const __gri
   const int quad = warp & 3, part = warp >> 2, row = quad * 32 + lane;
   const bool rows_here = quad * 32 < R;                                    // warps beyond have no rows of D
   const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16);
-  // sums of two blocks' products at most per accumulator (see kGrouped); without low parts one takes all
-  const int groups = kSplit ? (nb + 1) / 2 : 1, per_group = kSplit ? 2 : nb;
+  // With low parts an accumulator takes 32 of K, small products first, and the accumulators are added here, rounded to nearest: the
+  // tensor core cuts what does not fit its sums (see gemm_kernel).  128 x 1024 float32 updates, results off the 64-bit ones (float32
+  // operations 1.5e-6) and time: 4.4e-6 and 68 us with 128 of K in each and all of A A and B X in one, 2.7e-6 and 71 with 64, 1.8e-6 and 75 so.
+  // Without low parts one takes all.
+  constexpr int kGroupSteps = kSplit ? 2 : 1 << 20;                        // of 16 of K
+  const int k_steps = R / 16, groups = kSplit ? (k_steps + kGroupSteps - 1) / kGroupSteps : 1;       // of A A and B X: at most 4 of 128 columns
+  const int round_steps = kSplit ? 512 / R * kGroupSteps : nb * 4;         // of X X^T, as many as there are accumulators for
+  const int round_blocks = 8 / groups;                                     // of B X
 
   for (int step = 0; step < p.steps; ++step) {
     const bool first = step == 0, last = step == p.steps - 1;
     // ---- this CTA's share of A ----
-    if (warp == 0 && elect_one()) {
-      for (int gr = 0; gr < groups; ++gr) {
-        uint32_t more = 0;
-        // the small products first: what an addition cuts off goes by the sum's size
-        for (int seg = kSplit ? 0 : 2; seg < 3; ++seg)
-          for (int b = gr * per_group; b < min(nb, (gr + 1) * per_group); ++b) {
-            const int at = b * lay.block;
-            for (int k = 0; k < 4; ++k, more = 1)
-              mma_one(tmem + gr * R, desc(desc_k, at + (seg == 1 ? x_low : 0) + 32 * k), desc(desc_k, at + (seg == 0 ? x_low : 0) + 32 * k),
-                      idesc_sym, more);
-          }
+    float shares[kSideRows / 16 / kSideParts][16];                         // 16 columns of chunks part, part + kSideParts, ...
+    for (int k0 = 0; k0 < nb * 4; k0 += round_steps) {
+      const int k1 = min(nb * 4, k0 + round_steps);
+      if (warp == 0 && elect_one()) {
+        for (int from = k0, gr = 0; from < k1; ++gr) {
+          const int to = kSplit ? min(k1, from + kGroupSteps) : k1;
+          uint32_t more = 0;
+          // the small products first: what an addition cuts off goes by the sum's size
+          for (int seg = kSplit ? 0 : 2; seg < 3; ++seg)
+            for (int k = from; k < to; ++k, more = 1) {
+              const int at = (k >> 2) * lay.block + 32 * (k & 3);
+              mma_one(tmem + gr * R, desc(desc_k, at + (seg == 1 ? x_low : 0)), desc(desc_k, at + (seg == 0 ? x_low : 0)), idesc_sym, more);
+            }
+          from = to;
+        }
+        commit_one(bar);
       }
-      commit_one(bar);
+      __syncwarp();
+      finished();
+      if (rows_here) {
+#pragma unroll
+        for (int i = 0; i < kSideRows / 16 / kSideParts; ++i) {
+          const int j = part + i * kSideParts;
+          if (j >= R / 16) break;
+          __syncwarp();
+          if (k0 == 0) tc_ld16(lanes + j * 16, shares[i]);
+          for (int gr = k0 == 0 ? 1 : 0; kSplit && gr * kGroupSteps < k1 - k0; ++gr) {
+            float w[16];
+            tc_ld16(lanes + gr * R + j * 16, w);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) shares[i][e] += w[e];
+          }
+        }
+      }
+      if (k1 < nb * 4) {           // the accumulators are used again
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+      }
     }
-    __syncwarp();
-    finished();
     {
       float scale = first ? kScale : 1.0f / kScale;
       if (first) {
@@ -312,16 +342,11 @@ __global__ void __launch_bounds__(kSideThreads, 1) small_side_kernel(const __gri
         scale *= factor;
       }
       if (rows_here) {
-        for (int j = part; j < R / 16; j += kSideParts) {
-          __syncwarp();
-          float v[16];
-          tc_ld16(lanes + j * 16, v);
-          for (int gr = 1; gr < groups; ++gr) {
-            float w[16];
-            tc_ld16(lanes + gr * R + j * 16, w);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] += w[i];
-          }
+        for (int i = 0; i < kSideRows / 16 / kSideParts; ++i) {
+          const int j = part + i * kSideParts;
+          if (j >= R / 16) break;
+          const float (&v)[16] = shares[i];
           if (row < R && ctas == 1) {
             // the share is A
 #pragma unroll
@@ -330,22 +355,22 @@ __global__ void __launch_bounds__(kSideThreads, 1) small_side_kernel(const __gri
               uint8_t* at = base + lay.operand + (c >> 6) * lay.block + block_at(row, c & 63);
               float w[8];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) w[i] = v[8 * h + i] * scale;
+              for (int e = 0; e < 8; ++e) w[e] = v[8 * h + e] * scale;
               *reinterpret_cast<uint4*>(at) = halves(w);
               if (kSplit) *reinterpret_cast<uint4*>(at + op_low) = halves(w);
             }
           } else if (row < R) {
             float* at = reinterpret_cast<float*>(base + lay.share) + row * (R + 4) + j * 16;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              *reinterpret_cast<float4*>(at + 4 * i) = make_float4(v[4 * i] * scale, v[4 * i + 1] * scale, v[4 * i + 2] * scale, v[4 * i + 3] * scale);
+            for (int e = 0; e < 16; e += 4)
+              *reinterpret_cast<float4*>(at + e) = make_float4(v[e] * scale, v[e + 1] * scale, v[e + 2] * scale, v[e + 3] * scale);
           }
         }
       }
       tc_fence_before();
     }
     // ---- A: a slice of rows added up by each CTA, whole rows copied to the others (written piece by piece into all shared
-    // memories: 64 x 1024 float32 43.6 us, 37.9 so; 100 x 4000 91.5 and 82.5) ----
+    // memories, with longer accumulations than now: 64 x 1024 float32 43.6 us, 37.9 so; 100 x 4000 91.5 and 82.5) ----
     if (ctas > 1) {
       if (tid == 0) mbar_expect_tx(arrived, static_cast<uint32_t>((kSplit ? 2 : 1) * k_blocks * (R - slice) * 128));
       __syncwarp();
@@ -373,12 +398,15 @@ __global__ void __launch_bounds__(kSideThreads, 1) small_side_kernel(const __gri
     asm volatile("fence.proxy.async;" ::: "memory");
     tc_fence_after();
     if (warp == 0 && elect_one()) {
-      uint32_t more = 0;
-      for (int seg = kSplit ? 0 : 2; seg < 3; ++seg)
-        for (int k = 0; k < R / 16; ++k, more = 1) {
-          const int at = lay.operand + (k >> 2) * lay.block + 32 * (k & 3);
-          mma_one(tmem, desc(desc_k, at + (seg == 1 ? op_low : 0)), desc(desc_k, at + (seg == 0 ? op_low : 0)), idesc_sym, more);
-        }
+      for (int gr = 0; gr < groups; ++gr) {
+        uint32_t more = 0;
+        const int k0 = gr * kGroupSteps, k1 = kSplit ? min(k_steps, k0 + kGroupSteps) : k_steps;
+        for (int seg = kSplit ? 0 : 2; seg < 3; ++seg)
+          for (int k = k0; k < k1; ++k, more = 1) {
+            const int at = lay.operand + (k >> 2) * lay.block + 32 * (k & 3);
+            mma_one(tmem + gr * R, desc(desc_k, at + (seg == 1 ? op_low : 0)), desc(desc_k, at + (seg == 0 ? op_low : 0)), idesc_sym, more);
+          }
+      }
       commit_one(bar);
     }
     __syncwarp();
@@ -390,6 +418,12 @@ __global__ void __launch_bounds__(kSideThreads, 1) small_side_kernel(const __gri
         __syncwarp();
         float v[16];
         tc_ld16(lanes + j * 16, v);
+        for (int gr = 1; gr < groups; ++gr) {
+          float w[16];
+          tc_ld16(lanes + gr * R + j * 16, w);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] += w[i];
+        }
         if (row < R) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -424,21 +458,24 @@ __global__ void __launch_bounds__(kSideThreads, 1) small_side_kernel(const __gri
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    // ---- X <- B X, up to eight blocks at a time ----
+    // ---- X <- B X, up to eight blocks at a time (with low parts: accumulators) ----
     const float scale = (first ? factor : 1.0f / kScale) * (last ? 1.0f : kScale) / kScale;
-    for (int b0 = 0; b0 < nb; b0 += 8) {
-      const int b1 = min(nb, b0 + 8);
+    for (int b0 = 0; b0 < nb; b0 += round_blocks) {
+      const int b1 = min(nb, b0 + round_blocks);
       if (warp == 0 && elect_one()) {
-        for (int b = b0; b < b1; b += 4) {
-          const int n = min(4, b1 - b);
-          const uint32_t idesc = idesc0 | (1u << 16) | (static_cast<uint32_t>(n * kSideColumns >> 3) << 17);
-          uint32_t more = 0;
-          for (int seg = kSplit ? 0 : 2; seg < 3; ++seg)
-            for (int k = 0; k < R / 16; ++k, more = 1) {
-              const int at = lay.operand + (k >> 2) * lay.block + 32 * (k & 3) + (seg == 1 ? op_low : 0);
-              mma_one(tmem + (b - b0) * kSideColumns, desc(desc_k, at), desc(desc_mn, b * lay.block + (seg == 0 ? x_low : 0) + k * 2048), idesc,
-                      more);
-            }
+        for (int gr = 0; gr < groups; ++gr) {
+          const int k0 = gr * kGroupSteps, k1 = kSplit ? min(k_steps, k0 + kGroupSteps) : k_steps;
+          for (int b = b0; b < b1; b += 4) {
+            const int n = min(4, b1 - b);
+            const uint32_t idesc = idesc0 | (1u << 16) | (static_cast<uint32_t>(n * kSideColumns >> 3) << 17);
+            uint32_t more = 0;
+            for (int seg = kSplit ? 0 : 2; seg < 3; ++seg)
+              for (int k = k0; k < k1; ++k, more = 1) {
+                const int at = lay.operand + (k >> 2) * lay.block + 32 * (k & 3) + (seg == 1 ? op_low : 0);
+                mma_one(tmem + (gr * round_blocks + b - b0) * kSideColumns, desc(desc_k, at),
+                        desc(desc_mn, b * lay.block + (seg == 0 ? x_low : 0) + k * 2048), idesc, more);
+              }
+          }
         }
         commit_one(bar);
       }
@@ -449,6 +486,12 @@ __global__ void __launch_bounds__(kSideThreads, 1) small_side_kernel(const __gri
           __syncwarp();
           float v[16];
           tc_ld16(lanes + j * 16, v);
+          for (int gr = 1; gr < groups; ++gr) {
+            float w[16];
+            tc_ld16(lanes + gr * round_blocks * kSideColumns + j * 16, w);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] += w[i];
+          }
 #pragma unroll
           for (int i = 0; i < 16; ++i) v[i] *= scale;
           const int c = b0 * kSideColumns + j * 16;           // column of this CTA

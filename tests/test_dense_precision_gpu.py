@@ -119,3 +119,24 @@ def test_single_parts_through_the_c_interface(rows, cols, dtype):
                                        cols, rows * cols, p(room), size, _native.current_stream_ptr()))
     ns.check(out, update, 11)
     assert torch.equal(out, dense.orthogonalize(update, operand_bits=11))
+
+
+def _float32_operations(g):
+    a, b, c = ns.COEFFICIENTS
+    flip = g.shape[-2] > g.shape[-1]
+    x = g.mT if flip else g
+    x = x / (torch.linalg.matrix_norm(x, keepdim=True) + 1e-7)
+    for _ in range(5):
+        gram = x @ x.mT
+        x = a * x + (b * gram + c * (gram @ gram)) @ x
+    return x.mT if flip else x
+
+
+@pytest.mark.parametrize("shape", [(33, 40), (40, 500), (64, 64), (100, 100), (128, 128), (64, 1024), (128, 1024), (100, 4000), (700, 112), (3, 80, 300)])
+def test_float32_results_are_near_what_float32_operations_give(shape):
+    """Pairs round at 2^-23, twice float32's 2^-24, and their sums are cut where float32's are rounded, which doubles that error too."""
+    update = ns.update(shape, 1).cuda()
+    want = ns.steps_of(update)
+    off = lambda x: float((x.double() - want).norm() / want.norm())
+    here, plain = off(dense.orthogonalize(update)), off(_float32_operations(update))
+    assert here <= 2 * plain, (here, plain)
