@@ -145,14 +145,16 @@ class RuntimePredictor:
             raise RuntimeError("update_hidden needs the model on a GPU, in float32")
         with torch.no_grad():
             g = torch.stack([w.grad for w in weights])
-            if self._momentum is None or self._momentum.shape != g.shape or self._momentum.device != g.device:
-                self._momentum = torch.zeros_like(g)
-            self._momentum.mul_(momentum).add_(g)
-            update = torch.add(g, self._momentum, alpha=momentum) if nesterov else self._momentum
-            step = dense.orthogonalize(update, steps=steps)
+            kept = self._momentum
+            if kept is None or kept.shape != g.shape or kept.device != g.device:
+                kept = torch.zeros_like(g)
+            kept = kept.mul(momentum).add_(g)
+            update = torch.add(g, kept, alpha=momentum) if nesterov else kept
+            step = dense.orthogonalize(update, steps=steps)       # what this raises leaves weights and momentum as they were
             if weight_decay:
                 torch._foreach_mul_(weights, 1.0 - lr * weight_decay)
             torch._foreach_add_(weights, list(step.unbind(0)), alpha=-lr)
+        self._momentum = kept
         self.invalidate()
 
     # -- inference ----------------------------------------------------------

@@ -70,3 +70,38 @@ def test_retrained_under_queued_predictions():
     torch.cuda.synchronize()
     assert torch.equal(got, want) and not torch.equal(new, want)
     del held
+
+
+def _trained(seed=3, precision="int8", steps=1):
+    """A predictor with gradients, after some updates."""
+    torch.manual_seed(seed)
+    pred = RuntimePredictor("linear", 2, 128, precision=precision)
+    pred.model.cuda()
+    pred.mu, pred.sigma = np.zeros(8), np.full(8, 1e4)
+    x = torch.randn(64, 8, device="cuda")
+    for _ in range(steps):
+        pred.model.zero_grad()
+        pred.model(x).square().mean().backward()
+        pred.update_hidden(0.1)
+    pred.model.zero_grad()
+    pred.model(x).square().mean().backward()
+    return pred
+
+
+def _weights(pred):
+    return [p.detach().clone() for p in pred.model.parameters()]
+
+
+@pytest.mark.parametrize("failure", ["status", "steps"])
+@pytest.mark.parametrize("nesterov", [True, False])
+def test_an_update_that_raises_leaves_everything_as_it_was(failure, nesterov):
+    pred, other = _trained(), _trained()
+    before = _weights(pred)
+    if failure == "status":
+        _native.check(_native.load().hb_dense_inject_status(0x511))
+    with pytest.raises(_native.HabitatNativeError):
+        pred.update_hidden(0.1, nesterov=nesterov, steps=5 if failure == "status" else 0)
+    assert all(torch.equal(a, b) for a, b in zip(before, _weights(pred)))
+    for p in (pred, other):
+        p.update_hidden(0.1, nesterov=nesterov)
+    assert all(torch.equal(a, b) for a, b in zip(_weights(pred), _weights(other)))
