@@ -188,6 +188,7 @@ EXPORTS = {
     "hb_orthogonalize_workspace_bytes": (ctypes.c_int64, [
         ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32]),
     "hb_dense_status": (ctypes.c_int32, [ctypes.POINTER(ctypes.c_int32)]),
+    "hb_dense_failures": (ctypes.c_int32, [ctypes.c_int32, ctypes.POINTER(ctypes.c_int64)]),
     "hb_dense_inject_status": (ctypes.c_int32, [ctypes.c_int32]),
     "hb_peer_allreduce": (ctypes.c_int32, [
         ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p]),

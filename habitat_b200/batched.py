@@ -407,6 +407,7 @@ class Int8MLPHandle:
         stream = torch.cuda.current_stream(self.device)
         self._streams, self._captured = {stream.cuda_stream}, False       # that the pack is known to be used on; in a graph
         stream.synchronize()                                      # the pack is there for every stream
+        self._failures = dense.failures()                         # before this handle's first launch
 
     def _used_on(self, stream):
         """Tells the allocator that the pack is used on a stream, which its memory then waits for when it is given back."""
@@ -447,19 +448,23 @@ class Int8MLPHandle:
         flat = out.view(-1)
         pitch = (self.width + 15) // 16 * 16
         with torch.cuda.device(self.device):
-            self._used_on(torch.cuda.current_stream())
-            stream = _native.current_stream_ptr()
-            for at in range(0, n, self.chunk):
-                m = min(self.chunk, n - at)
-                q = torch.empty((m, pitch), dtype=torch.int8, device=self.device)[:, :self.width]
-                scales = torch.empty((m,), dtype=torch.float32, device=self.device)
-                _native.check(_call("hb_int8_mlp_input", lib.hb_int8_mlp_input, _ptr(op_features[at:]), self.n_op_features, _ptr(rows[at:]),
-                                    _ptr(self._devices), self.n_device_rows, _ptr(self._mu), _ptr(self._sigma), _ptr(self._fc1[0]),
-                                    _ptr(self._fc1[1]), m, self.width, _ptr(q), pitch, _ptr(scales), stream))
-                for weight, weight_scales, bias in self._layers:
-                    q, scales = dense.int8_matmul_quantized(q, scales, weight, weight_scales, bias=bias, relu=True)
-                _native.check(_call("hb_int8_mlp_output", lib.hb_int8_mlp_output, _ptr(q), pitch, _ptr(scales), _ptr(self._fc2[0]),
-                                    _ptr(self._fc2[1]), m, self.width, _ptr(flat[at:]), stream))
+            try:
+                self._used_on(torch.cuda.current_stream())
+                stream = _native.current_stream_ptr()
+                for at in range(0, n, self.chunk):
+                    m = min(self.chunk, n - at)
+                    q = torch.empty((m, pitch), dtype=torch.int8, device=self.device)[:, :self.width]
+                    scales = torch.empty((m,), dtype=torch.float32, device=self.device)
+                    _native.check(_call("hb_int8_mlp_input", lib.hb_int8_mlp_input, _ptr(op_features[at:]), self.n_op_features, _ptr(rows[at:]),
+                                        _ptr(self._devices), self.n_device_rows, _ptr(self._mu), _ptr(self._sigma), _ptr(self._fc1[0]),
+                                        _ptr(self._fc1[1]), m, self.width, _ptr(q), pitch, _ptr(scales), stream))
+                    for weight, weight_scales, bias in self._layers:
+                        q, scales = dense.int8_matmul_quantized(q, scales, weight, weight_scales, bias=bias, relu=True)
+                    _native.check(_call("hb_int8_mlp_output", lib.hb_int8_mlp_output, _ptr(q), pitch, _ptr(scales), _ptr(self._fc2[0]),
+                                        _ptr(self._fc2[1]), m, self.width, _ptr(flat[at:]), stream))
+            except _native.HabitatNativeError:
+                self._failures = dense.failures()         # what this reports, check_status need not
+                raise
         return out
 
     def predict_host(self, op_features, device_row):
@@ -477,10 +482,12 @@ class Int8MLPHandle:
         return float(self.predict_host(np.asarray([op_features], np.float32), [device_row])[0])
 
     def check_status(self):
-        """Synchronises and raises if a launch gave up on a bounded device wait (reported once)."""
+        """Synchronises and raises if a launch gave up on a bounded device wait since the last check, this handle's or (they share
+        the GPU's status word) another's, whoever has been told of it meanwhile.  Reported once."""
         from habitat_b200 import dense
         with torch.cuda.device(self.device):
-            dense.check_status()
+            since, self._failures = self._failures, dense.failures(synchronise=True)
+            dense.check_since(since)
 
 
 def special_scale(run_time_ms, pred_dest, pred_orig, negative_count=None):

@@ -14,9 +14,8 @@ namespace dense {
 cudaError_t encode_planes(CUtensorMap* map, const void* base, int elem_bytes, int64_t cols, int64_t rows, int64_t planes,
                           int64_t pitch, int64_t plane_stride, int box_rows);
 
-// The word that kernels on the current GPU write when a bounded wait runs out (page-locked, created on first use).
-hb_status status_word(int32_t** word);
-// The same, and HB_ERR_DEVICE_TIMEOUT (reported once) when an earlier launch has written it.
+// The word that kernels on the current GPU write when a bounded wait runs out (page-locked, created on first use), and
+// HB_ERR_DEVICE_TIMEOUT (once for each host thread) when an earlier launch has written it.
 hb_status begin_call(const char* name, int32_t** word);
 
 hb_status sm_count(int* sms);

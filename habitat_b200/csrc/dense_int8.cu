@@ -615,34 +615,84 @@ cudaError_t encode_planes(CUtensorMap* map, const void* base, int elem_bytes, in
 namespace {
 std::mutex g_status_mu;
 int32_t* g_status[64];
-}  // namespace
+// Codes that the host has found in each GPU's word, and the last of them.  The word says nothing about whose launch it was, and whoever looks
+// first takes it; so everyone who asks compares the count with the one they were last told of, host threads here
+// (one more than that; 0: none yet), handles for themselves (hb_dense_failures).
+std::atomic<int64_t> g_failures[64];
+std::atomic<int32_t> g_code[64];
+thread_local int64_t t_told[64];
 
-hb_status status_word(int32_t** word) {
-  int dev = 0;
-  HB_CUDA_TRY(cudaGetDevice(&dev));
-  if (dev < 0 || dev >= 64) {
-    hb::set_error("device ordinal %d out of range", dev);
+hb_status status_word_of(int* dev, int32_t** word) {
+  HB_CUDA_TRY(cudaGetDevice(dev));
+  if (*dev < 0 || *dev >= 64) {
+    hb::set_error("device ordinal %d out of range", *dev);
     return HB_ERR_UNSUPPORTED;
   }
   std::lock_guard<std::mutex> lock(g_status_mu);
-  if (!g_status[dev]) {
+  if (!g_status[*dev]) {
     void* p = nullptr;
     HB_CUDA_TRY(cudaHostAlloc(&p, 64, cudaHostAllocDefault));
-    g_status[dev] = static_cast<int32_t*>(p);
-    *static_cast<volatile int32_t*>(g_status[dev]) = 0;
+    g_status[*dev] = static_cast<int32_t*>(p);
+    *static_cast<volatile int32_t*>(g_status[*dev]) = 0;
   }
-  *word = g_status[dev];
+  *word = g_status[*dev];
   return HB_OK;
 }
 
+int64_t count_failures(int dev, int32_t* word) {
+  if (*static_cast<volatile int32_t*>(word)) {
+    if (const int32_t code = __atomic_exchange_n(word, 0, __ATOMIC_ACQ_REL)) {
+      g_code[dev].store(code);
+      g_failures[dev].fetch_add(1);
+    }
+  }
+  return g_failures[dev].load();
+}
+
+// The last code where a launch has given up since this thread was last told, else 0.
+int32_t news(int dev, int32_t* word) {
+  int64_t& told = t_told[dev];
+  if (told == 0) told = g_failures[dev].load() + 1;      // what others met before this thread's first call is theirs
+  const int64_t now = count_failures(dev, word) + 1;
+  if (now == told) return 0;
+  told = now;
+  return g_code[dev].load();
+}
+}  // namespace
+
 hb_status begin_call(const char* name, int32_t** word) {
-  if (const hb_status st = status_word(word)) return st;
-  volatile int32_t* w = *word;
-  if (const int32_t code = *w) {
-    *w = 0;
+  int dev = 0;
+  if (const hb_status st = status_word_of(&dev, word)) return st;
+  if (const int32_t code = news(dev, *word)) {
     hb::set_error("%s: an earlier dense-layer launch gave up on a bounded wait (code 0x%x)", name, code);
     return HB_ERR_DEVICE_TIMEOUT;
   }
+  return HB_OK;
+}
+
+hb_status dense_status(int32_t* code) {
+  int dev = 0;
+  int32_t* word = nullptr;
+  if (const hb_status st = status_word_of(&dev, &word)) return st;
+  HB_CUDA_TRY(cudaDeviceSynchronize());
+  *code = news(dev, word);
+  return HB_OK;
+}
+
+hb_status dense_failures(bool synchronise, int64_t* failures) {
+  int dev = 0;
+  int32_t* word = nullptr;
+  if (const hb_status st = status_word_of(&dev, &word)) return st;
+  if (synchronise) HB_CUDA_TRY(cudaDeviceSynchronize());
+  *failures = count_failures(dev, word);
+  return HB_OK;
+}
+
+hb_status inject_status(int32_t code) {
+  int dev = 0;
+  int32_t* word = nullptr;
+  if (const hb_status st = status_word_of(&dev, &word)) return st;
+  *static_cast<volatile int32_t*>(word) = code;
   return HB_OK;
 }
 
@@ -653,12 +703,7 @@ extern "C" hb_status hb_dense_status(int32_t* device_status) {
     hb::set_error("hb_dense_status: NULL argument");
     return HB_ERR_INVALID_ARGUMENT;
   }
-  int32_t* word = nullptr;
-  if (const hb_status st = dense::status_word(&word)) return st;
-  HB_CUDA_TRY(cudaDeviceSynchronize());
-  volatile int32_t* w = word;
-  *device_status = *w;
-  *w = 0;
+  if (const hb_status st = dense::dense_status(device_status)) return st;
   if (*device_status) {
     hb::set_error("a dense-layer launch gave up on a bounded wait (code 0x%x)", *device_status);
     return HB_ERR_DEVICE_TIMEOUT;
@@ -666,12 +711,15 @@ extern "C" hb_status hb_dense_status(int32_t* device_status) {
   return HB_OK;
 }
 
-extern "C" hb_status hb_dense_inject_status(int32_t device_status) {
-  int32_t* word = nullptr;
-  if (const hb_status st = dense::status_word(&word)) return st;
-  *static_cast<volatile int32_t*>(word) = device_status;
-  return HB_OK;
+extern "C" hb_status hb_dense_failures(int32_t synchronise, int64_t* failures) {
+  if (!failures) {
+    hb::set_error("hb_dense_failures: NULL argument");
+    return HB_ERR_INVALID_ARGUMENT;
+  }
+  return dense::dense_failures(synchronise != 0, failures);
 }
+
+extern "C" hb_status hb_dense_inject_status(int32_t device_status) { return dense::inject_status(device_status); }
 
 extern "C" hb_status hb_quantize_rows(const void* x, int32_t x_type, int64_t rows, int64_t cols, int64_t x_pitch, int8_t* q,
                                       int64_t q_pitch, float* scales, void* stream) {

@@ -119,6 +119,22 @@ def orthogonalize(update, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1
 
 
 def check_status():
-    """Synchronises the current GPU and raises if a launch of this module gave up on a bounded device wait (reported once)."""
+    """Synchronises the current GPU and raises if a launch of this module gave up on a bounded device wait.  The calls above raise for
+    that, too, without synchronising.  Each thread is told once, whoever's launch it was."""
     code = ctypes.c_int32(0)
     _native.check(_native.load().hb_dense_status(ctypes.byref(code)))
+
+
+def failures(synchronise=False):
+    """How often a launch of this module is known to have given up on the current GPU.  Results are good if the count from before their
+    calls is still the one that `failures(synchronise=True)` gives behind them, whichever thread was told in between."""
+    count = ctypes.c_int64(0)
+    _native.check(_native.load().hb_dense_failures(int(synchronise), ctypes.byref(count)))
+    return count.value
+
+
+def check_since(count):
+    """Synchronises and raises if a launch has given up since `failures` gave `count`."""
+    if failures(synchronise=True) != count:
+        check_status()            # raises unless this thread has been told by another call
+        raise _native.HabitatNativeError(_native.HB_ERR_DEVICE_TIMEOUT, "a dense-layer launch gave up on a bounded wait")

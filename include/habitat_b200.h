@@ -527,8 +527,12 @@ hb_status hb_orthogonalize(const void* update, int32_t type, int64_t batch, int6
 int64_t hb_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols, int32_t split);
 
 /* Synchronises the current GPU and reports whether one of the launches above gave up on a bounded device wait (reported
- * once; without this call the next one of them on that GPU reports it). */
+ * once to each host thread that has made such calls, whoever's launch it was; without this call the thread's next one of them on
+ * that GPU reports it). */
 hb_status hb_dense_status(int32_t* device_status);
+/* How often one of them is known to have given up on the current GPU, `synchronise`: after waiting for it.  For callers that keep track
+ * of their own results: whether the count is still the one from before their calls.  Reports nothing to the thread. */
+hb_status hb_dense_failures(int32_t synchronise, int64_t* failures);
 /* Writes that word from the host (tests of the error path). */
 hb_status hb_dense_inject_status(int32_t device_status);
 

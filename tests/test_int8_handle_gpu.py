@@ -105,3 +105,79 @@ def test_an_update_that_raises_leaves_everything_as_it_was(failure, nesterov):
     for p in (pred, other):
         p.update_hidden(0.1, nesterov=nesterov)
     assert all(torch.equal(a, b) for a, b in zip(_weights(pred), _weights(other)))
+
+
+# -- launches that gave up: the word as a kernel leaves it, written from the host ----------------
+
+def _gives_up(code=0x531):
+    torch.cuda.synchronize()
+    _native.check(_native.load().hb_dense_inject_status(code))
+
+
+def _other_call():
+    dense.quantize_rows(torch.ones((2, 16), device="cuda"))
+    dense.orthogonalize(torch.ones((4, 4), device="cuda"))
+
+
+def test_a_failure_that_another_call_reported_is_not_lost_to_the_handle():
+    h, f, d = _handle()
+    h.predict(f, d)
+    _gives_up()
+    with pytest.raises(_native.HabitatNativeError, match="gave up"):
+        _other_call()
+    _other_call()                                     # told once
+    with pytest.raises(_native.HabitatNativeError, match="gave up"):
+        h.check_status()
+    h.check_status()
+    h.predict(f, d)
+    h.check_status()
+
+
+def test_every_handle_learns_of_a_failure_and_none_twice():
+    h, f, d = _handle()
+    other, _, _ = _handle(seed=2)
+    h.predict(f, d), other.predict(f, d)
+    _gives_up()
+    for each in (h, other):
+        with pytest.raises(_native.HabitatNativeError, match="gave up"):
+            each.check_status()
+    h.predict(f, d), other.predict(f, d)
+    h.check_status(), other.check_status()
+    late, _, _ = _handle(seed=3)
+    late.predict(f, d)
+    late.check_status()                               # of before its time
+    _gives_up()
+    with pytest.raises(_native.HabitatNativeError, match="gave up"):
+        h.predict(f, d)
+    h.predict(f, d)
+    h.check_status()                                  # its predict has said so
+    assert np.isfinite(h.predict_host(f.cpu().numpy(), d.cpu().numpy())).all()
+    for each in (other, late):
+        with pytest.raises(_native.HabitatNativeError, match="gave up"):
+            each.check_status()
+
+
+def test_every_thread_learns_of_a_failure():
+    import threading
+    dense.check_status()
+    heard = []
+
+    def look():
+        try:
+            dense.check_status()
+            heard.append(False)
+        except _native.HabitatNativeError:
+            heard.append(True)
+    count = dense.failures()
+    _gives_up()
+    for _ in range(2):                                # the first to look is told, a thread that starts afterwards is not
+        t = threading.Thread(target=look)
+        t.start()
+        t.join()
+    assert heard == [True, False] and dense.failures() == count + 1
+    with pytest.raises(_native.HabitatNativeError, match="gave up"):
+        dense.check_status()
+    dense.check_status()
+    dense.check_since(count + 1)
+    with pytest.raises(_native.HabitatNativeError, match="gave up"):
+        dense.check_since(count)
