@@ -106,6 +106,7 @@ class RuntimePredictor:
         self._handle = None
         self._device_rows = None
         self._momentum = None
+        self._unchecked = None               # (GPU, dense.failures()) from before updates whose launches may have given up
         if model_path is not None:
             self.load_state(model_path)
 
@@ -117,10 +118,11 @@ class RuntimePredictor:
         self.mu = checkpoint["mu"]
         self.sigma = checkpoint["sigma"]
         self.model.load_state_dict(checkpoint["model"])
-        self._momentum = None
+        self._momentum = self._unchecked = None
         self.invalidate()
 
     def save_state(self, path):
+        self._check_updates()
         torch.save({"mu": self.mu, "sigma": self.sigma, "model": self.model.state_dict()}, path)
 
     def invalidate(self):
@@ -136,7 +138,8 @@ class RuntimePredictor:
         and m the kept momentum, m <- momentum m + g, the update is g + momentum m (nesterov) or m, made nearly orthogonal
         by `steps` Newton-Schulz steps (dense.orthogonalize, all layers in one call), and
         w <- (1 - lr weight_decay) w - lr update.  Biases, fc1 and fc2 are left to the caller's optimizer.
-        The next prediction packs the new weights (`invalidate`)."""
+        The next prediction packs the new weights (`invalidate`).  Does not synchronise: whether a launch gave up on a bounded
+        device wait, which leaves weights that mean nothing, is seen and raised before they are packed or saved."""
         from habitat_b200 import dense
         weights = [block.weight for block in self.model.mlp.layers if isinstance(block, nn.Linear)]
         if any(w.grad is None for w in weights):
@@ -150,12 +153,24 @@ class RuntimePredictor:
                 kept = torch.zeros_like(g)
             kept = kept.mul(momentum).add_(g)
             update = torch.add(g, kept, alpha=momentum) if nesterov else kept
+            if self._unchecked is None:
+                with torch.cuda.device(g.device):
+                    unchecked = g.device, dense.failures()
+            else:
+                unchecked = self._unchecked
             step = dense.orthogonalize(update, steps=steps)       # what this raises leaves weights and momentum as they were
             if weight_decay:
                 torch._foreach_mul_(weights, 1.0 - lr * weight_decay)
             torch._foreach_add_(weights, list(step.unbind(0)), alpha=-lr)
-        self._momentum = kept
+        self._momentum, self._unchecked = kept, unchecked
         self.invalidate()
+
+    def _check_updates(self):
+        if self._unchecked is not None:
+            from habitat_b200 import dense
+            (device, since), self._unchecked = self._unchecked, None
+            with torch.cuda.device(device):
+                dense.check_since(since)
 
     # -- inference ----------------------------------------------------------
     def _ensure_handle(self):
@@ -164,6 +179,7 @@ class RuntimePredictor:
         from habitat_b200.batched import Int8MLPHandle, MLPHandle
         if self.mu is None or self.sigma is None:
             raise RuntimeError("RuntimePredictor has no mu/sigma (load a checkpoint first)")
+        self._check_updates()
         devices = get_all_devices(self.device_params)
         names = sorted(devices)
         self._device_rows = {name: i for i, name in enumerate(names)}

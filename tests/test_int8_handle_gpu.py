@@ -181,3 +181,23 @@ def test_every_thread_learns_of_a_failure():
     dense.check_since(count + 1)
     with pytest.raises(_native.HabitatNativeError, match="gave up"):
         dense.check_since(count)
+
+
+@pytest.mark.parametrize("precision", ["bf16", "bf16x3", "int8"])
+@pytest.mark.parametrize("told", [False, True])
+@pytest.mark.parametrize("how", ["predict", "save"])
+def test_updates_that_gave_up_are_neither_served_nor_saved(precision, told, how, tmp_path):
+    pred = _trained(precision=precision, steps=2)
+    _gives_up()
+    if told:
+        with pytest.raises(_native.HabitatNativeError):
+            _other_call()
+    feats, dev = (torch.from_numpy(a).cuda() for a in workloads.make_queries("linear", 20, seed=4))
+    path = str(tmp_path / "model.pth")
+    with pytest.raises(_native.HabitatNativeError, match="gave up"):
+        pred.predict_batch(feats, dev) if how == "predict" else pred.save_state(path)
+    assert not (tmp_path / "model.pth").exists()
+    pred.save_state(path)                             # the caller has been told
+    pred.load_state(path)
+    assert bool(torch.isfinite(pred.predict_batch(feats, dev)).all())
+    dense.check_status()
