@@ -364,9 +364,9 @@ class Int8MLPHandle:
     and the weights half the memory; the error is that of 8-bit rows, about 1 % of a layer's spread per layer.  A call is one
     launch per layer, so batches of up to 8,192 queries are quicker in bf16 (110 us against 139).  Queries go through in pieces of `chunk`, whose rows are allocated through torch.
 
-    The pack lies in torch's memory, which goes back when the handle is dropped.  It is not used again before the
+    The pack lies in torch's memory, which goes back when the handle is closed or dropped.  It is not used again before the
     predictions that any stream has queued by then have ended; graphs that hold predictions are to be replayed only while the handle is kept,
-    as with MLPHandle, and dropping it waits for replays under way."""
+    as with MLPHandle, and closing it waits for replays under way."""
 
     chunk = 131072
 
@@ -393,41 +393,52 @@ class Int8MLPHandle:
                 raise ValueError("%s must be %s" % (name, list(shape)))
             return torch.from_numpy(a).to(self.device)
         c = n_op_features + 4
-        self._fc1 = up(fc1_w, np.float32, (width, c), "fc1 weight"), up(fc1_b, np.float32, (width,), "fc1 bias")
-        self._fc2 = (up(np.asarray(fc2_w).reshape(-1), np.float32, (width,), "fc2 weight"),
-                     up(np.asarray(fc2_b).reshape(-1), np.float32, (1,), "fc2 bias"))
-        self._mu, self._sigma = up(mu, np.float64, (c,), "mu"), up(sigma, np.float64, (c,), "sigma")
-        self._devices = up(device_features, np.float64, device_features.shape, "device_features")
+        fc1 = up(fc1_w, np.float32, (width, c), "fc1 weight"), up(fc1_b, np.float32, (width,), "fc1 bias")
+        fc2 = (up(np.asarray(fc2_w).reshape(-1), np.float32, (width,), "fc2 weight"),
+               up(np.asarray(fc2_b).reshape(-1), np.float32, (1,), "fc2 bias"))
+        mu, sigma = up(mu, np.float64, (c,), "mu"), up(sigma, np.float64, (c,), "sigma")
+        devices = up(device_features, np.float64, device_features.shape, "device_features")
         biases = up(hidden_b, np.float32, (layers, width), "hidden bias")
-        self._layers = [dense.quantize_rows(torch.from_numpy(np.ascontiguousarray(hidden_w[i])).to(self.device)) + (biases[i],)
-                        for i in range(layers)]
-        self._pack = [*self._fc1, *self._fc2, self._mu, self._sigma, self._devices, biases]
-        for weight, scales, _ in self._layers:
-            self._pack += [weight, scales]
+        hidden = [dense.quantize_rows(torch.from_numpy(np.ascontiguousarray(hidden_w[i])).to(self.device)) + (biases[i],)
+                  for i in range(layers)]
+        pack = [*fc1, *fc2, mu, sigma, devices, biases]
+        for weight, scales, _ in hidden:
+            pack += [weight, scales]
+        self._weights = fc1, fc2, mu, sigma, devices, hidden, pack      # None: closed
         stream = torch.cuda.current_stream(self.device)
         self._streams, self._captured = {stream.cuda_stream}, False       # that the pack is known to be used on; in a graph
         stream.synchronize()                                      # the pack is there for every stream
         self._failures = dense.failures()                         # before this handle's first launch
 
-    def _used_on(self, stream):
+    def _used_on(self, stream, pack):
         """Tells the allocator that the pack is used on a stream, which its memory then waits for when it is given back."""
         if torch.cuda.is_current_stream_capturing():
-            self._captured = True               # replays may be on any stream: __del__ waits for them
+            self._captured = True               # replays may be on any stream: close waits for them
         elif stream.cuda_stream not in self._streams:
-            for t in self._pack:
+            for t in pack:
                 t.record_stream(stream)
             self._streams.add(stream.cuda_stream)
 
-    def __del__(self):
-        try:
+    def close(self):
+        """Gives the pack back; predictions that are queued keep theirs, later ones raise."""
+        if self._weights is not None:
             if self._captured:
                 torch.cuda.synchronize(self.device)
+            self._weights = None
+
+    def __del__(self):
+        try:
+            self.close()
         except Exception:
             pass
 
     def predict(self, op_features, device_row, out=None):
         """op_features [Q, F] float32 CUDA, device_row [Q] uint8 CUDA -> [Q] float32."""
         from habitat_b200 import dense
+        weights = self._weights
+        if weights is None:
+            raise _native.HabitatNativeError(_native.HB_ERR_INVALID_ARGUMENT, "the handle is closed")
+        (fc1_w, fc1_b), (fc2_w, fc2_b), mu, sigma, devices, layers, pack = weights
         _require_cuda(op_features, torch.float32, "op_features")
         _require_cuda(device_row, torch.uint8, "device_row")
         if op_features.ndim != 2 or op_features.shape[1] != self.n_op_features:
@@ -449,19 +460,18 @@ class Int8MLPHandle:
         pitch = (self.width + 15) // 16 * 16
         with torch.cuda.device(self.device):
             try:
-                self._used_on(torch.cuda.current_stream())
+                self._used_on(torch.cuda.current_stream(), pack)
                 stream = _native.current_stream_ptr()
                 for at in range(0, n, self.chunk):
                     m = min(self.chunk, n - at)
                     q = torch.empty((m, pitch), dtype=torch.int8, device=self.device)[:, :self.width]
                     scales = torch.empty((m,), dtype=torch.float32, device=self.device)
                     _native.check(_call("hb_int8_mlp_input", lib.hb_int8_mlp_input, _ptr(op_features[at:]), self.n_op_features, _ptr(rows[at:]),
-                                        _ptr(self._devices), self.n_device_rows, _ptr(self._mu), _ptr(self._sigma), _ptr(self._fc1[0]),
-                                        _ptr(self._fc1[1]), m, self.width, _ptr(q), pitch, _ptr(scales), stream))
-                    for weight, weight_scales, bias in self._layers:
+                                        _ptr(devices), self.n_device_rows, _ptr(mu), _ptr(sigma), _ptr(fc1_w), _ptr(fc1_b), m, self.width, _ptr(q), pitch, _ptr(scales), stream))
+                    for weight, weight_scales, bias in layers:
                         q, scales = dense.int8_matmul_quantized(q, scales, weight, weight_scales, bias=bias, relu=True)
-                    _native.check(_call("hb_int8_mlp_output", lib.hb_int8_mlp_output, _ptr(q), pitch, _ptr(scales), _ptr(self._fc2[0]),
-                                        _ptr(self._fc2[1]), m, self.width, _ptr(flat[at:]), stream))
+                    _native.check(_call("hb_int8_mlp_output", lib.hb_int8_mlp_output, _ptr(q), pitch, _ptr(scales), _ptr(fc2_w),
+                                        _ptr(fc2_b), m, self.width, _ptr(flat[at:]), stream))
             except _native.HabitatNativeError:
                 self._failures = dense.failures()         # what this reports, check_status need not
                 raise

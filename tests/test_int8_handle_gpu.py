@@ -50,6 +50,26 @@ def test_weights_stay_until_queued_predictions_have_ended(captured):
     del held
 
 
+def test_closed():
+    h, f, d = _handle()
+    want = h.predict(f, d)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)
+        got = h.predict(f, d)
+    h.close()
+    held = _overwrite()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    del held
+    h.close()
+    for call in (lambda: h.predict(f, d), lambda: h.predict_host(f.cpu().numpy(), d.cpu().numpy()), lambda: h.predict_one([1.0] * 4, 0)):
+        with pytest.raises(_native.HabitatNativeError, match="closed"):
+            call()
+    h.check_status()
+
+
 def test_retrained_under_queued_predictions():
     """The same through the predictor: an update drops the pack and the next prediction uploads another."""
     torch.manual_seed(2)
