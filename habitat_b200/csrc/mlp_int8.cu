@@ -49,7 +49,7 @@ mlp_input_kernel(const float* __restrict__ features, int n_op_feat, const uint8_
   // thread e of the first 96 brings input e mod 12 of query e / 12
   const int mine_k = tid / kMaxInFeat, mine_c = tid - mine_k * kMaxInFeat;
   const bool brings = tid < kInputQueries * kMaxInFeat && mine_c < inputs;
-  const double mine_mu = brings ? mu[mine_c] : 0.0, mine_per_sigma = brings ? 1.0 / sigma[mine_c] : 1.0;
+  const double mine_mu = brings ? mu[mine_c] : 0.0, mine_sigma = brings ? sigma[mine_c] : 1.0;
   float raw = 0.0f;
   int row = 0;
   auto request = [&](int64_t q0) {
@@ -59,7 +59,7 @@ mlp_input_kernel(const float* __restrict__ features, int n_op_feat, const uint8_
   };
   auto put = [&](int buf) {
     if (!brings) return;
-    x[buf][mine_k][mine_c] = mine_c < n_op_feat ? static_cast<float>((static_cast<double>(raw) - mine_mu) * mine_per_sigma)
+    x[buf][mine_k][mine_c] = mine_c < n_op_feat ? static_cast<float>((static_cast<double>(raw) - mine_mu) / mine_sigma)
                                                 : devices[row < n_dev ? row : n_dev - 1][mine_c - n_op_feat];
   };
   const int64_t step = static_cast<int64_t>(gridDim.x) * kInputQueries;

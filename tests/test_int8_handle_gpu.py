@@ -1,4 +1,6 @@
 """What an 8-bit predictor owes its caller beyond the numbers: its memory, its errors, its weights' updates."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -221,3 +223,27 @@ def test_updates_that_gave_up_are_neither_served_nor_saved(precision, told, how,
     pred.load_state(path)
     assert bool(torch.isfinite(pred.predict_batch(feats, dev)).all())
     dense.check_status()
+
+
+def test_features_are_divided_by_sigma():
+    """The quotient rounded to float32, as in the other predictors, not a product with 1 / sigma: features whose quotient lies half-way between two
+    float32 numbers, where the two differ."""
+    rng = np.random.default_rng(1)
+    cases = []
+    while len(cases) < 40:
+        x = np.float32(rng.uniform(1.0, 1000.0))
+        half_way = (2 * int(rng.integers(2 ** 23, 2 ** 24)) + 1) * 2.0 ** -24       # 25 bits
+        sigma = float(x) / half_way
+        if np.float32(float(x) / sigma) != np.float32(float(x) * (1.0 / sigma)):
+            cases.append((x, sigma))
+    lib, p = _native.load(), lambda t: ctypes.c_void_p(t.data_ptr())
+    f64 = lambda a: torch.tensor(a, dtype=torch.float64, device="cuda")
+    w, b, devices, mu = torch.zeros((1, 5), device="cuda"), torch.zeros((1,), device="cuda"), f64([[1.0] * 4]), f64([0.0] * 5)
+    w[0, 0] = 1.0
+    row, q = torch.zeros((1,), dtype=torch.uint8, device="cuda"), torch.empty((1, 16), dtype=torch.int8, device="cuda")
+    for x, sigma in cases:
+        scales, feature, sigmas = torch.empty((1,), device="cuda"), torch.tensor([x], device="cuda"), f64([sigma] + [1.0] * 4)
+        _native.check(lib.hb_int8_mlp_input(p(feature), 1, p(row), p(devices), 1, p(mu), p(sigmas), p(w), p(b), 1, 1, p(q), 16, p(scales),
+                                            _native.current_stream_ptr()))
+        # one feature through a weight of one: the row's scale is the quotient / 127
+        assert float(scales) == np.float32(float(x) / sigma) / np.float32(127), (x, sigma)
