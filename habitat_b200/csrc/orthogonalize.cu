@@ -579,6 +579,23 @@ int64_t lower_tiles(int64_t s, int bn) {
 
 constexpr int kMostPairs = 128;
 
+// Times in units of 240 cycles: a slot of operands with low parts takes 4, of others 1, a second launch that adds shares from
+// memory about 55, and sums that the pairs of a cluster exchange 15 and 7 (fitted to updates of 200 x 200 to 1024 x 1024).
+constexpr int kSecondLaunch = 55;
+int64_t slot_time(int64_t slots, bool split) { return slots * (split ? 4 : 1); }
+
+// How many ways K of a symmetric product is split, the shares added by a second launch: as many as there are SM pairs for the
+// tiles, of at least four slots; one unless that saves more than the launch takes.
+int splits_of(int64_t batch, int64_t s, int64_t K, bool split, int pairs) {
+  const int64_t tiles = batch * lower_tiles(s, 128), slots = (K + 63) / 64;
+  int64_t n = pairs / tiles;
+  if (n > slots / 4) n = slots / 4;
+  if (n < 2) return 1;
+  const int64_t each = (slots + n - 1) / n;
+  if (slot_time(slots - each, split) < kSecondLaunch) return 1;
+  return static_cast<int>((slots + each - 1) / each);      // none without slots
+}
+
 struct Layout {
   int64_t s, l, sp, lp;           // sides, and the pitches of rows of them
   int64_t x_bytes, a_bytes;       // one buffer of X, of A or B (all batches and planes)
@@ -594,8 +611,14 @@ Layout layout_of(int64_t batch, int64_t rows, int64_t cols, bool split) {
   const int64_t planes = split ? 2 : 1;
   r.x_bytes = up(batch * planes * r.s * r.lp * 2, 256);
   r.a_bytes = up(batch * planes * r.s * r.sp * 2, 256);
-  // splits never make more tiles than there are SM pairs, of which a GPU has at most 128
-  r.shares = lower_tiles(r.s, 128) * batch <= kMostPairs / 2 ? static_cast<int64_t>(kMostPairs) * kPairRows * 128 * 4 : 0;
+  // of both symmetric products, for as many SM pairs as a GPU may have: with fewer there are no more splits
+  if (batch > 0 && r.s > 0) {
+    const int64_t tiles = batch * lower_tiles(r.s, 128);
+    for (const int64_t K : {r.l, r.s}) {
+      const int64_t n = splits_of(batch, r.s, K, split, kMostPairs), bytes = n > 1 ? tiles * n * kPairRows * 128 * 4 : 0;
+      if (bytes > r.shares) r.shares = bytes;
+    }
+  }
   r.total = 2 * r.x_bytes + 2 * r.a_bytes + up(batch * 4, 256) + up(batch * kMostPartials * 8, 256) + r.shares;
   return r;
 }
@@ -625,23 +648,6 @@ hb_status launch(Product p, const typename Epi::Params& ep, cudaStream_t s, Prod
   HB_CUDA_TRY(launch_clusters(kernel, clusters, 2 * Epi::kShares, Shape<BN>::kThreads, Ring<BN, Epi>::kSmem, s, p, ep));
   if (as_launched) *as_launched = p;
   return HB_OK;
-}
-
-// Times in units of 240 cycles: a slot of operands with low parts takes 4, of others 1, a second launch that adds shares from
-// memory about 55, and sums that the pairs of a cluster exchange 15 and 7 (fitted to updates of 200 x 200 to 1024 x 1024).
-constexpr int kSecondLaunch = 55;
-int64_t slot_time(int64_t slots, bool split) { return slots * (split ? 4 : 1); }
-
-// How many ways K of a symmetric product is split, the shares added by a second launch: as many as there are SM pairs for the
-// tiles, of at least four slots; one unless that saves more than the launch takes.
-int splits_of(int64_t batch, int64_t s, int64_t K, bool split, int pairs) {
-  const int64_t tiles = batch * lower_tiles(s, 128), slots = (K + 63) / 64;
-  int64_t n = pairs / tiles;
-  if (n > slots / 4) n = slots / 4;
-  if (n < 2) return 1;
-  const int64_t each = (slots + n - 1) / n;
-  if (slot_time(slots - each, split) < kSecondLaunch) return 1;
-  return static_cast<int>((slots + each - 1) / each);      // none without slots
 }
 
 // How many pairs of a cluster share K of a product with `tiles` tiles of 128 columns: as many as make it shortest, where all its

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from habitat_b200 import _native
 from tests import newton_schulz as ns
 
 SHAPES = [(12, 1024), (64, 200), (128, 700), (300, 260), (2, 150, 180)]
@@ -38,3 +39,15 @@ def test_faults_do_not(shape, dtype):
         with pytest.raises(AssertionError):
             ns.check(ns.steps_of(g, bits=bits).to(dtype), g, _operands(shape))
     assert float((want - lost).norm() / want.norm()) < 0.5             # (no gross ones)
+
+
+def test_workspaces_have_room_for_shares_only_where_there_are_some():
+    """Symmetric products of few tiles and a long K leave shares of 256 x 128 float32 in memory; nothing else does."""
+    size = _native.load().hb_orthogonalize_workspace_bytes
+    for batch, rows, cols in ((1, 1, 1), (1, 1024, 12), (1, 64, 64), (1, 128, 300), (3, 100, 90), (1, 200, 200)):
+        for split in (0, 1):
+            s, l = min(rows, cols), max(rows, cols)
+            up = lambda x, m: (x + m - 1) // m * m
+            planes = 2 * batch * (1 + split) * 2 * s * (up(l, 64) + up(s, 64)) + 4 * batch * 257 * 2
+            assert planes <= size(batch, rows, cols, split) <= planes + 6 * 256
+    assert size(1, 150, 8000, 1) >= 2 * 2 * 2 * 150 * 8000 + 2 * 25 * 256 * 128 * 4

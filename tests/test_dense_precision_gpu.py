@@ -140,3 +140,39 @@ def test_float32_results_are_near_what_float32_operations_give(shape):
     off = lambda x: float((x.double() - want).norm() / want.norm())
     here, plain = off(dense.orthogonalize(update)), off(_float32_operations(update))
     assert here <= 2 * plain, (here, plain)
+
+
+# tiles with other numbers of steps (the buffers of X change places), K of all products split over clusters and over launches, batches
+@pytest.mark.parametrize("shape", [(64, 500), (100, 180), (300, 260), (200, 200), (150, 8000), (300, 3000), (2, 650, 700), (12, 140, 150), (1200, 1100)])
+@pytest.mark.parametrize("steps", [1, 2, 3, 4, 7])
+def test_steps_of_larger_matrices(shape, steps):
+    for dtype in (torch.float32, torch.bfloat16):
+        update = ns.update(shape, steps, dtype).cuda()
+        ns.check(dense.orthogonalize(update, steps=steps), update, 22, steps=steps)
+
+
+def test_streams_and_graphs_share_nothing():
+    """Updates whose shares lie in workspaces, on several streams and in two graphs at once."""
+    updates = [ns.update(shape, 9).cuda() for shape in ((150, 8000), (150, 9000), (300, 3000), (12, 1000), (100, 2000))]
+    run = lambda: [dense.orthogonalize(u) for u in updates] + [dense.orthogonalize(updates[3], steps=20)]
+    want = run()
+    graphs, results = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            results.append(run())
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    for _ in range(4):
+        torch.cuda.synchronize()
+        for st, g in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                g.replay()
+        eager = []
+        for st in streams[2:]:
+            with torch.cuda.stream(st):
+                eager.append(run())
+        torch.cuda.synchronize()
+        for got in results + eager:
+            assert all(torch.equal(x, y) for x, y in zip(got, want))
+    dense.check_status()
