@@ -176,3 +176,14 @@ def test_streams_and_graphs_share_nothing():
         for got in results + eager:
             assert all(torch.equal(x, y) for x, y in zip(got, want))
     dense.check_status()
+
+
+@pytest.mark.parametrize("shape", [(20, 30), (64, 200), (200, 100), (300, 260), (260, 300)])
+@pytest.mark.parametrize("largest", [1e-32, 1e-36, 1e-38, 1e-41, 3e38])
+def test_updates_next_to_the_ends_of_float32(shape, largest):
+    update = ns.update(shape, 4).double()
+    update = (update * (largest / update.abs().max())).float().cuda()
+    for eps in (0.0, 1e-30 if largest < 1 else 1e30):
+        want = ns.steps_of(update, eps=eps)
+        if float(want.abs().max()) > 1e-3:                # else there is little left beside 2^-32
+            ns.check(dense.orthogonalize(update, eps=eps), update, 64 if min(shape) <= 32 else 22, eps=eps)
