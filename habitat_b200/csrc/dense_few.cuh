@@ -27,7 +27,6 @@ struct FewParams {
   int8_t* out_q;                         // or quantised rows
   int64_t out_pitch;
   float* out_scales;
-  int32_t* status;
 };
 
 __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {

@@ -423,8 +423,8 @@ __device__ __forceinline__ void expect_shares(const EpiContext& c) {
 // cluster that share rows, one pair per BN columns), kShares (above 1: the pairs of a cluster share K, a tile per cluster) and
 //   static void begin(const Params&, const Product&, EpiContext&, sums)         before a tile's accumulators are waited for
 //   static void fetch(const Params&, const Product&, EpiContext&, row0, n0)     requests what a tile's results need, a tile ahead
-//   static void drain(const Params&, const Product&, EpiContext&, sums, release)   calls release() once the accumulators are read,
-//                                                                                  and c.fetch_next() once that is used
+//   static void drain(const Params&, const Product&, EpiContext&, sums, release)   calls release() once the accumulators are read, and,
+//                                                                                  where it has used what fetch() brought, requests the next tile's
 // kSplit: the tensor core adds 16 products of K at a time to its float32 sums and cuts what does not fit, which over long K is
 // off by as many units as there are additions, all to the same side (1024 x 1024 float32 updates: 3.7e-5).  So every
 // slot has an accumulation of its own, the small products of high and low parts first, and drain() adds them in

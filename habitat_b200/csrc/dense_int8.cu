@@ -4,8 +4,9 @@
 // Definition (float32 arithmetic, every operation rounded to nearest): amax = max |x| of the row, q = rint(x * (127 / amax)),
 // scale = amax / 127; y = (float(sum q w) * channel scale) * row scale + bias, then ReLU.  The integer sums are exact, so
 // results do not depend on the order of the additions: all kernels here, and any other program that follows the
-// definition, give the same bits.  A row whose amax is below 2^-119 counts as zeros (127 / amax would overflow); a row with
-// an infinity or a NaN gets zeros and the scale NaN, so that its results are NaN and not finite numbers that look like some.
+// definition, give the same bits.  Two exceptions to the formula: a row whose amax is below 2^-119 counts as zeros, since its scale would
+// be a subnormal number of a few bits (and below 2^-121 127 / amax overflows); a row with an infinity or a NaN gets zeros and the
+// scale NaN, so that its results are NaN and not finite numbers that look like some.
 #include <atomic>
 #include <cmath>
 #include <type_traits>
@@ -498,9 +499,9 @@ bool through_memory(int64_t M, int64_t N, int64_t K) { return N > 1024 || (M <= 
 
 // Operands that TMA can read: as they are, or copied to the workspace.
 hb_status align_operands(const char* name, Operands* o, int64_t M, int64_t N, int64_t K, uint8_t* workspace, int64_t workspace_bytes,
-                         int64_t more, cudaStream_t s) {
+                         cudaStream_t s) {
   const bool q_ok = tma_rows(o->q, o->q_pitch), w_ok = tma_rows(o->w, o->w_pitch);
-  const int64_t need = align_bytes(M, K, q_ok) + align_bytes(N, K, w_ok) + more;
+  const int64_t need = align_bytes(M, K, q_ok) + align_bytes(N, K, w_ok);
   if (need > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256)) {
     hb::set_error("%s: the workspace has to have %lld bytes, on a 256-byte boundary", name, static_cast<long long>(need));
     return HB_ERR_INVALID_ARGUMENT;
@@ -766,12 +767,12 @@ extern "C" hb_status hb_int8_matmul(const int8_t* q, int64_t q_pitch, const floa
   if (M == 0 || N == 0) return HB_OK;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   Operands o{q, q_pitch, w, w_pitch};
-  if (const hb_status st = align_operands(name, &o, M, N, K, static_cast<uint8_t*>(workspace), workspace_bytes, 0, s)) return st;
+  if (const hb_status st = align_operands(name, &o, M, N, K, static_cast<uint8_t*>(workspace), workspace_bytes, s)) return st;
   FloatOut::Params ep{{q_scales, w_scales, bias, relu ? 1 : 0, 1.0f}, {out, out_pitch, 0, out_type, 0}};
   ep.out.vec = row_alignment(out, out_pitch, 0, out_type == HB_F32 ? 4 : 2);
   if (M <= kFewRows) {
     FewParams few{o.q, o.w, o.q_pitch, o.w_pitch, ep.s, static_cast<int32_t>(M), static_cast<int32_t>(N), static_cast<int32_t>(K), ep.out, nullptr, 0,
-                  nullptr, status};
+                  nullptr};
     return launch_few(few, s);
   }
   int sms = 0;
@@ -812,11 +813,11 @@ extern "C" hb_status hb_int8_matmul_quantized(const int8_t* q, int64_t q_pitch, 
       return st;
     return hb_quantize_rows(y, HB_F32, M, N, pitch, out, out_pitch, out_scales, stream);
   }
-  if (const hb_status st = align_operands(name, &o, M, N, K, ws, workspace_bytes, 0, s)) return st;
+  if (const hb_status st = align_operands(name, &o, M, N, K, ws, workspace_bytes, s)) return st;
   const LayerScales scales{q_scales, w_scales, bias, relu ? 1 : 0, 1.0f};
   if (M <= kFewRows) {
     FewParams few{o.q, o.w, o.q_pitch, o.w_pitch, scales, static_cast<int32_t>(M), static_cast<int32_t>(N), static_cast<int32_t>(K), Out{}, out,
-                  out_pitch, out_scales, status};
+                  out_pitch, out_scales};
     return launch_few(few, s);
   }
   switch ((N + 255) / 256) {

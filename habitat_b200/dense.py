@@ -7,7 +7,8 @@
 
 All take CUDA tensors, queue their work on the current stream without synchronising, allocate results and workspaces
 through torch, and run in the library's sm_100a kernels (habitat_b200/csrc/dense_int8.cu, orthogonalize.cu).  The first
-call on a GPU sets up a status word there: make it before a stream capture.
+call on a GPU sets up a status word there: make it before a stream capture.  Results carry no gradient, whatever the
+arguments require.
 """
 import ctypes
 
@@ -47,8 +48,8 @@ def _check_vector(t, n, name, device):
 def quantize_rows(x):
     """Rows of a float32, bfloat16 or float16 matrix in 8-bit integers: (q [rows, cols] int8, scales [rows] float32), so that
     q[i, j] * scales[i] is x[i, j] to within half a scale.  In float32: scale = max |x| / 127, q = rint(x * (127 / max |x|)),
-    ties to even.  Rows of zeros (magnitudes below 2^-119) get the scale 0, rows with an infinity or a NaN zeros and the scale
-    NaN.  q's rows start on 16-byte boundaries, as the products want them."""
+    ties to even.  Rows of zeros (magnitudes below 2^-119, whose scale would be subnormal) get the scale 0, rows with an infinity
+    or a NaN zeros and the scale NaN.  q's rows start on 16-byte boundaries, as the products want them."""
     res = _native.binding().quantize_rows(x)
     if res is None:
         _check_rows(x, tuple(_TYPES), "x")
@@ -120,7 +121,7 @@ def orthogonalize(update, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1
 
 def check_status():
     """Synchronises the current GPU and raises if a launch of this module gave up on a bounded device wait.  The calls above raise for
-    that, too, without synchronising.  Each thread is told once, whoever's launch it was."""
+    that, too, without synchronising.  Each thread is told once, whichever thread launched it."""
     code = ctypes.c_int32(0)
     _native.check(_native.load().hb_dense_status(ctypes.byref(code)))
 

@@ -527,7 +527,7 @@ hb_status hb_orthogonalize(const void* update, int32_t type, int64_t batch, int6
 int64_t hb_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols, int32_t split);
 
 /* Synchronises the current GPU and reports whether one of the launches above gave up on a bounded device wait (reported
- * once to each host thread that has made such calls, whoever's launch it was; without this call the thread's next one of them on
+ * once to each host thread that has made such calls, whichever thread launched it; without this call the thread's next one of them on
  * that GPU reports it). */
 hb_status hb_dense_status(int32_t* device_status);
 /* How often one of them is known to have given up on the current GPU, `synchronise`: after waiting for it.  For callers that keep track

@@ -247,3 +247,11 @@ def test_features_are_divided_by_sigma():
                                             _native.current_stream_ptr()))
         # one feature through a weight of one: the row's scale is the quotient / 127
         assert float(scales) == np.float32(float(x) / sigma) / np.float32(127), (x, sigma)
+
+
+def test_results_carry_no_gradient():
+    x = torch.randn(40, 64, device="cuda", requires_grad=True)
+    q, scales = dense.quantize_rows(x)
+    for y in (scales, dense.int8_matmul(q, scales, q, scales, bias=scales.detach().requires_grad_()), dense.orthogonalize(x)):
+        assert not y.requires_grad and y.grad_fn is None
+    assert "carry no gradient" in dense.__doc__
