@@ -107,6 +107,7 @@ class RuntimePredictor:
         self._device_rows = None
         self._momentum = None
         self._unchecked = None               # (GPU, dense.failures()) from before updates whose launches may have given up
+        self._given_up = False               # one of them has
         if model_path is not None:
             self.load_state(model_path)
 
@@ -128,6 +129,7 @@ class RuntimePredictor:
     def invalidate(self):
         """Drops the device-side weight pack (call after changing weights, mu or sigma).  A prediction that another
         thread is making keeps it until it has ended."""
+        self._given_up = False
         self._handle = None
         self._device_rows = None
 
@@ -139,7 +141,8 @@ class RuntimePredictor:
         by `steps` Newton-Schulz steps (dense.orthogonalize, all layers in one call), and
         w <- (1 - lr weight_decay) w - lr update.  Biases, fc1 and fc2 are left to the caller's optimizer.
         The next prediction packs the new weights (`invalidate`).  Does not synchronise: whether a launch gave up on a bounded
-        device wait, which leaves weights that mean nothing, is seen and raised before they are packed or saved."""
+        device wait, which leaves weights that mean nothing, is seen before they are packed or saved, and raised until they are
+        replaced (`load_state`, or `invalidate` behind weights of the caller's)."""
         from habitat_b200 import dense
         weights = [block.weight for block in self.model.mlp.layers if isinstance(block, nn.Linear)]
         if any(w.grad is None for w in weights):
@@ -153,6 +156,8 @@ class RuntimePredictor:
                 kept = torch.zeros_like(g)
             kept = kept.mul(momentum).add_(g)
             update = torch.add(g, kept, alpha=momentum) if nesterov else kept
+            if self._given_up or (self._unchecked is not None and self._unchecked[0] != g.device):
+                self._check_updates()
             if self._unchecked is None:
                 with torch.cuda.device(g.device):
                     unchecked = g.device, dense.failures()
@@ -166,11 +171,19 @@ class RuntimePredictor:
         self.invalidate()
 
     def _check_updates(self):
+        from habitat_b200 import _native, dense
         if self._unchecked is not None:
-            from habitat_b200 import dense
             (device, since), self._unchecked = self._unchecked, None
-            with torch.cuda.device(device):
-                dense.check_since(since)
+            try:
+                with torch.cuda.device(device):
+                    dense.check_since(since)
+            except _native.HabitatNativeError as e:
+                if e.status != _native.HB_ERR_DEVICE_TIMEOUT:
+                    raise
+                self._given_up = True
+        if self._given_up:
+            raise _native.HabitatNativeError(_native.HB_ERR_DEVICE_TIMEOUT,
+                                             "an update of the hidden layers gave up on a bounded wait: their weights mean nothing")
 
     # -- inference ----------------------------------------------------------
     def _ensure_handle(self):

@@ -498,6 +498,7 @@ class Int8MLPHandle:
         with torch.cuda.device(self.device):
             since, self._failures = self._failures, dense.failures(synchronise=True)
             dense.check_since(since)
+            dense.check_status()          # what another thread's predict has reported there
 
 
 def special_scale(run_time_ms, pred_dest, pred_orig, negative_count=None):

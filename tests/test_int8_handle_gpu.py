@@ -216,10 +216,14 @@ def test_updates_that_gave_up_are_neither_served_nor_saved(precision, told, how,
             _other_call()
     feats, dev = (torch.from_numpy(a).cuda() for a in workloads.make_queries("linear", 20, seed=4))
     path = str(tmp_path / "model.pth")
-    with pytest.raises(_native.HabitatNativeError, match="gave up"):
-        pred.predict_batch(feats, dev) if how == "predict" else pred.save_state(path)
+    for _ in range(2):
+        with pytest.raises(_native.HabitatNativeError, match="gave up"):
+            pred.predict_batch(feats, dev) if how == "predict" else pred.save_state(path)
     assert not (tmp_path / "model.pth").exists()
-    pred.save_state(path)                             # the caller has been told
+    with pytest.raises(_native.HabitatNativeError, match="gave up"):
+        pred.update_hidden(0.1)
+    pred.invalidate()                                 # the caller says that the weights are good
+    pred.save_state(path)
     pred.load_state(path)
     assert bool(torch.isfinite(pred.predict_batch(feats, dev)).all())
     dense.check_status()
@@ -247,6 +251,59 @@ def test_features_are_divided_by_sigma():
                                             _native.current_stream_ptr()))
         # one feature through a weight of one: the row's scale is the quotient / 127
         assert float(scales) == np.float32(float(x) / sigma) / np.float32(127), (x, sigma)
+
+
+def test_invalidate_does_not_hide_an_update_that_gave_up():
+    """It belongs behind every change of weights, a step of the caller's optimizer after update_hidden for one."""
+    pred = _trained(precision="bf16", steps=2)
+    _gives_up()
+    pred.invalidate()
+    with pytest.raises(_native.HabitatNativeError, match="gave up"):
+        pred.device_row("V100")
+
+
+@pytest.mark.parametrize("precision", ["bf16", "int8"])
+def test_traces_are_not_predicted_with_an_update_that_gave_up(precision):
+    """Predictions of traces start their predictors early and try again where that raises."""
+    from habitat_b200.analysis import Device
+    from habitat_b200.analysis.arguments import Arguments
+    from habitat_b200.analysis.operation import MeasuredOperation
+    from habitat_b200.analysis.predictor import Predictor
+    from habitat_b200.analysis.run_time import RunTimeMeasurement
+    from habitat_b200.analysis.trace import Trace
+    predictor = Predictor(precision=precision)
+    predictor.linear_pred = _trained(precision=precision, steps=2)
+    _gives_up()
+    operation = MeasuredOperation("linear", Arguments(((64, 512), (256, 512), None), {}), RunTimeMeasurement(3.0, [], Device.V100), None, Device.V100)
+    for _ in range(2):
+        with pytest.raises(_native.HabitatNativeError, match="gave up"):
+            Trace(Device.V100, [operation]).to_devices([Device.T4, Device.P100], predictor)
+    predictor.linear_pred.invalidate()
+    Trace(Device.V100, [operation]).to_devices([Device.T4, Device.P100], predictor)
+
+
+def test_a_failure_that_another_threads_prediction_reported_is_not_lost():
+    import threading
+    h, f, d = _handle()
+    h.predict(f, d)
+    _gives_up()
+    raised = []
+
+    def other():
+        dense.quantize_rows(torch.ones((2, 16), device="cuda"))
+        for _ in range(2):
+            try:
+                h.predict(f, d)
+                raised.append(False)
+            except _native.HabitatNativeError:
+                raised.append(True)
+    t = threading.Thread(target=other)
+    t.start()
+    t.join()
+    assert raised == [True, False]
+    with pytest.raises(_native.HabitatNativeError, match="gave up"):
+        h.check_status()
+    h.check_status()
 
 
 def test_results_carry_no_gradient():
